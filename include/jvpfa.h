@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define JVPFA_VERSION 103 /* major*100 + minor; 101: fields after the last of 100 in four structs; 102: workspace in two; 103: kv_len_host in two */
+#define JVPFA_VERSION 104 /* major*100 + minor; 101: fields after the last of 100 in four structs; 102: workspace in two; 103: kv_len_host in two; 104: jvpfa_rotary */
 
 typedef enum {
   JVPFA_OK = 0,
@@ -357,6 +357,39 @@ typedef struct {
 } jvpfa_pad_bias_args;
 
 int jvpfa_pad_bias(const jvpfa_pad_bias_args* args, void* stream);
+
+/*
+ * jvpfa_rotary -- rotary positions: each pair (a, b) of a row's entries turned by position * frequency,
+ *   (a', b') = amplitude * (a cos - b sin, a sin + b cos),
+ * for up to four tensors (queries, keys, their tangents) in one launch.  No upstream counterpart.
+ *
+ * The first 2 * n_freq of the D entries of a row are turned, the others copied.  Pair i is entries (i, n_freq + i), or with
+ * `interleaved` (2 i, 2 i + 1).  `transposed` turns the other way, which is the gradient.  Tensors are (B, H, L, D) with the head
+ * dimension contiguous and any other strides (in elements); x and y may be the same memory, and y must not overlap itself.
+ */
+typedef struct {
+  const void* x;
+  void* y;
+  int32_t H; /* heads: each tensor its own number */
+  int64_t x_stride[3], y_stride[3]; /* batch, head, row */
+} jvpfa_rotary_tensor;
+
+typedef struct {
+  int32_t struct_size; /* sizeof(jvpfa_rotary_args) */
+  int32_t dtype;       /* JVPFA_BF16, JVPFA_FP16 or JVPFA_FP32 */
+  int32_t B, L, D, n_freq;
+  int32_t n_tensors; /* 1 to 4 */
+  int32_t interleaved, transposed;
+  int32_t position_bits;  /* 32 or 64: the type of positions */
+  float amplitude;        /* of cosine and sine */
+  const double* freq;     /* n_freq radians per position */
+  const void* positions;  /* (B, L) signed integers through position_stride (0 = broadcast), |position| < 2^53; NULL: offset + row */
+  int64_t position_stride[2];
+  int64_t offset;
+  jvpfa_rotary_tensor t[4];
+} jvpfa_rotary_args;
+
+int jvpfa_rotary(const jvpfa_rotary_args* args, void* stream);
 
 /* Human-readable text for a jvpfa_status (static storage, never NULL). */
 const char* jvpfa_strerror(int status);

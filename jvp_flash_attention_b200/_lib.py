@@ -53,6 +53,7 @@ EXPORTS = (
     "jvpfa_mask_check",
     "jvpfa_mask_tiles",
     "jvpfa_pad_bias",
+    "jvpfa_rotary",
 )
 
 NOALLOC_MAX_ROWS = 524288  # JVPFA_NOALLOC_MAX_ROWS
@@ -227,6 +228,37 @@ class PadBiasArgs(C.Structure):
     ]
 
 
+class RotaryTensor(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("y", C.c_void_p),
+        ("H", C.c_int32),
+        ("x_stride", C.c_int64 * 3),
+        ("y_stride", C.c_int64 * 3),
+    ]
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_int32),
+        ("dtype", C.c_int32),
+        ("B", C.c_int32),
+        ("L", C.c_int32),
+        ("D", C.c_int32),
+        ("n_freq", C.c_int32),
+        ("n_tensors", C.c_int32),
+        ("interleaved", C.c_int32),
+        ("transposed", C.c_int32),
+        ("position_bits", C.c_int32),
+        ("amplitude", C.c_float),
+        ("freq", C.c_void_p),
+        ("positions", C.c_void_p),
+        ("position_stride", C.c_int64 * 2),
+        ("offset", C.c_int64),
+        ("t", RotaryTensor * 4),
+    ]
+
+
 _lib = None
 
 
@@ -273,6 +305,8 @@ def load() -> C.CDLL:
     lib.jvpfa_mask_tiles.restype = C.c_int
     lib.jvpfa_pad_bias.argtypes = [C.POINTER(PadBiasArgs), C.c_void_p]
     lib.jvpfa_pad_bias.restype = C.c_int
+    lib.jvpfa_rotary.argtypes = [C.POINTER(RotaryArgs), C.c_void_p]
+    lib.jvpfa_rotary.restype = C.c_int
     _lib = lib
     return lib
 

@@ -3,8 +3,8 @@
 Usage: ``python -m jvp_flash_attention_b200.build [--force] [--verbose]``.
 Each ``csrc/*.cu`` is compiled to an object file under ``csrc/_obj`` (in parallel) and the
 objects are linked into ``jvp_flash_attention_b200/libjvpfa.so``.  A translation unit is rebuilt
-only when it or a header is newer than its object.  ``csrc/native.cpp``, the host side of a call
-(``_native.so``, a Python extension module linked against torch and libjvpfa.so), is built with g++, again also when
+only when it or a header is newer than its object.  ``csrc/native*.cpp``, the host side of a call
+(``_native.so``, a Python extension module linked against torch and libjvpfa.so), are built with g++, again also when
 the command or the version of torch is another one than it was built with.
 """
 from __future__ import annotations
@@ -60,7 +60,7 @@ def _native_cmd() -> list[str]:
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_native",
         "-I", str(INCLUDE), "-I", str(CSRC / "compat"), "-I", sysconfig.get_paths()["include"],
         *(f"-isystem{p}" for p in cpp_extension.include_paths("cuda")),
-        str(CSRC / "native.cpp"), "-o", str(NATIVE),
+        *(str(f) for f in sorted(CSRC.glob("native*.cpp"))), "-o", str(NATIVE),
         f"-L{torch_lib}", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10",
         f"-L{PKG_DIR}", "-l:libjvpfa.so", "-Wl,-rpath,$ORIGIN",
     ]
@@ -73,7 +73,7 @@ def _native_with() -> str:
 
 
 def _native_stale() -> bool:
-    sources = [CSRC / "native.cpp", INCLUDE / "jvpfa.h", *(CSRC / "compat").rglob("*.hpp")]
+    sources = [*CSRC.glob("native*"), INCLUDE / "jvpfa.h", *(CSRC / "compat").rglob("*.hpp")]
     if not NATIVE.exists() or NATIVE.stat().st_mtime < max(f.stat().st_mtime for f in sources):
         return True
     return not NATIVE_STAMP.exists() or NATIVE_STAMP.read_text() != _native_with()

@@ -327,6 +327,28 @@ int jvpfa_pad_bias(const jvpfa_pad_bias_args* a, void* stream) {
   return launch_pad_bias(*a, static_cast<cudaStream_t>(stream));
 }
 
+int jvpfa_rotary(const jvpfa_rotary_args* a, void* stream) {
+  if (!a) return JVPFA_ERR_NULL;
+  if (a->struct_size != (int32_t)sizeof(jvpfa_rotary_args)) return JVPFA_ERR_STRUCT;
+  if (a->dtype != JVPFA_BF16 && a->dtype != JVPFA_FP16 && a->dtype != JVPFA_FP32) return JVPFA_ERR_DTYPE;
+  if (a->B < 1 || a->L < 1 || a->D < 1 || a->n_freq < 0 || a->n_freq > a->D / 2) return JVPFA_ERR_SHAPE;
+  if (a->n_tensors < 1 || a->n_tensors > 4) return JVPFA_ERR_SHAPE;
+  if (a->n_freq > 0 && !a->freq) return JVPFA_ERR_NULL;
+  if (a->positions && a->position_bits != 32 && a->position_bits != 64) return JVPFA_ERR_DTYPE;
+  const uintptr_t size = a->dtype == JVPFA_FP32 ? 4 : 2;
+  for (int t = 0; t < a->n_tensors; ++t) {
+    const jvpfa_rotary_tensor& x = a->t[t];
+    if (!x.x || !x.y) return JVPFA_ERR_NULL;
+    if (x.H < 1) return JVPFA_ERR_SHAPE;
+    if ((reinterpret_cast<uintptr_t>(x.x) | reinterpret_cast<uintptr_t>(x.y)) % size) return JVPFA_ERR_ALIGN;
+    for (int d = 0; d < 3; ++d)
+      if (x.x_stride[d] < 0 || x.y_stride[d] < 0) return JVPFA_ERR_SHAPE;
+  }
+  const int rc = check_arch();
+  if (rc) return rc;
+  return launch_rotary(*a, static_cast<cudaStream_t>(stream));
+}
+
 int jvpfa_device_status(int* status, int clear) {
   if (!status) return JVPFA_ERR_NULL;
   return tc5_read_status(status, clear);
