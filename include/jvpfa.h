@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define JVPFA_VERSION 104 /* major*100 + minor; 101: fields after the last of 100 in four structs; 102: workspace in two; 103: kv_len_host in two; 104: jvpfa_rotary */
+#define JVPFA_VERSION 104 /* major*100 + minor; 101: fields after the last of 100 in four structs; 102: workspace in two; 103: kv_len_host in two; 104: jvpfa_rotary, jvpfa_gated_fwd, jvpfa_gated_bwd */
 
 typedef enum {
   JVPFA_OK = 0,
@@ -390,6 +390,66 @@ typedef struct {
 } jvpfa_rotary_args;
 
 int jvpfa_rotary(const jvpfa_rotary_args* args, void* stream);
+
+/*
+ * jvpfa_gated_fwd, jvpfa_gated_bwd -- the widening half of a gated feed-forward block, value and tangent, and the gradients through
+ * both.  No upstream counterpart.
+ *
+ *   g = x wg^T, u = x wu^T, h = a(g) u                       x, tx: (M, K); wg, wu: (F, K); all others (M, F)
+ *   tg = tx wg^T, tu = tx wu^T, th = a'(g) tg u + a(g) tu
+ *
+ * and for cotangents gh of h and gth of th
+ *
+ *   dg = gh a' u + gth (a'' tg u + a' tu),  du = gh a + gth a' tg,  dtg = gth a' u,  dtu = gth a
+ *   dx = dg wg + du wu,  dtx = dtg wg + dtu wu,  dwg = dg^T x + dtg^T tx,  dwu = du^T x + dtu^T tx
+ *
+ * Sums are held in 32 bits; g, u, tg, tu and the four between the two steps of the backward are kept in the tensors' type.
+ * JVPFA_FP32 multiplies three bf16 parts of every entry (error ~1e-6 relative).  x, tx, wg, wu have contiguous columns and row
+ * strides in elements; all other tensors are row-major.
+ */
+typedef enum {
+  JVPFA_ACT_SILU = 0,      /* g / (1 + exp(-g)) */
+  JVPFA_ACT_SIGMOID = 1,   /* 1 / (1 + exp(-g)) */
+  JVPFA_ACT_GELU = 2,      /* g times the normal distribution function of g */
+  JVPFA_ACT_GELU_TANH = 3  /* its approximation 0.5 g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) */
+} jvpfa_activation;
+
+typedef struct {
+  int32_t struct_size; /* sizeof(jvpfa_gated_fwd_args) */
+  int32_t dtype;       /* JVPFA_BF16, JVPFA_FP16 or JVPFA_FP32 */
+  int32_t M, K, F;
+  int32_t activation;
+  const void *x, *tx; /* tx NULL: the value alone */
+  const void *wg, *wu;
+  int64_t x_stride, tx_stride, wg_stride, wu_stride;
+  void *h, *th;           /* th iff tx */
+  void *g, *u, *tg, *tu;  /* for jvpfa_gated_bwd: g and u or neither, tg and tu iff tx and g */
+  void* workspace;        /* jvpfa_gated_fwd_workspace() bytes of scratch, 16-byte aligned (0: NULL) */
+  int64_t workspace_bytes;
+} jvpfa_gated_fwd_args;
+
+int jvpfa_gated_fwd(const jvpfa_gated_fwd_args* args, void* stream);
+/* Bytes of scratch that this call needs (workspace itself not looked at), 0 for arguments that it refuses; host logic. */
+int64_t jvpfa_gated_fwd_workspace(const jvpfa_gated_fwd_args* args);
+
+typedef struct {
+  int32_t struct_size; /* sizeof(jvpfa_gated_bwd_args) */
+  int32_t dtype;
+  int32_t M, K, F;
+  int32_t activation;
+  const void *x, *tx; /* tx iff gth; x and tx are read for dwg and dwu alone */
+  const void *wg, *wu;
+  int64_t x_stride, tx_stride, wg_stride, wu_stride;
+  const void *g, *u, *tg, *tu; /* as the forward left them; tg and tu iff gth */
+  const void *gh, *gth;        /* either may be NULL, not both */
+  void *dx, *dtx;              /* (M, K) row-major; NULL: not formed; dtx only with gth */
+  void *dwg, *dwu;             /* (F, K) row-major; both or neither */
+  void* workspace;             /* jvpfa_gated_bwd_workspace() bytes of scratch, 16-byte aligned */
+  int64_t workspace_bytes;
+} jvpfa_gated_bwd_args;
+
+int jvpfa_gated_bwd(const jvpfa_gated_bwd_args* args, void* stream);
+int64_t jvpfa_gated_bwd_workspace(const jvpfa_gated_bwd_args* args);
 
 /* Human-readable text for a jvpfa_status (static storage, never NULL). */
 const char* jvpfa_strerror(int status);

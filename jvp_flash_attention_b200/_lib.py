@@ -54,6 +54,10 @@ EXPORTS = (
     "jvpfa_mask_tiles",
     "jvpfa_pad_bias",
     "jvpfa_rotary",
+    "jvpfa_gated_fwd",
+    "jvpfa_gated_fwd_workspace",
+    "jvpfa_gated_bwd",
+    "jvpfa_gated_bwd_workspace",
 )
 
 NOALLOC_MAX_ROWS = 524288  # JVPFA_NOALLOC_MAX_ROWS
@@ -259,6 +263,64 @@ class RotaryArgs(C.Structure):
     ]
 
 
+class GatedFwdArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_int32),
+        ("dtype", C.c_int32),
+        ("M", C.c_int32),
+        ("K", C.c_int32),
+        ("F", C.c_int32),
+        ("activation", C.c_int32),
+        ("x", C.c_void_p),
+        ("tx", C.c_void_p),
+        ("wg", C.c_void_p),
+        ("wu", C.c_void_p),
+        ("x_stride", C.c_int64),
+        ("tx_stride", C.c_int64),
+        ("wg_stride", C.c_int64),
+        ("wu_stride", C.c_int64),
+        ("h", C.c_void_p),
+        ("th", C.c_void_p),
+        ("g", C.c_void_p),
+        ("u", C.c_void_p),
+        ("tg", C.c_void_p),
+        ("tu", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
+    ]
+
+
+class GatedBwdArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_int32),
+        ("dtype", C.c_int32),
+        ("M", C.c_int32),
+        ("K", C.c_int32),
+        ("F", C.c_int32),
+        ("activation", C.c_int32),
+        ("x", C.c_void_p),
+        ("tx", C.c_void_p),
+        ("wg", C.c_void_p),
+        ("wu", C.c_void_p),
+        ("x_stride", C.c_int64),
+        ("tx_stride", C.c_int64),
+        ("wg_stride", C.c_int64),
+        ("wu_stride", C.c_int64),
+        ("g", C.c_void_p),
+        ("u", C.c_void_p),
+        ("tg", C.c_void_p),
+        ("tu", C.c_void_p),
+        ("gh", C.c_void_p),
+        ("gth", C.c_void_p),
+        ("dx", C.c_void_p),
+        ("dtx", C.c_void_p),
+        ("dwg", C.c_void_p),
+        ("dwu", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
+    ]
+
+
 _lib = None
 
 
@@ -307,6 +369,14 @@ def load() -> C.CDLL:
     lib.jvpfa_pad_bias.restype = C.c_int
     lib.jvpfa_rotary.argtypes = [C.POINTER(RotaryArgs), C.c_void_p]
     lib.jvpfa_rotary.restype = C.c_int
+    lib.jvpfa_gated_fwd.argtypes = [C.POINTER(GatedFwdArgs), C.c_void_p]
+    lib.jvpfa_gated_fwd.restype = C.c_int
+    lib.jvpfa_gated_fwd_workspace.argtypes = [C.POINTER(GatedFwdArgs)]
+    lib.jvpfa_gated_fwd_workspace.restype = C.c_int64
+    lib.jvpfa_gated_bwd.argtypes = [C.POINTER(GatedBwdArgs), C.c_void_p]
+    lib.jvpfa_gated_bwd.restype = C.c_int
+    lib.jvpfa_gated_bwd_workspace.argtypes = [C.POINTER(GatedBwdArgs)]
+    lib.jvpfa_gated_bwd_workspace.restype = C.c_int64
     _lib = lib
     return lib
 

@@ -3,6 +3,7 @@
 #include <cstddef>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 
 #include "common.cuh"
 
@@ -196,6 +197,47 @@ int check_bwd_request(const jvpfa_bwd_args* a) {
   return JVPFA_OK;
 }
 
+static int check_gated(int dtype, int M, int K, int F, int activation) {
+  if (dtype != JVPFA_BF16 && dtype != JVPFA_FP16 && dtype != JVPFA_FP32) return JVPFA_ERR_DTYPE;
+  if (M < 1 || K < 1 || F < 1) return JVPFA_ERR_SHAPE;
+  if (activation < JVPFA_ACT_SILU || activation > JVPFA_ACT_GELU_TANH) return JVPFA_ERR_UNSUPPORTED;
+  return JVPFA_OK;
+}
+// Operands that may be anywhere their elements may, and tensors that are read and written in whole pieces.
+static int check_gated_memory(int dtype, std::initializer_list<const void*> operands, std::initializer_list<int64_t> strides,
+                              std::initializer_list<const void*> tensors) {
+  for (const void* p : operands)
+    if (reinterpret_cast<uintptr_t>(p) % (dtype == JVPFA_FP32 ? 4 : 2)) return JVPFA_ERR_ALIGN;
+  for (const int64_t st : strides)
+    if (st < 0) return JVPFA_ERR_SHAPE;
+  for (const void* p : tensors)
+    if (!aligned16(p)) return JVPFA_ERR_ALIGN;
+  return JVPFA_OK;
+}
+
+static int validate_gated_fwd(const jvpfa_gated_fwd_args* a) {
+  if (!a) return JVPFA_ERR_NULL;
+  if (a->struct_size != (int32_t)sizeof(jvpfa_gated_fwd_args)) return JVPFA_ERR_STRUCT;
+  const int rc = check_gated(a->dtype, a->M, a->K, a->F, a->activation);
+  if (rc) return rc;
+  if (!a->x || !a->wg || !a->wu || !a->h || !a->th != !a->tx || !a->g != !a->u || !a->tg != !a->tu || !a->tg != !(a->tx && a->g))
+    return JVPFA_ERR_NULL;
+  return check_gated_memory(a->dtype, {a->x, a->tx, a->wg, a->wu}, {a->x_stride, a->tx_stride, a->wg_stride, a->wu_stride},
+                            {a->h, a->th, a->g, a->u, a->tg, a->tu, a->workspace});
+}
+
+static int validate_gated_bwd(const jvpfa_gated_bwd_args* a) {
+  if (!a) return JVPFA_ERR_NULL;
+  if (a->struct_size != (int32_t)sizeof(jvpfa_gated_bwd_args)) return JVPFA_ERR_STRUCT;
+  const int rc = check_gated(a->dtype, a->M, a->K, a->F, a->activation);
+  if (rc) return rc;
+  if (!a->x || !a->wg || !a->wu || !a->g || !a->u || (!a->gh && !a->gth)) return JVPFA_ERR_NULL;
+  if (!a->tx != !a->gth || !a->tg != !a->gth || !a->tu != !a->gth || (a->dtx && !a->gth)) return JVPFA_ERR_NULL;
+  if (!a->dwg != !a->dwu || (!a->dx && !a->dtx && !a->dwg)) return JVPFA_ERR_NULL;
+  return check_gated_memory(a->dtype, {a->x, a->tx, a->wg, a->wu}, {a->x_stride, a->tx_stride, a->wg_stride, a->wu_stride},
+                            {a->g, a->u, a->tg, a->tu, a->gh, a->gth, a->dx, a->dtx, a->dwg, a->dwu, a->workspace});
+}
+
 }  // namespace jvpfa
 
 using namespace jvpfa;
@@ -347,6 +389,36 @@ int jvpfa_rotary(const jvpfa_rotary_args* a, void* stream) {
   const int rc = check_arch();
   if (rc) return rc;
   return launch_rotary(*a, static_cast<cudaStream_t>(stream));
+}
+
+int64_t jvpfa_gated_fwd_workspace(const jvpfa_gated_fwd_args* a) {
+  return validate_gated_fwd(a) == JVPFA_OK ? gated_fwd_workspace(*a) : 0;
+}
+
+int jvpfa_gated_fwd(const jvpfa_gated_fwd_args* a, void* stream) {
+  int rc = validate_gated_fwd(a);
+  if (rc) return rc;
+  const int64_t need = gated_fwd_workspace(*a);
+  if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return JVPFA_ERR_NULL;
+  rc = check_arch();
+  if (rc) return rc;
+  if (tc5_status_peek() != 0) return JVPFA_ERR_DEVICE_STATUS;
+  return launch_gated_fwd(*a, static_cast<cudaStream_t>(stream));
+}
+
+int64_t jvpfa_gated_bwd_workspace(const jvpfa_gated_bwd_args* a) {
+  return validate_gated_bwd(a) == JVPFA_OK ? gated_bwd_workspace(*a) : 0;
+}
+
+int jvpfa_gated_bwd(const jvpfa_gated_bwd_args* a, void* stream) {
+  int rc = validate_gated_bwd(a);
+  if (rc) return rc;
+  const int64_t need = gated_bwd_workspace(*a);
+  if (!a->workspace || a->workspace_bytes < need) return JVPFA_ERR_NULL;
+  rc = check_arch();
+  if (rc) return rc;
+  if (tc5_status_peek() != 0) return JVPFA_ERR_DEVICE_STATUS;
+  return launch_gated_bwd(*a, static_cast<cudaStream_t>(stream));
 }
 
 int jvpfa_device_status(int* status, int clear) {

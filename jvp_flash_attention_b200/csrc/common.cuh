@@ -613,6 +613,10 @@ int launch_mask_check(const jvpfa_mask_check_args& a, cudaStream_t stream);
 int launch_mask_tiles(const jvpfa_mask_tiles_args& a, cudaStream_t stream);
 int launch_pad_bias(const jvpfa_pad_bias_args& a, cudaStream_t stream);
 int launch_rotary(const jvpfa_rotary_args& a, cudaStream_t stream);
+int64_t gated_fwd_workspace(const jvpfa_gated_fwd_args& a);
+int launch_gated_fwd(const jvpfa_gated_fwd_args& a, cudaStream_t stream);
+int64_t gated_bwd_workspace(const jvpfa_gated_bwd_args& a);
+int launch_gated_bwd(const jvpfa_gated_bwd_args& a, cudaStream_t stream);
 int launch_fwd_tc5(const jvpfa_fwd_args& a, cudaStream_t stream);
 bool fwd_tc5_eligible(const jvpfa_fwd_args& a);
 bool tc5_head_dim(int D, int L);

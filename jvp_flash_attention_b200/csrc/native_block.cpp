@@ -14,6 +14,12 @@ py::object& rotary_module() {
   return *m;
 }
 
+py::object& gated_module() {
+  static py::object* m = new py::object(py::module_::import("jvp_flash_attention_b200.gated"));
+  return *m;
+}
+py::object or_none(const Tensor& t) { return t.defined() ? py::cast(t) : py::object(py::none()); }
+
 // The level of the lone torch.func.jvp that is active, -1 without any transform, -2 under others.
 int64_t jvp_level() {
   const auto& stack = at::functorch::getDynamicLayerStack();
@@ -75,7 +81,7 @@ std::vector<Tensor> launch_rotary(std::vector<Tensor> xs, const std::vector<Orde
     auto launch = rotary_module().attr("_launch");
     for (size_t i = 0; i < xs.size(); ++i)
       if (xs[i].defined())
-        ys[i] = launch(xs[i], freq, positions.defined() ? py::cast(positions) : py::object(py::none()), turn.offset, turn.interleaved,
+        ys[i] = launch(xs[i], freq, or_none(positions), turn.offset, turn.interleaved,
                        turn.amplitude, turn.transposed).cast<Tensor>();
     return ys;
   }
@@ -136,7 +142,7 @@ struct RotaryNode : public Node {
         auto turned = rotary_module().attr("_turn");
         for (size_t j = 0; j < grads.size(); ++j)
           if (grads[j].defined() && task_should_compute_output(j))
-            out[j] = turned(grads[j], f, p.defined() ? py::cast(p) : py::object(py::none()), back.offset, back.interleaved,
+            out[j] = turned(grads[j], f, or_none(p), back.offset, back.interleaved,
                             back.amplitude, back.transposed).cast<Tensor>();
         return out;
       }
@@ -227,9 +233,297 @@ py::object rotary(const Tensor& q_in, const std::optional<Tensor>& k_in, const T
   return py::make_tuple(q, dual(ys[1], ys[3], level));
 }
 
+// ---- gated projection ----------------------------------------------------------------------------------------------------
+struct GatedOut {
+  Tensor h, th, g, u, tg, tu;
+};
+struct GatedGrads {
+  Tensor dx, dtx, dwg, dwu;
+};
+
+Tensor from_python(const py::handle& o) { return o.is_none() ? Tensor() : o.cast<Tensor>(); }
+
+// (rows, K) with contiguous columns.
+Tensor as_rows(const Tensor& x) {
+  if (!x.defined() || (x.dim() == 2 && x.stride(1) == 1)) return x;
+  NoFunctorch nf;
+  at::AutoDispatchBelowADInplaceOrView below;
+  const int64_t K = x.size(-1);
+  Tensor r = x.dim() == 2 ? x : x.reshape({x.numel() / K, K});
+  return r.stride(1) == 1 ? r : r.contiguous();
+}
+// Row-major, on a 16-byte boundary, of the type of `like`.
+Tensor as_dense(const Tensor& x, const Tensor& like) {
+  if (!x.defined()) return x;
+  const bool aligned = (reinterpret_cast<uintptr_t>(x.const_data_ptr()) & 15u) == 0;
+  if (x.is_contiguous() && aligned && x.scalar_type() == like.scalar_type()) return x;
+  NoFunctorch nf;
+  at::AutoDispatchBelowADInplaceOrView below;
+  return at::empty_like(x, x.options().dtype(like.scalar_type()), at::MemoryFormat::Contiguous).copy_(x);
+}
+Tensor workspace_for(int64_t bytes, const Tensor& x) { return bytes > 0 ? empty({bytes}, at::kByte, x.device()) : Tensor(); }
+
+// h, with tx also th, and with `keep` the projections that a backward reads.
+GatedOut launch_gated_fwd(const Tensor& x, const Tensor& tx, const Tensor& wg, const Tensor& wu, int activation, bool keep) {
+  GatedOut r;
+  if (!x.is_cuda()) {
+    py::gil_scoped_acquire gil;
+    NoFunctorch nf;
+    at::AutoGradMode no_grad(false);
+    py::tuple out = gated_module().attr("_launch_fwd")(x, or_none(tx), wg, wu, activation, keep);
+    Tensor* to[] = {&r.h, &r.th, &r.g, &r.u, &r.tg, &r.tu};
+    for (int i = 0; i < 6; ++i) *to[i] = from_python(out[i]);
+    return r;
+  }
+  c10::cuda::OptionalCUDAGuard guard;
+  if (x.get_device() != c10::cuda::current_device()) guard.set_index(x.get_device());
+  std::vector<int64_t> sizes = x.sizes().vec();
+  sizes.back() = wg.size(0);
+  auto make = [&]() { return empty(sizes, x.scalar_type(), x.device()); };
+  r.h = make();
+  if (tx.defined()) r.th = make();
+  if (keep) {
+    r.g = make(), r.u = make();
+    if (tx.defined()) r.tg = make(), r.tu = make();
+  }
+  if (x.numel() == 0) return r;
+  const Tensor x2 = as_rows(x), tx2 = as_rows(tx), wg2 = as_rows(wg), wu2 = as_rows(wu);
+  jvpfa_gated_fwd_args a{};
+  a.struct_size = sizeof(a);
+  a.dtype = dtype_of(x, false);
+  a.M = (int)x2.size(0), a.K = (int)x2.size(1), a.F = (int)wg.size(0);
+  a.activation = activation;
+  a.x = data(x2), a.tx = data(tx2), a.wg = data(wg2), a.wu = data(wu2);
+  a.x_stride = x2.stride(0), a.tx_stride = tx2.defined() ? tx2.stride(0) : 0, a.wg_stride = wg2.stride(0), a.wu_stride = wu2.stride(0);
+  a.h = r.h.data_ptr(), a.th = r.th.defined() ? r.th.data_ptr() : nullptr;
+  if (keep) {
+    a.g = r.g.data_ptr(), a.u = r.u.data_ptr();
+    if (tx.defined()) a.tg = r.tg.data_ptr(), a.tu = r.tu.data_ptr();
+  }
+  const Tensor workspace = workspace_for(jvpfa_gated_fwd_workspace(&a), x);
+  if (workspace.defined()) a.workspace = workspace.data_ptr(), a.workspace_bytes = workspace.numel();
+  check_status(jvpfa_gated_fwd(&a, c10::cuda::getCurrentCUDAStream(x.get_device()).stream()), "jvpfa_gated_fwd");
+  return r;
+}
+
+// Gradients of <gh, h> + <gth, th>; of `kept` the forward's g, u, tg, tu are read.
+GatedGrads launch_gated_bwd(const Tensor& x, const Tensor& tx, const Tensor& wg, const Tensor& wu, const GatedOut& kept, Tensor gh, Tensor gth,
+                            int activation, bool need_x, bool need_tx, bool need_w) {
+  GatedGrads r;
+  need_tx = need_tx && gth.defined();
+  if (!need_x && !need_tx && !need_w) return r;
+  if (!x.is_cuda()) {
+    py::gil_scoped_acquire gil;
+    NoFunctorch nf;
+    at::AutoGradMode no_grad(false);
+    py::tuple out = gated_module().attr("_launch_bwd")(x, or_none(tx), wg, wu, kept.g, kept.u, or_none(kept.tg), or_none(kept.tu), or_none(gh),
+                                                       or_none(gth), activation, need_x, need_tx, need_w);
+    Tensor* to[] = {&r.dx, &r.dtx, &r.dwg, &r.dwu};
+    for (int i = 0; i < 4; ++i) *to[i] = from_python(out[i]);
+    return r;
+  }
+  c10::cuda::OptionalCUDAGuard guard;
+  if (x.get_device() != c10::cuda::current_device()) guard.set_index(x.get_device());
+  if (x.numel() == 0) {
+    NoFunctorch nf;
+    at::AutoDispatchBelowADInplaceOrView below;
+    if (need_x) r.dx = at::zeros_like(x);
+    if (need_tx) r.dtx = at::zeros_like(x);
+    if (need_w) r.dwg = at::zeros_like(wg), r.dwu = at::zeros_like(wu);
+    return r;
+  }
+  gh = as_dense(gh, x), gth = as_dense(gth, x);
+  const bool dual = gth.defined();
+  if (need_x) r.dx = empty(x.sizes(), x.scalar_type(), x.device());
+  if (need_tx) r.dtx = empty(x.sizes(), x.scalar_type(), x.device());
+  if (need_w) r.dwg = empty(wg.sizes(), x.scalar_type(), x.device()), r.dwu = empty(wu.sizes(), x.scalar_type(), x.device());
+  const Tensor x2 = as_rows(x), tx2 = dual ? as_rows(tx) : Tensor(), wg2 = as_rows(wg), wu2 = as_rows(wu);
+  const Tensor g = as_dense(kept.g, x), u = as_dense(kept.u, x), tg = dual ? as_dense(kept.tg, x) : Tensor(), tu = dual ? as_dense(kept.tu, x) : Tensor();
+  jvpfa_gated_bwd_args a{};
+  a.struct_size = sizeof(a);
+  a.dtype = dtype_of(x, false);
+  a.M = (int)x2.size(0), a.K = (int)x2.size(1), a.F = (int)wg.size(0);
+  a.activation = activation;
+  a.x = data(x2), a.tx = data(tx2), a.wg = data(wg2), a.wu = data(wu2);
+  a.x_stride = x2.stride(0), a.tx_stride = dual ? tx2.stride(0) : 0, a.wg_stride = wg2.stride(0), a.wu_stride = wu2.stride(0);
+  a.g = data(g), a.u = data(u), a.tg = data(tg), a.tu = data(tu);
+  a.gh = data(gh), a.gth = data(gth);
+  if (need_x) a.dx = r.dx.data_ptr();
+  if (need_tx) a.dtx = r.dtx.data_ptr();
+  if (need_w) a.dwg = r.dwg.data_ptr(), a.dwu = r.dwu.data_ptr();
+  const Tensor workspace = workspace_for(jvpfa_gated_bwd_workspace(&a), x);
+  if (workspace.defined()) a.workspace = workspace.data_ptr(), a.workspace_bytes = workspace.numel();
+  check_status(jvpfa_gated_bwd(&a, c10::cuda::getCurrentCUDAStream(x.get_device()).stream()), "jvpfa_gated_bwd");
+  return r;
+}
+
+// (dx, dwg, dwu) of <gh, h> as a node that can be differentiated once more, along x: with v the incoming gradient of dx,
+//   d<dx, v>/d(x, wg, wu) = d<th(x; v), gh>/d(x, wg, wu)   and   d<dx, v>/d(gh) = th(x; v),
+// one value-and-tangent forward and one backward through the tangent.
+struct GatedGradNode : public Node {
+  int activation;
+  SavedVariable x, wg, wu, gh;
+
+  variable_list apply(variable_list&& v) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out(4);
+    if (v[1].defined() || v[2].defined())
+      throw std::runtime_error("the gradients of gated_linear with respect to its weights cannot be differentiated a second time");
+    if (!v[0].defined()) return out;
+    const Tensor x_ = x.unpack(), wg_ = wg.unpack(), wu_ = wu.unpack(), gh_ = gh.unpack();
+    const Tensor xp = unwrap(x_), wgp = unwrap(wg_), wup = unwrap(wu_), t = unwrap(v[0]);
+    const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1) || task_should_compute_output(2);
+    const GatedOut f = launch_gated_fwd(xp, t, wgp, wup, activation, need_x || need_w);
+    if (need_x || need_w) {
+      const GatedGrads g = launch_gated_bwd(xp, t, wgp, wup, f, Tensor(), unwrap(gh_), activation, need_x, false, need_w);
+      out[0] = g.dx, out[1] = g.dwg, out[2] = g.dwu;
+    }
+    if (task_should_compute_output(3)) out[3] = f.th;
+    if (at::GradMode::is_enabled())
+      attach_refusal("gated_linear cannot be differentiated a third time", {&out[0], &out[1], &out[2], &out[3]}, x_, wg_, wu_, gh_, v[0]);
+    return out;
+  }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* s : {&x, &wg, &wu, &gh}) s->reset_data();
+  }
+  std::string name() const override { return "GatedLinearBackwardBackward"; }
+};
+
+// The node of a call: outputs h (0) and, with a tangent, th (1); edges to x, wg, wu and, with a tangent, tx.
+struct GatedNode : public Node {
+  int activation;
+  SavedVariable x, tx, wg, wu, g, u, tg, tu;
+
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out(num_outputs());
+    const Tensor gh = primal_of(grads[0]), gth = grads.size() > 1 ? primal_of(grads[1]) : Tensor();
+    if (!gh.defined() && !gth.defined()) return out;
+    const Tensor x_ = primal_of(x.unpack()), wg_ = primal_of(wg.unpack()), wu_ = primal_of(wu.unpack());
+    const Tensor xp = unwrap(x_), wgp = unwrap(wg_), wup = unwrap(wu_);
+    GatedOut kept;
+    kept.g = unwrap(g.unpack()), kept.u = unwrap(u.unpack());
+    Tensor tx_;
+    if (gth.defined()) tx_ = tx.unpack(), kept.tg = unwrap(tg.unpack()), kept.tu = unwrap(tu.unpack());
+    const Tensor txp = unwrap(tx_);
+    const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1) || task_should_compute_output(2);
+    const bool need_tx = num_outputs() > 3 && task_should_compute_output(3);
+    if ((gh.defined() && is_wrapped(gh)) || (gth.defined() && is_wrapped(gth))) {
+      // the cotangents belong to a functorch transform, which differentiates Functions
+      py::gil_scoped_acquire gil;
+      py::tuple d = gated_module().attr("_backward_under_functorch")(x_, or_none(tx_), wg_, wu_, kept.g, kept.u, or_none(kept.tg),
+                                                                      or_none(kept.tu), or_none(gh), or_none(gth), activation);
+      const int at[] = {0, 3, 1, 2};  // of (dx, dtx, dwg, dwu) among the edges
+      for (int i = 0; i < 4; ++i)
+        if (at[i] < (int)out.size()) out[at[i]] = from_python(d[i]);
+      return out;
+    }
+    // Under create_graph the part through h stays a node of its own, which can be differentiated again.
+    const bool again = at::GradMode::is_enabled() && torch::autograd::compute_requires_grad(x_, wg_, wu_, tx_, gh, gth);
+    GatedGrads d;
+    if (gth.defined()) {
+      d = launch_gated_bwd(xp, txp, wgp, wup, kept, again ? Tensor() : gh, gth, activation, need_x, need_tx, need_w);
+      if (again)
+        attach_refusal("the gradient through the tangent output of gated_linear cannot be differentiated a second time",
+                       {&d.dx, &d.dtx, &d.dwg, &d.dwu}, x_, wg_, wu_, tx_, gth);
+    }
+    if (gh.defined() && (again || !gth.defined())) {
+      GatedGrads e = launch_gated_bwd(xp, Tensor(), wgp, wup, kept, gh, Tensor(), activation, need_x, false, need_w);
+      if (again) {
+        auto node = std::shared_ptr<GatedGradNode>(new GatedGradNode(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(x_, wg_, wu_, gh));
+        node->activation = activation;
+        node->x = SavedVariable(x_, false);
+        node->wg = SavedVariable(wg_, false);
+        node->wu = SavedVariable(wu_, false);
+        node->gh = SavedVariable(gh, false);
+        for (Tensor* t : {&e.dx, &e.dwg, &e.dwu}) {
+          if (t->defined())
+            torch::autograd::set_history(*t, node);
+          else
+            node->add_input_metadata(Node::undefined_input());
+        }
+      }
+      auto add = [](Tensor& to, const Tensor& t) {
+        if (t.defined()) to = to.defined() ? to + t : t;
+      };
+      add(d.dx, e.dx), add(d.dwg, e.dwg), add(d.dwu, e.dwu);
+    }
+    out[0] = d.dx;
+    if (task_should_compute_output(1)) out[1] = d.dwg;
+    if (task_should_compute_output(2)) out[2] = d.dwu;
+    if (need_tx) out[3] = d.dtx;
+    return out;
+  }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* s : {&x, &tx, &wg, &wu, &g, &u, &tg, &tu}) s->reset_data();
+  }
+  std::string name() const override { return "GatedLinearBackward"; }
+};
+
+bool gated_acceptable(const Tensor& x, const Tensor& wg, const Tensor& wu) {
+  if (x.dim() < 1 || wg.dim() != 2 || wu.sizes() != wg.sizes() || x.size(-1) != wg.size(1)) return false;
+  if (wg.size(0) < 1 || wg.size(1) < 1) return false;
+  for (const Tensor* t : {&x, &wg, &wu})
+    if (t->layout() != at::kStrided || t->scalar_type() != x.scalar_type() || t->device() != x.device()) return false;
+  const int64_t K = wg.size(1), F = wg.size(0);
+  if (x.numel() / K > INT32_MAX || K > INT32_MAX || F > INT32_MAX) return false;
+  return !x.is_cuda() || dtype_of(x, false) >= 0;
+}
+
+// None: not a case for this path; the caller takes its general route.
+py::object gated(const Tensor& x_in, const Tensor& wg_in, const Tensor& wu_in, int activation) {
+  const int64_t level = jvp_level();
+  if (level == -2 || wg_in._fw_grad(0).defined() || wu_in._fw_grad(0).defined()) return py::none();
+  Tensor x = x_in, tx = x._fw_grad(0);
+  if (level >= 0 && !tx.defined()) return py::none();
+  // (inside torch.func.jvp the function may use the weights as they are, or wrapped at its level without a tangent)
+  x = at_level_below(x, level), tx = at_level_below(tx, level);
+  const Tensor wg = at_level_below(wg_in, level), wu = at_level_below(wu_in, level);
+  if (level < 0 && tx.defined()) x = x._fw_primal(0);
+  for (const Tensor* t : std::initializer_list<const Tensor*>{&x, &tx, &wg, &wu})
+    if (t->defined() && is_wrapped(*t)) return py::none();
+  if (!gated_acceptable(x, wg, wu)) return py::none();
+  if (tx.defined()) {
+    if (tx.sizes() != x.sizes() || tx.device() != x.device()) return py::none();
+    tx = as_tangent(tx, x);
+  }
+  const bool grad_h = torch::autograd::compute_requires_grad(x, wg, wu), grad = grad_h || torch::autograd::compute_requires_grad(tx);
+  GatedOut r;
+  {
+    std::optional<py::gil_scoped_release> no_gil;
+    if (x.is_cuda()) no_gil.emplace();
+    r = launch_gated_fwd(x, tx, wg, wu, activation, grad);
+  }
+  if (grad) {
+    auto node = std::shared_ptr<GatedNode>(new GatedNode(), torch::autograd::deleteNode);
+    node->set_next_edges(tx.defined() ? torch::autograd::collect_next_edges(x, wg, wu, tx) : torch::autograd::collect_next_edges(x, wg, wu));
+    node->activation = activation;
+    node->x = SavedVariable(x, false);
+    node->wg = SavedVariable(wg, false);
+    node->wu = SavedVariable(wu, false);
+    node->g = SavedVariable(r.g, false);
+    node->u = SavedVariable(r.u, false);
+    if (grad_h)
+      torch::autograd::set_history(r.h, node);
+    else
+      node->add_input_metadata(Node::undefined_input());
+    if (tx.defined()) {
+      node->tx = SavedVariable(tx, false);
+      node->tg = SavedVariable(r.tg, false);
+      node->tu = SavedVariable(r.tu, false);
+      torch::autograd::set_history(r.th, node);
+    }
+  }
+  return dual(r.h, r.th, level);
+}
+
 }  // namespace
 
 void bind_block(py::module_& m) {
   m.def("rotary", &rotary, py::arg("q"), py::arg("k").none(true), py::arg("inv_freq"), py::arg("positions").none(true), py::arg("offset"),
         py::arg("interleaved"), py::arg("amplitude"));
+  m.def("gated", &gated);
 }

@@ -1,0 +1,239 @@
+"""The widening half of a gated feed-forward block with its tangent (csrc/gated.cu): ``h = a(x Wg^T) * (x Wu^T)`` in one kernel, both
+products, the activation and the gate.
+
+``gated_linear`` is to such a block what ``JVPAttn.fwd_dual`` is to attention: where x carries a tangent (``torch.func.jvp``, forward-AD
+dual tensors) value and tangent come from one launch, and the gradient goes through both, to x, its tangent and the weights.  The
+gradient of the value can be differentiated once more along x (Hessian-vector products, gradient penalties).  What follows in a block,
+the product with the narrowing weights, is ``torch.nn.functional.linear``.  No upstream counterpart: upstream leaves it to the model.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+import torch.autograd.forward_ad as fwAD
+from torch import Tensor
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .jvp_attention import _JVP, _is_tracing, _peek_functorch, _require_cuda, _unwrap
+
+ACTIVATIONS = {"silu": 0, "sigmoid": 1, "gelu": 2, "gelu_tanh": 3}  # jvpfa_activation
+
+
+def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, activation: str = "silu") -> Tensor:
+    """``activation(x @ w_gate.T) * (x @ w_up.T)``.
+
+    x: (..., K), plain or dual; w_gate, w_up: (F, K), as ``torch.nn.Linear`` keeps them (two halves of one (2 F, K) tensor will do); all
+    bfloat16, float16 or float32, of one type and device.  ``activation``: ``"silu"``, ``"sigmoid"``, ``"gelu"`` (exact) or ``"gelu_tanh"``.
+    Rows of whole 16-byte pieces (K a multiple of 8) are read in place, others, and float32, through a copy.
+
+    Sums are in 32 bits, and the result is rounded once.  For a backward the projections are kept in x's type (a
+    float16 projection beyond 65504 becomes infinite there).  float32 is multiplied as three bfloat16 parts, about 1e-6 relative,
+    whatever ``set_fp32_precision`` says of attention; an infinite entry gives NaN in its row.  Results are the same from run to run.
+
+    The weights have no tangents, and their gradients cannot be differentiated again: both are refused.
+    """
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation is one of {', '.join(ACTIVATIONS)}; got {activation!r}")
+    act = ACTIVATIONS[activation]
+    interp = _peek_functorch()
+    if (interp is None or (interp.level() == 1 and interp.key() == _JVP)) and not _is_tracing():
+        if not x.is_cuda:  # (the native layer checks CUDA tensors itself)
+            _check(x, w_gate, w_up)
+        out = _lib.native().gated(x, w_gate, w_up, act)
+        if out is not None:
+            return out
+    _check(x, w_gate, w_up)
+    return _Gated.apply(x, w_gate, w_up, act)[0]
+
+
+def _check(x, w_gate, w_up) -> None:
+    if x.dim() < 1 or w_gate.dim() != 2 or w_up.shape != w_gate.shape or x.shape[-1] != w_gate.shape[1]:
+        raise ValueError("x, w_gate and w_up must have the shapes (..., K), (F, K) and (F, K); got "
+                         f"{tuple(x.shape)}, {tuple(w_gate.shape)} and {tuple(w_up.shape)}")
+    if w_gate.numel() == 0:
+        raise ValueError(f"the weights must not be empty, got {tuple(w_gate.shape)}")
+    if x.numel() // x.shape[-1] >= 2**31:
+        raise ValueError("x must have less than 2**31 rows")
+    for name, t in (("x", x), ("w_gate", w_gate), ("w_up", w_up)):
+        if t.is_cuda and t.dtype not in _lib.DTYPE_ENUM:
+            raise TypeError(f"unsupported dtype {t.dtype} of {name}; expected bfloat16, float16 or float32")
+        if t.dtype != x.dtype:
+            raise TypeError(f"x, w_gate and w_up must have one dtype, got {x.dtype} and {t.dtype}")
+        if t.device != x.device:
+            raise ValueError(f"x, w_gate and w_up must be on one device, got {x.device} and {t.device}")
+    if any(fwAD.unpack_dual(w).tangent is not None for w in (w_gate, w_up)):
+        raise NotImplementedError("gated_linear has no tangent with respect to its weights")
+    _require_cuda(x, w_gate, w_up)
+
+
+# ---- the general route (functorch transforms other than a lone torch.func.jvp) --------------------------------------------
+def _launch_fwd(x, tx, w_gate, w_up, activation, keep):
+    """Runs jvpfa_gated_fwd on plain tensors: (h, th, g, u, tg, tu), the last four with ``keep``, and those of the tangent with tx."""
+    F, K = w_gate.shape
+    x2, tx2, wg, wu = (None if t is None else _rows(t) for t in (x, tx, w_gate, w_up))
+    out = [torch.empty(*x.shape[:-1], F, device=x.device, dtype=x.dtype) if wanted else None
+           for wanted in (True, tx is not None, keep, keep, keep and tx is not None, keep and tx is not None)]
+    if x.numel():
+        a = _lib.GatedFwdArgs()
+        _describe(a, x2, tx2, wg, wu, activation)
+        a.h, a.th, a.g, a.u, a.tg, a.tu = (_lib.ptr(t) for t in out)
+        _run(a, x2, "jvpfa_gated_fwd")
+    return tuple(out)
+
+
+def _launch_bwd(x, tx, w_gate, w_up, g, u, tg, tu, gh, gth, activation, need_x, need_tx, need_w):
+    """Runs jvpfa_gated_bwd on plain tensors: (dx, dtx, dwg, dwu), None for those not asked for."""
+    F, K = w_gate.shape
+    x2, wg, wu = _rows(x), _rows(w_gate), _rows(w_up)
+    tx2 = _rows(tx) if gth is not None else None
+    gh, gth = (None if c is None else c.to(x.dtype).contiguous() for c in (gh, gth))
+    make = torch.empty if x.numel() else torch.zeros
+    out = [make(shape, device=x.device, dtype=x.dtype) if wanted else None
+           for wanted, shape in ((need_x, x.shape), (need_tx and gth is not None, x.shape), (need_w, (F, K)), (need_w, (F, K)))]
+    if x.numel() and any(t is not None for t in out):
+        a = _lib.GatedBwdArgs()
+        _describe(a, x2, tx2, wg, wu, activation)
+        a.g, a.u, a.gh, a.gth = (_lib.ptr(t) for t in (g, u, gh, gth))
+        if gth is not None:
+            a.tg, a.tu = _lib.ptr(tg), _lib.ptr(tu)
+        a.dx, a.dtx, a.dwg, a.dwu = (_lib.ptr(t) for t in out)
+        _run(a, x2, "jvpfa_gated_bwd")
+    return tuple(out)
+
+
+def _rows(t):
+    t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 else t.contiguous()
+
+
+def _describe(a, x, tx, wg, wu, activation):
+    a.struct_size = C.sizeof(a)
+    a.dtype = _lib.DTYPE_ENUM[x.dtype]
+    (a.M, a.K), a.F, a.activation = x.shape, wg.shape[0], activation
+    for name, t in (("x", x), ("tx", tx), ("wg", wg), ("wu", wu)):
+        if t is not None:
+            setattr(a, name, t.data_ptr())
+            setattr(a, name + "_stride", t.stride(0))
+
+
+def _run(a, x, entry):
+    lib = _lib.load()
+    with torch.cuda.device(x.device):
+        n = getattr(lib, entry + "_workspace")(C.byref(a))
+    workspace = torch.empty(n, device=x.device, dtype=torch.uint8) if n else None
+    a.workspace, a.workspace_bytes = _lib.ptr(workspace), n
+    _lib.check(_lib._launch(x, getattr(lib, entry), a), entry)
+
+
+class _Gated(Function):
+    """h, and the projections g and u that its backward reads."""
+
+    @staticmethod
+    def forward(x, w_gate, w_up, activation):
+        h, _, g, u, _, _ = _launch_fwd(_unwrap(x), None, _unwrap(w_gate), _unwrap(w_up), activation, True)
+        return h, g, u
+
+    @staticmethod
+    def setup_context(ctx, inputs, outputs):
+        x, w_gate, w_up, ctx.activation = inputs
+        _, g, u = outputs
+        ctx.mark_non_differentiable(g, u)
+        ctx.save_for_backward(x, w_gate, w_up, g, u)
+        ctx.save_for_forward(x, w_gate, w_up)
+        ctx.set_materialize_grads(False)
+
+    @staticmethod
+    def jvp(ctx, tx, t_gate, t_up, *_):
+        if t_gate is not None or t_up is not None:
+            raise NotImplementedError("gated_linear has no tangent with respect to its weights")
+        x, w_gate, w_up = ctx.saved_tensors
+        return (None if tx is None else _GatedTangent.apply(x, tx.to(x.dtype), w_gate, w_up, ctx.activation)[0]), None, None
+
+    @staticmethod
+    def backward(ctx, gh, *_):
+        if gh is None:
+            return None, None, None, None
+        x, w_gate, w_up, g, u = (fwAD.unpack_dual(t).primal for t in ctx.saved_tensors)
+        return (*_GatedGrad.apply(x, w_gate, w_up, g, u, fwAD.unpack_dual(gh).primal, ctx.activation), None)
+
+
+class _GatedTangent(Function):
+    """th, differentiable once with respect to x, its tangent and the weights."""
+
+    @staticmethod
+    def forward(x, tx, w_gate, w_up, activation):
+        _, th, g, u, tg, tu = _launch_fwd(*(_unwrap(t) for t in (x, tx, w_gate, w_up)), activation, True)
+        return th, g, u, tg, tu
+
+    @staticmethod
+    def setup_context(ctx, inputs, outputs):
+        *tensors, ctx.activation = inputs
+        ctx.mark_non_differentiable(*outputs[1:])
+        ctx.save_for_backward(*tensors, *outputs[1:])
+        ctx.set_materialize_grads(False)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gth, *_):
+        if gth is None:
+            return (None,) * 5
+        x, tx, w_gate, w_up, g, u, tg, tu = (_unwrap(t) for t in ctx.saved_tensors)
+        dx, dtx, dwg, dwu = _launch_bwd(x, tx, w_gate, w_up, g, u, tg, tu, None, _unwrap(gth), ctx.activation, True, True, True)
+        return dx, dtx, dwg, dwu, None
+
+
+class _GatedGrad(Function):
+    """(dx, dwg, dwu) of <gh, h>, differentiable once more along x (see GatedGradNode in csrc/native_block.cpp)."""
+
+    @staticmethod
+    def forward(x, w_gate, w_up, g, u, gh, activation):
+        x, w_gate, w_up, g, u, gh = (_unwrap(t) for t in (x, w_gate, w_up, g, u, gh))
+        dx, _, dwg, dwu = _launch_bwd(x, None, w_gate, w_up, g, u, None, None, gh, None, activation, True, False, True)
+        return dx, dwg, dwu
+
+    @staticmethod
+    def setup_context(ctx, inputs, outputs):
+        x, w_gate, w_up, g, u, gh, ctx.activation = inputs
+        ctx.save_for_backward(x, w_gate, w_up, gh)
+        ctx.set_materialize_grads(False)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, vx, v_gate, v_up):
+        if v_gate is not None or v_up is not None:
+            raise RuntimeError("the gradients of gated_linear with respect to its weights cannot be differentiated a second time")
+        if vx is None:
+            return (None,) * 7
+        x, w_gate, w_up, gh = (_unwrap(t) for t in ctx.saved_tensors)
+        vx = _unwrap(vx).to(x.dtype)
+        _, th, g, u, tg, tu = _launch_fwd(x, vx, w_gate, w_up, ctx.activation, True)
+        dx, _, dwg, dwu = _launch_bwd(x, vx, w_gate, w_up, g, u, tg, tu, None, gh, ctx.activation, True, False, True)
+        return dx, dwg, dwu, None, None, th, None
+
+
+class _GatedDualGrad(Function):
+    """(dx, dtx, dwg, dwu) of <gh, h> + <gth, th>."""
+
+    @staticmethod
+    def forward(x, tx, w_gate, w_up, g, u, tg, tu, gh, gth, activation):
+        tensors = [None if t is None else _unwrap(t) for t in (x, tx, w_gate, w_up, g, u, tg, tu, gh, gth)]
+        return _launch_bwd(*tensors, activation, True, True, True)
+
+    @staticmethod
+    def setup_context(ctx, inputs, outputs):
+        pass
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("the gradient through the tangent output of gated_linear cannot be differentiated a second time")
+
+
+def _backward_under_functorch(x, tx, w_gate, w_up, g, u, tg, tu, gh, gth, activation):
+    """The native layer's backward where a cotangent is a tensor of a functorch transform: Functions take part in it."""
+    if gth is not None:
+        return _GatedDualGrad.apply(x, tx, w_gate, w_up, g, u, tg, tu, gh, gth, activation)
+    dx, dwg, dwu = _GatedGrad.apply(x, w_gate, w_up, g, u, gh, activation)
+    return dx, None, dwg, dwu

@@ -25,3 +25,47 @@ def pair_norm(x, n, interleaved):
     r = torch.hypot(a, b)
     r = torch.stack((r, r), -1).flatten(-2) if interleaved else torch.cat((r, r), -1)
     return torch.cat((r, torch.zeros_like(z[..., 2 * n:])), -1)
+
+
+def activation(kind, g):
+    """a, a', a'' of jvpfa_activation ``kind`` at g."""
+    if kind in (0, 1):
+        s, r = torch.sigmoid(g), torch.sigmoid(-g)
+        d = s * r
+        return (s, d, d * (r - s)) if kind == 1 else (g * s, s + g * d, d * (2 + g * (r - s)))
+    if kind == 2:
+        p, d = torch.special.ndtr(g), torch.exp(-0.5 * g * g) * (2 * torch.pi) ** -0.5
+        return g * p, p + g * d, d * (2 - g * g)
+    c, c3 = (2 / torch.pi) ** 0.5, 0.044715
+    s, r = torch.sigmoid(2 * c * (g + c3 * g**3)), torch.sigmoid(-2 * c * (g + c3 * g**3))
+    z1, z2, d = 2 * c * (1 + 3 * c3 * g * g), 12 * c * c3 * g, s * r
+    return g * s, s + g * d * z1, d * (2 * z1 + g * (z2 + (r - s) * z1 * z1))
+
+
+def gated_fwd(x, tx, w_gate, w_up, kind, keep=True):
+    """(h, th, g, u, tg, tu) as ``gated._launch_fwd`` returns them."""
+    x, tx, w_gate, w_up = (None if t is None else t.double() for t in (x, tx, w_gate, w_up))
+    g, u = x @ w_gate.T, x @ w_up.T
+    a, a1, _ = activation(kind, g)
+    if tx is None:
+        return (a * u, None, *((g, u) if keep else (None, None)), None, None)
+    tg, tu = tx @ w_gate.T, tx @ w_up.T
+    return (a * u, a1 * tg * u + a * tu, *((g, u, tg, tu) if keep else (None,) * 4))
+
+
+def gated_bwd(x, tx, w_gate, w_up, g, u, tg, tu, gh, gth, kind, need_x=True, need_tx=True, need_w=True):
+    """(dx, dtx, dwg, dwu) as ``gated._launch_bwd`` returns them."""
+    x, tx, w_gate, w_up, g, u, tg, tu, gh, gth = (None if t is None else t.double() for t in (x, tx, w_gate, w_up, g, u, tg, tu, gh, gth))
+    a, a1, a2 = activation(kind, g)
+    dg, du = (torch.zeros_like(g), torch.zeros_like(g)) if gh is None else (gh * a1 * u, gh * a)
+    dtg = dtu = None
+    if gth is not None:
+        dg, du = dg + gth * (a2 * tg * u + a1 * tu), du + gth * a1 * tg
+        dtg, dtu = gth * a1 * u, gth * a
+    flat = lambda t: t.reshape(-1, t.shape[-1])  # noqa: E731
+    dx = dg @ w_gate + du @ w_up if need_x else None
+    dtx = dtg @ w_gate + dtu @ w_up if need_tx and gth is not None else None
+    dwg, dwu = (flat(d).T @ flat(x) for d in (dg, du)) if need_w else (None, None)
+    if need_w and gth is not None:
+        dwg, dwu = dwg + flat(dtg).T @ flat(tx), dwu + flat(dtu).T @ flat(tx)
+    return dx, dtx, dwg, dwu

@@ -1,0 +1,199 @@
+"""CPU tests of gated_linear: graph, tangents, second derivatives and refusals.  Launches go to the formulas (tests/_block_formulas.py),
+which are themselves held against torch's differentiation."""
+import ctypes
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+import jvp_flash_attention_b200.gated as gated
+from jvp_flash_attention_b200 import _lib
+from jvp_flash_attention_b200.gated import gated_linear
+from tests import _block_formulas as formulas
+
+F = torch.nn.functional
+PLAIN = {"silu": F.silu, "sigmoid": torch.sigmoid, "gelu": F.gelu, "gelu_tanh": lambda g: F.gelu(g, approximate="tanh")}
+
+
+@pytest.fixture()
+def cpu_kernels(monkeypatch):
+    calls = []
+    monkeypatch.setattr(gated, "_launch_fwd", lambda *a: (calls.append(("fwd", a[1] is not None, a[5])), formulas.gated_fwd(*a))[1])
+    monkeypatch.setattr(gated, "_launch_bwd", lambda *a: (calls.append(("bwd", *a[11:])), formulas.gated_bwd(*a))[1])
+    monkeypatch.setattr(gated, "_require_cuda", lambda *a: None)
+    return calls
+
+
+def _inputs(seed, rows=(2, 5), k=4, f=3):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)  # noqa: E731
+    return r(*rows, k), r(*rows, k), r(f, k), r(f, k), r(*rows, f), r(*rows, f)
+
+
+def _plain(name):
+    return lambda x, wg, wu: PLAIN[name](x @ wg.T) * (x @ wu.T)
+
+
+@pytest.mark.parametrize("route", ["func", "fwad"])
+@pytest.mark.parametrize("name", list(PLAIN))
+@pytest.mark.parametrize("through", ["h", "t", "both"])
+def test_values_tangents_and_gradients(cpu_kernels, route, name, through):
+    x, tx, wg, wu, gh, gth = _inputs(1)
+    leaves = [t.requires_grad_() for t in (x, tx, wg, wu)]
+    want = torch.func.jvp(lambda v: _plain(name)(v, wg, wu), (x,), (tx,))
+    if route == "func":
+        got = torch.func.jvp(lambda v: gated_linear(v, wg, wu, name), (x,), (tx,))
+    else:
+        with fwAD.dual_level():
+            got = fwAD.unpack_dual(gated_linear(fwAD.make_dual(x, tx), wg, wu, name))
+    pick = {"h": [0], "t": [1], "both": [0, 1]}[through]
+    for a, b in zip(got, want):
+        torch.testing.assert_close(a, b)
+    args = [[o[i] for i in pick] for o in (got, want)]
+    cots = [(gh, gth)[i] for i in pick]
+    for a, b in zip(torch.autograd.grad(args[0], leaves, cots, allow_unused=True), torch.autograd.grad(args[1], leaves, cots, allow_unused=True)):
+        assert (a is None) == (b is None) or not (a if b is None else b).any()
+        if a is not None and b is not None:
+            torch.testing.assert_close(a, b)
+
+
+@pytest.mark.parametrize("name", list(PLAIN))
+def test_gradients_against_differences(cpu_kernels, name):
+    x, _, wg, wu, _, _ = _inputs(2)
+    torch.autograd.gradcheck(lambda *a: gated_linear(*a, name), tuple(t.requires_grad_() for t in (x, wg, wu)))
+    torch.autograd.gradgradcheck(lambda v: gated_linear(v, wg.detach(), wu.detach(), name), (x,))
+
+
+def test_a_gradient_penalty_reaches_the_weights(cpu_kernels):
+    x, _, wg, wu, gh, v = _inputs(3)
+    leaves = [t.requires_grad_() for t in (x, wg, wu)]
+    gh.requires_grad_()
+    out = []
+    for f in (gated_linear, _plain("silu")):
+        (dx,) = torch.autograd.grad(f(*leaves), x, gh, create_graph=True)
+        out.append(torch.autograd.grad((dx**2).sum(), (*leaves, gh)))
+    for a, b in zip(*out):
+        torch.testing.assert_close(a, b)
+
+
+def test_what_cannot_be_differentiated_says_so(cpu_kernels):
+    x, tx, wg, wu, gh, gth = _inputs(4)
+    leaves = [t.requires_grad_() for t in (x, wg, wu)]
+    dx, dw = torch.autograd.grad(gated_linear(*leaves), (x, wg), gh, create_graph=True)
+    with pytest.raises(RuntimeError, match="cannot be differentiated a second time"):
+        torch.autograd.grad(dw.sum(), x, retain_graph=True)
+    h, th = torch.func.jvp(lambda v: gated_linear(v, wg, wu), (x,), (tx,))
+    (dx,) = torch.autograd.grad(th, x, gth, create_graph=True, retain_graph=True)
+    with pytest.raises(RuntimeError, match="cannot be differentiated a second time"):
+        torch.autograd.grad(dx.sum(), x)
+    # ... but the part through h can
+    (dx,) = torch.autograd.grad(h, x, gh, create_graph=True)
+    torch.autograd.grad(dx.sum(), x)
+
+
+def test_nested_transforms_take_the_general_route(cpu_kernels):
+    x, tx, wg, wu, gh, v = _inputs(5)
+    f, plain = (lambda a: (gated_linear(a, wg, wu) * gh).sum()), (lambda a: (_plain("silu")(a, wg, wu) * gh).sum())
+    torch.testing.assert_close(torch.func.grad(f)(x), torch.func.grad(plain)(x))
+    torch.testing.assert_close(torch.func.grad(lambda w: (gated_linear(x, w, wu) * gh).sum())(wg),
+                               torch.func.grad(lambda w: (_plain("silu")(x, w, wu) * gh).sum())(wg))
+    torch.testing.assert_close(torch.func.grad(lambda a: (torch.func.grad(f)(a) * tx).sum())(x),
+                               torch.func.grad(lambda a: (torch.func.grad(plain)(a) * tx).sum())(x))
+
+
+def test_only_what_is_asked_for_is_computed(cpu_kernels):
+    x, tx, wg, wu, gh, gth = _inputs(6)
+    gated_linear(x, wg, wu)
+    assert cpu_kernels == [("fwd", False, False)]  # nothing kept without a graph
+    cpu_kernels.clear()
+    h = gated_linear(x, wg.requires_grad_(), wu)
+    torch.autograd.grad(h, wg, gh)
+    assert cpu_kernels == [("fwd", False, True), ("bwd", False, False, True)]
+    cpu_kernels.clear()
+    wg.requires_grad_(False)
+    _, th = torch.func.jvp(lambda v: gated_linear(v, wg, wu), (x,), (tx.requires_grad_(),))
+    torch.autograd.grad(th, tx, gth)
+    assert cpu_kernels == [("fwd", True, True), ("bwd", False, True, False)]
+
+
+def test_a_run_of_operators_under_one_jvp(cpu_kernels):
+    """A feed-forward block: the gated projection, the narrowing product and the residual."""
+    x, tx, wg, wu, _, _ = _inputs(7)
+    wd = _inputs(8, k=3, f=4)[2]
+    leaves = [t.requires_grad_() for t in (x, wg, wu, wd)]
+    block = lambda f: lambda v: v + F.linear(f(v, wg, wu), wd)  # noqa: E731
+    out = []
+    for f in (gated_linear, _plain("silu")):
+        y, ty = torch.func.jvp(block(f), (x,), (tx,))
+        out.append((y, ty, *torch.autograd.grad((y.sum() + (ty**2).sum()), leaves)))
+    for a, b in zip(*out):
+        torch.testing.assert_close(a, b)
+
+
+def test_refusals(cpu_kernels):
+    x, tx, wg, wu, _, _ = _inputs(9)
+    for error, args in [(ValueError, (x, wg, wu, "relu")), (ValueError, (x, wg[0], wu[0])), (ValueError, (x, wg, wu[:2])),
+                        (ValueError, (x[..., :3], wg, wu)), (ValueError, (x, wg[:0], wu[:0])), (TypeError, (x, wg.float(), wu)),
+                        (ValueError, (x[..., 0:0], wg[:, :0], wu[:, :0]))]:
+        with pytest.raises(error):
+            gated_linear(*args)
+    with fwAD.dual_level(), pytest.raises(NotImplementedError, match="no tangent with respect to its weights"):
+        gated_linear(x, fwAD.make_dual(wg, wu), wu)
+    with pytest.raises(NotImplementedError, match="no tangent with respect to its weights"):
+        torch.func.jvp(lambda w: gated_linear(x, w, wu), (wg,), (wu,))
+
+
+def test_no_cpu_fallback():
+    x, _, wg, wu, _, _ = (t.float() for t in _inputs(10))
+    with pytest.raises(RuntimeError, match="runs only on CUDA tensors"):
+        gated_linear(x, wg, wu)
+
+
+def _fwd_args(**kw):
+    a = _lib.GatedFwdArgs()
+    a.struct_size = ctypes.sizeof(a)
+    a.M = a.K = a.F = 64
+    a.x = a.wg = a.wu = a.h = 256
+    a.x_stride = a.wg_stride = a.wu_stride = 64
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def _bwd_args(**kw):
+    a = _lib.GatedBwdArgs()
+    a.struct_size = ctypes.sizeof(a)
+    a.M = a.K = a.F = 64
+    a.x = a.wg = a.wu = a.g = a.u = a.gh = a.dx = a.workspace = 256
+    a.x_stride = a.wg_stride = a.wu_stride = 64
+    a.workspace_bytes = 1 << 30
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def test_the_c_entries_refuse():
+    lib = _lib.load()
+    assert lib.jvpfa_gated_fwd(None, None) == -1 and lib.jvpfa_gated_bwd(None, None) == -1
+    common = [(-7, dict(struct_size=4)), (-3, dict(dtype=3)), (-2, dict(M=0)), (-2, dict(K=0)), (-2, dict(F=0)), (-9, dict(activation=4)),
+              (-9, dict(activation=-1)), (-1, dict(x=None)), (-1, dict(wg=None)), (-1, dict(wu=None)), (-8, dict(x=257)), (-2, dict(x_stride=-8))]
+    for want, kw in common + [(-1, dict(h=None)), (-8, dict(h=264)), (-1, dict(tx=256)), (-1, dict(th=256)), (-1, dict(g=256)), (-1, dict(tg=256, tu=256)),
+                              (-1, dict(x=258)), (-1, dict(dtype=2))]:  # the last two need a workspace
+        assert lib.jvpfa_gated_fwd(ctypes.byref(_fwd_args(**kw)), None) == want, kw
+    for want, kw in common + [(-1, dict(g=None)), (-1, dict(gh=None)), (-1, dict(gth=256)), (-1, dict(dtx=256)), (-1, dict(dwg=256)), (-1, dict(dx=None)),
+                              (-8, dict(dx=264)), (-8, dict(gh=258)), (-1, dict(workspace=None)), (-1, dict(workspace_bytes=16))]:
+        assert lib.jvpfa_gated_bwd(ctypes.byref(_bwd_args(**kw)), None) == want, kw
+
+
+def test_workspaces():
+    lib = _lib.load()
+    fwd = lambda **kw: lib.jvpfa_gated_fwd_workspace(ctypes.byref(_fwd_args(**kw)))  # noqa: E731
+    assert fwd() == 0
+    assert fwd(x=258) == 64 * 64 * 2  # rows that begin elsewhere are copied
+    assert fwd(x_stride=65) == 64 * 64 * 2 and fwd(K=63, x_stride=63) == 64 * 64 * 2  # rows padded to 16 bytes; wg and wu have them
+    assert fwd(dtype=2) == 3 * 3 * 64 * 64 * 2  # three parts of three operands
+    assert fwd(x_stride=0) == 64 * 64 * 2  # one row for all
+    bwd = lambda **kw: lib.jvpfa_gated_bwd_workspace(ctypes.byref(_bwd_args(**kw)))  # noqa: E731
+    assert bwd() == 2 * 64 * 64 * 2
+    assert bwd(gth=256, tx=256, tg=256, tu=256, tx_stride=64) == 2 * 2 * 64 * 64 * 2
+    assert bwd(M=0) == 0
