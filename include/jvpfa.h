@@ -403,7 +403,8 @@ int jvpfa_rotary(const jvpfa_rotary_args* args, void* stream);
  *   dg = gh a' u + gth (a'' tg u + a' tu),  du = gh a + gth a' tg,  dtg = gth a' u,  dtu = gth a
  *   dx = dg wg + du wu,  dtx = dtg wg + dtu wu,  dwg = dg^T x + dtg^T tx,  dwu = du^T x + dtu^T tx
  *
- * Sums are held in 32 bits; g, u, tg, tu and the four between the two steps of the backward are kept in the tensors' type.
+ * Sums are held in 32 bits.  g, u, tg, tu are kept for the backward in a form of the library's own (24 bits an entry, 32 for JVPFA_FP32);
+ * dg, du, dtg, dtu are rounded to the tensors' type.
  * JVPFA_FP32 multiplies three bf16 parts of every entry (error ~1e-6 relative).  x, tx, wg, wu have contiguous columns and row
  * strides in elements; all other tensors are row-major.
  */
@@ -423,12 +424,14 @@ typedef struct {
   const void *wg, *wu;
   int64_t x_stride, tx_stride, wg_stride, wu_stride;
   void *h, *th;           /* th iff tx */
-  void *g, *u, *tg, *tu;  /* for jvpfa_gated_bwd: g and u or neither, tg and tu iff tx and g */
+  void* kept;             /* NULL, or for jvpfa_gated_bwd: jvpfa_gated_kept_bytes() bytes, 16-byte aligned */
   void* workspace;        /* jvpfa_gated_fwd_workspace() bytes of scratch, 16-byte aligned (0: NULL) */
   int64_t workspace_bytes;
 } jvpfa_gated_fwd_args;
 
 int jvpfa_gated_fwd(const jvpfa_gated_fwd_args* args, void* stream);
+/* Bytes of jvpfa_gated_fwd_args.kept for these M and F, with a tangent (tangent != 0) or without; 0 for a size or type that is refused. */
+int64_t jvpfa_gated_kept_bytes(int dtype, int32_t M, int32_t F, int tangent);
 /* Bytes of scratch that this call needs (workspace itself not looked at), 0 for arguments that it refuses; host logic. */
 int64_t jvpfa_gated_fwd_workspace(const jvpfa_gated_fwd_args* args);
 
@@ -440,7 +443,8 @@ typedef struct {
   const void *x, *tx; /* tx iff gth; x and tx are read for dwg and dwu alone */
   const void *wg, *wu;
   int64_t x_stride, tx_stride, wg_stride, wu_stride;
-  const void *g, *u, *tg, *tu; /* as the forward left them; tg and tu iff gth */
+  const void* kept;            /* as the forward of these operands left it */
+  int32_t kept_tangent;        /* whether that had a tangent: it must for gth */
   const void *gh, *gth;        /* either may be NULL, not both */
   void *dx, *dtx;              /* (M, K) row-major; NULL: not formed; dtx only with gth */
   void *dwg, *dwu;             /* (F, K) row-major; both or neither */

@@ -54,6 +54,7 @@ EXPORTS = (
     "jvpfa_mask_tiles",
     "jvpfa_pad_bias",
     "jvpfa_rotary",
+    "jvpfa_gated_kept_bytes",
     "jvpfa_gated_fwd",
     "jvpfa_gated_fwd_workspace",
     "jvpfa_gated_bwd",
@@ -281,10 +282,7 @@ class GatedFwdArgs(C.Structure):
         ("wu_stride", C.c_int64),
         ("h", C.c_void_p),
         ("th", C.c_void_p),
-        ("g", C.c_void_p),
-        ("u", C.c_void_p),
-        ("tg", C.c_void_p),
-        ("tu", C.c_void_p),
+        ("kept", C.c_void_p),
         ("workspace", C.c_void_p),
         ("workspace_bytes", C.c_int64),
     ]
@@ -306,10 +304,8 @@ class GatedBwdArgs(C.Structure):
         ("tx_stride", C.c_int64),
         ("wg_stride", C.c_int64),
         ("wu_stride", C.c_int64),
-        ("g", C.c_void_p),
-        ("u", C.c_void_p),
-        ("tg", C.c_void_p),
-        ("tu", C.c_void_p),
+        ("kept", C.c_void_p),
+        ("kept_tangent", C.c_int32),
         ("gh", C.c_void_p),
         ("gth", C.c_void_p),
         ("dx", C.c_void_p),
@@ -369,6 +365,8 @@ def load() -> C.CDLL:
     lib.jvpfa_pad_bias.restype = C.c_int
     lib.jvpfa_rotary.argtypes = [C.POINTER(RotaryArgs), C.c_void_p]
     lib.jvpfa_rotary.restype = C.c_int
+    lib.jvpfa_gated_kept_bytes.argtypes = [C.c_int, C.c_int32, C.c_int32, C.c_int]
+    lib.jvpfa_gated_kept_bytes.restype = C.c_int64
     lib.jvpfa_gated_fwd.argtypes = [C.POINTER(GatedFwdArgs), C.c_void_p]
     lib.jvpfa_gated_fwd.restype = C.c_int
     lib.jvpfa_gated_fwd_workspace.argtypes = [C.POINTER(GatedFwdArgs)]

@@ -220,10 +220,9 @@ static int validate_gated_fwd(const jvpfa_gated_fwd_args* a) {
   if (a->struct_size != (int32_t)sizeof(jvpfa_gated_fwd_args)) return JVPFA_ERR_STRUCT;
   const int rc = check_gated(a->dtype, a->M, a->K, a->F, a->activation);
   if (rc) return rc;
-  if (!a->x || !a->wg || !a->wu || !a->h || !a->th != !a->tx || !a->g != !a->u || !a->tg != !a->tu || !a->tg != !(a->tx && a->g))
-    return JVPFA_ERR_NULL;
+  if (!a->x || !a->wg || !a->wu || !a->h || !a->th != !a->tx) return JVPFA_ERR_NULL;
   return check_gated_memory(a->dtype, {a->x, a->tx, a->wg, a->wu}, {a->x_stride, a->tx_stride, a->wg_stride, a->wu_stride},
-                            {a->h, a->th, a->g, a->u, a->tg, a->tu, a->workspace});
+                            {a->h, a->th, a->kept, a->workspace});
 }
 
 static int validate_gated_bwd(const jvpfa_gated_bwd_args* a) {
@@ -231,11 +230,11 @@ static int validate_gated_bwd(const jvpfa_gated_bwd_args* a) {
   if (a->struct_size != (int32_t)sizeof(jvpfa_gated_bwd_args)) return JVPFA_ERR_STRUCT;
   const int rc = check_gated(a->dtype, a->M, a->K, a->F, a->activation);
   if (rc) return rc;
-  if (!a->x || !a->wg || !a->wu || !a->g || !a->u || (!a->gh && !a->gth)) return JVPFA_ERR_NULL;
-  if (!a->tx != !a->gth || !a->tg != !a->gth || !a->tu != !a->gth || (a->dtx && !a->gth)) return JVPFA_ERR_NULL;
+  if (!a->x || !a->wg || !a->wu || !a->kept || (!a->gh && !a->gth)) return JVPFA_ERR_NULL;
+  if (!a->tx != !a->gth || (a->gth && !a->kept_tangent) || (a->dtx && !a->gth)) return JVPFA_ERR_NULL;
   if (!a->dwg != !a->dwu || (!a->dx && !a->dtx && !a->dwg)) return JVPFA_ERR_NULL;
   return check_gated_memory(a->dtype, {a->x, a->tx, a->wg, a->wu}, {a->x_stride, a->tx_stride, a->wg_stride, a->wu_stride},
-                            {a->g, a->u, a->tg, a->tu, a->gh, a->gth, a->dx, a->dtx, a->dwg, a->dwu, a->workspace});
+                            {a->kept, a->gh, a->gth, a->dx, a->dtx, a->dwg, a->dwu, a->workspace});
 }
 
 }  // namespace jvpfa
@@ -389,6 +388,10 @@ int jvpfa_rotary(const jvpfa_rotary_args* a, void* stream) {
   const int rc = check_arch();
   if (rc) return rc;
   return launch_rotary(*a, static_cast<cudaStream_t>(stream));
+}
+
+int64_t jvpfa_gated_kept_bytes(int dtype, int32_t M, int32_t F, int tangent) {
+  return check_gated(dtype, M, 1, F, JVPFA_ACT_SILU) == JVPFA_OK ? gated_kept_bytes(dtype, M, F, tangent != 0) : 0;
 }
 
 int64_t jvpfa_gated_fwd_workspace(const jvpfa_gated_fwd_args* a) {

@@ -2,12 +2,13 @@
 //
 // Forward: one launch (value, or value and tangent).  Backward: a pass that turns the cotangents into those of the projections,
 //   dg = gh a' u + gth (a'' tg u + a' tu),  du = gh a + gth a' tg,  dtg = gth a' u,  dtu = gth a,
-// bound by memory (four tensors read and two written for the value alone), then a product over the features for dx and dtx, and one over
+// bound by memory (12 bytes an entry for the value of a 16-bit tensor: gh, 3 each for g and u, dg, du), then a product over the features for dx and dtx, and one over
 // the rows for dwg and dwu.  Tangents are further rows of the first (dx beside dtx, the weights shared) and further depth of the second.
 //
 // Operands go to the tensor cores by TMA, which takes rows of whole 16-byte pieces; others are copied once into the workspace with padded
 // rows.  fp32 operands become three planes of bf16 parts there (f32_tc5_common.cuh).
 #include <algorithm>
+#include <initializer_list>
 
 #include "gated_common.cuh"
 
@@ -28,50 +29,58 @@ struct alignas(V * sizeof(T)) Pack {
 };
 
 // ---- operands as TMA takes them ------------------------------------------------------------------------------------------
-// rows x cols, row stride `stride`, into rows of `width`; fp32: into three planes of bf16 parts.
+// rows x cols, row stride `stride`, into rows of up8(cols); fp32: into three planes of bf16 parts.  All of a call's in one launch.
+struct StageItem {
+  const void* src;
+  void* dst;
+  int rows, cols;
+  long long stride;
+};
+struct StageArgs {
+  StageItem item[4];
+};
+
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) stage_kernel(const T* src, long long rows, int cols, long long stride, void* dst, int width) {
-  const long long per_row = (cols + V - 1) / V, total = rows * per_row;
-  for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < total; i += (long long)gridDim.x * kThreads) {
-    const long long r = i / per_row;
-    const int c = (int)(i - r * per_row) * V;
-    const Pack<T, V> x = *reinterpret_cast<const Pack<T, V>*>(src + r * stride + c);
+__device__ __forceinline__ void stage_matrix(const StageItem& m) {
+  const int width = (m.cols + 7) / 8 * 8;
+  const int per_row = (m.cols + V - 1) / V;
+  const long long step = (long long)gridDim.x * kThreads, plane = (long long)m.rows * width;
+  long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
+  long long r = i / per_row;
+  int c = (int)(i - r * per_row);
+  const long long step_r = step / per_row;
+  const int step_c = (int)(step - step_r * per_row);
+  for (; r < m.rows; r += step_r, c += step_c) {
+    if (c >= per_row) {
+      c -= per_row;
+      if (++r >= m.rows) break;
+    }
+    const Pack<T, V> x = *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(m.src) + r * m.stride + c * V);
     if constexpr (sizeof(T) == 4) {
-      const long long plane = rows * width;
       Pack<__nv_bfloat16, V> part[3];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        float h, m, l;
-        split3(x.e[j], h, m, l);
-        part[0].e[j] = __float2bfloat16_rn(h), part[1].e[j] = __float2bfloat16_rn(m), part[2].e[j] = __float2bfloat16_rn(l);
+        float h, mid, l;
+        split3(x.e[j], h, mid, l);
+        part[0].e[j] = __float2bfloat16_rn(h), part[1].e[j] = __float2bfloat16_rn(mid), part[2].e[j] = __float2bfloat16_rn(l);
       }
-      __nv_bfloat16* d = static_cast<__nv_bfloat16*>(dst) + r * width + c;
+      __nv_bfloat16* d = static_cast<__nv_bfloat16*>(m.dst) + r * width + c * V;
 #pragma unroll
       for (int k = 0; k < 3; ++k) *reinterpret_cast<Pack<__nv_bfloat16, V>*>(d + k * plane) = part[k];
     } else {
-      *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(dst) + r * width + c) = x;
+      *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(m.dst) + r * width + c * V) = x;
     }
   }
 }
 
-template <typename T, int V>
-int run_stage(const void* src, int rows, int cols, int64_t stride, void* dst, cudaStream_t s) {
-  const long long blocks = ((long long)rows * ((cols + V - 1) / V) + kThreads - 1) / kThreads;
-  stage_kernel<T, V><<<(unsigned)std::min<long long>(blocks, 148 * 16), kThreads, 0, s>>>(static_cast<const T*>(src), rows, cols, stride, dst,
-                                                                                         (int)up8(cols));
-  const cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess) return JVPFA_OK;
-  set_last_cuda_error(e, "gated stage_kernel");
-  return JVPFA_ERR_CUDA;
-}
-// `stride` in elements; pieces of 16 bytes where the source has them.
-int stage(int dtype, const void* src, int rows, int cols, int64_t stride, void* dst, cudaStream_t s) {
-  const uint64_t address = reinterpret_cast<uint64_t>(src);
-  if (dtype == JVPFA_FP32)
-    return address % 16 == 0 && cols % 4 == 0 && stride % 4 == 0 ? run_stage<float, 4>(src, rows, cols, stride, dst, s)
-                                                                 : run_stage<float, 1>(src, rows, cols, stride, dst, s);
-  return address % 16 == 0 && cols % 8 == 0 && stride % 8 == 0 ? run_stage<__half, 8>(src, rows, cols, stride, dst, s)
-                                                               : run_stage<__half, 1>(src, rows, cols, stride, dst, s);
+template <typename T>
+__global__ void __launch_bounds__(kThreads) stage_kernel(const __grid_constant__ StageArgs a) {
+  constexpr int V = 16 / sizeof(T);
+  const StageItem& m = a.item[blockIdx.y];
+  if (reinterpret_cast<uint64_t>(m.src) % 16 == 0 && m.cols % V == 0 && m.stride % V == 0)
+    stage_matrix<T, V>(m);
+  else
+    stage_matrix<T, 1>(m);
 }
 
 // A matrix as the products read it: in place, or in the workspace.
@@ -94,11 +103,12 @@ struct Matrix {
     width = up8(cols);
     workspace += up256(2 * planes * width * rows);
   }
-  int make(int dtype, void* workspace, cudaStream_t s) {
-    if (at < 0) return JVPFA_OK;
+  // Its place in the workspace, and what has to be copied there.
+  void put(void* workspace, StageArgs& stage, int& n) {
+    if (at < 0) return;
     void* dst = static_cast<char*>(workspace) + at;
     ptr = dst;
-    return stage(dtype, src, rows, cols, stride, dst, s);
+    stage.item[n++] = {src, dst, rows, cols, stride};
   }
   bool map(CUtensorMap* m, int dtype, int box_rows) const { return encode_matrix(m, dtype, ptr, rows, cols, width, planes, box_rows); }
 };
@@ -108,12 +118,33 @@ int map_error() {
   return JVPFA_ERR_CUDA;
 }
 
+int stage(int dtype, std::initializer_list<Matrix*> matrices, void* workspace, cudaStream_t s) {
+  StageArgs a{};
+  int n = 0;
+  long long most = 0;
+  for (Matrix* m : matrices) {
+    m->put(workspace, a, n);
+    if (m->at >= 0) most = std::max<long long>(most, (long long)m->rows * m->cols);
+  }
+  if (n == 0) return JVPFA_OK;
+  const dim3 grid((unsigned)std::min<long long>((most + 8 * kThreads - 1) / (8 * kThreads), 148 * 8), n);
+  if (dtype == JVPFA_FP32)
+    stage_kernel<float><<<grid, kThreads, 0, s>>>(a);
+  else
+    stage_kernel<__half><<<grid, kThreads, 0, s>>>(a);  // (bits alone are moved)
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) return JVPFA_OK;
+  set_last_cuda_error(e, "gated stage_kernel");
+  return JVPFA_ERR_CUDA;
+}
+
 // ---- cotangents of the projections ---------------------------------------------------------------------------------------
 struct CotangentArgs {
-  const void *g, *u, *tg, *tu, *gh, *gth;
+  const uint8_t* kept;
+  const void *gh, *gth;
   void *d, *td;  // [dg | du] and [dtg | dtu], rows of 2 * width; fp32: three planes each
-  long long rows;
-  int cols, width, activation;
+  int rows, cols, width, tensors;  // tensors: that were kept
+  long long units;
 };
 
 template <typename T, int V>
@@ -129,91 +160,143 @@ __device__ __forceinline__ void store_parts(void* base, long long plane, long lo
 #pragma unroll
     for (int k = 0; k < 3; ++k) *reinterpret_cast<Pack<__nv_bfloat16, V>*>(static_cast<__nv_bfloat16*>(base) + k * plane + at) = part[k];
   } else {
-    Pack<T, V> x;
-#pragma unroll
-    for (int j = 0; j < V; ++j) x.e[j] = Elem<T>::from_float(v[j]);
-    *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(base) + at) = x;
+    uint4 x;
+    x = make_uint4(Elem<T>::pack(v[0], v[1]), Elem<T>::pack(v[2], v[3]), Elem<T>::pack(v[4], v[5]), Elem<T>::pack(v[6], v[7]));
+    *reinterpret_cast<uint4*>(static_cast<T*>(base) + at) = x;
   }
 }
 
-template <typename T, int V>
-__device__ __forceinline__ void load_floats(const void* base, long long at, float (&v)[V]) {
-  const Pack<T, V> x = *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(base) + at);
+// V entries of a row from column c on; rows that are no whole pieces entry by entry (0 beyond the end).
+template <typename T, int V, bool ALIGNED>
+__device__ __forceinline__ void load_floats(const void* base, long long at, int left, float (&v)[V]) {
+  const T* p = static_cast<const T*>(base) + at;
+  Pack<T, V> x;
+  if constexpr (ALIGNED) {
+    x = *reinterpret_cast<const Pack<T, V>*>(p);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) x.e[j] = j < left ? p[j] : Elem<T>::from_float(0.f);
+  }
 #pragma unroll
   for (int j = 0; j < V; ++j) v[j] = Elem<T>::to_float(x.e[j]);
 }
 
-template <typename T, int V>
+// A warp takes an eighth or a quarter of a kept block at a time: 8 rows x 4 pieces.
+template <typename T, int KIND, bool DUAL, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads) cotangent_kernel(const __grid_constant__ CotangentArgs p) {
+  constexpr int V = Kept<T>::kPiece, kParts = 32 / V;  // of a block: 4 x 8 rows, 1 x or 2 x 4 pieces
   constexpr bool EXACT = sizeof(T) == 4;
-  const long long per_row = p.cols / V, total = p.rows * per_row, plane = p.rows * 2 * p.width;
-  for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < total; i += (long long)gridDim.x * kThreads) {
-    const long long r = i / per_row;
-    const int c = (int)(i - r * per_row) * V;
-    const long long from = r * p.cols + c, to = r * 2 * p.width + c;
+  const int lane = threadIdx.x & 31, blocks = (p.cols + 31) / 32;
+  const long long plane = (long long)p.rows * 2 * p.width;
+  for (long long unit = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); unit < p.units; unit += (long long)gridDim.x * (kThreads / 32)) {
+    const unsigned block = (unsigned)(unit / kParts), part = (unsigned)(unit % kParts);
+    const unsigned rb = block / (unsigned)blocks, fb = block - rb * (unsigned)blocks;
+    const int r = (int)(part & 3) * 8 + (lane >> 2), piece = (int)(part >> 2) * 4 + (lane & 3);
+    const int c = (int)fb * 32 + piece * V;
+    const long long i = (long long)rb * 32 + r;
+    if (i >= p.rows || c >= p.cols) continue;
+    const uint8_t* kept = p.kept + (size_t)block * p.tensors * Kept<T>::kBlock;
+    const long long from = i * p.cols + c, to = i * 2 * p.width + c;
     float g[V], u[V], gh[V], dg[V], du[V];
-    load_floats<T, V>(p.g, from, g);
-    load_floats<T, V>(p.u, from, u);
-    if (p.gh) load_floats<T, V>(p.gh, from, gh);
-    Activated y[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      y[j] = activate<EXACT>(p.activation, g[j]);
-      dg[j] = p.gh ? gh[j] * y[j].d1 * u[j] : 0.f;
-      du[j] = p.gh ? gh[j] * y[j].a : 0.f;
-    }
-    if (p.gth) {
+    kept_piece<T>(kept, r, piece, g);
+    kept_piece<T>(kept + Kept<T>::kBlock, r, piece, u);
+    if (!DUAL || p.gh) load_floats<T, V, ALIGNED>(p.gh, from, p.cols - c, gh);
+    if constexpr (DUAL) {
       float gth[V], tg[V], tu[V];
-      load_floats<T, V>(p.gth, from, gth);
-      load_floats<T, V>(p.tg, from, tg);
-      load_floats<T, V>(p.tu, from, tu);
+      load_floats<T, V, ALIGNED>(p.gth, from, p.cols - c, gth);
+      kept_piece<T>(kept + 2 * Kept<T>::kBlock, r, piece, tg);
+      kept_piece<T>(kept + 3 * Kept<T>::kBlock, r, piece, tu);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        dg[j] += gth[j] * (y[j].d2 * tg[j] * u[j] + y[j].d1 * tu[j]);
-        du[j] += gth[j] * y[j].d1 * tg[j];
-        tg[j] = gth[j] * y[j].d1 * u[j];
-        tu[j] = gth[j] * y[j].a;
+        const Activated y = activate<KIND, EXACT>(g[j]);
+        const float slope = y.d1 * u[j];
+        dg[j] = gth[j] * (y.d2 * tg[j] * u[j] + y.d1 * tu[j]);
+        du[j] = gth[j] * y.d1 * tg[j];
+        if (p.gh) dg[j] += gh[j] * slope, du[j] += gh[j] * y.a;
+        tg[j] = gth[j] * slope;
+        tu[j] = gth[j] * y.a;
       }
       store_parts<T, V>(p.td, plane, to, tg);
       store_parts<T, V>(p.td, plane, to + p.width, tu);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const Activated y = activate<KIND, EXACT>(g[j]);
+        dg[j] = gh[j] * y.d1 * u[j];
+        du[j] = gh[j] * y.a;
+      }
     }
     store_parts<T, V>(p.d, plane, to, dg);
     store_parts<T, V>(p.d, plane, to + p.width, du);
   }
 }
 
-template <typename T, int V>
-int run_cotangents(const CotangentArgs& p, cudaStream_t s) {
-  const long long blocks = (p.rows * (p.cols / V) + kThreads - 1) / kThreads;
-  cotangent_kernel<T, V><<<(unsigned)std::min<long long>(blocks, 148 * 8), kThreads, 0, s>>>(p);
+template <typename T, int KIND, bool DUAL>
+void run_cotangents(const CotangentArgs& p, cudaStream_t s) {
+  const unsigned blocks = (unsigned)std::min<long long>((p.units + kThreads / 32 - 1) / (kThreads / 32), 148 * 16);
+  if (p.cols % Kept<T>::kPiece == 0)
+    cotangent_kernel<T, KIND, DUAL, true><<<blocks, kThreads, 0, s>>>(p);
+  else
+    cotangent_kernel<T, KIND, DUAL, false><<<blocks, kThreads, 0, s>>>(p);
+}
+template <typename T>
+void run_cotangents(int kind, CotangentArgs& p, cudaStream_t s) {
+  p.units = (long long)((p.rows + 31) / 32) * ((p.cols + 31) / 32) * (32 / Kept<T>::kPiece);
+  auto run = [&](auto k) {
+    if (p.gth)
+      run_cotangents<T, decltype(k)::value, true>(p, s);
+    else
+      run_cotangents<T, decltype(k)::value, false>(p, s);
+  };
+  switch (kind) {
+    case JVPFA_ACT_SILU: return run(Kind<JVPFA_ACT_SILU>{});
+    case JVPFA_ACT_SIGMOID: return run(Kind<JVPFA_ACT_SIGMOID>{});
+    case JVPFA_ACT_GELU: return run(Kind<JVPFA_ACT_GELU>{});
+    default: return run(Kind<JVPFA_ACT_GELU_TANH>{});
+  }
+}
+int cotangents(int dtype, int kind, CotangentArgs& p, cudaStream_t s) {
+  if (dtype == JVPFA_FP32)
+    run_cotangents<float>(kind, p, s);
+  else if (dtype == JVPFA_BF16)
+    run_cotangents<__nv_bfloat16>(kind, p, s);
+  else
+    run_cotangents<__half>(kind, p, s);
   const cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) return JVPFA_OK;
   set_last_cuda_error(e, "gated cotangent_kernel");
   return JVPFA_ERR_CUDA;
 }
-int cotangents(int dtype, const CotangentArgs& p, cudaStream_t s) {
-  if (dtype == JVPFA_FP32) return p.cols % 4 == 0 ? run_cotangents<float, 4>(p, s) : run_cotangents<float, 1>(p, s);
-  const bool bf16 = dtype == JVPFA_BF16;
-  if (p.cols % 8 == 0) return bf16 ? run_cotangents<__nv_bfloat16, 8>(p, s) : run_cotangents<__half, 8>(p, s);
-  return bf16 ? run_cotangents<__nv_bfloat16, 1>(p, s) : run_cotangents<__half, 1>(p, s);
-}
 
 // ---- plans ---------------------------------------------------------------------------------------------------------------
 struct FwdPlan {
+  int rc;
   int64_t bytes = 0;
   Matrix x, tx, wg, wu;
+  int kind;
+  int64_t partial_at = 0;
+  PairArgs pair{};
   explicit FwdPlan(const jvpfa_gated_fwd_args& a)
       : x(a.dtype, a.x, a.M, a.K, a.x_stride, bytes),
         tx(a.dtype, a.tx, a.M, a.K, a.tx_stride, bytes),
         wg(a.dtype, a.wg, a.F, a.K, a.wg_stride, bytes),
-        wu(a.dtype, a.wu, a.F, a.K, a.wu_stride, bytes) {}
+        wu(a.dtype, a.wu, a.F, a.K, a.wu_stride, bytes),
+        kind(a.tx ? kPairGatedDual : kPairGated),
+        partial_at(bytes) {
+    pair.groups = 1, pair.rows = a.M, pair.cols = a.F, pair.depth = a.K, pair.sources = 1;
+    rc = plan_pair(a.dtype, kind, pair);
+    if (rc == JVPFA_OK) bytes += pair_workspace(pair);
+  }
 };
 
 struct BwdPlan {
+  int rc = JVPFA_OK;
   int64_t bytes = 0;
   int64_t width, d_bytes, d_at, td_at = -1;
   bool data, weights;  // which products are asked for
   Matrix x, tx, wg, wu;
+  int64_t partial_at;  // (one product's at a time)
+  PairArgs dx{}, dw{};
   explicit BwdPlan(const jvpfa_gated_bwd_args& a)
       : width(up8(a.F)),
         d_bytes(up256(2 * (a.dtype == JVPFA_FP32 ? 3 : 1) * 2 * width * a.M)),
@@ -224,7 +307,21 @@ struct BwdPlan {
         x(a.dtype, weights ? a.x : nullptr, a.M, a.K, a.x_stride, bytes),
         tx(a.dtype, weights && a.gth ? a.tx : nullptr, a.M, a.K, a.tx_stride, bytes),
         wg(a.dtype, data ? a.wg : nullptr, a.F, a.K, a.wg_stride, bytes),
-        wu(a.dtype, data ? a.wu : nullptr, a.F, a.K, a.wu_stride, bytes) {}
+        wu(a.dtype, data ? a.wu : nullptr, a.F, a.K, a.wu_stride, bytes),
+        partial_at(bytes) {
+    int64_t partial = 0;
+    if (data) {
+      dx.groups = (a.dx != nullptr) + (a.dtx != nullptr), dx.rows = a.M, dx.cols = a.K, dx.depth = a.F, dx.sources = 2;
+      rc = plan_pair(a.dtype, kPairDx, dx);
+      if (rc == JVPFA_OK) partial = pair_workspace(dx);
+    }
+    if (weights && rc == JVPFA_OK) {
+      dw.groups = 2, dw.rows = a.F, dw.cols = a.K, dw.depth = a.M, dw.sources = a.gth ? 2 : 1;
+      rc = plan_pair(a.dtype, kPairDw, dw);
+      if (rc == JVPFA_OK) partial = std::max(partial, pair_workspace(dw));
+    }
+    bytes += partial;
+  }
   int64_t take(int64_t n) {
     const int64_t at = bytes;
     bytes += n;
@@ -234,15 +331,21 @@ struct BwdPlan {
 
 }  // namespace
 
-int64_t gated_fwd_workspace(const jvpfa_gated_fwd_args& a) { return FwdPlan(a).bytes; }
-int64_t gated_bwd_workspace(const jvpfa_gated_bwd_args& a) { return BwdPlan(a).bytes; }
+int64_t gated_kept_bytes(int dtype, int64_t M, int64_t F, bool tangent) { return kept_bytes(dtype, M, F, tangent); }
+int64_t gated_fwd_workspace(const jvpfa_gated_fwd_args& a) {
+  const FwdPlan plan(a);
+  return plan.rc ? 0 : plan.bytes;
+}
+int64_t gated_bwd_workspace(const jvpfa_gated_bwd_args& a) {
+  const BwdPlan plan(a);
+  return plan.rc ? 0 : plan.bytes;
+}
 
 int launch_gated_fwd(const jvpfa_gated_fwd_args& a, cudaStream_t s) {
   FwdPlan plan(a);
-  for (Matrix* m : {&plan.x, &plan.tx, &plan.wg, &plan.wu}) {
-    const int rc = m->make(a.dtype, a.workspace, s);
-    if (rc) return rc;
-  }
+  if (plan.rc) return plan.rc;
+  const int rc = stage(a.dtype, {&plan.x, &plan.tx, &plan.wg, &plan.wu}, a.workspace, s);
+  if (rc) return rc;
   const bool dual = a.tx != nullptr;
   PairMaps maps;
   bool ok = plan.x.map(&maps.a[0], a.dtype, dual ? 64 : 128) && plan.wg.map(&maps.b[0], a.dtype, 128) && plan.wu.map(&maps.b[1], a.dtype, 128);
@@ -250,26 +353,28 @@ int launch_gated_fwd(const jvpfa_gated_fwd_args& a, cudaStream_t s) {
   if (dual) ok = ok && plan.tx.map(&maps.a[1], a.dtype, 64);
   maps.a[2] = maps.a[3] = maps.a[0];
   if (!ok) return map_error();
-  PairArgs p{};
-  p.groups = 1, p.rows = a.M, p.cols = a.F, p.depth = a.K, p.sources = 1;
-  p.h = a.h, p.th = a.th, p.g = a.g, p.u = a.u, p.tg = a.tg, p.tu = a.tu;
+  PairArgs& p = plan.pair;
+  p.partial = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + plan.partial_at);
+  p.h = a.h, p.th = a.th, p.kept = static_cast<uint8_t*>(a.kept);
   p.activation = a.activation;
-  return launch_pair(a.dtype, dual ? kPairGatedDual : kPairGated, p, maps, s);
+  return launch_pair(a.dtype, plan.kind, p, maps, s);
 }
 
 int launch_gated_bwd(const jvpfa_gated_bwd_args& a, cudaStream_t s) {
   BwdPlan plan(a);
+  if (plan.rc) return plan.rc;
   char* const ws = static_cast<char*>(a.workspace);
   CotangentArgs c{};
-  c.g = a.g, c.u = a.u, c.tg = a.tg, c.tu = a.tu, c.gh = a.gh, c.gth = a.gth;
+  c.kept = static_cast<const uint8_t*>(a.kept), c.tensors = a.kept_tangent ? 4 : 2;
+  c.gh = a.gh, c.gth = a.gth;
   c.d = ws + plan.d_at;
   c.td = a.gth ? ws + plan.td_at : nullptr;
-  c.rows = a.M, c.cols = a.F, c.width = (int)plan.width, c.activation = a.activation;
-  int rc = cotangents(a.dtype, c, s);
-  for (Matrix* m : {&plan.x, &plan.tx, &plan.wg, &plan.wu})
-    if (!rc) rc = m->make(a.dtype, a.workspace, s);
+  c.rows = a.M, c.cols = a.F, c.width = (int)plan.width;
+  int rc = cotangents(a.dtype, a.activation, c, s);
+  if (!rc) rc = stage(a.dtype, {&plan.x, &plan.tx, &plan.wg, &plan.wu}, a.workspace, s);
   if (rc) return rc;
   const int planes = a.dtype == JVPFA_FP32 ? 3 : 1;
+  float* const partial = reinterpret_cast<float*>(ws + plan.partial_at);
   // half of [dg | du] or of [dtg | dtu]
   auto half = [&](CUtensorMap* m, bool tangent, bool up, int box_rows) {
     return encode_matrix(m, a.dtype, static_cast<const char*>(tangent ? c.td : c.d) + (up ? 2 * plan.width : 0), a.M, a.F, 2 * plan.width, planes,
@@ -277,24 +382,25 @@ int launch_gated_bwd(const jvpfa_gated_bwd_args& a, cudaStream_t s) {
   };
   if (plan.data) {
     PairMaps maps;
-    PairArgs p{};
-    p.rows = a.M, p.cols = a.K, p.depth = a.F, p.sources = 2;
+    PairArgs& p = plan.dx;
+    p.partial = partial;
     bool ok = plan.wg.map(&maps.b[0], a.dtype, 64) && plan.wu.map(&maps.b[1], a.dtype, 64);
+    int group = 0;
     for (int tangent = 0; tangent < 2; ++tangent) {
       if (!(tangent ? a.dtx : a.dx)) continue;
-      p.out[p.groups] = tangent ? a.dtx : a.dx;
-      for (int up = 0; up < 2; ++up) ok = ok && half(&maps.a[2 * p.groups + up], tangent, up, 128);
-      ++p.groups;
+      p.out[group] = tangent ? a.dtx : a.dx;
+      for (int up = 0; up < 2; ++up) ok = ok && half(&maps.a[2 * group + up], tangent, up, 128);
+      ++group;
     }
-    if (p.groups == 1) maps.a[2] = maps.a[0], maps.a[3] = maps.a[1];
+    if (group == 1) maps.a[2] = maps.a[0], maps.a[3] = maps.a[1];
     if (!ok) return map_error();
     rc = launch_pair(a.dtype, kPairDx, p, maps, s);
     if (rc) return rc;
   }
   if (plan.weights) {
     PairMaps maps;
-    PairArgs p{};
-    p.groups = 2, p.rows = a.F, p.cols = a.K, p.depth = a.M, p.sources = a.gth ? 2 : 1;
+    PairArgs& p = plan.dw;
+    p.partial = partial;
     p.out[0] = a.dwg, p.out[1] = a.dwu;
     bool ok = plan.x.map(&maps.b[0], a.dtype, 64);
     maps.b[1] = maps.b[0];

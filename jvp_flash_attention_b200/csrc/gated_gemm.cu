@@ -6,16 +6,18 @@
 //
 // Forward (kPairGated): the columns are 128 features of wg (CTA 0's) beside the same 128 of wu (CTA 1's), so that g and u of a feature
 // end up in one lane of one CTA and the gate is applied on the way out.  With tangents (kPairGatedDual) a CTA's 128 rows
-// are 64 of x and the same 64 of tx: all four products of a (row, feature) are in one CTA, and the lanes of the value hand a'(g) u and a(g)
-// to those of the tangent through shared memory.
+// are 64 of x and the same 64 of tx: all four products of a (row, feature) are in one CTA, and of every 32 features the warp that has a
+// row's value finishes 16 and the one that has its tangent the others, for which they hand each other what they hold through shared memory.
 // Backward: products over the features (kPairDx: weights read across the contraction) and over the rows (kPairDw: both operands are).
 //
 // Sums are fp32 accumulators in TMEM, two of them (2 x 256 columns), so that a tile is written while the next is computed.  The tensor cores
 // round a sum towards zero at every step of 16; fp32 results, whose products are six each of bf16 parts, are taken up in registers
-// every 16 k-blocks and summed there to nearest.
+// every 4 k-blocks and summed there to nearest (every 16: an error of 2.6e-6 of the norm at K = 768).
 //
 // Roles: warp 0 loads (TMA), warp 1 of CTA 0 issues the products, warp 2 owns TMEM, warps 4 to 11 write results.  Persistent: each cluster
-// takes every (clusters)-th tile, in bands of 8 tiles of rows so that what runs at once shares its operands in L2.
+// takes every (clusters)-th tile, in bands of 8 tiles of rows so that what runs at once shares its operands in L2.  Tiles of the last,
+// partly empty round are cut along their depth into as many pieces as there are clusters for; the pieces' sums go through the workspace and
+// join_kernel adds them in their order (plan_pair).
 #include "gated_common.cuh"
 
 namespace jvpfa {
@@ -24,14 +26,16 @@ namespace tc5 {
 namespace {
 
 constexpr int kPairThreads = 384;
-constexpr int kPairStages = 6;
+template <typename T>
+constexpr int kPairStages = sizeof(T) == 4 ? 5 : 6;  // (fp32: more room for what warps write through)
 constexpr int kStageBytes = 32768;  // of a CTA: A 128 x 64, B 128 x 64
 constexpr int kBand = 8;
-constexpr int kExchangeBytes = 32768;
+constexpr int kExchangeBytes = 32768;  // 4 pairs of warps x two directions x 2 x 16 features x 32 rows
+constexpr int kMinPieceSteps = 4, kMinSavedSteps = 24;
 constexpr int kAbortPairFull = 14, kAbortPairEmpty = 15, kAbortPairAcc = 16, kAbortPairAccEmpty = 17;
 
 struct PairBarriers {
-  uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2];
+  uint64_t full[6], empty[6], acc_full[2], acc_empty[2];
   uint32_t tmem;
   int abort_flag;
 };
@@ -83,24 +87,87 @@ __device__ __forceinline__ void tile_at(const PairArgs& p, int t, int& mt, int& 
   mt = band * kBand + r - nt * high;
 }
 
-// 32 neighbouring entries of a row.
-template <typename T>
-__device__ __forceinline__ void store32(T* row, int c, int n, bool pieces, const float (&v)[32]) {
-  if (pieces && c + 32 <= n) {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(row + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; j += 8)
-        *reinterpret_cast<uint4*>(row + c + j) = make_uint4(Elem<T>::pack(v[j], v[j + 1]), Elem<T>::pack(v[j + 2], v[j + 3]),
-                                                            Elem<T>::pack(v[j + 4], v[j + 5]), Elem<T>::pack(v[j + 6], v[j + 7]));
-    }
-    return;
+// What cluster `cluster` takes up as its `i`-th: a tile and the k-blocks of it, [begin, end); piece -1: all of them.
+struct Item {
+  int mt, nt, begin, end, piece;
+};
+__device__ __forceinline__ Item item_at(const PairArgs& p, int i) {
+  Item r;
+  int t = i;
+  r.begin = 0, r.end = p.steps, r.piece = -1;
+  if (i >= p.whole) {
+    r.piece = i - p.whole;
+    const int rest = r.piece / p.cut;
+    t = p.whole + rest;
+    r.begin = (r.piece - rest * p.cut) * p.piece;
+    r.end = min(p.steps, r.begin + p.piece);
   }
+  tile_at(p, t, r.mt, r.nt);
+  return r;
+}
+
+// N entries of each of 32 rows (a lane has a row) of a row-major matrix, from column c on, through the warp's own shared memory: lanes that
+// write at once write next to each other.
+template <typename T, int N>
+__device__ __forceinline__ void write_rows(T* out, const PairArgs& p, int row0, int c, int lane, uint8_t* mine, const float (&v)[N]) {
+  constexpr int E = 16 / sizeof(T), U = N / E, pitch = N * sizeof(T) + 16;
+  __syncwarp();
 #pragma unroll
-  for (int j = 0; j < 32; ++j)
-    if (c + j < n) row[c + j] = Elem<T>::from_float(v[j]);
+  for (int k = 0; k < U; ++k) {
+    uint4 x;
+    if constexpr (sizeof(T) == 4)
+      x = make_uint4(__float_as_uint(v[k * 4]), __float_as_uint(v[k * 4 + 1]), __float_as_uint(v[k * 4 + 2]), __float_as_uint(v[k * 4 + 3]));
+    else
+      x = make_uint4(Elem<T>::pack(v[k * 8], v[k * 8 + 1]), Elem<T>::pack(v[k * 8 + 2], v[k * 8 + 3]),
+                     Elem<T>::pack(v[k * 8 + 4], v[k * 8 + 5]), Elem<T>::pack(v[k * 8 + 6], v[k * 8 + 7]));
+    *reinterpret_cast<uint4*>(mine + lane * pitch + k * 16) = x;
+  }
+  __syncwarp();
+  if (p.aligned) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int r = (i * 32 + lane) / U, k = (i * 32 + lane) % U;
+      if (row0 + r < p.rows && c + k * E < p.cols)
+        *reinterpret_cast<uint4*>(out + (size_t)(row0 + r) * p.cols + c + k * E) = *reinterpret_cast<const uint4*>(mine + r * pitch + k * 16);
+    }
+  } else {
+#pragma unroll 4
+    for (int i = 0; i < N; ++i) {
+      const int r = (i * 32 + lane) / N, k = (i * 32 + lane) % N;
+      if (row0 + r < p.rows && c + k < p.cols) out[(size_t)(row0 + r) * p.cols + c + k] = reinterpret_cast<const T*>(mine + r * pitch)[k];
+    }
+  }
+}
+
+// The gate, for N features from c on of 32 rows: h (and th), and what a backward reads.
+template <typename T, bool DUAL, int N>
+__device__ __forceinline__ void finish_gated(const PairArgs& p, int row0, int c, int lane, uint8_t* mine, float (&g)[N], float (&u)[N],
+                                             float (&tg)[N], float (&tu)[N]) {
+  constexpr bool EXACT = sizeof(T) == 4;
+  if (p.kept && row0 < p.rows && c < p.cols) {
+    uint8_t* block = p.kept + (size_t)((row0 >> 5) * ((p.cols + 31) >> 5) + (c >> 5)) * (DUAL ? 4 : 2) * Kept<T>::kBlock;
+    keep<T>(block, lane, c & 31, g);
+    keep<T>(block + Kept<T>::kBlock, lane, c & 31, u);
+    if constexpr (DUAL) {
+      keep<T>(block + 2 * Kept<T>::kBlock, lane, c & 31, tg);
+      keep<T>(block + 3 * Kept<T>::kBlock, lane, c & 31, tu);
+    }
+  }
+  with_activation(p.activation, [&](auto kind) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const Activated y = activate<decltype(kind)::value, EXACT>(g[j]);
+      if constexpr (DUAL) tg[j] = y.d1 * tg[j] * u[j] + y.a * tu[j];
+      g[j] = y.a * u[j];
+    }
+  });
+  write_rows<T, N>(static_cast<T*>(p.h), p, row0, c, lane, mine, g);
+  if constexpr (DUAL) write_rows<T, N>(static_cast<T*>(p.th), p, row0, c, lane, mine, tg);
+}
+
+// A thread's 32 sums of block b among those of its piece.
+__device__ __forceinline__ float4* partial_at(const PairArgs& p, int piece, int rank, int warp, int b, int lane) {
+  return reinterpret_cast<float4*>(p.partial + ((((size_t)piece * 2 + rank) * 8 + warp) * 4 + b) * 1024) + lane;
 }
 
 template <typename T>
@@ -115,14 +182,18 @@ struct Operand<float> {
 };
 
 template <typename T, int KIND>
+constexpr int kThroughBytes = KIND == kPairGatedDual ? kExchangeBytes : 8 * 32 * (32 * (int)sizeof(T) + 16);
+
+template <typename T, int KIND>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     pair_kernel(const __grid_constant__ PairArgs p, const __grid_constant__ PairMaps maps) {
   constexpr bool GATED = KIND <= kPairGatedDual, DUAL = KIND == kPairGatedDual, A_MN = KIND == kPairDw, B_MN = KIND >= kPairDx;
   constexpr bool PARTS = Operand<T>::kParts;
+  constexpr int STAGES = kPairStages<T>;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
-  float* exchange = reinterpret_cast<float*>(smem + kPairStages * kStageBytes);
-  PairBarriers& bar = *reinterpret_cast<PairBarriers*>(smem + kPairStages * kStageBytes + (DUAL ? kExchangeBytes : 0));
+  uint8_t* through = smem + STAGES * kStageBytes;  // for the warps that write
+  PairBarriers& bar = *reinterpret_cast<PairBarriers*>(through + kThroughBytes<T, KIND>);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
@@ -130,7 +201,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   if (threadIdx.x == 0) {
     const int before = *reinterpret_cast<volatile int*>(p.status);
     bar.abort_flag = before;
-    for (int i = 0; i < kPairStages; ++i) mbar_init(&bar.full[i], 1), mbar_init(&bar.empty[i], 1);
+    for (int i = 0; i < STAGES; ++i) mbar_init(&bar.full[i], 1), mbar_init(&bar.empty[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&bar.acc_full[i], 1), mbar_init(&bar.acc_empty[i], 16);
     fence_mbar_init();
   }
@@ -151,42 +222,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       const int rows_of_tile = DUAL ? 128 : 256;
       int n = 0;  // k-blocks so far
       bool ok = true;
-      for (int t = cluster; t < p.tiles && ok; t += clusters) {
-        int mt, nt;
-        tile_at(p, t, mt, nt);
-        const int group = mt / p.tiles_m, m0 = (mt - group * p.tiles_m) * rows_of_tile + (int)rank * (rows_of_tile / 2);
-        const int n0 = GATED ? nt * 128 : nt * 256 + (int)rank * 128;
-        for (int s = 0; s < p.sources && ok; ++s) {
-          const CUtensorMap* ma = &maps.a[GATED ? 0 : 2 * group + s];
-          const CUtensorMap* mb = &maps.b[GATED ? rank : s];
-          for (int pair = 0; pair < p.pairs && ok; ++pair) {
-            const int pa = PARTS ? 0x850 >> (2 * pair) & 3 : 0, pb = PARTS ? 0x244 >> (2 * pair) & 3 : 0;
-            for (int kb = 0; kb < p.kblocks; ++kb, ++n) {
-              const int stage = n % kPairStages;
-              ok = mbar_wait(&bar.empty[stage], (n / kPairStages & 1) ^ 1, ab, kAbortPairEmpty);
-              if (!ok) break;
-              if (rank == 0) mbar_expect_tx(&bar.full[stage], 2 * kStageBytes);
-              const uint32_t full = in_leader(&bar.full[stage]), to = smem_u32(smem + stage * kStageBytes);
-              if constexpr (A_MN) {
-                tma_load_pair(to, ma, full, m0, kb * 64, pa);
-                tma_load_pair(to + 8192, ma, full, m0 + 64, kb * 64, pa);
-              } else {
-                tma_load_pair(to, ma, full, kb * 64, m0, pa);
-                if constexpr (DUAL) tma_load_pair(to + 8192, &maps.a[1], full, kb * 64, m0, pa);
-              }
-              if constexpr (B_MN) {
-                tma_load_pair(to + 16384, mb, full, n0, kb * 64, pb);
-                tma_load_pair(to + 16384 + 8192, mb, full, n0 + 64, kb * 64, pb);
-              } else {
-                tma_load_pair(to + 16384, mb, full, kb * 64, n0, pb);
-              }
-            }
+      for (int i = cluster; i < p.items && ok; i += clusters) {
+        const Item it = item_at(p, i);
+        const int group = it.mt / p.tiles_m, m0 = (it.mt - group * p.tiles_m) * rows_of_tile + (int)rank * (rows_of_tile / 2);
+        const int n0 = GATED ? it.nt * 128 : it.nt * 256 + (int)rank * 128;
+        int segment = it.begin / p.kblocks, kb = it.begin - segment * p.kblocks, source = segment / p.pairs, pair = segment - source * p.pairs;
+        for (int step = it.begin; step < it.end; ++step, ++n) {
+          const CUtensorMap* ma = &maps.a[GATED ? 0 : 2 * group + source];
+          const CUtensorMap* mb = &maps.b[GATED ? rank : source];
+          const int pa = PARTS ? 0x850 >> (2 * pair) & 3 : 0, pb = PARTS ? 0x244 >> (2 * pair) & 3 : 0;
+          const int stage = n % STAGES;
+          ok = mbar_wait(&bar.empty[stage], (n / STAGES & 1) ^ 1, ab, kAbortPairEmpty);
+          if (!ok) break;
+          if (rank == 0) mbar_expect_tx(&bar.full[stage], 2 * kStageBytes);
+          const uint32_t full = in_leader(&bar.full[stage]), to = smem_u32(smem + stage * kStageBytes);
+          if constexpr (A_MN) {
+            tma_load_pair(to, ma, full, m0, kb * 64, pa);
+            tma_load_pair(to + 8192, ma, full, m0 + 64, kb * 64, pa);
+          } else {
+            tma_load_pair(to, ma, full, kb * 64, m0, pa);
+            if constexpr (DUAL) tma_load_pair(to + 8192, &maps.a[1], full, kb * 64, m0, pa);
+          }
+          if constexpr (B_MN) {
+            tma_load_pair(to + 16384, mb, full, n0, kb * 64, pb);
+            tma_load_pair(to + 16384 + 8192, mb, full, n0 + 64, kb * 64, pb);
+          } else {
+            tma_load_pair(to + 16384, mb, full, kb * 64, n0, pb);
+          }
+          if (++kb == p.kblocks) {
+            kb = 0;
+            if (++pair == p.pairs) pair = 0, ++source;
           }
         }
       }
       // What the products have still to say to this CTA's barriers arrives before it ends.
-      for (int i = 0; i < kPairStages && ok; ++i, ++n)
-        ok = mbar_wait(&bar.empty[n % kPairStages], (n / kPairStages & 1) ^ 1, ab, kAbortPairEmpty);
+      for (int i = 0; i < STAGES && ok; ++i, ++n)
+        ok = mbar_wait(&bar.empty[n % STAGES], (n / STAGES & 1) ^ 1, ab, kAbortPairEmpty);
     }
   } else if (warp == 1) {
     if (rank == 0 && !refused) {
@@ -195,15 +266,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       constexpr uint32_t step_a = A_MN ? 128 : 2, step_b = B_MN ? 128 : 2;  // 16 of the contraction, in 16 bytes
       int n = 0, acc = 0;
       bool ok = true;
-      for (int t = cluster; t < p.tiles && ok; t += clusters) {
-        for (int done = 0; done < p.steps && ok; ++acc) {
-          const int upto = min(p.steps, done + p.chunk), buf = acc & 1;
+      for (int i = cluster; i < p.items && ok; i += clusters) {
+        const Item it = item_at(p, i);
+        for (int done = it.begin; done < it.end && ok; ++acc) {
+          const int upto = min(it.end, done + p.chunk), buf = acc & 1;
           ok = mbar_wait_warp(&bar.acc_empty[buf], (acc >> 1 & 1) ^ 1, ab, kAbortPairAccEmpty);
           if (!ok) break;
           tc_fence_after();
           for (bool first = true; done < upto; ++done, ++n) {
-            const int stage = n % kPairStages;
-            ok = mbar_wait_warp(&bar.full[stage], n / kPairStages & 1, ab, kAbortPairFull);
+            const int stage = n % STAGES;
+            ok = mbar_wait_warp(&bar.full[stage], n / STAGES & 1, ab, kAbortPairFull);
             if (!ok) break;
             tc_fence_after();
             const uint32_t a = (smem_u32(smem + stage * kStageBytes) & 0x3ffff) >> 4, b = a + (16384 >> 4);
@@ -223,19 +295,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       }
     }
   } else if (warp >= 4) {
-    const int q = warp & 3, half = (warp - 4) >> 2;
+    const int e = warp - 4, q = warp & 3, half = e >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
-    constexpr int kPieces = 16 / sizeof(T);
-    const bool pieces = p.cols % kPieces == 0;
+    uint8_t* const mine = through + (DUAL ? ((half * 2 + (q & 1)) * 2 + (q >> 1)) * 4096 : e * 32 * (32 * (int)sizeof(T) + 16));
     int acc = 0;
     bool ok = !refused;
-    for (int t = cluster; t < p.tiles; t += clusters) {
-      int mt, nt;
-      tile_at(p, t, mt, nt);
-      const int group = mt / p.tiles_m, m = mt - group * p.tiles_m;
-      const int row = DUAL ? m * 128 + (int)rank * 64 + (q & 1) * 32 + lane : m * 256 + (int)rank * 128 + q * 32 + lane;
-      const bool inside = row < p.rows;
-      const size_t at = (size_t)row * p.cols;
+    for (int i = cluster; i < p.items; i += clusters) {
+      const Item it = item_at(p, i);
+      const int group = it.mt / p.tiles_m, m = it.mt - group * p.tiles_m;
+      const int row0 = DUAL ? m * 128 + (int)rank * 64 + (q & 1) * 32 : m * 256 + (int)rank * 128 + q * 32;
       float sum[PARTS ? 4 : 1][32];
       uint32_t col = 0;
       // this thread's 4 x 32 accumulators: gated g, g, u, u of 2 x 32 features, else 128 columns
@@ -250,7 +318,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         for (int b = 0; b < 4; ++b)
 #pragma unroll
           for (int j = 0; j < 32; ++j) sum[b][j] = 0.f;
-        for (int done = 0; done < p.steps; done += p.chunk, ++acc) {
+        for (int done = it.begin; done < it.end; done += p.chunk, ++acc) {
           const int buf = acc & 1;
           ok = ok && mbar_wait_warp(&bar.acc_full[buf], acc >> 1 & 1, ab, kAbortPairAcc);
           if (!ok) continue;
@@ -271,68 +339,79 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         if (ok) tc_fence_after();
         col = lanes + (acc & 1) * 256;
       }
-      // 32 accumulators of this thread
+      // 32 accumulators of this thread (to be waited for), NaN after a wait that gave up
       auto take = [&](int b, float (&v)[32]) {
-        if constexpr (PARTS) {
+        if (!ok) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = poison_f32();
+        } else if constexpr (PARTS) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = sum[b][j];
-        } else if (ok) {
+        } else {
           tmem_ld32(column(b), reinterpret_cast<uint32_t(&)[32]>(v));
         }
       };
-      if constexpr (GATED) {
-        const bool tangent = DUAL && q >= 2;
-        T* const out = static_cast<T*>(tangent ? p.th : p.h) + at;
-        T* const save_g = static_cast<T*>(tangent ? p.tg : p.g);
-        T* const save_u = static_cast<T*>(tangent ? p.tu : p.u);
-        float* const ex = exchange + half * (kExchangeBytes / 8) + (q & 1) * 32 + lane;
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const int c = nt * 128 + half * 64 + b * 32;
-          float g[32], u[32], o[32];
-          take(b, g);
-          take(b + 2, u);
-          if (!PARTS && ok) {
-            tmem_wait_ld();
-            if (b == 1) release(acc & 1);
-          }
-          if (!tangent) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const Activated y = activate<PARTS>(p.activation, g[j]);
-              o[j] = y.a * u[j];
-              if constexpr (DUAL) ex[j * 64] = y.d1 * u[j], ex[(32 + j) * 64] = y.a;
-            }
-          }
-          if constexpr (DUAL) {
-            asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
-            if (tangent) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = ex[j * 64] * g[j] + ex[(32 + j) * 64] * u[j];
-            }
-            asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
-          }
-          if (inside && ok) {
-            store32(out, c, p.cols, pieces, o);
-            if (save_g) store32(save_g + at, c, p.cols, pieces, g), store32(save_u + at, c, p.cols, pieces, u);
-          }
-          __syncwarp();
-        }
-        if (!ok && inside && nt * 128 + half * 64 < p.cols) out[nt * 128 + half * 64] = Elem<T>::from_float(poison_f32());
-      } else {
-        T* const out = static_cast<T*>(p.out[group]) + at;
+      auto taken = [&](bool last) {
+        if (PARTS || !ok) return;
+        tmem_wait_ld();
+        if (last) release(acc & 1);
+      };
+      if (it.piece >= 0) {
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
           float v[32];
           take(b, v);
-          if (!PARTS && ok) {
-            tmem_wait_ld();
-            if (b == 3) release(acc & 1);
-          }
-          if (inside && ok) store32(out, nt * 256 + half * 128 + b * 32, p.cols, pieces, v);
-          __syncwarp();
+          taken(b == 3);
+          float4* to = partial_at(p, it.piece, (int)rank, e, b, lane);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) to[j * 32] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
         }
-        if (!ok && inside && nt * 256 + half * 128 < p.cols) out[nt * 256 + half * 128] = Elem<T>::from_float(poison_f32());
+      } else if constexpr (GATED) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int c = it.nt * 128 + half * 64 + b * 32;
+          float g[32], u[32];
+          take(b, g);
+          take(b + 2, u);
+          taken(b == 1);
+          if constexpr (DUAL) {
+            // The warp of the value finishes features 0 to 15 of the 32, that of the tangent the others.
+            const bool tangent = q >= 2;
+            const int pair_id = half * 2 + (q & 1);
+            float* const to = reinterpret_cast<float*>(mine) + lane;
+            const float* const from = reinterpret_cast<const float*>(through + (pair_id * 2 + (tangent ? 0 : 1)) * 4096) + lane;
+            float own_g[16], own_u[16], got_g[16], got_u[16];
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              to[j * 32] = tangent ? g[j] : g[16 + j];
+              to[(16 + j) * 32] = tangent ? u[j] : u[16 + j];
+              own_g[j] = tangent ? g[16 + j] : g[j];
+              own_u[j] = tangent ? u[16 + j] : u[j];
+            }
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + pair_id) : "memory");
+#pragma unroll
+            for (int j = 0; j < 16; ++j) got_g[j] = from[j * 32], got_u[j] = from[(16 + j) * 32];
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + pair_id) : "memory");
+            float vg[16], vu[16], vtg[16], vtu[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              vg[j] = tangent ? got_g[j] : own_g[j], vu[j] = tangent ? got_u[j] : own_u[j];
+              vtg[j] = tangent ? own_g[j] : got_g[j], vtu[j] = tangent ? own_u[j] : got_u[j];
+            }
+            finish_gated<T, true, 16>(p, row0, c + (tangent ? 16 : 0), lane, mine, vg, vu, vtg, vtu);
+          } else {
+            finish_gated<T, false, 32>(p, row0, c, lane, mine, g, u, g, u);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          float v[32];
+          take(b, v);
+          taken(b == 3);
+          write_rows<T, 32>(static_cast<T*>(p.out[group]), p, row0, it.nt * 256 + half * 128 + b * 32, lane, mine, v);
+        }
       }
       if constexpr (!PARTS) ++acc;
     }
@@ -354,6 +433,55 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   cluster_sync();
 }
 
+// The sums of a cut tile's pieces, in their order, and what becomes of them.  A warp takes 32 rows x 32 columns, as one of pair_kernel's did.
+constexpr int kJoinWarps = 4;
+template <typename T, int KIND>
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ PairArgs p) {
+  constexpr bool GATED = KIND <= kPairGatedDual, DUAL = KIND == kPairGatedDual;
+  constexpr int kBlocks = GATED ? 2 : 4, kQ = DUAL ? 2 : 4;  // tasks: tile, rank, half, q, block
+  __shared__ __align__(16) uint8_t through[kJoinWarps * 32 * (32 * sizeof(T) + 16)];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int task = blockIdx.x * kJoinWarps + warp;
+  const int b = task % kBlocks, q = task / kBlocks % kQ, half = task / (kBlocks * kQ) % 2, rank = task / (kBlocks * kQ * 2) % 2;
+  const int rest = task / (kBlocks * kQ * 4);
+  if (rest * p.cut >= p.items - p.whole) return;
+  uint8_t* const mine = through + warp * 32 * (32 * sizeof(T) + 16);
+  int mt, nt;
+  tile_at(p, p.whole + rest, mt, nt);
+  const int group = mt / p.tiles_m, m = mt - group * p.tiles_m;
+  const int row0 = DUAL ? m * 128 + rank * 64 + q * 32 : m * 256 + rank * 128 + q * 32;
+  const int c = GATED ? nt * 128 + half * 64 + b * 32 : nt * 256 + half * 128 + b * 32;
+  if (row0 >= p.rows || c >= p.cols) return;
+  auto add_up = [&](int q_, int b_, float (&v)[32]) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = 0.f;
+    for (int k = 0; k < p.cut; ++k) {
+      const float4* from = partial_at(p, rest * p.cut + k, rank, half * 4 + q_, b_, lane);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float4 x = from[j * 32];
+        v[4 * j] += x.x, v[4 * j + 1] += x.y, v[4 * j + 2] += x.z, v[4 * j + 3] += x.w;
+      }
+    }
+  };
+  if constexpr (GATED) {
+    float g[32], u[32], tg[DUAL ? 32 : 1], tu[DUAL ? 32 : 1];
+    add_up(q, b, g);
+    add_up(q, b + 2, u);
+    if constexpr (DUAL) {
+      add_up(q + 2, b, tg);
+      add_up(q + 2, b + 2, tu);
+      finish_gated<T, true, 32>(p, row0, c, lane, mine, g, u, tg, tu);
+    } else {
+      finish_gated<T, false, 32>(p, row0, c, lane, mine, g, u, g, u);
+    }
+  } else {
+    float v[32];
+    add_up(q, b, v);
+    write_rows<T, 32>(static_cast<T*>(p.out[group]), p, row0, c, lane, mine, v);
+  }
+}
+
 int device_sms() {
   static int cached[64];
   int dev = 0, n = 0;
@@ -366,21 +494,27 @@ int device_sms() {
   return n;
 }
 
+int launched(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) return JVPFA_OK;
+  set_last_cuda_error(e, what);
+  return JVPFA_ERR_CUDA;
+}
+
 template <typename T, int KIND>
 int launch_kind(const PairArgs& p, const PairMaps& maps, cudaStream_t s) {
-  constexpr size_t smem = kPairStages * kStageBytes + (KIND == kPairGatedDual ? kExchangeBytes : 0) + sizeof(PairBarriers) + 1024;
+  constexpr size_t smem = kPairStages<T> * kStageBytes + kThroughBytes<T, KIND> + sizeof(PairBarriers) + 1024;
   static_assert(smem <= 232448, "shared memory of a CTA");
   auto kern = pair_kernel<T, KIND>;
   static SmemOptIn opt_in;
   if (!opt_in.ensure(reinterpret_cast<const void*>(kern), smem)) return JVPFA_ERR_CUDA;
   const int pairs = device_sms() / 2;
-  kern<<<2 * (p.tiles < pairs ? p.tiles : pairs), kPairThreads, smem, s>>>(p, maps);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) {
-    set_last_cuda_error(e, "gated pair_kernel");
-    return JVPFA_ERR_CUDA;
-  }
-  return JVPFA_OK;
+  kern<<<2 * (p.items < pairs ? p.items : pairs), kPairThreads, smem, s>>>(p, maps);
+  const int rc = launched("gated pair_kernel");
+  if (rc || p.items == p.whole) return rc;
+  constexpr int tasks = KIND <= kPairGated ? 2 * 4 * 4 : KIND == kPairGatedDual ? 2 * 2 * 4 : 4 * 4 * 4;  // of a tile
+  join_kernel<T, KIND><<<(p.items - p.whole) / p.cut * (tasks / kJoinWarps), kJoinWarps * 32, 0, s>>>(p);
+  return launched("gated join_kernel");
 }
 
 template <typename T>
@@ -401,7 +535,7 @@ bool encode_matrix(CUtensorMap* m, int dtype, const void* ptr, int rows, int col
   return encode_map4d(m, dt, ptr, cols, rows, planes, 1, st, box_rows);
 }
 
-int launch_pair(int dtype, int kind, PairArgs& p, const PairMaps& maps, cudaStream_t s) {
+int plan_pair(int dtype, int kind, PairArgs& p) {
   const bool gated = kind <= kPairGatedDual;
   const int rows = kind == kPairGatedDual ? 128 : 256, cols = gated ? 128 : 256;
   p.kblocks = (p.depth + 63) / 64;
@@ -413,8 +547,33 @@ int launch_pair(int dtype, int kind, PairArgs& p, const PairMaps& maps, cudaStre
   // (what a CTA counts, k-blocks of its tiles and tiles of a band, stays in 32 bits)
   if (steps > 2147483647LL || tiles > 2147483647LL - 1024 || steps * (tiles / 64 + 1) > 2147483647LL) return JVPFA_ERR_TOO_LARGE;
   p.steps = (int)steps;
-  p.tiles = (int)tiles;
-  p.chunk = dtype == JVPFA_FP32 ? 16 : p.steps;
+  p.chunk = dtype == JVPFA_FP32 ? 4 : p.steps;
+  p.aligned = p.cols % (dtype == JVPFA_FP32 ? 4 : 8) == 0;
+  // The tiles of the last round are cut into as many pieces as there are clusters for, where that saves more than a launch and the way
+  // through memory cost.
+  const int clusters = device_sms() / 2, rest = (int)(tiles % clusters);
+  p.whole = p.items = (int)tiles;
+  p.cut = 1, p.piece = p.steps;
+  if (rest > 0) {
+    int cut = clusters / rest;
+    if (cut > p.steps / kMinPieceSteps) cut = p.steps / kMinPieceSteps;
+    if (cut > 1) {
+      const int piece = (p.steps + cut - 1) / cut;
+      cut = (p.steps + piece - 1) / piece;
+      if (cut > 1 && p.steps - piece >= kMinSavedSteps) {
+        p.whole = (int)tiles - rest;
+        p.cut = cut, p.piece = piece;
+        p.items = p.whole + rest * cut;
+      }
+    }
+  }
+  return JVPFA_OK;
+}
+
+int64_t pair_workspace(const PairArgs& p) { return (int64_t)(p.items - p.whole) * 256 * 256 * 4; }
+
+int launch_pair(int dtype, int kind, const PairArgs& planned, const PairMaps& maps, cudaStream_t s) {
+  PairArgs p = planned;
   p.status = tc5_status_device_ptr();
   if (!p.status) {
     set_last_cuda_error(cudaErrorUnknown, "status word address");

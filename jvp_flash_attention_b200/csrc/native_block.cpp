@@ -235,7 +235,7 @@ py::object rotary(const Tensor& q_in, const std::optional<Tensor>& k_in, const T
 
 // ---- gated projection ----------------------------------------------------------------------------------------------------
 struct GatedOut {
-  Tensor h, th, g, u, tg, tu;
+  Tensor h, th, kept;  // kept: what a backward reads (jvpfa_gated_fwd_args)
 };
 struct GatedGrads {
   Tensor dx, dtx, dwg, dwu;
@@ -263,7 +263,7 @@ Tensor as_dense(const Tensor& x, const Tensor& like) {
 }
 Tensor workspace_for(int64_t bytes, const Tensor& x) { return bytes > 0 ? empty({bytes}, at::kByte, x.device()) : Tensor(); }
 
-// h, with tx also th, and with `keep` the projections that a backward reads.
+// h, with tx also th, and with `keep` what a backward reads.
 GatedOut launch_gated_fwd(const Tensor& x, const Tensor& tx, const Tensor& wg, const Tensor& wu, int activation, bool keep) {
   GatedOut r;
   if (!x.is_cuda()) {
@@ -271,22 +271,19 @@ GatedOut launch_gated_fwd(const Tensor& x, const Tensor& tx, const Tensor& wg, c
     NoFunctorch nf;
     at::AutoGradMode no_grad(false);
     py::tuple out = gated_module().attr("_launch_fwd")(x, or_none(tx), wg, wu, activation, keep);
-    Tensor* to[] = {&r.h, &r.th, &r.g, &r.u, &r.tg, &r.tu};
-    for (int i = 0; i < 6; ++i) *to[i] = from_python(out[i]);
+    r.h = from_python(out[0]), r.th = from_python(out[1]), r.kept = from_python(out[2]);
     return r;
   }
   c10::cuda::OptionalCUDAGuard guard;
   if (x.get_device() != c10::cuda::current_device()) guard.set_index(x.get_device());
   std::vector<int64_t> sizes = x.sizes().vec();
   sizes.back() = wg.size(0);
-  auto make = [&]() { return empty(sizes, x.scalar_type(), x.device()); };
-  r.h = make();
-  if (tx.defined()) r.th = make();
-  if (keep) {
-    r.g = make(), r.u = make();
-    if (tx.defined()) r.tg = make(), r.tu = make();
-  }
-  if (x.numel() == 0) return r;
+  const int64_t rows = x.numel() / wg.size(1);
+  r.h = empty(sizes, x.scalar_type(), x.device());
+  if (tx.defined()) r.th = empty(sizes, x.scalar_type(), x.device());
+  if (keep)
+    r.kept = empty({jvpfa_gated_kept_bytes(dtype_of(x, false), (int)rows, (int)wg.size(0), tx.defined())}, at::kByte, x.device());
+  if (rows == 0) return r;
   const Tensor x2 = as_rows(x), tx2 = as_rows(tx), wg2 = as_rows(wg), wu2 = as_rows(wu);
   jvpfa_gated_fwd_args a{};
   a.struct_size = sizeof(a);
@@ -296,18 +293,15 @@ GatedOut launch_gated_fwd(const Tensor& x, const Tensor& tx, const Tensor& wg, c
   a.x = data(x2), a.tx = data(tx2), a.wg = data(wg2), a.wu = data(wu2);
   a.x_stride = x2.stride(0), a.tx_stride = tx2.defined() ? tx2.stride(0) : 0, a.wg_stride = wg2.stride(0), a.wu_stride = wu2.stride(0);
   a.h = r.h.data_ptr(), a.th = r.th.defined() ? r.th.data_ptr() : nullptr;
-  if (keep) {
-    a.g = r.g.data_ptr(), a.u = r.u.data_ptr();
-    if (tx.defined()) a.tg = r.tg.data_ptr(), a.tu = r.tu.data_ptr();
-  }
+  if (keep) a.kept = r.kept.data_ptr();
   const Tensor workspace = workspace_for(jvpfa_gated_fwd_workspace(&a), x);
   if (workspace.defined()) a.workspace = workspace.data_ptr(), a.workspace_bytes = workspace.numel();
   check_status(jvpfa_gated_fwd(&a, c10::cuda::getCurrentCUDAStream(x.get_device()).stream()), "jvpfa_gated_fwd");
   return r;
 }
 
-// Gradients of <gh, h> + <gth, th>; of `kept` the forward's g, u, tg, tu are read.
-GatedGrads launch_gated_bwd(const Tensor& x, const Tensor& tx, const Tensor& wg, const Tensor& wu, const GatedOut& kept, Tensor gh, Tensor gth,
+// Gradients of <gh, h> + <gth, th>; tx as in the forward that left `kept`.
+GatedGrads launch_gated_bwd(const Tensor& x, const Tensor& tx, const Tensor& wg, const Tensor& wu, const Tensor& kept, Tensor gh, Tensor gth,
                             int activation, bool need_x, bool need_tx, bool need_w) {
   GatedGrads r;
   need_tx = need_tx && gth.defined();
@@ -316,8 +310,8 @@ GatedGrads launch_gated_bwd(const Tensor& x, const Tensor& tx, const Tensor& wg,
     py::gil_scoped_acquire gil;
     NoFunctorch nf;
     at::AutoGradMode no_grad(false);
-    py::tuple out = gated_module().attr("_launch_bwd")(x, or_none(tx), wg, wu, kept.g, kept.u, or_none(kept.tg), or_none(kept.tu), or_none(gh),
-                                                       or_none(gth), activation, need_x, need_tx, need_w);
+    py::tuple out = gated_module().attr("_launch_bwd")(x, or_none(tx), wg, wu, kept, or_none(gh), or_none(gth), activation, need_x,
+                                                       need_tx, need_w);
     Tensor* to[] = {&r.dx, &r.dtx, &r.dwg, &r.dwu};
     for (int i = 0; i < 4; ++i) *to[i] = from_python(out[i]);
     return r;
@@ -338,7 +332,6 @@ GatedGrads launch_gated_bwd(const Tensor& x, const Tensor& tx, const Tensor& wg,
   if (need_tx) r.dtx = empty(x.sizes(), x.scalar_type(), x.device());
   if (need_w) r.dwg = empty(wg.sizes(), x.scalar_type(), x.device()), r.dwu = empty(wu.sizes(), x.scalar_type(), x.device());
   const Tensor x2 = as_rows(x), tx2 = dual ? as_rows(tx) : Tensor(), wg2 = as_rows(wg), wu2 = as_rows(wu);
-  const Tensor g = as_dense(kept.g, x), u = as_dense(kept.u, x), tg = dual ? as_dense(kept.tg, x) : Tensor(), tu = dual ? as_dense(kept.tu, x) : Tensor();
   jvpfa_gated_bwd_args a{};
   a.struct_size = sizeof(a);
   a.dtype = dtype_of(x, false);
@@ -346,7 +339,7 @@ GatedGrads launch_gated_bwd(const Tensor& x, const Tensor& tx, const Tensor& wg,
   a.activation = activation;
   a.x = data(x2), a.tx = data(tx2), a.wg = data(wg2), a.wu = data(wu2);
   a.x_stride = x2.stride(0), a.tx_stride = dual ? tx2.stride(0) : 0, a.wg_stride = wg2.stride(0), a.wu_stride = wu2.stride(0);
-  a.g = data(g), a.u = data(u), a.tg = data(tg), a.tu = data(tu);
+  a.kept = data(kept), a.kept_tangent = tx.defined();
   a.gh = data(gh), a.gth = data(gth);
   if (need_x) a.dx = r.dx.data_ptr();
   if (need_tx) a.dtx = r.dtx.data_ptr();
@@ -375,7 +368,7 @@ struct GatedGradNode : public Node {
     const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1) || task_should_compute_output(2);
     const GatedOut f = launch_gated_fwd(xp, t, wgp, wup, activation, need_x || need_w);
     if (need_x || need_w) {
-      const GatedGrads g = launch_gated_bwd(xp, t, wgp, wup, f, Tensor(), unwrap(gh_), activation, need_x, false, need_w);
+      const GatedGrads g = launch_gated_bwd(xp, t, wgp, wup, f.kept, Tensor(), unwrap(gh_), activation, need_x, false, need_w);
       out[0] = g.dx, out[1] = g.dwg, out[2] = g.dwu;
     }
     if (task_should_compute_output(3)) out[3] = f.th;
@@ -393,7 +386,7 @@ struct GatedGradNode : public Node {
 // The node of a call: outputs h (0) and, with a tangent, th (1); edges to x, wg, wu and, with a tangent, tx.
 struct GatedNode : public Node {
   int activation;
-  SavedVariable x, tx, wg, wu, g, u, tg, tu;
+  SavedVariable x, tx, wg, wu, kept;
 
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -402,18 +395,13 @@ struct GatedNode : public Node {
     if (!gh.defined() && !gth.defined()) return out;
     const Tensor x_ = primal_of(x.unpack()), wg_ = primal_of(wg.unpack()), wu_ = primal_of(wu.unpack());
     const Tensor xp = unwrap(x_), wgp = unwrap(wg_), wup = unwrap(wu_);
-    GatedOut kept;
-    kept.g = unwrap(g.unpack()), kept.u = unwrap(u.unpack());
-    Tensor tx_;
-    if (gth.defined()) tx_ = tx.unpack(), kept.tg = unwrap(tg.unpack()), kept.tu = unwrap(tu.unpack());
-    const Tensor txp = unwrap(tx_);
+    const Tensor tx_ = num_outputs() > 3 ? tx.unpack() : Tensor(), txp = unwrap(tx_), kept_ = unwrap(kept.unpack());
     const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1) || task_should_compute_output(2);
     const bool need_tx = num_outputs() > 3 && task_should_compute_output(3);
     if ((gh.defined() && is_wrapped(gh)) || (gth.defined() && is_wrapped(gth))) {
       // the cotangents belong to a functorch transform, which differentiates Functions
       py::gil_scoped_acquire gil;
-      py::tuple d = gated_module().attr("_backward_under_functorch")(x_, or_none(tx_), wg_, wu_, kept.g, kept.u, or_none(kept.tg),
-                                                                      or_none(kept.tu), or_none(gh), or_none(gth), activation);
+      py::tuple d = gated_module().attr("_backward_under_functorch")(x_, or_none(tx_), wg_, wu_, kept_, or_none(gh), or_none(gth), activation);
       const int at[] = {0, 3, 1, 2};  // of (dx, dtx, dwg, dwu) among the edges
       for (int i = 0; i < 4; ++i)
         if (at[i] < (int)out.size()) out[at[i]] = from_python(d[i]);
@@ -423,13 +411,13 @@ struct GatedNode : public Node {
     const bool again = at::GradMode::is_enabled() && torch::autograd::compute_requires_grad(x_, wg_, wu_, tx_, gh, gth);
     GatedGrads d;
     if (gth.defined()) {
-      d = launch_gated_bwd(xp, txp, wgp, wup, kept, again ? Tensor() : gh, gth, activation, need_x, need_tx, need_w);
+      d = launch_gated_bwd(xp, txp, wgp, wup, kept_, again ? Tensor() : gh, gth, activation, need_x, need_tx, need_w);
       if (again)
         attach_refusal("the gradient through the tangent output of gated_linear cannot be differentiated a second time",
                        {&d.dx, &d.dtx, &d.dwg, &d.dwu}, x_, wg_, wu_, tx_, gth);
     }
     if (gh.defined() && (again || !gth.defined())) {
-      GatedGrads e = launch_gated_bwd(xp, Tensor(), wgp, wup, kept, gh, Tensor(), activation, need_x, false, need_w);
+      GatedGrads e = launch_gated_bwd(xp, txp, wgp, wup, kept_, gh, Tensor(), activation, need_x, false, need_w);
       if (again) {
         auto node = std::shared_ptr<GatedGradNode>(new GatedGradNode(), torch::autograd::deleteNode);
         node->set_next_edges(torch::autograd::collect_next_edges(x_, wg_, wu_, gh));
@@ -458,7 +446,7 @@ struct GatedNode : public Node {
   }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
-    for (SavedVariable* s : {&x, &tx, &wg, &wu, &g, &u, &tg, &tu}) s->reset_data();
+    for (SavedVariable* s : {&x, &tx, &wg, &wu, &kept}) s->reset_data();
   }
   std::string name() const override { return "GatedLinearBackward"; }
 };
@@ -504,16 +492,13 @@ py::object gated(const Tensor& x_in, const Tensor& wg_in, const Tensor& wu_in, i
     node->x = SavedVariable(x, false);
     node->wg = SavedVariable(wg, false);
     node->wu = SavedVariable(wu, false);
-    node->g = SavedVariable(r.g, false);
-    node->u = SavedVariable(r.u, false);
+    node->kept = SavedVariable(r.kept, false);
     if (grad_h)
       torch::autograd::set_history(r.h, node);
     else
       node->add_input_metadata(Node::undefined_input());
     if (tx.defined()) {
       node->tx = SavedVariable(tx, false);
-      node->tg = SavedVariable(r.tg, false);
-      node->tu = SavedVariable(r.tu, false);
       torch::autograd::set_history(r.th, node);
     }
   }

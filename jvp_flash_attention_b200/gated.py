@@ -29,8 +29,7 @@ def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, activation: str = "sil
     bfloat16, float16 or float32, of one type and device.  ``activation``: ``"silu"``, ``"sigmoid"``, ``"gelu"`` (exact) or ``"gelu_tanh"``.
     Rows of whole 16-byte pieces (K a multiple of 8) are read in place, others, and float32, through a copy.
 
-    Sums are in 32 bits, and the result is rounded once.  For a backward the projections are kept in x's type (a
-    float16 projection beyond 65504 becomes infinite there).  float32 is multiplied as three bfloat16 parts, about 1e-6 relative,
+    Sums are in 32 bits, and the result is rounded once.  For a backward the projections are kept in 24 bits an entry (float32: 32).  float32 is multiplied as three bfloat16 parts, about 1e-6 relative,
     whatever ``set_fp32_precision`` says of attention; an infinite entry gives NaN in its row.  Results are the same from run to run.
 
     The weights have no tangents, and their gradients cannot be differentiated again: both are refused.
@@ -71,21 +70,23 @@ def _check(x, w_gate, w_up) -> None:
 
 # ---- the general route (functorch transforms other than a lone torch.func.jvp) --------------------------------------------
 def _launch_fwd(x, tx, w_gate, w_up, activation, keep):
-    """Runs jvpfa_gated_fwd on plain tensors: (h, th, g, u, tg, tu), the last four with ``keep``, and those of the tangent with tx."""
+    """Runs jvpfa_gated_fwd on plain tensors: (h, th, kept), what a backward reads with ``keep``."""
     F, K = w_gate.shape
     x2, tx2, wg, wu = (None if t is None else _rows(t) for t in (x, tx, w_gate, w_up))
-    out = [torch.empty(*x.shape[:-1], F, device=x.device, dtype=x.dtype) if wanted else None
-           for wanted in (True, tx is not None, keep, keep, keep and tx is not None, keep and tx is not None)]
+    h, th = (torch.empty(*x.shape[:-1], F, device=x.device, dtype=x.dtype) if wanted else None for wanted in (True, tx is not None))
+    n = _lib.load().jvpfa_gated_kept_bytes(_lib.DTYPE_ENUM[x.dtype], x2.shape[0], F, tx is not None)
+    kept = torch.empty(n, device=x.device, dtype=torch.uint8) if keep else None
     if x.numel():
         a = _lib.GatedFwdArgs()
         _describe(a, x2, tx2, wg, wu, activation)
-        a.h, a.th, a.g, a.u, a.tg, a.tu = (_lib.ptr(t) for t in out)
+        a.h, a.th, a.kept = (_lib.ptr(t) for t in (h, th, kept))
         _run(a, x2, "jvpfa_gated_fwd")
-    return tuple(out)
+    return h, th, kept
 
 
-def _launch_bwd(x, tx, w_gate, w_up, g, u, tg, tu, gh, gth, activation, need_x, need_tx, need_w):
-    """Runs jvpfa_gated_bwd on plain tensors: (dx, dtx, dwg, dwu), None for those not asked for."""
+def _launch_bwd(x, tx, w_gate, w_up, kept, gh, gth, activation, need_x, need_tx, need_w):
+    """Runs jvpfa_gated_bwd on plain tensors: (dx, dtx, dwg, dwu), None for those not asked for.  tx as in the forward
+    that left ``kept``."""
     F, K = w_gate.shape
     x2, wg, wu = _rows(x), _rows(w_gate), _rows(w_up)
     tx2 = _rows(tx) if gth is not None else None
@@ -96,9 +97,8 @@ def _launch_bwd(x, tx, w_gate, w_up, g, u, tg, tu, gh, gth, activation, need_x, 
     if x.numel() and any(t is not None for t in out):
         a = _lib.GatedBwdArgs()
         _describe(a, x2, tx2, wg, wu, activation)
-        a.g, a.u, a.gh, a.gth = (_lib.ptr(t) for t in (g, u, gh, gth))
-        if gth is not None:
-            a.tg, a.tu = _lib.ptr(tg), _lib.ptr(tu)
+        a.kept, a.gh, a.gth = (_lib.ptr(t) for t in (kept, gh, gth))
+        a.kept_tangent = tx is not None
         a.dx, a.dtx, a.dwg, a.dwu = (_lib.ptr(t) for t in out)
         _run(a, x2, "jvpfa_gated_bwd")
     return tuple(out)
@@ -129,19 +129,18 @@ def _run(a, x, entry):
 
 
 class _Gated(Function):
-    """h, and the projections g and u that its backward reads."""
+    """h, and what its backward reads."""
 
     @staticmethod
     def forward(x, w_gate, w_up, activation):
-        h, _, g, u, _, _ = _launch_fwd(_unwrap(x), None, _unwrap(w_gate), _unwrap(w_up), activation, True)
-        return h, g, u
+        h, _, kept = _launch_fwd(_unwrap(x), None, _unwrap(w_gate), _unwrap(w_up), activation, True)
+        return h, kept
 
     @staticmethod
     def setup_context(ctx, inputs, outputs):
         x, w_gate, w_up, ctx.activation = inputs
-        _, g, u = outputs
-        ctx.mark_non_differentiable(g, u)
-        ctx.save_for_backward(x, w_gate, w_up, g, u)
+        ctx.mark_non_differentiable(outputs[1])
+        ctx.save_for_backward(x, w_gate, w_up, outputs[1])
         ctx.save_for_forward(x, w_gate, w_up)
         ctx.set_materialize_grads(False)
 
@@ -150,14 +149,14 @@ class _Gated(Function):
         if t_gate is not None or t_up is not None:
             raise NotImplementedError("gated_linear has no tangent with respect to its weights")
         x, w_gate, w_up = ctx.saved_tensors
-        return (None if tx is None else _GatedTangent.apply(x, tx.to(x.dtype), w_gate, w_up, ctx.activation)[0]), None, None
+        return (None if tx is None else _GatedTangent.apply(x, tx.to(x.dtype), w_gate, w_up, ctx.activation)[0]), None
 
     @staticmethod
     def backward(ctx, gh, *_):
         if gh is None:
             return None, None, None, None
-        x, w_gate, w_up, g, u = (fwAD.unpack_dual(t).primal for t in ctx.saved_tensors)
-        return (*_GatedGrad.apply(x, w_gate, w_up, g, u, fwAD.unpack_dual(gh).primal, ctx.activation), None)
+        x, w_gate, w_up, kept = (fwAD.unpack_dual(t).primal for t in ctx.saved_tensors)
+        return (*_GatedGrad.apply(x, None, w_gate, w_up, kept, fwAD.unpack_dual(gh).primal, ctx.activation), None)
 
 
 class _GatedTangent(Function):
@@ -165,14 +164,14 @@ class _GatedTangent(Function):
 
     @staticmethod
     def forward(x, tx, w_gate, w_up, activation):
-        _, th, g, u, tg, tu = _launch_fwd(*(_unwrap(t) for t in (x, tx, w_gate, w_up)), activation, True)
-        return th, g, u, tg, tu
+        _, th, kept = _launch_fwd(*(_unwrap(t) for t in (x, tx, w_gate, w_up)), activation, True)
+        return th, kept
 
     @staticmethod
     def setup_context(ctx, inputs, outputs):
         *tensors, ctx.activation = inputs
-        ctx.mark_non_differentiable(*outputs[1:])
-        ctx.save_for_backward(*tensors, *outputs[1:])
+        ctx.mark_non_differentiable(outputs[1])
+        ctx.save_for_backward(*tensors, outputs[1])
         ctx.set_materialize_grads(False)
 
     @staticmethod
@@ -180,23 +179,23 @@ class _GatedTangent(Function):
     def backward(ctx, gth, *_):
         if gth is None:
             return (None,) * 5
-        x, tx, w_gate, w_up, g, u, tg, tu = (_unwrap(t) for t in ctx.saved_tensors)
-        dx, dtx, dwg, dwu = _launch_bwd(x, tx, w_gate, w_up, g, u, tg, tu, None, _unwrap(gth), ctx.activation, True, True, True)
-        return dx, dtx, dwg, dwu, None
+        tensors = (_unwrap(t) for t in ctx.saved_tensors)
+        return (*_launch_bwd(*tensors, None, _unwrap(gth), ctx.activation, True, True, True), None)
 
 
 class _GatedGrad(Function):
-    """(dx, dwg, dwu) of <gh, h>, differentiable once more along x (see GatedGradNode in csrc/native_block.cpp)."""
+    """(dx, dwg, dwu) of <gh, h>, differentiable once more along x (see GatedGradNode in csrc/native_block.cpp).  ``tx``: of the forward that
+    left ``kept``, or None."""
 
     @staticmethod
-    def forward(x, w_gate, w_up, g, u, gh, activation):
-        x, w_gate, w_up, g, u, gh = (_unwrap(t) for t in (x, w_gate, w_up, g, u, gh))
-        dx, _, dwg, dwu = _launch_bwd(x, None, w_gate, w_up, g, u, None, None, gh, None, activation, True, False, True)
+    def forward(x, tx, w_gate, w_up, kept, gh, activation):
+        x, tx, w_gate, w_up, kept, gh = (None if t is None else _unwrap(t) for t in (x, tx, w_gate, w_up, kept, gh))
+        dx, _, dwg, dwu = _launch_bwd(x, tx, w_gate, w_up, kept, gh, None, activation, True, False, True)
         return dx, dwg, dwu
 
     @staticmethod
     def setup_context(ctx, inputs, outputs):
-        x, w_gate, w_up, g, u, gh, ctx.activation = inputs
+        x, _, w_gate, w_up, _, gh, ctx.activation = inputs
         ctx.save_for_backward(x, w_gate, w_up, gh)
         ctx.set_materialize_grads(False)
 
@@ -209,17 +208,17 @@ class _GatedGrad(Function):
             return (None,) * 7
         x, w_gate, w_up, gh = (_unwrap(t) for t in ctx.saved_tensors)
         vx = _unwrap(vx).to(x.dtype)
-        _, th, g, u, tg, tu = _launch_fwd(x, vx, w_gate, w_up, ctx.activation, True)
-        dx, _, dwg, dwu = _launch_bwd(x, vx, w_gate, w_up, g, u, tg, tu, None, gh, ctx.activation, True, False, True)
-        return dx, dwg, dwu, None, None, th, None
+        _, th, kept = _launch_fwd(x, vx, w_gate, w_up, ctx.activation, True)
+        dx, _, dwg, dwu = _launch_bwd(x, vx, w_gate, w_up, kept, None, gh, ctx.activation, True, False, True)
+        return dx, None, dwg, dwu, None, th, None
 
 
 class _GatedDualGrad(Function):
     """(dx, dtx, dwg, dwu) of <gh, h> + <gth, th>."""
 
     @staticmethod
-    def forward(x, tx, w_gate, w_up, g, u, tg, tu, gh, gth, activation):
-        tensors = [None if t is None else _unwrap(t) for t in (x, tx, w_gate, w_up, g, u, tg, tu, gh, gth)]
+    def forward(x, tx, w_gate, w_up, kept, gh, gth, activation):
+        tensors = [None if t is None else _unwrap(t) for t in (x, tx, w_gate, w_up, kept, gh, gth)]
         return _launch_bwd(*tensors, activation, True, True, True)
 
     @staticmethod
@@ -231,9 +230,9 @@ class _GatedDualGrad(Function):
         raise RuntimeError("the gradient through the tangent output of gated_linear cannot be differentiated a second time")
 
 
-def _backward_under_functorch(x, tx, w_gate, w_up, g, u, tg, tu, gh, gth, activation):
+def _backward_under_functorch(x, tx, w_gate, w_up, kept, gh, gth, activation):
     """The native layer's backward where a cotangent is a tensor of a functorch transform: Functions take part in it."""
     if gth is not None:
-        return _GatedDualGrad.apply(x, tx, w_gate, w_up, g, u, tg, tu, gh, gth, activation)
-    dx, dwg, dwu = _GatedGrad.apply(x, w_gate, w_up, g, u, gh, activation)
+        return _GatedDualGrad.apply(x, tx, w_gate, w_up, kept, gh, gth, activation)
+    dx, dwg, dwu = _GatedGrad.apply(x, tx, w_gate, w_up, kept, gh, activation)
     return dx, None, dwg, dwu

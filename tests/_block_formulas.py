@@ -69,3 +69,15 @@ def gated_bwd(x, tx, w_gate, w_up, g, u, tg, tu, gh, gth, kind, need_x=True, nee
     if need_w and gth is not None:
         dwg, dwu = dwg + flat(dtg).T @ flat(tx), dwu + flat(dtu).T @ flat(tx)
     return dx, dtx, dwg, dwu
+
+
+def launch_gated_fwd(x, tx, w_gate, w_up, kind, keep):
+    """Stand-in for ``gated._launch_fwd``."""
+    h, th, *projections = gated_fwd(x, tx, w_gate, w_up, kind)
+    return h, th, torch.stack([t for t in projections if t is not None]) if keep else None
+
+
+def launch_gated_bwd(x, tx, w_gate, w_up, kept, *args):
+    """Stand-in for ``gated._launch_bwd``."""
+    assert kept.shape[0] == (2 if tx is None else 4)
+    return gated_bwd(x, tx, w_gate, w_up, *(*kept, None, None)[:4], *args)

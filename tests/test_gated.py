@@ -18,8 +18,8 @@ PLAIN = {"silu": F.silu, "sigmoid": torch.sigmoid, "gelu": F.gelu, "gelu_tanh": 
 @pytest.fixture()
 def cpu_kernels(monkeypatch):
     calls = []
-    monkeypatch.setattr(gated, "_launch_fwd", lambda *a: (calls.append(("fwd", a[1] is not None, a[5])), formulas.gated_fwd(*a))[1])
-    monkeypatch.setattr(gated, "_launch_bwd", lambda *a: (calls.append(("bwd", *a[11:])), formulas.gated_bwd(*a))[1])
+    monkeypatch.setattr(gated, "_launch_fwd", lambda *a: (calls.append(("fwd", a[1] is not None, a[5])), formulas.launch_gated_fwd(*a))[1])
+    monkeypatch.setattr(gated, "_launch_bwd", lambda *a: (calls.append(("bwd", *a[8:])), formulas.launch_gated_bwd(*a))[1])
     monkeypatch.setattr(gated, "_require_cuda", lambda *a: None)
     return calls
 
@@ -164,7 +164,7 @@ def _bwd_args(**kw):
     a = _lib.GatedBwdArgs()
     a.struct_size = ctypes.sizeof(a)
     a.M = a.K = a.F = 64
-    a.x = a.wg = a.wu = a.g = a.u = a.gh = a.dx = a.workspace = 256
+    a.x = a.wg = a.wu = a.kept = a.gh = a.dx = a.workspace = 256
     a.x_stride = a.wg_stride = a.wu_stride = 64
     a.workspace_bytes = 1 << 30
     for k, v in kw.items():
@@ -177,10 +177,10 @@ def test_the_c_entries_refuse():
     assert lib.jvpfa_gated_fwd(None, None) == -1 and lib.jvpfa_gated_bwd(None, None) == -1
     common = [(-7, dict(struct_size=4)), (-3, dict(dtype=3)), (-2, dict(M=0)), (-2, dict(K=0)), (-2, dict(F=0)), (-9, dict(activation=4)),
               (-9, dict(activation=-1)), (-1, dict(x=None)), (-1, dict(wg=None)), (-1, dict(wu=None)), (-8, dict(x=257)), (-2, dict(x_stride=-8))]
-    for want, kw in common + [(-1, dict(h=None)), (-8, dict(h=264)), (-1, dict(tx=256)), (-1, dict(th=256)), (-1, dict(g=256)), (-1, dict(tg=256, tu=256)),
+    for want, kw in common + [(-1, dict(h=None)), (-8, dict(h=264)), (-1, dict(tx=256)), (-1, dict(th=256)), (-8, dict(kept=264)),
                               (-1, dict(x=258)), (-1, dict(dtype=2))]:  # the last two need a workspace
         assert lib.jvpfa_gated_fwd(ctypes.byref(_fwd_args(**kw)), None) == want, kw
-    for want, kw in common + [(-1, dict(g=None)), (-1, dict(gh=None)), (-1, dict(gth=256)), (-1, dict(dtx=256)), (-1, dict(dwg=256)), (-1, dict(dx=None)),
+    for want, kw in common + [(-1, dict(kept=None)), (-1, dict(gh=None)), (-1, dict(gth=256)), (-1, dict(gth=256, tx=256)), (-1, dict(dtx=256)), (-1, dict(dwg=256)), (-1, dict(dx=None)),
                               (-8, dict(dx=264)), (-8, dict(gh=258)), (-1, dict(workspace=None)), (-1, dict(workspace_bytes=16))]:
         assert lib.jvpfa_gated_bwd(ctypes.byref(_bwd_args(**kw)), None) == want, kw
 
@@ -195,5 +195,9 @@ def test_workspaces():
     assert fwd(x_stride=0) == 64 * 64 * 2  # one row for all
     bwd = lambda **kw: lib.jvpfa_gated_bwd_workspace(ctypes.byref(_bwd_args(**kw)))  # noqa: E731
     assert bwd() == 2 * 64 * 64 * 2
-    assert bwd(gth=256, tx=256, tg=256, tu=256, tx_stride=64) == 2 * 2 * 64 * 64 * 2
+    assert bwd(gth=256, tx=256, kept_tangent=1, tx_stride=64) == 2 * 2 * 64 * 64 * 2
     assert bwd(M=0) == 0
+    # a tile whose depth is worth cutting: 2 x 28 672 of the contraction, one row of 16 tiles, 4 pieces each of 256 x 256 sums
+    assert bwd(M=64, K=4096, F=28672, x_stride=4096, wg_stride=4096, wu_stride=4096) == 2 * 64 * 28672 * 2 + 16 * 4 * 256 * 256 * 4
+    kept = lib.jvpfa_gated_kept_bytes
+    assert kept(0, 1, 1, 0) == 2 * 1024 * 3 and kept(2, 33, 40, 1) == 4 * 4 * 1024 * 4 and kept(3, 1, 1, 0) == kept(0, 0, 1, 0) == 0
