@@ -5,6 +5,8 @@
 // bound by memory (12 bytes an entry for the value of a 16-bit tensor: gh, 3 each for g and u, dg, du), then a product over the features for dx and dtx, and one over
 // the rows for dwg and dwu.  Tangents are further rows of the first (dx beside dtx, the weights shared) and further depth of the second.
 //
+// Up to 128 rows (value and tangent together) the forward and dx are the kernels of gated_few.cu.
+//
 // Operands go to the tensor cores by TMA, which takes rows of whole 16-byte pieces; others are copied once into the workspace with padded
 // rows.  fp32 operands become three planes of bf16 parts there (f32_tc5_common.cuh).
 #include <algorithm>
@@ -93,11 +95,12 @@ struct Matrix {
   int64_t width;
   int planes;
 
-  Matrix(int dtype, const void* p, int rows_, int cols_, int64_t stride_, int64_t& workspace)
-      : src(p), rows(rows_), cols(cols_), stride(stride_), ptr(p), width(stride_), planes(dtype == JVPFA_FP32 ? 3 : 1) {
-    if (!p) return;
-    if (rows == 1) stride = width = up8(cols);
-    const bool in_place = dtype != JVPFA_FP32 && reinterpret_cast<uint64_t>(p) % 16 == 0 && width % 8 == 0 && width >= cols && width < 1ll << 38;
+  Matrix(int dtype, const void* p, int rows_, int cols_, int64_t stride_)
+      : src(p), rows(rows_), cols(cols_), stride(rows_ == 1 ? up8(cols_) : stride_), ptr(p), width(stride), planes(dtype == JVPFA_FP32 ? 3 : 1) {}
+  // Takes a place in the workspace where it cannot be read in place.
+  void use(int64_t& workspace) {
+    if (!src) return;
+    const bool in_place = planes == 1 && reinterpret_cast<uint64_t>(src) % 16 == 0 && width % 8 == 0 && width >= cols && width < 1ll << 38;
     if (in_place) return;
     at = workspace;
     width = up8(cols);
@@ -270,19 +273,27 @@ int cotangents(int dtype, int kind, CotangentArgs& p, cudaStream_t s) {
 
 // ---- plans ---------------------------------------------------------------------------------------------------------------
 struct FwdPlan {
-  int rc;
+  int rc = JVPFA_OK;
   int64_t bytes = 0;
   Matrix x, tx, wg, wu;
   int kind;
   int64_t partial_at = 0;
   PairArgs pair{};
+  bool is_few;
+  FewArgs few{};
   explicit FwdPlan(const jvpfa_gated_fwd_args& a)
-      : x(a.dtype, a.x, a.M, a.K, a.x_stride, bytes),
-        tx(a.dtype, a.tx, a.M, a.K, a.tx_stride, bytes),
-        wg(a.dtype, a.wg, a.F, a.K, a.wg_stride, bytes),
-        wu(a.dtype, a.wu, a.F, a.K, a.wu_stride, bytes),
-        kind(a.tx ? kPairGatedDual : kPairGated),
-        partial_at(bytes) {
+      : x(a.dtype, a.x, a.M, a.K, a.x_stride),
+        tx(a.dtype, a.tx, a.M, a.K, a.tx_stride),
+        wg(a.dtype, a.wg, a.F, a.K, a.wg_stride),
+        wu(a.dtype, a.wu, a.F, a.K, a.wu_stride),
+        kind(a.tx ? kPairGatedDual : kPairGated) {
+    few.groups = a.tx ? 2 : 1, few.rows = a.M, few.features = a.F, few.width = a.K;
+    is_few = plan_few(a.dtype, kFewGated, few);
+    x.use(bytes), tx.use(bytes);
+    if (is_few && a.dtype == JVPFA_FP32) return;  // (reads the weights as they are)
+    wg.use(bytes), wu.use(bytes);
+    if (is_few) return;
+    partial_at = bytes;
     pair.groups = 1, pair.rows = a.M, pair.cols = a.F, pair.depth = a.K, pair.sources = 1;
     rc = plan_pair(a.dtype, kind, pair);
     if (rc == JVPFA_OK) bytes += pair_workspace(pair);
@@ -297,6 +308,8 @@ struct BwdPlan {
   Matrix x, tx, wg, wu;
   int64_t partial_at;  // (one product's at a time)
   PairArgs dx{}, dw{};
+  bool is_few;
+  FewArgs few{};
   explicit BwdPlan(const jvpfa_gated_bwd_args& a)
       : width(up8(a.F)),
         d_bytes(up256(2 * (a.dtype == JVPFA_FP32 ? 3 : 1) * 2 * width * a.M)),
@@ -304,13 +317,17 @@ struct BwdPlan {
         td_at(a.gth ? take(d_bytes) : -1),
         data(a.dx || a.dtx),
         weights(a.dwg != nullptr),
-        x(a.dtype, weights ? a.x : nullptr, a.M, a.K, a.x_stride, bytes),
-        tx(a.dtype, weights && a.gth ? a.tx : nullptr, a.M, a.K, a.tx_stride, bytes),
-        wg(a.dtype, data ? a.wg : nullptr, a.F, a.K, a.wg_stride, bytes),
-        wu(a.dtype, data ? a.wu : nullptr, a.F, a.K, a.wu_stride, bytes),
-        partial_at(bytes) {
+        x(a.dtype, weights ? a.x : nullptr, a.M, a.K, a.x_stride),
+        tx(a.dtype, weights && a.gth ? a.tx : nullptr, a.M, a.K, a.tx_stride),
+        wg(a.dtype, data ? a.wg : nullptr, a.F, a.K, a.wg_stride),
+        wu(a.dtype, data ? a.wu : nullptr, a.F, a.K, a.wu_stride) {
+    few.groups = (a.dx != nullptr) + (a.dtx != nullptr), few.rows = a.M, few.features = a.F, few.width = a.K;
+    is_few = data && plan_few(a.dtype, kFewDx, few);
+    x.use(bytes), tx.use(bytes);
+    if (!is_few || a.dtype != JVPFA_FP32) wg.use(bytes), wu.use(bytes);
+    partial_at = bytes;
     int64_t partial = 0;
-    if (data) {
+    if (data && !is_few) {
       dx.groups = (a.dx != nullptr) + (a.dtx != nullptr), dx.rows = a.M, dx.cols = a.K, dx.depth = a.F, dx.sources = 2;
       rc = plan_pair(a.dtype, kPairDx, dx);
       if (rc == JVPFA_OK) partial = pair_workspace(dx);
@@ -328,6 +345,18 @@ struct BwdPlan {
     return at;
   }
 };
+
+// The weights of a product of few rows: 64 x 64 boxes of 16-bit ones, fp32 ones as they are.
+template <typename Args, typename Plan>
+void few_weights(const Args& a, Plan& plan, FewMaps& maps, bool& ok) {
+  FewArgs& p = plan.few;
+  if (a.dtype != JVPFA_FP32) {
+    ok = ok && plan.wg.map(&maps.w[0], a.dtype, 64) && plan.wu.map(&maps.w[1], a.dtype, 64);
+    return;
+  }
+  p.wg = a.wg, p.wu = a.wu, p.wg_stride = a.wg_stride, p.wu_stride = a.wu_stride;
+  p.pieces = (reinterpret_cast<uint64_t>(a.wg) | reinterpret_cast<uint64_t>(a.wu)) % 16 == 0 && (a.wg_stride | a.wu_stride) % 4 == 0;
+}
 
 }  // namespace
 
@@ -347,6 +376,18 @@ int launch_gated_fwd(const jvpfa_gated_fwd_args& a, cudaStream_t s) {
   const int rc = stage(a.dtype, {&plan.x, &plan.tx, &plan.wg, &plan.wu}, a.workspace, s);
   if (rc) return rc;
   const bool dual = a.tx != nullptr;
+  if (plan.is_few) {
+    FewMaps maps;
+    FewArgs& p = plan.few;
+    bool ok = plan.x.map(&maps.rows[0], a.dtype, p.padded);
+    maps.rows[1] = maps.rows[2] = maps.rows[3] = maps.w[0] = maps.w[1] = maps.rows[0];
+    if (dual) ok = ok && plan.tx.map(&maps.rows[1], a.dtype, p.padded);
+    few_weights(a, plan, maps, ok);
+    if (!ok) return map_error();
+    p.h = a.h, p.th = a.th, p.kept = static_cast<uint8_t*>(a.kept);
+    p.activation = a.activation;
+    return launch_few(a.dtype, kFewGated, p, maps, s);
+  }
   PairMaps maps;
   bool ok = plan.x.map(&maps.a[0], a.dtype, dual ? 64 : 128) && plan.wg.map(&maps.b[0], a.dtype, 128) && plan.wu.map(&maps.b[1], a.dtype, 128);
   maps.a[1] = maps.a[0];
@@ -380,7 +421,24 @@ int launch_gated_bwd(const jvpfa_gated_bwd_args& a, cudaStream_t s) {
     return encode_matrix(m, a.dtype, static_cast<const char*>(tangent ? c.td : c.d) + (up ? 2 * plan.width : 0), a.M, a.F, 2 * plan.width, planes,
                          box_rows);
   };
-  if (plan.data) {
+  if (plan.is_few) {
+    FewMaps maps;
+    FewArgs& p = plan.few;
+    bool ok = true;
+    int group = 0;
+    for (int tangent = 0; tangent < 2; ++tangent) {
+      if (!(tangent ? a.dtx : a.dx)) continue;
+      p.out[group] = tangent ? a.dtx : a.dx;
+      for (int up = 0; up < 2; ++up) ok = ok && half(&maps.rows[2 * group + up], tangent, up, p.padded);
+      ++group;
+    }
+    if (group == 1) maps.rows[2] = maps.rows[0], maps.rows[3] = maps.rows[1];
+    maps.w[0] = maps.w[1] = maps.rows[0];
+    few_weights(a, plan, maps, ok);
+    if (!ok) return map_error();
+    rc = launch_few(a.dtype, kFewDx, p, maps, s);
+    if (rc) return rc;
+  } else if (plan.data) {
     PairMaps maps;
     PairArgs& p = plan.dx;
     p.partial = partial;

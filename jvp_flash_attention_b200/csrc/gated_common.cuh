@@ -105,6 +105,19 @@ __device__ __forceinline__ void keep(uint8_t* block, int lane, int first, const 
     }
   }
 }
+// One entry.
+template <typename T>
+__device__ __forceinline__ void keep_entry(uint8_t* block, int row, int f, float v) {
+  constexpr int P = Kept<T>::kPiece;
+  const uint32_t w = __float_as_uint(v);
+  uint8_t* at = block + f / P * 512 + row * 16;
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<uint32_t*>(at)[f % P] = w;
+  } else {
+    reinterpret_cast<uint16_t*>(at)[f % P] = (uint16_t)(w >> 16);
+    block[2048 + f / P * 256 + row * 8 + f % P] = (uint8_t)(w >> 8);
+  }
+}
 // Piece `c` of row `row` of a tensor's block.
 template <typename T>
 __device__ __forceinline__ void kept_piece(const uint8_t* block, int row, int c, float (&v)[Kept<T>::kPiece]) {
@@ -141,7 +154,7 @@ struct PairArgs {
   int depth, sources;                // each is a sum over `sources` products of this depth
   int kblocks, pairs, steps;         // ceil(depth / 64); 1, or 6 products of bf16 parts (fp32); k-blocks of a tile
   int chunk;                         // k-blocks summed on the tensor cores before the sum goes on in registers
-  int tiles_m, tiles_n;              // tiles of a group
+  int tiles_m, tiles_n, band;        // tiles of a group, and how many rows of tiles are gone through together
   int whole, items;                  // tiles that are computed whole, and what clusters take up: these, then pieces of the others
   int cut, piece;                    // pieces of a tile, and their k-blocks
   float* partial;                    // 256 x 256 sums of each piece
@@ -156,6 +169,31 @@ struct PairArgs {
 int plan_pair(int dtype, int kind, PairArgs& p);
 int64_t pair_workspace(const PairArgs& p);
 int launch_pair(int dtype, int kind, const PairArgs& p, const PairMaps& maps, cudaStream_t s);
+
+// A product of few rows with the weights (gated_few.cu).
+enum FewKind {
+  kFewGated = 0,  // x (wg | wu)^T, the gate, h and with a second group th
+  kFewDx = 1      // dx, and as a second group dtx
+};
+struct FewMaps {
+  CUtensorMap w[2];     // wg, wu (16-bit types)
+  CUtensorMap rows[4];  // gated: x, tx; dx: [2 * group + source], source 0 the gate's cotangents, 1 the other's
+};
+struct FewArgs {
+  int groups, rows;          // 1 or 2 groups (value, tangent) of so many rows
+  int features, width;       // of the weights: rows F, columns K
+  const void *wg, *wu;       // fp32: read as they are
+  int64_t wg_stride, wu_stride;
+  bool pieces;               // ... and in whole 16-byte pieces
+  int padded, kblocks, steps, tiles, cluster, stages, accumulators, tmem_columns;
+  void *out[2], *h, *th;
+  uint8_t* kept;
+  int activation;
+  int* status;
+};
+// Fills in what follows from groups, rows, features and width; false: too many rows for these kernels.
+bool plan_few(int dtype, int kind, FewArgs& p);
+int launch_few(int dtype, int kind, const FewArgs& p, const FewMaps& maps, cudaStream_t s);
 // The map of a (planes of) row-major matrix: boxes of 64 columns x box_rows rows.
 bool encode_matrix(CUtensorMap* m, int dtype, const void* ptr, int rows, int cols, int64_t stride, int planes, int box_rows);
 

@@ -1,0 +1,356 @@
+// The gated projection's products for few rows (up to 128, value and tangent together): what counts is how quickly the weights arrive.
+//
+// The roles of rows and columns are exchanged: a tile of 128 weight rows (or columns, for dx) is the instruction's M, the rows of x are
+// its N, so nothing is computed for rows that are not there beyond the next multiple of 16.
+//   kFewGated  64 features: 64 rows of wg beside the same 64 of wu, contraction over K; then the gate
+//   kFewDx     128 columns of dx: the weights across the contraction, which runs over the features of wg and then of wu
+// A cluster of 1 to 8 CTAs shares a tile, a part of the depth each, so that all SMs have a part of the weights under way also where there are few
+// tiles; the parts' sums meet in the CTAs' shared memory and are added in their order, each CTA finishing a part of the tile.
+//
+// fp32 weights are read once, as they are: eight warps load them, split them into three bf16 parts and lay these down for the tensor cores
+// (a copy of the parts in memory would be written and read again, four times the bytes).  The tensor cores round towards zero at every
+// step of 16, so consecutive k-blocks go to different accumulators, as many as TMEM has room for, which are added to nearest at the end.
+#include "gated_common.cuh"
+
+namespace jvpfa {
+namespace tc5 {
+
+namespace {
+
+constexpr int kFewThreads = 384;  // warps 0: TMA, 1: products, 2: TMEM, 4 to 11: fp32 weights, results
+constexpr int kAbortFewFull = 18, kAbortFewEmpty = 19, kAbortFewAcc = 20;
+constexpr int kTile = 16384;  // 128 x 64 weights, 16 bits
+
+struct FewBarriers {
+  uint64_t full[8], empty[8], acc;
+  uint32_t tmem;
+  int abort_flag;
+};
+
+template <typename T>
+struct FewOperand {
+  using type = T;
+  static constexpr int kParts = 1;
+};
+template <>
+struct FewOperand<float> {
+  using type = __nv_bfloat16;
+  static constexpr int kParts = 3;
+};
+
+__device__ __forceinline__ uint32_t few_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void few_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A word of another CTA's shared memory.
+__device__ __forceinline__ float remote(uint32_t address, int rank) {
+  uint32_t at;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(address), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+
+// fp32 weights of k-block `step`: this thread's four pieces of eight neighbouring entries (zeros beyond the matrix).
+template <int KIND>
+struct Piece8 {
+  float v[4][8];
+  __device__ __forceinline__ static void place(const FewArgs& p, int tile, int step, int unit, const float*& row, int& c, bool& inside) {
+    if constexpr (KIND == kFewGated) {
+      const int r = unit >> 3, f = tile * 64 + (r & 63);
+      inside = f < p.features;
+      row = static_cast<const float*>(r < 64 ? p.wg : p.wu) + (size_t)f * (r < 64 ? p.wg_stride : p.wu_stride);
+      c = step * 64 + (unit & 7) * 8;
+    } else {
+      const int up = step >= p.kblocks, f = (step - (up ? p.kblocks : 0)) * 64 + (unit >> 4);
+      inside = f < p.features;
+      row = static_cast<const float*>(up ? p.wu : p.wg) + (size_t)f * (up ? p.wu_stride : p.wg_stride);
+      c = tile * 128 + (unit & 15) * 8;
+    }
+  }
+  __device__ __forceinline__ void load(const FewArgs& p, int tile, int step, int tid) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float* row;
+      int c;
+      bool inside;
+      place(p, tile, step, i * 256 + tid, row, c, inside);
+      const int left = inside ? p.width - c : 0;
+      if (p.pieces && left >= 8) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(row + c)), b = __ldg(reinterpret_cast<const float4*>(row + c) + 1);
+        v[i][0] = a.x, v[i][1] = a.y, v[i][2] = a.z, v[i][3] = a.w, v[i][4] = b.x, v[i][5] = b.y, v[i][6] = b.z, v[i][7] = b.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = j < left ? __ldg(row + c + j) : 0.f;
+      }
+    }
+  }
+  // ... as three parts, in the 128-byte-swizzled form of a tile contiguous along the contraction, or across it.
+  __device__ __forceinline__ void store(uint8_t* stage, int tid) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int unit = i * 256 + tid;
+      const int r = KIND == kFewGated ? unit >> 3 : unit >> 4, ch = KIND == kFewGated ? unit & 7 : unit & 15;
+      uint8_t* at = stage + (ch >> 3) * 8192 + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+      uint32_t w[3][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float h[2], m[2], l[2];
+        split3(v[i][2 * j], h[0], m[0], l[0]);
+        split3(v[i][2 * j + 1], h[1], m[1], l[1]);
+        w[0][j] = pack_bf16(h[0], h[1]), w[1][j] = pack_bf16(m[0], m[1]), w[2][j] = pack_bf16(l[0], l[1]);
+      }
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4*>(at + k * kTile) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+    }
+  }
+};
+
+template <typename T, int KIND>
+__global__ void __launch_bounds__(kFewThreads, 1) few_kernel(const __grid_constant__ FewArgs p, const __grid_constant__ FewMaps maps) {
+  constexpr int PARTS = FewOperand<T>::kParts;
+  constexpr bool SPLIT = PARTS > 1, GATED = KIND == kFewGated;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  const int N = p.padded * p.groups, rows_bytes = N * 128;
+  const int stage_bytes = PARTS * (kTile + rows_bytes);  // weights, then rows, part by part
+  FewBarriers& bar = *reinterpret_cast<FewBarriers*>(smem + p.stages * stage_bytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = p.cluster > 1 ? (int)few_rank() : 0, tile = (int)blockIdx.x / p.cluster;
+  const int begin = (int)((long long)p.steps * rank / p.cluster), end = (int)((long long)p.steps * (rank + 1) / p.cluster);
+
+  if (threadIdx.x == 0) {
+    bar.abort_flag = *reinterpret_cast<volatile int*>(p.status);
+    for (int i = 0; i < p.stages; ++i) mbar_init(&bar.full[i], SPLIT ? 9 : 1), mbar_init(&bar.empty[i], 1);
+    mbar_init(&bar.acc, 1);
+    fence_mbar_init();
+  }
+  if (warp == 2) {
+    tmem_alloc(&bar.tmem, p.tmem_columns);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bar.tmem;
+  const AbortState ab{&bar.abort_flag, p.status};
+  bool ok = bar.abort_flag == 0;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int step = begin, n = 0; step < end && ok; ++step, ++n) {
+        const int stage = n % p.stages;
+        ok = mbar_wait(&bar.empty[stage], (n / p.stages & 1) ^ 1, ab, kAbortFewEmpty);
+        if (!ok) break;
+        uint8_t* to = smem + stage * stage_bytes;
+        mbar_expect_tx(&bar.full[stage], PARTS * rows_bytes + (SPLIT ? 0 : kTile));
+        const int source = !GATED && step >= p.kblocks, kb = step - source * p.kblocks;
+        if constexpr (!SPLIT) {
+          if constexpr (GATED) {
+            tma_load_4d(to, &maps.w[0], &bar.full[stage], kb * 64, tile * 64, 0, 0);
+            tma_load_4d(to + 8192, &maps.w[1], &bar.full[stage], kb * 64, tile * 64, 0, 0);
+          } else {
+            tma_load_4d(to, &maps.w[source], &bar.full[stage], tile * 128, kb * 64, 0, 0);
+            tma_load_4d(to + 8192, &maps.w[source], &bar.full[stage], tile * 128 + 64, kb * 64, 0, 0);
+          }
+        }
+        for (int part = 0; part < PARTS; ++part)
+          for (int g = 0; g < p.groups; ++g)
+            tma_load_4d(to + PARTS * kTile + part * rows_bytes + g * p.padded * 128, &maps.rows[GATED ? g : 2 * g + source], &bar.full[stage], kb * 64,
+                        0, part, 0);
+      }
+    }
+  } else if (warp == 1) {
+    const uint32_t idesc = make_idesc(Fmt<typename FewOperand<T>::type>::kIdesc, 128, 0, !GATED, 0) | (uint32_t)(N >> 3) << 17;
+    constexpr uint32_t a_form = GATED ? kDescLo : (8192u >> 4) << 16, step_a = GATED ? 2 : 128;
+    for (int step = begin, n = 0; step < end && ok; ++step, ++n) {
+      const int stage = n % p.stages;
+      ok = mbar_wait_warp(&bar.full[stage], n / p.stages & 1, ab, kAbortFewFull);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t a = (smem_u32(smem + stage * stage_bytes) & 0x3ffff) >> 4, b = a + PARTS * (kTile >> 4);
+      const uint32_t d = tmem + n % p.accumulators * N;
+      if (elect_one()) {
+#pragma unroll
+        for (int pair = 0; pair < (SPLIT ? 6 : 1); ++pair) {
+          const int pa = SPLIT ? 0x850 >> (2 * pair) & 3 : 0, pb = SPLIT ? 0x244 >> (2 * pair) & 3 : 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_ss_lo_dyn(d, a_form | (a + pa * (kTile >> 4) + k * step_a), kDescLo | (b + pb * (rows_bytes >> 4) + k * 2), idesc,
+                           n >= p.accumulators || pair > 0 || k > 0);
+        }
+        tc_commit(&bar.empty[stage]);
+        if (step + 1 == end) tc_commit(&bar.acc);
+      }
+      __syncwarp();
+    }
+  } else if (warp >= 4) {
+    const int tid = threadIdx.x - 128;
+    if constexpr (SPLIT) {
+      Piece8<KIND> now, next;
+      if (begin < end) now.load(p, tile, begin, tid);
+      for (int step = begin, n = 0; step < end && ok; ++step, ++n) {
+        const int stage = n % p.stages;
+        if (step + 1 < end) next.load(p, tile, step + 1, tid);
+        ok = mbar_wait_warp(&bar.empty[stage], (n / p.stages & 1) ^ 1, ab, kAbortFewEmpty);
+        if (!ok) break;
+        now.store(smem + stage * stage_bytes, tid);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.full[stage]);
+        now = next;
+      }
+    }
+    // All products done: the stages' memory takes the sums, column by column.
+    ok = ok && mbar_wait_warp(&bar.acc, 0, ab, kAbortFewAcc);
+    if (ok) tc_fence_after();
+    float* const sums = reinterpret_cast<float*>(smem);
+    const int q = warp & 3, used = min(p.accumulators, end - begin);
+    for (int c = (warp >> 2 & 1) * 16; c < N; c += 32) {
+      float v[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = ok ? 0.f : poison_f32();
+      for (int i = 0; ok && i < used; ++i) {
+        uint32_t r[16];
+        tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + i * N + c, r);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] += __uint_as_float(r[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sums[(c + j) * 128 + q * 32 + lane] = v[j];
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (bar.abort_flag != 0) {
+    // Something gave up: copies and products that may still be in flight get time to land before shared memory and TMEM go.
+    const long long t0 = clock64();
+    while (clock64() - t0 < (1ll << 22)) {
+    }
+  }
+  if (p.cluster > 1) few_cluster_sync();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc(tmem, p.tmem_columns);
+  }
+
+  // This CTA's part of the tile.
+  const uint32_t sums = smem_u32(smem);
+  auto add_up = [&](int column, int line) {
+    const int at = (column * 128 + line) * 4;
+    if (p.cluster == 1) return *reinterpret_cast<const float*>(smem + at);
+    float v = 0.f;
+    for (int r = 0; r < p.cluster; ++r) v += remote(sums + at, r);
+    return v;
+  };
+  constexpr int kLines = GATED ? 64 : 128;  // of the tile: features, or columns of dx
+  const int total = kLines * p.rows * (GATED ? 1 : p.groups);
+  const int from = (int)((long long)total * rank / p.cluster), to = (int)((long long)total * (rank + 1) / p.cluster);
+  if constexpr (GATED) {
+    with_activation(p.activation, [&](auto kind) {
+      for (int i = from + (int)threadIdx.x; i < to; i += kFewThreads) {
+        const int row = i / kLines, line = i % kLines, f = tile * 64 + line;
+        if (f >= p.features) continue;
+        const float g = add_up(row, line), u = add_up(row, 64 + line);
+        const Activated y = activate<decltype(kind)::value, sizeof(T) == 4>(g);
+        static_cast<T*>(p.h)[(size_t)row * p.features + f] = Elem<T>::from_float(y.a * u);
+        float v[4] = {g, u, 0.f, 0.f};
+        if (p.groups > 1) {
+          v[2] = add_up(p.padded + row, line), v[3] = add_up(p.padded + row, 64 + line);
+          static_cast<T*>(p.th)[(size_t)row * p.features + f] = Elem<T>::from_float(y.d1 * v[2] * u + y.a * v[3]);
+        }
+        if (p.kept) {
+          uint8_t* block = p.kept + (size_t)((row >> 5) * ((p.features + 31) >> 5) + (f >> 5)) * (2 * p.groups) * Kept<T>::kBlock;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (k < 2 * p.groups) keep_entry<T>(block + k * Kept<T>::kBlock, row & 31, f & 31, v[k]);
+        }
+      }
+    });
+  } else {
+    for (int i = from + (int)threadIdx.x; i < to; i += kFewThreads) {
+      const int line = i % kLines, g = i / kLines / p.rows, row = i / kLines - g * p.rows, c = tile * 128 + line;
+      if (c < p.width) static_cast<T*>(p.out[g])[(size_t)row * p.width + c] = Elem<T>::from_float(add_up(g * p.padded + row, line));
+    }
+  }
+  if (p.cluster > 1) {
+    __syncwarp();
+    few_cluster_sync();  // the others have read what is here
+  }
+}
+
+template <typename T, int KIND>
+int launch_kind(const FewArgs& p, const FewMaps& maps, cudaStream_t s) {
+  constexpr int PARTS = FewOperand<T>::kParts;
+  const size_t smem = (size_t)p.stages * PARTS * (kTile + p.padded * p.groups * 128) + sizeof(FewBarriers) + 1024;
+  auto kern = few_kernel<T, KIND>;
+  static SmemOptIn opt_in;
+  if (!opt_in.ensure(reinterpret_cast<const void*>(kern), 232448)) return JVPFA_ERR_CUDA;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3((unsigned)(p.tiles * p.cluster));
+  config.blockDim = dim3(kFewThreads);
+  config.dynamicSmemBytes = smem;
+  config.stream = s;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = (unsigned)p.cluster;
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = p.cluster > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&config, kern, p, maps);
+  if (e == cudaSuccess) return JVPFA_OK;
+  (void)cudaGetLastError();
+  set_last_cuda_error(e, "gated few_kernel");
+  return JVPFA_ERR_CUDA;
+}
+
+}  // namespace
+
+bool plan_few(int dtype, int kind, FewArgs& p) {
+  const int parts = dtype == JVPFA_FP32 ? 3 : 1;
+  if (p.rows > 128) return false;
+  p.padded = p.groups == 1 ? (p.rows + 15) / 16 * 16 : (p.rows + 7) / 8 * 8;
+  const int N = p.padded * p.groups;
+  if (N > 128) return false;
+  const int depth = kind == kFewGated ? p.width : p.features;
+  p.kblocks = (depth + 63) / 64;
+  p.steps = kind == kFewGated ? p.kblocks : 2 * p.kblocks;
+  p.tiles = kind == kFewGated ? (p.features + 63) / 64 : (p.width + 127) / 128;
+  // fp32: one CTA an SM, whose registers hold what is under way; else two, of some 100 KB of stages each
+  const int stage = parts * (kTile + N * 128), room = parts > 1 ? 224 * 1024 : 108 * 1024;
+  p.stages = room / stage < 8 ? room / stage : 8;
+  const int at_once = parts > 1 ? 148 : 296;
+  p.cluster = 1;
+  while (p.cluster < 8 && p.tiles * 2 * p.cluster <= at_once && 4 * p.cluster <= p.steps) p.cluster *= 2;
+  const int per_cta = (p.steps + p.cluster - 1) / p.cluster;
+  p.accumulators = 1;
+  if (parts > 1) {
+    p.accumulators = 512 / N < 16 ? 512 / N : 16;
+    if (p.accumulators > per_cta) p.accumulators = per_cta;
+  }
+  p.tmem_columns = 32;
+  while (p.tmem_columns < p.accumulators * N) p.tmem_columns *= 2;
+  return true;
+}
+
+int launch_few(int dtype, int kind, const FewArgs& planned, const FewMaps& maps, cudaStream_t s) {
+  FewArgs p = planned;
+  p.status = tc5_status_device_ptr();
+  if (!p.status) {
+    set_last_cuda_error(cudaErrorUnknown, "status word address");
+    return JVPFA_ERR_CUDA;
+  }
+  const bool gated = kind == kFewGated;
+  if (dtype == JVPFA_BF16) return gated ? launch_kind<__nv_bfloat16, kFewGated>(p, maps, s) : launch_kind<__nv_bfloat16, kFewDx>(p, maps, s);
+  if (dtype == JVPFA_FP16) return gated ? launch_kind<__half, kFewGated>(p, maps, s) : launch_kind<__half, kFewDx>(p, maps, s);
+  return gated ? launch_kind<float, kFewGated>(p, maps, s) : launch_kind<float, kFewDx>(p, maps, s);
+}
+
+}  // namespace tc5
+}  // namespace jvpfa

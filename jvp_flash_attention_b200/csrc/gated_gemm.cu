@@ -15,7 +15,7 @@
 // every 4 k-blocks and summed there to nearest (every 16: an error of 2.6e-6 of the norm at K = 768).
 //
 // Roles: warp 0 loads (TMA), warp 1 of CTA 0 issues the products, warp 2 owns TMEM, warps 4 to 11 write results.  Persistent: each cluster
-// takes every (clusters)-th tile, in bands of 8 tiles of rows so that what runs at once shares its operands in L2.  Tiles of the last,
+// takes every (clusters)-th tile, in bands of tile rows, so that what runs at once shares its operands in L2.  Tiles of the last,
 // partly empty round are cut along their depth into as many pieces as there are clusters for; the pieces' sums go through the workspace and
 // join_kernel adds them in their order (plan_pair).
 #include "gated_common.cuh"
@@ -29,7 +29,6 @@ constexpr int kPairThreads = 384;
 template <typename T>
 constexpr int kPairStages = sizeof(T) == 4 ? 5 : 6;  // (fp32: more room for what warps write through)
 constexpr int kStageBytes = 32768;  // of a CTA: A 128 x 64, B 128 x 64
-constexpr int kBand = 8;
 constexpr int kExchangeBytes = 32768;  // 4 pairs of warps x two directions x 2 x 16 features x 32 rows
 constexpr int kMinPieceSteps = 4, kMinSavedSteps = 24;
 constexpr int kAbortPairFull = 14, kAbortPairEmpty = 15, kAbortPairAcc = 16, kAbortPairAccEmpty = 17;
@@ -79,12 +78,17 @@ __device__ __forceinline__ void umma_pair(uint32_t d, uint32_t a_lo, uint32_t b_
       : "memory");
 }
 
-// Tile t of the launch: the row of tiles (over all groups) and the column.
+// Tile t of the launch: the row of tiles (over all groups) and the column, in bands of p.band rows.
 __device__ __forceinline__ void tile_at(const PairArgs& p, int t, int& mt, int& nt) {
-  const int band = t / (kBand * p.tiles_n), r = t - band * kBand * p.tiles_n;
-  const int high = min(kBand, p.tiles_m * p.groups - band * kBand);
+  const int band = t / (p.band * p.tiles_n), r = t - band * p.band * p.tiles_n;
+  const int high = min(p.band, p.tiles_m * p.groups - band * p.band);
   nt = r / high;
-  mt = band * kBand + r - nt * high;
+  mt = band * p.band + r - nt * high;
+}
+
+// A result warp's wait, which is long: it looks every 100 ns and leaves the issue slots and the power to the others.
+__device__ __forceinline__ bool wait_for_sums(uint64_t* bar, uint32_t parity, const AbortState& ab) {
+  return __all_sync(0xffffffffu, mbar_wait_backoff<100>(bar, parity, ab, kAbortPairAcc));
 }
 
 // What cluster `cluster` takes up as its `i`-th: a tile and the k-blocks of it, [begin, end); piece -1: all of them.
@@ -320,7 +324,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           for (int j = 0; j < 32; ++j) sum[b][j] = 0.f;
         for (int done = it.begin; done < it.end; done += p.chunk, ++acc) {
           const int buf = acc & 1;
-          ok = ok && mbar_wait_warp(&bar.acc_full[buf], acc >> 1 & 1, ab, kAbortPairAcc);
+          ok = ok && wait_for_sums(&bar.acc_full[buf], acc >> 1 & 1, ab);
           if (!ok) continue;
           tc_fence_after();
           col = lanes + buf * 256;
@@ -335,7 +339,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           release(buf);
         }
       } else {
-        ok = ok && mbar_wait_warp(&bar.acc_full[acc & 1], acc >> 1 & 1, ab, kAbortPairAcc);
+        ok = ok && wait_for_sums(&bar.acc_full[acc & 1], acc >> 1 & 1, ab);
         if (ok) tc_fence_after();
         col = lanes + (acc & 1) * 256;
       }
@@ -548,6 +552,10 @@ int plan_pair(int dtype, int kind, PairArgs& p) {
   if (steps > 2147483647LL || tiles > 2147483647LL - 1024 || steps * (tiles / 64 + 1) > 2147483647LL) return JVPFA_ERR_TOO_LARGE;
   p.steps = (int)steps;
   p.chunk = dtype == JVPFA_FP32 ? 4 : p.steps;
+  // 74 tiles at once read band + 74 / band panels of their operands.  8 is the fewest, and best for the backward's, whose panels are as deep as the
+  // features or the rows are many; the forward's are shallow enough that a band of 16 stays in L2 while all columns go by (M8192
+  // K4096 F11008, sustained: forward 1092 -> 1051 us; all three products at 16 instead of 8 differ by less than they do between runs).
+  p.band = gated ? 16 : 8;
   p.aligned = p.cols % (dtype == JVPFA_FP32 ? 4 : 8) == 0;
   // The tiles of the last round are cut into as many pieces as there are clusters for, where that saves more than a launch and the way
   // through memory cost.

@@ -191,13 +191,15 @@ def test_workspaces():
     assert fwd() == 0
     assert fwd(x=258) == 64 * 64 * 2  # rows that begin elsewhere are copied
     assert fwd(x_stride=65) == 64 * 64 * 2 and fwd(K=63, x_stride=63) == 64 * 64 * 2  # rows padded to 16 bytes; wg and wu have them
-    assert fwd(dtype=2) == 3 * 3 * 64 * 64 * 2  # three parts of three operands
     assert fwd(x_stride=0) == 64 * 64 * 2  # one row for all
+    assert fwd(dtype=2) == 3 * 64 * 64 * 2  # fp32: three parts, up to 128 rows of x alone
+    assert fwd(dtype=2, M=256) == 3 * (256 + 2 * 64) * 64 * 2
     bwd = lambda **kw: lib.jvpfa_gated_bwd_workspace(ctypes.byref(_bwd_args(**kw)))  # noqa: E731
     assert bwd() == 2 * 64 * 64 * 2
     assert bwd(gth=256, tx=256, kept_tangent=1, tx_stride=64) == 2 * 2 * 64 * 64 * 2
+    assert bwd(dtype=2) == 3 * 2 * 64 * 64 * 2 and bwd(dtype=2, M=256) == 3 * (2 * 256 * 64 + 2 * 64 * 64) * 2
     assert bwd(M=0) == 0
-    # a tile whose depth is worth cutting: 2 x 28 672 of the contraction, one row of 16 tiles, 4 pieces each of 256 x 256 sums
-    assert bwd(M=64, K=4096, F=28672, x_stride=4096, wg_stride=4096, wu_stride=4096) == 2 * 64 * 28672 * 2 + 16 * 4 * 256 * 256 * 4
+    # tiles whose depth is worth cutting: 2 x 28 672 of the contraction, two rows of 16 tiles, 2 pieces each of 256 x 256 sums
+    assert bwd(M=300, K=4096, F=28672, x_stride=4096, wg_stride=4096, wu_stride=4096) == 2 * 300 * 28672 * 2 + 32 * 2 * 256 * 256 * 4
     kept = lib.jvpfa_gated_kept_bytes
     assert kept(0, 1, 1, 0) == 2 * 1024 * 3 and kept(2, 33, 40, 1) == 4 * 4 * 1024 * 4 and kept(3, 1, 1, 0) == kept(0, 0, 1, 0) == 0

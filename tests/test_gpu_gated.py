@@ -141,6 +141,15 @@ def test_several_tiles_of_a_cluster(dt, step):
     _case(400, 2500, 900, dt, "gelu_tanh", step)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("M", [1, 2, 17, 64, 65, 128, 129])
+@pytest.mark.parametrize("step", ["fwd_bwd", "jvp_bwd"])
+def test_few_rows(M, dt, step):
+    """Around the number of rows up to which the weights set the pace (128, value and tangent together), with clusters of one to eight CTAs."""
+    for K, F in ((1032, 264), (4100, 72), (200, 3300), (64, 20000)):
+        _case(M, K, F, dt, "silu" if K > 1000 else "gelu", step)
+
+
 @pytest.mark.parametrize("rows", [(0,), (0, 3), (3, 0)])
 def test_no_rows(rows):
     x, tx, wg, wu, gh, gth = _inputs(0, 16, 8, "bf16", 1, rows=rows)
