@@ -185,7 +185,7 @@ struct FewArgs {
   const void *wg, *wu;       // fp32: read as they are
   int64_t wg_stride, wu_stride;
   bool pieces;               // ... and in whole 16-byte pieces
-  int padded, kblocks, steps, tiles, cluster, stages, accumulators, tmem_columns;
+  int padded, kblocks, steps, tiles, cluster, stages, tmem_columns;
   void *out[2], *h, *th;
   uint8_t* kept;
   int activation;
@@ -194,6 +194,7 @@ struct FewArgs {
 // Fills in what follows from groups, rows, features and width; false: too many rows for these kernels.
 bool plan_few(int dtype, int kind, FewArgs& p);
 int launch_few(int dtype, int kind, const FewArgs& p, const FewMaps& maps, cudaStream_t s);
+int device_sms();  // of the current device
 // The map of a (planes of) row-major matrix: boxes of 64 columns x box_rows rows.
 bool encode_matrix(CUtensorMap* m, int dtype, const void* ptr, int rows, int cols, int64_t stride, int planes, int box_rows);
 

@@ -9,7 +9,8 @@
 //
 // fp32 weights are read once, as they are: eight warps load them, split them into three bf16 parts and lay these down for the tensor cores
 // (a copy of the parts in memory would be written and read again, four times the bytes).  The tensor cores round towards zero at every
-// step of 16, so consecutive k-blocks go to different accumulators, as many as TMEM has room for, which are added to nearest at the end.
+// step of 16, so those warps take the sums up in registers every 4 k-blocks, while the next go to another accumulator; and the five lesser
+// products of parts have accumulators of their own, where what is rounded away is that much smaller.
 #include "gated_common.cuh"
 
 namespace jvpfa {
@@ -17,12 +18,17 @@ namespace tc5 {
 
 namespace {
 
-constexpr int kFewThreads = 384;  // warps 0: TMA, 1: products, 2: TMEM, 4 to 11: fp32 weights, results
-constexpr int kAbortFewFull = 18, kAbortFewEmpty = 19, kAbortFewAcc = 20;
+// Warps 0: TMA, 1: products, 2: TMEM, from 4 on: fp32 weights, results
+template <typename T>
+constexpr int kFewThreads = sizeof(T) == 4 ? 640 : 384;
+constexpr int kSplitThreads = 512, kUnits = 1024 / kSplitThreads;  // fp32: a k-block's 1024 pieces of eight entries
+constexpr int kAbortFewFull = 18, kAbortFewEmpty = 19, kAbortFewAcc = 20, kAbortFewAccEmpty = 21;
+constexpr int kTakeUp = 4;   // fp32: k-blocks between two looks at the accumulators
+constexpr int kFewOpen = 1;    // what beginning and ending a CTA's share costs, in k-blocks
 constexpr int kTile = 16384;  // 128 x 64 weights, 16 bits
 
 struct FewBarriers {
-  uint64_t full[8], empty[8], acc;
+  uint64_t full[8], empty[8], acc[2], acc_empty[2];
   uint32_t tmem;
   int abort_flag;
 };
@@ -55,10 +61,10 @@ __device__ __forceinline__ float remote(uint32_t address, int rank) {
   return v;
 }
 
-// fp32 weights of k-block `step`: this thread's four pieces of eight neighbouring entries (zeros beyond the matrix).
+// fp32 weights of k-block `step`: this thread's pieces of eight neighbouring entries (zeros beyond the matrix).
 template <int KIND>
 struct Piece8 {
-  float v[4][8];
+  float v[kUnits][8];
   __device__ __forceinline__ static void place(const FewArgs& p, int tile, int step, int unit, const float*& row, int& c, bool& inside) {
     if constexpr (KIND == kFewGated) {
       const int r = unit >> 3, f = tile * 64 + (r & 63);
@@ -74,11 +80,11 @@ struct Piece8 {
   }
   __device__ __forceinline__ void load(const FewArgs& p, int tile, int step, int tid) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kUnits; ++i) {
       const float* row;
       int c;
       bool inside;
-      place(p, tile, step, i * 256 + tid, row, c, inside);
+      place(p, tile, step, i * kSplitThreads + tid, row, c, inside);
       const int left = inside ? p.width - c : 0;
       if (p.pieces && left >= 8) {
         const float4 a = __ldg(reinterpret_cast<const float4*>(row + c)), b = __ldg(reinterpret_cast<const float4*>(row + c) + 1);
@@ -92,17 +98,21 @@ struct Piece8 {
   // ... as three parts, in the 128-byte-swizzled form of a tile contiguous along the contraction, or across it.
   __device__ __forceinline__ void store(uint8_t* stage, int tid) const {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int unit = i * 256 + tid;
+    for (int i = 0; i < kUnits; ++i) {
+      const int unit = i * kSplitThreads + tid;
       const int r = KIND == kFewGated ? unit >> 3 : unit >> 4, ch = KIND == kFewGated ? unit & 7 : unit & 15;
       uint8_t* at = stage + (ch >> 3) * 8192 + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
       uint32_t w[3][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        float h[2], m[2], l[2];
-        split3(v[i][2 * j], h[0], m[0], l[0]);
-        split3(v[i][2 * j + 1], h[1], m[1], l[1]);
-        w[0][j] = pack_bf16(h[0], h[1]), w[1][j] = pack_bf16(m[0], m[1]), w[2][j] = pack_bf16(l[0], l[1]);
+        // Cut, not rounded (24 bits are 8 + 8 + 8 that way too): conversions run at an eighth of the rate of these, and would take longer
+        // than the weights need to arrive.  What the six products leave out is at most 2^-21 of one, 2^-24 on average.
+        float a = v[i][2 * j], b = v[i][2 * j + 1];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          w[k][j] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+          a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u), b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+        }
       }
 #pragma unroll
       for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4*>(at + k * kTile) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
@@ -110,8 +120,9 @@ struct Piece8 {
   }
 };
 
-template <typename T, int KIND>
-__global__ void __launch_bounds__(kFewThreads, 1) few_kernel(const __grid_constant__ FewArgs p, const __grid_constant__ FewMaps maps) {
+// BIG: more than 64 columns (fp32: a thread holds 32 sums, and has one k-block less under way).
+template <typename T, int KIND, bool BIG>
+__global__ void __launch_bounds__(kFewThreads<T>, 1) few_kernel(const __grid_constant__ FewArgs p, const __grid_constant__ FewMaps maps) {
   constexpr int PARTS = FewOperand<T>::kParts;
   constexpr bool SPLIT = PARTS > 1, GATED = KIND == kFewGated;
   extern __shared__ uint8_t raw[];
@@ -125,8 +136,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_kernel(const __grid_consta
 
   if (threadIdx.x == 0) {
     bar.abort_flag = *reinterpret_cast<volatile int*>(p.status);
-    for (int i = 0; i < p.stages; ++i) mbar_init(&bar.full[i], SPLIT ? 9 : 1), mbar_init(&bar.empty[i], 1);
-    mbar_init(&bar.acc, 1);
+    for (int i = 0; i < p.stages; ++i) mbar_init(&bar.full[i], SPLIT ? 1 + kSplitThreads / 32 : 1), mbar_init(&bar.empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&bar.acc[i], 1), mbar_init(&bar.acc_empty[i], kSplitThreads / 32);
     fence_mbar_init();
   }
   if (warp == 2) {
@@ -173,56 +184,118 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_kernel(const __grid_consta
       if (!ok) break;
       tc_fence_after();
       const uint32_t a = (smem_u32(smem + stage * stage_bytes) & 0x3ffff) >> 4, b = a + PARTS * (kTile >> 4);
-      const uint32_t d = tmem + n % p.accumulators * N;
-      if (elect_one()) {
-#pragma unroll
-        for (int pair = 0; pair < (SPLIT ? 6 : 1); ++pair) {
-          const int pa = SPLIT ? 0x850 >> (2 * pair) & 3 : 0, pb = SPLIT ? 0x244 >> (2 * pair) & 3 : 0;
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_ss_lo_dyn(d, a_form | (a + pa * (kTile >> 4) + k * step_a), kDescLo | (b + pb * (rows_bytes >> 4) + k * 2), idesc,
-                           n >= p.accumulators || pair > 0 || k > 0);
+      if constexpr (SPLIT) {
+        const int chunk = n / kTakeUp, buf = chunk & 1;
+        const uint32_t d = tmem + buf * 2 * N;  // the leading products' accumulator, and the others'
+        const bool first = n % kTakeUp == 0;
+        if (first) {
+          ok = mbar_wait_warp(&bar.acc_empty[buf], (chunk >> 1 & 1) ^ 1, ab, kAbortFewAccEmpty);
+          if (!ok) break;
+          tc_fence_after();
         }
+        if (elect_one()) {
+#pragma unroll
+          for (int pair = 0; pair < 6; ++pair) {
+            const int pa = 0x850 >> (2 * pair) & 3, pb = 0x244 >> (2 * pair) & 3;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_ss_lo_dyn(pair ? d + N : d, a_form | (a + pa * (kTile >> 4) + k * step_a), kDescLo | (b + pb * (rows_bytes >> 4) + k * 2), idesc,
+                             !first || pair > 1 || k > 0);
+          }
+          tc_commit(&bar.empty[stage]);
+          if (n % kTakeUp == kTakeUp - 1 || step + 1 == end) tc_commit(&bar.acc[buf]);
+        }
+      } else if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) umma_ss_lo_dyn(tmem, a_form | (a + k * step_a), kDescLo | (b + k * 2), idesc, n > 0 || k > 0);
         tc_commit(&bar.empty[stage]);
-        if (step + 1 == end) tc_commit(&bar.acc);
+        if (step + 1 == end) tc_commit(&bar.acc[0]);
       }
       __syncwarp();
     }
   } else if (warp >= 4) {
-    const int tid = threadIdx.x - 128;
+    const int tid = threadIdx.x - 128, q = warp & 3, set = (warp >> 2) - 1;
+    constexpr int kSets = kFewThreads<T> / 128 - 1;  // of four warps, which have 16 columns in turn
+    constexpr int kRun = SPLIT ? (BIG ? 2 : 1) : 1, kAhead = BIG ? 1 : 2;
+    const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
+    float run[kRun][16];
     if constexpr (SPLIT) {
-      Piece8<KIND> now, next;
-      if (begin < end) now.load(p, tile, begin, tid);
-      for (int step = begin, n = 0; step < end && ok; ++step, ++n) {
-        const int stage = n % p.stages;
-        if (step + 1 < end) next.load(p, tile, step + 1, tid);
-        ok = mbar_wait_warp(&bar.empty[stage], (n / p.stages & 1) ^ 1, ab, kAbortFewEmpty);
-        if (!ok) break;
-        now.store(smem + stage * stage_bytes, tid);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+#pragma unroll
+      for (int c = 0; c < kRun; ++c)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) run[c][j] = 0.f;
+      int taken = 0;
+      auto take_up = [&]() {
+        const int buf = taken & 1;
+        ok = ok && mbar_wait_warp(&bar.acc[buf], taken >> 1 & 1, ab, kAbortFewAcc);
+        if (!ok) return;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < kRun; ++c) {
+          const int column = (c * kSets + set) * 16;
+          if (column >= N) break;
+          uint32_t r[16];
+          tmem_ld16(lanes + (buf * 2 + 1) * N + column, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) run[c][j] += __uint_as_float(r[j]);
+          tmem_ld16(lanes + buf * 2 * N + column, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) run[c][j] += __uint_as_float(r[j]);
+        }
+        tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.full[stage]);
-        now = next;
+        if (lane == 0) mbar_arrive(&bar.acc_empty[buf]);
+        ++taken;
+      };
+      // One or two k-blocks are under way while another is split: up to 64 KB of each SM's, which is what memory's latency asks for.
+      Piece8<KIND> piece[kAhead + 1];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (begin + i < end) piece[i].load(p, tile, begin + i, tid);
+      for (int first = 0; begin + first < end && ok; first += kAhead + 1) {
+#pragma unroll
+        for (int i = 0; i <= kAhead; ++i) {
+          const int n = first + i, step = begin + n;
+          if (step >= end || !ok) break;
+          if (step + kAhead < end) piece[(i + kAhead) % (kAhead + 1)].load(p, tile, step + kAhead, tid);
+          const int stage = n % p.stages;
+          ok = mbar_wait_warp(&bar.empty[stage], (n / p.stages & 1) ^ 1, ab, kAbortFewEmpty);
+          if (!ok) break;
+          piece[i].store(smem + stage * stage_bytes, tid);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar.full[stage]);
+          if (n % kTakeUp == kTakeUp - 1 && n >= kTakeUp) take_up();  // what the k-blocks before these four gave
+        }
       }
+      const int all = (end - begin + kTakeUp - 1) / kTakeUp;
+      while (ok && taken < all) take_up();
+    } else {
+      ok = ok && mbar_wait_warp(&bar.acc[0], 0, ab, kAbortFewAcc);
+      if (ok) tc_fence_after();
     }
-    // All products done: the stages' memory takes the sums, column by column.
-    ok = ok && mbar_wait_warp(&bar.acc, 0, ab, kAbortFewAcc);
-    if (ok) tc_fence_after();
+    // All products are done (by every warp's account): the stages' memory takes the sums, column by column.
     float* const sums = reinterpret_cast<float*>(smem);
-    const int q = warp & 3, used = min(p.accumulators, end - begin);
-    for (int c = (warp >> 2 & 1) * 16; c < N; c += 32) {
+    for (int c = 0; (c * kSets + set) * 16 < N; ++c) {
+      const int column = (c * kSets + set) * 16;
       float v[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = ok ? 0.f : poison_f32();
-      for (int i = 0; ok && i < used; ++i) {
-        uint32_t r[16];
-        tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + i * N + c, r);
-        tmem_wait_ld();
+      for (int j = 0; j < 16; ++j) v[j] = poison_f32();
+      if constexpr (SPLIT) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] += __uint_as_float(r[j]);
+        for (int k = 0; k < kRun; ++k)
+          if (ok && k == c) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = run[k][j];
+          }
+      } else if (ok) {
+        tmem_ld16(lanes + column, reinterpret_cast<uint32_t(&)[16]>(v));
+        tmem_wait_ld();
       }
 #pragma unroll
-      for (int j = 0; j < 16; ++j) sums[(c + j) * 128 + q * 32 + lane] = v[j];
+      for (int j = 0; j < 16; ++j) sums[(column + j) * 128 + q * 32 + lane] = v[j];
     }
   }
   __syncwarp();
@@ -254,7 +327,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_kernel(const __grid_consta
   const int from = (int)((long long)total * rank / p.cluster), to = (int)((long long)total * (rank + 1) / p.cluster);
   if constexpr (GATED) {
     with_activation(p.activation, [&](auto kind) {
-      for (int i = from + (int)threadIdx.x; i < to; i += kFewThreads) {
+      for (int i = from + (int)threadIdx.x; i < to; i += kFewThreads<T>) {
         const int row = i / kLines, line = i % kLines, f = tile * 64 + line;
         if (f >= p.features) continue;
         const float g = add_up(row, line), u = add_up(row, 64 + line);
@@ -274,7 +347,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_kernel(const __grid_consta
       }
     });
   } else {
-    for (int i = from + (int)threadIdx.x; i < to; i += kFewThreads) {
+    for (int i = from + (int)threadIdx.x; i < to; i += kFewThreads<T>) {
       const int line = i % kLines, g = i / kLines / p.rows, row = i / kLines - g * p.rows, c = tile * 128 + line;
       if (c < p.width) static_cast<T*>(p.out[g])[(size_t)row * p.width + c] = Elem<T>::from_float(add_up(g * p.padded + row, line));
     }
@@ -285,16 +358,18 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_kernel(const __grid_consta
   }
 }
 
-template <typename T, int KIND>
+template <typename T, int KIND, bool BIG = false>
 int launch_kind(const FewArgs& p, const FewMaps& maps, cudaStream_t s) {
+  if constexpr (sizeof(T) == 4 && !BIG)
+    if (p.padded * p.groups > 64) return launch_kind<T, KIND, true>(p, maps, s);
   constexpr int PARTS = FewOperand<T>::kParts;
   const size_t smem = (size_t)p.stages * PARTS * (kTile + p.padded * p.groups * 128) + sizeof(FewBarriers) + 1024;
-  auto kern = few_kernel<T, KIND>;
+  auto kern = few_kernel<T, KIND, BIG>;
   static SmemOptIn opt_in;
   if (!opt_in.ensure(reinterpret_cast<const void*>(kern), 232448)) return JVPFA_ERR_CUDA;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3((unsigned)(p.tiles * p.cluster));
-  config.blockDim = dim3(kFewThreads);
+  config.blockDim = dim3(kFewThreads<T>);
   config.dynamicSmemBytes = smem;
   config.stream = s;
   cudaLaunchAttribute attribute{};
@@ -325,17 +400,16 @@ bool plan_few(int dtype, int kind, FewArgs& p) {
   // fp32: one CTA an SM, whose registers hold what is under way; else two, of some 100 KB of stages each
   const int stage = parts * (kTile + N * 128), room = parts > 1 ? 224 * 1024 : 108 * 1024;
   p.stages = room / stage < 8 ? room / stage : 8;
-  const int at_once = parts > 1 ? 148 : 296;
+  const int at_once = parts > 1 ? device_sms() : 2 * device_sms();
+  // So many CTAs to a tile that the rounds of the SMs are the shortest, in k-blocks; the fewest of those that are alike.
   p.cluster = 1;
-  while (p.cluster < 8 && p.tiles * 2 * p.cluster <= at_once && 4 * p.cluster <= p.steps) p.cluster *= 2;
-  const int per_cta = (p.steps + p.cluster - 1) / p.cluster;
-  p.accumulators = 1;
-  if (parts > 1) {
-    p.accumulators = 512 / N < 16 ? 512 / N : 16;
-    if (p.accumulators > per_cta) p.accumulators = per_cta;
+  long long best = -1;
+  for (int c = 1; c <= 8 && (c == 1 || 2 * c <= p.steps); c *= 2) {
+    const long long rounds = ((long long)p.tiles * c + at_once - 1) / at_once, blocks = rounds * ((p.steps + c - 1) / c + kFewOpen);
+    if (best < 0 || blocks < best) best = blocks, p.cluster = c;
   }
   p.tmem_columns = 32;
-  while (p.tmem_columns < p.accumulators * N) p.tmem_columns *= 2;
+  while (p.tmem_columns < (parts > 1 ? 4 : 1) * N) p.tmem_columns *= 2;
   return true;
 }
 

@@ -53,8 +53,10 @@ __device__ __forceinline__ uint32_t in_leader(const void* p) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
   return r;
 }
+// What it tells is that TMEM has been read (tcgen05.wait::ld, tcgen05.fence), nothing that was written: a release at cluster scope would wait for
+// every store of the thread on its way to memory first (half of the time of the fp32 kernels, which arrive once for 4 k-blocks).
 __device__ __forceinline__ void arrive_in_leader(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // A load into this CTA's shared memory whose bytes CTA 0's barrier counts.
 __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
@@ -329,12 +331,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           tc_fence_after();
           col = lanes + buf * 256;
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            uint32_t r[32];
-            tmem_ld32(column(b), r);
+          for (int b = 0; b < 8; ++b) {  // (16 at a time: what is left of the registers)
+            uint32_t r[16];
+            tmem_ld16(column(b >> 1) + (b & 1) * 16, r);
             tmem_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) sum[b][j] += __uint_as_float(r[j]);
+            for (int j = 0; j < 16; ++j) sum[b >> 1][(b & 1) * 16 + j] += __uint_as_float(r[j]);
           }
           release(buf);
         }
@@ -486,18 +488,6 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
   }
 }
 
-int device_sms() {
-  static int cached[64];
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  n = __atomic_load_n(&cached[dev], __ATOMIC_RELAXED);
-  if (n == 0) {
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 2) n = 148;
-    __atomic_store_n(&cached[dev], n, __ATOMIC_RELAXED);
-  }
-  return n;
-}
-
 int launched(const char* what) {
   const cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) return JVPFA_OK;
@@ -532,6 +522,18 @@ int launch_type(int kind, const PairArgs& p, const PairMaps& maps, cudaStream_t 
 }
 
 }  // namespace
+
+int device_sms() {
+  static int cached[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  n = __atomic_load_n(&cached[dev], __ATOMIC_RELAXED);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 2) n = 148;
+    __atomic_store_n(&cached[dev], n, __ATOMIC_RELAXED);
+  }
+  return n;
+}
 
 bool encode_matrix(CUtensorMap* m, int dtype, const void* ptr, int rows, int cols, int64_t stride, int planes, int box_rows) {
   const int64_t plane = (int64_t)rows * stride, st[3] = {plane * planes, plane, stride};

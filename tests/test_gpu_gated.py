@@ -2,8 +2,8 @@
 
 Entrywise bounds, propagated through the formulas.  e: half a step of the type (2^-8 bf16, 2^-11 fp16, 2^-24 fp32).  A sum of n products that
 the tensor cores form is off by at most 17 n / 16 * 2^-23 of the sum of the products' magnitudes (every instruction of 16 rounds 17
-numbers towards zero), fp32 ones, which are taken up every 1024, by as much for n = 1024, 2^-24 for each of these pieces and 2^-22 for the
-parts left out.  An activation and its derivatives are off by eta (1 + |g|): 2^-17 by the fast exponential and division, 2^-20 for fp32.
+numbers towards zero), fp32 ones, which are taken up every 1024, by as much for n = 1024, 2^-24 for each of these pieces and 2^-21 for the
+parts left out (where the parts are cut: mid < 2^-7, lo < 2^-15 of the leading bit's, two products of one of each and lo lo).  An activation and its derivatives are off by eta (1 + |g|): 2^-17 by the fast exponential and division, 2^-20 for fp32.
 Projections and their cotangents are rounded to the type on the way to the gradients.  |a'''| <= 2 for each activation.
 
 Those bounds are the worst case.  Random inputs' errors add up as random numbers do, so the norm of an output's error is held to e (a
@@ -25,7 +25,7 @@ DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 
 def _sum_error(n, dtype):
     if dtype == torch.float32:
-        return 17 * min(n, 1024) / 16 * 2.0**-23 + (n // 1024 + 2) * 2.0**-24 + 2.0**-22
+        return 17 * min(n, 1024) / 16 * 2.0**-23 + (n // 1024 + 2) * 2.0**-24 + 2.0**-21
     return 17 * n / 16 * 2.0**-23 + 2.0**-23
 
 
