@@ -24,7 +24,7 @@ constexpr int kFewThreads = sizeof(T) == 4 ? 640 : 384;
 constexpr int kSplitThreads = 512, kUnits = 1024 / kSplitThreads;  // fp32: a k-block's 1024 pieces of eight entries
 constexpr int kAbortFewFull = 18, kAbortFewEmpty = 19, kAbortFewAcc = 20, kAbortFewAccEmpty = 21;
 constexpr int kTakeUp = 4;   // fp32: k-blocks between two looks at the accumulators
-constexpr int kFewOpen = 1;    // what beginning and ending a CTA's share costs, in k-blocks
+constexpr int kFewOpen = 6;    // fp32: what beginning and ending a CTA's share costs, in k-blocks
 constexpr int kTile = 16384;  // 128 x 64 weights, 16 bits
 
 struct FewBarriers {
@@ -400,13 +400,17 @@ bool plan_few(int dtype, int kind, FewArgs& p) {
   // fp32: one CTA an SM, whose registers hold what is under way; else two, of some 100 KB of stages each
   const int stage = parts * (kTile + N * 128), room = parts > 1 ? 224 * 1024 : 108 * 1024;
   p.stages = room / stage < 8 ? room / stage : 8;
-  const int at_once = parts > 1 ? device_sms() : 2 * device_sms();
-  // So many CTAs to a tile that the rounds of the SMs are the shortest, in k-blocks; the fewest of those that are alike.
+  // CTAs of a tile.  16 bits: as many as find room at once, for memory sets the pace whoever asks for what.  fp32, where a CTA has an SM
+  // to itself and splitting costs as much as loading: so many that the SMs' rounds are the shortest, in k-blocks.
   p.cluster = 1;
-  long long best = -1;
-  for (int c = 1; c <= 8 && (c == 1 || 2 * c <= p.steps); c *= 2) {
-    const long long rounds = ((long long)p.tiles * c + at_once - 1) / at_once, blocks = rounds * ((p.steps + c - 1) / c + kFewOpen);
-    if (best < 0 || blocks < best) best = blocks, p.cluster = c;
+  if (parts == 1) {
+    while (p.cluster < 8 && p.tiles * 2 * p.cluster <= 2 * device_sms() && 4 * p.cluster <= p.steps) p.cluster *= 2;
+  } else {
+    long long best = -1;
+    for (int c = 1; c <= 8 && (c == 1 || 2 * c <= p.steps); c *= 2) {
+      const long long rounds = ((long long)p.tiles * c + device_sms() - 1) / device_sms(), blocks = rounds * ((p.steps + c - 1) / c + kFewOpen);
+      if (best < 0 || blocks < best) best = blocks, p.cluster = c;
+    }
   }
   p.tmem_columns = 32;
   while (p.tmem_columns < (parts > 1 ? 4 : 1) * N) p.tmem_columns *= 2;

@@ -145,11 +145,12 @@ __device__ __forceinline__ void write_rows(T* out, const PairArgs& p, int row0, 
   }
 }
 
-// The gate, for N features from c on of 32 rows: h (and th), and what a backward reads.
-template <typename T, bool DUAL, int N>
-__device__ __forceinline__ void finish_gated(const PairArgs& p, int row0, int c, int lane, uint8_t* mine, float (&g)[N], float (&u)[N],
-                                             float (&tg)[N], float (&tu)[N]) {
+// The gate, for 16 features from c on of 32 rows: h (and th), and what a backward reads.
+template <typename T, bool DUAL>
+__device__ __forceinline__ void finish_gated(const PairArgs& p, int row0, int c, int lane, uint8_t* mine, float (&g)[16],
+                                             float (&u)[16], float (&tg)[16], float (&tu)[16]) {
   constexpr bool EXACT = sizeof(T) == 4;
+  constexpr int N = 16;
   if (p.kept && row0 < p.rows && c < p.cols) {
     uint8_t* block = p.kept + (size_t)((row0 >> 5) * ((p.cols + 31) >> 5) + (c >> 5)) * (DUAL ? 4 : 2) * Kept<T>::kBlock;
     keep<T>(block, lane, c & 31, g);
@@ -171,9 +172,9 @@ __device__ __forceinline__ void finish_gated(const PairArgs& p, int row0, int c,
   if constexpr (DUAL) write_rows<T, N>(static_cast<T*>(p.th), p, row0, c, lane, mine, tg);
 }
 
-// A thread's 32 sums of block b among those of its piece.
+// A thread's b-th 16 sums of its piece.
 __device__ __forceinline__ float4* partial_at(const PairArgs& p, int piece, int rank, int warp, int b, int lane) {
-  return reinterpret_cast<float4*>(p.partial + ((((size_t)piece * 2 + rank) * 8 + warp) * 4 + b) * 1024) + lane;
+  return reinterpret_cast<float4*>(p.partial + ((((size_t)piece * 2 + rank) * 8 + warp) * 8 + b) * 512) + lane;
 }
 
 template <typename T>
@@ -204,6 +205,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   const uint32_t rank = cluster_rank();
   const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
 
+  if (threadIdx.x == 32) {
+    for (int i = 0; i < 4; ++i) prefetch_tmap(&maps.a[i]);
+    for (int i = 0; i < 2; ++i) prefetch_tmap(&maps.b[i]);
+  }
   if (threadIdx.x == 0) {
     const int before = *reinterpret_cast<volatile int*>(p.status);
     bar.abort_flag = before;
@@ -310,116 +315,122 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       const Item it = item_at(p, i);
       const int group = it.mt / p.tiles_m, m = it.mt - group * p.tiles_m;
       const int row0 = DUAL ? m * 128 + (int)rank * 64 + (q & 1) * 32 : m * 256 + (int)rank * 128 + q * 32;
-      float sum[PARTS ? 4 : 1][32];
-      uint32_t col = 0;
-      // this thread's 4 x 32 accumulators: gated g, g, u, u of 2 x 32 features, else 128 columns
-      auto column = [&](int b) { return col + (GATED ? (b >> 1) * 128 + half * 64 + (b & 1) * 32 : half * 128 + b * 32); };
       auto release = [&](int buf) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) arrive_in_leader(in_leader(&bar.acc_empty[buf]));
       };
+      // this thread's 128 accumulators: gated 64 of g and the 64 of u that belong to them, else 128 columns
+      uint32_t col = 0;
+      auto column = [&](int c) { return col + (GATED ? (c >> 6) * 128 + half * 64 + (c & 63) : half * 128 + c); };
       if constexpr (PARTS) {
+        float sum[8][16];
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
+        for (int b = 0; b < 8; ++b)
 #pragma unroll
-          for (int j = 0; j < 32; ++j) sum[b][j] = 0.f;
-        for (int done = it.begin; done < it.end; done += p.chunk, ++acc) {
+          for (int j = 0; j < 16; ++j) sum[b][j] = 0.f;
+        for (int done = it.begin; done < it.end; done += p.chunk) {
           const int buf = acc & 1;
           ok = ok && wait_for_sums(&bar.acc_full[buf], acc >> 1 & 1, ab);
-          if (!ok) continue;
+          if (!ok) break;
           tc_fence_after();
           col = lanes + buf * 256;
 #pragma unroll
-          for (int b = 0; b < 8; ++b) {  // (16 at a time: what is left of the registers)
+          for (int b = 0; b < 8; ++b) {
             uint32_t r[16];
-            tmem_ld16(column(b >> 1) + (b & 1) * 16, r);
+            tmem_ld16(column(b * 16), r);
             tmem_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) sum[b >> 1][(b & 1) * 16 + j] += __uint_as_float(r[j]);
+            for (int j = 0; j < 16; ++j) sum[b][j] += __uint_as_float(r[j]);
           }
-          release(buf);
+          if (done + p.chunk < it.end) release(acc++ & 1);
+        }
+        // The sums go back where the last of their terms came from, so that what follows can go through them in a loop.
+        if (ok) {
+#pragma unroll
+          for (int b = 0; b < 8; ++b) tmem_st16(column(b * 16), reinterpret_cast<const uint32_t(&)[16]>(sum[b]));
+          tmem_wait_st();
         }
       } else {
         ok = ok && wait_for_sums(&bar.acc_full[acc & 1], acc >> 1 & 1, ab);
         if (ok) tc_fence_after();
         col = lanes + (acc & 1) * 256;
       }
-      // 32 accumulators of this thread (to be waited for), NaN after a wait that gave up
-      auto take = [&](int b, float (&v)[32]) {
-        if (!ok) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = poison_f32();
-        } else if constexpr (PARTS) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = sum[b][j];
+      // Neighbouring accumulators of this thread (to be waited for), NaN after a wait that gave up.
+      auto take16 = [&](int c, float (&v)[16]) {
+        if (ok) {
+          tmem_ld16(column(c), reinterpret_cast<uint32_t(&)[16]>(v));
         } else {
-          tmem_ld32(column(b), reinterpret_cast<uint32_t(&)[32]>(v));
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = poison_f32();
         }
       };
       auto taken = [&](bool last) {
-        if (PARTS || !ok) return;
+        if (!ok) return;
         tmem_wait_ld();
         if (last) release(acc & 1);
       };
+      // (Loops that stay loops: a CTA of a short call goes through this once, and the time of straight-line code is that of fetching it.)
       if (it.piece >= 0) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          float v[32];
-          take(b, v);
-          taken(b == 3);
+#pragma unroll 1
+        for (int b = 0; b < 8; ++b) {
+          float v[16];
+          take16(b * 16, v);
+          taken(b == 7);
           float4* to = partial_at(p, it.piece, (int)rank, e, b, lane);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) to[j * 32] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          for (int j = 0; j < 4; ++j) to[j * 32] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        }
+      } else if constexpr (DUAL) {
+        // Of 32 features the warp of the value finishes 0 to 15, that of the tangent the others.
+        const bool tangent = q >= 2;
+        const int pair_id = half * 2 + (q & 1);
+        float* const to = reinterpret_cast<float*>(mine) + lane;
+        const float* const from = reinterpret_cast<const float*>(through + (pair_id * 2 + (tangent ? 0 : 1)) * 4096) + lane;
+#pragma unroll 1
+        for (int b = 0; b < 2; ++b) {
+          float g[16], u[16], tg[16], tu[16];  // first what is handed over, of the other's 16 features, then one's own
+          take16(b * 32 + (tangent ? 0 : 16), tg);
+          take16(64 + b * 32 + (tangent ? 0 : 16), tu);
+          take16(b * 32 + (tangent ? 16 : 0), g);
+          take16(64 + b * 32 + (tangent ? 16 : 0), u);
+          taken(b == 1);
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) to[j * 32] = tg[j], to[(16 + j) * 32] = tu[j];
+          asm volatile("bar.sync %0, 64;" ::"r"(1 + pair_id) : "memory");
+#pragma unroll
+          for (int j = 0; j < 16; ++j) tg[j] = from[j * 32], tu[j] = from[(16 + j) * 32];
+          asm volatile("bar.sync %0, 64;" ::"r"(1 + pair_id) : "memory");
+          if (tangent) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float x = g[j], y = u[j];
+              g[j] = tg[j], u[j] = tu[j], tg[j] = x, tu[j] = y;
+            }
+          }
+          finish_gated<T, true>(p, row0, it.nt * 128 + half * 64 + b * 32 + (tangent ? 16 : 0), lane, mine, g, u, tg, tu);
         }
       } else if constexpr (GATED) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const int c = it.nt * 128 + half * 64 + b * 32;
-          float g[32], u[32];
-          take(b, g);
-          take(b + 2, u);
-          taken(b == 1);
-          if constexpr (DUAL) {
-            // The warp of the value finishes features 0 to 15 of the 32, that of the tangent the others.
-            const bool tangent = q >= 2;
-            const int pair_id = half * 2 + (q & 1);
-            float* const to = reinterpret_cast<float*>(mine) + lane;
-            const float* const from = reinterpret_cast<const float*>(through + (pair_id * 2 + (tangent ? 0 : 1)) * 4096) + lane;
-            float own_g[16], own_u[16], got_g[16], got_u[16];
-            __syncwarp();
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              to[j * 32] = tangent ? g[j] : g[16 + j];
-              to[(16 + j) * 32] = tangent ? u[j] : u[16 + j];
-              own_g[j] = tangent ? g[16 + j] : g[j];
-              own_u[j] = tangent ? u[16 + j] : u[j];
-            }
-            asm volatile("bar.sync %0, 64;" ::"r"(1 + pair_id) : "memory");
-#pragma unroll
-            for (int j = 0; j < 16; ++j) got_g[j] = from[j * 32], got_u[j] = from[(16 + j) * 32];
-            asm volatile("bar.sync %0, 64;" ::"r"(1 + pair_id) : "memory");
-            float vg[16], vu[16], vtg[16], vtu[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              vg[j] = tangent ? got_g[j] : own_g[j], vu[j] = tangent ? got_u[j] : own_u[j];
-              vtg[j] = tangent ? own_g[j] : got_g[j], vtu[j] = tangent ? own_u[j] : got_u[j];
-            }
-            finish_gated<T, true, 16>(p, row0, c + (tangent ? 16 : 0), lane, mine, vg, vu, vtg, vtu);
-          } else {
-            finish_gated<T, false, 32>(p, row0, c, lane, mine, g, u, g, u);
-          }
+#pragma unroll 1
+        for (int b = 0; b < 4; ++b) {
+          float g[16], u[16];
+          take16(b * 16, g);
+          take16(64 + b * 16, u);
+          taken(b == 3);
+          finish_gated<T, false>(p, row0, it.nt * 128 + half * 64 + b * 16, lane, mine, g, u, g, u);
         }
       } else {
-#pragma unroll
+#pragma unroll 1
         for (int b = 0; b < 4; ++b) {
           float v[32];
-          take(b, v);
+          take16(b * 32, reinterpret_cast<float(&)[16]>(v[0]));
+          take16(b * 32 + 16, reinterpret_cast<float(&)[16]>(v[16]));
           taken(b == 3);
           write_rows<T, 32>(static_cast<T*>(p.out[group]), p, row0, it.nt * 256 + half * 128 + b * 32, lane, mine, v);
         }
       }
-      if constexpr (!PARTS) ++acc;
+      ++acc;
     }
   }
   __syncwarp();
@@ -439,52 +450,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   cluster_sync();
 }
 
-// The sums of a cut tile's pieces, in their order, and what becomes of them.  A warp takes 32 rows x 32 columns, as one of pair_kernel's did.
+// The sums of a cut tile's pieces, in their order, and what becomes of them.  A warp takes 32 rows x 16 columns, as one of pair_kernel's did.
 constexpr int kJoinWarps = 4;
 template <typename T, int KIND>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ PairArgs p) {
   constexpr bool GATED = KIND <= kPairGatedDual, DUAL = KIND == kPairGatedDual;
-  constexpr int kBlocks = GATED ? 2 : 4, kQ = DUAL ? 2 : 4;  // tasks: tile, rank, half, q, block
-  __shared__ __align__(16) uint8_t through[kJoinWarps * 32 * (32 * sizeof(T) + 16)];
+  constexpr int kBlocks = GATED ? 4 : 8, kQ = DUAL ? 2 : 4;  // tasks: tile, rank, half, q, block
+  constexpr int kBytes = 32 * (16 * sizeof(T) + 16);
+  __shared__ __align__(16) uint8_t through[kJoinWarps * kBytes];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int task = blockIdx.x * kJoinWarps + warp;
   const int b = task % kBlocks, q = task / kBlocks % kQ, half = task / (kBlocks * kQ) % 2, rank = task / (kBlocks * kQ * 2) % 2;
   const int rest = task / (kBlocks * kQ * 4);
   if (rest * p.cut >= p.items - p.whole) return;
-  uint8_t* const mine = through + warp * 32 * (32 * sizeof(T) + 16);
+  uint8_t* const mine = through + warp * kBytes;
   int mt, nt;
   tile_at(p, p.whole + rest, mt, nt);
   const int group = mt / p.tiles_m, m = mt - group * p.tiles_m;
   const int row0 = DUAL ? m * 128 + rank * 64 + q * 32 : m * 256 + rank * 128 + q * 32;
-  const int c = GATED ? nt * 128 + half * 64 + b * 32 : nt * 256 + half * 128 + b * 32;
+  const int c = GATED ? nt * 128 + half * 64 + b * 16 : nt * 256 + half * 128 + b * 16;
   if (row0 >= p.rows || c >= p.cols) return;
-  auto add_up = [&](int q_, int b_, float (&v)[32]) {
+  auto add_up = [&](int q_, int b_, float (&v)[16]) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = 0.f;
+    for (int j = 0; j < 16; ++j) v[j] = 0.f;
+#pragma unroll 2
     for (int k = 0; k < p.cut; ++k) {
       const float4* from = partial_at(p, rest * p.cut + k, rank, half * 4 + q_, b_, lane);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 4; ++j) {
         const float4 x = from[j * 32];
         v[4 * j] += x.x, v[4 * j + 1] += x.y, v[4 * j + 2] += x.z, v[4 * j + 3] += x.w;
       }
     }
   };
   if constexpr (GATED) {
-    float g[32], u[32], tg[DUAL ? 32 : 1], tu[DUAL ? 32 : 1];
+    float g[16], u[16], tg[DUAL ? 16 : 1], tu[DUAL ? 16 : 1];
     add_up(q, b, g);
-    add_up(q, b + 2, u);
+    add_up(q, b + 4, u);
     if constexpr (DUAL) {
       add_up(q + 2, b, tg);
-      add_up(q + 2, b + 2, tu);
-      finish_gated<T, true, 32>(p, row0, c, lane, mine, g, u, tg, tu);
+      add_up(q + 2, b + 4, tu);
+      finish_gated<T, true>(p, row0, c, lane, mine, g, u, tg, tu);
     } else {
-      finish_gated<T, false, 32>(p, row0, c, lane, mine, g, u, g, u);
+      finish_gated<T, false>(p, row0, c, lane, mine, g, u, g, u);
     }
   } else {
-    float v[32];
+    float v[16];
     add_up(q, b, v);
-    write_rows<T, 32>(static_cast<T*>(p.out[group]), p, row0, c, lane, mine, v);
+    write_rows<T, 16>(static_cast<T*>(p.out[group]), p, row0, c, lane, mine, v);
   }
 }
 
@@ -506,7 +519,7 @@ int launch_kind(const PairArgs& p, const PairMaps& maps, cudaStream_t s) {
   kern<<<2 * (p.items < pairs ? p.items : pairs), kPairThreads, smem, s>>>(p, maps);
   const int rc = launched("gated pair_kernel");
   if (rc || p.items == p.whole) return rc;
-  constexpr int tasks = KIND <= kPairGated ? 2 * 4 * 4 : KIND == kPairGatedDual ? 2 * 2 * 4 : 4 * 4 * 4;  // of a tile
+  constexpr int tasks = KIND <= kPairGated ? 4 * 4 * 4 : KIND == kPairGatedDual ? 4 * 2 * 4 : 8 * 4 * 4;  // of a tile
   join_kernel<T, KIND><<<(p.items - p.whole) / p.cut * (tasks / kJoinWarps), kJoinWarps * 32, 0, s>>>(p);
   return launched("gated join_kernel");
 }
