@@ -40,11 +40,12 @@ py::object dual(Tensor value, Tensor tangent, int64_t level) {
   value._set_fw_grad(tangent, /*level=*/0, /*is_inplace_op=*/false);
   return py::cast(value);
 }
-// The tangent in its value's type.
+// The tangent in its value's type, and in memory (torch keeps some that are zero as a shape alone).
 Tensor as_tangent(const Tensor& t, const Tensor& x) {
-  if (!t.defined() || t.scalar_type() == x.scalar_type()) return t;
+  if (!t.defined()) return t;
   NoFunctorch nf;
-  return t.to(x.scalar_type());
+  if (t._is_zerotensor()) return at::zeros(t.sizes(), x.options().requires_grad(false));
+  return t.scalar_type() == x.scalar_type() ? t : t.to(x.scalar_type());
 }
 
 // ---- rotary --------------------------------------------------------------------------------------------------------------
@@ -178,6 +179,9 @@ struct RotaryNode : public Node {
 };
 
 bool rotary_acceptable(const Tensor& q, const Tensor& k, const Tensor& freq, const Tensor& positions) {
+  for (const Tensor* t : {&q, &k})
+    for (int64_t d = 0; t->defined() && d < t->dim(); ++d)
+      if (t->size(d) > INT32_MAX) return false;
   if (q.dim() != 4 || q.layout() != at::kStrided || (q.is_cuda() && dtype_of(q, false) < 0)) return false;
   if (k.defined() && (k.dim() != 4 || k.layout() != at::kStrided || k.scalar_type() != q.scalar_type() || k.device() != q.device() ||
                       k.size(0) != q.size(0) || k.size(2) != q.size(2) || k.size(3) != q.size(3)))
@@ -363,6 +367,7 @@ struct GatedGradNode : public Node {
     if (v[1].defined() || v[2].defined())
       throw std::runtime_error("the gradients of gated_linear with respect to its weights cannot be differentiated a second time");
     if (!v[0].defined()) return out;
+    if (is_wrapped(v[0])) throw std::runtime_error("gated_linear cannot be differentiated a second time under a functorch transform");
     const Tensor x_ = x.unpack(), wg_ = wg.unpack(), wu_ = wu.unpack(), gh_ = gh.unpack();
     const Tensor xp = unwrap(x_), wgp = unwrap(wg_), wup = unwrap(wu_), t = unwrap(v[0]);
     const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1) || task_should_compute_output(2);

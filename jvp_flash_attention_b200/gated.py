@@ -29,7 +29,8 @@ def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, activation: str = "sil
     bfloat16, float16 or float32, of one type and device.  ``activation``: ``"silu"``, ``"sigmoid"``, ``"gelu"`` (exact) or ``"gelu_tanh"``.
     Rows of whole 16-byte pieces (K a multiple of 8) are read in place, others, and float32, through a copy.
 
-    Sums are in 32 bits, and the result is rounded once.  For a backward the projections are kept in 24 bits an entry (float32: 32).  float32 is multiplied as three bfloat16 parts, about 1e-6 relative,
+    Sums are in 32 bits, and the result is rounded once.  For a backward the projections are kept in 24 bits an entry (float32: 32); their
+    cotangents are rounded to x's type, so where one passes float16's 65504 the gradients of its row are not finite.  float32 is multiplied as three bfloat16 parts, about 1e-6 relative,
     whatever ``set_fp32_precision`` says of attention; an infinite entry gives NaN in its row.  Results are the same from run to run.
 
     The weights have no tangents, and their gradients cannot be differentiated again: both are refused.

@@ -89,6 +89,8 @@ def _check(q, k, inv_freq, positions) -> None:
             continue
         if x.dim() != 4:
             raise ValueError(f"{name} must have 4 dimensions (B, H, L, D), got {tuple(x.shape)}")
+        if max(x.shape) >= 2**31:
+            raise ValueError(f"{name} must have less than 2**31 entries along each dimension, got {tuple(x.shape)}")
         if x.dtype not in _lib.DTYPE_ENUM and x.is_cuda:
             raise TypeError(f"unsupported dtype {x.dtype} of {name}; expected bfloat16, float16 or float32")
         if x.dtype != q.dtype:

@@ -232,6 +232,66 @@ def test_a_gradient_penalty():
         assert (a.double() - b).norm() <= 1e-5 * b.norm()
 
 
+def test_projections_beyond_the_types_range():
+    """fp16 gates of 10^5.  h is formed from sums in 32 bits, and the projections are kept with fp32's range; their cotangents are rounded to
+    fp16, as documented, so a row in which one passes 65504 has a gradient that is not finite, and others are as exact as ever."""
+    K, F = 64, 72
+    x, _, wg, wu, gh, _ = _inputs(40, K, F, "fp16", 13)
+    x = (x * 50).half()
+    wg = (wg * 3000).half()  # |g| of 10^5 and more
+    wu = (wu * 1e-4).half()
+    want = [t.double().detach().requires_grad_() for t in (x, wg, wu)]
+    g = want[0] @ want[1].T
+    hw = torch.nn.functional.silu(g) * (want[0] @ want[2].T)
+    assert (g.abs() > 65504).any() and (hw.abs() < 65504).all()
+    for scale in (1.0, 2.0**-8):
+        leaves = [t.detach().requires_grad_() for t in (x, wg, wu)]
+        h = gated_linear(*leaves)
+        assert (h.double() - hw).abs().max() <= 2.0**-10 * hw.abs().max()
+        c = (gh * scale).half()
+        du = (c.double() * torch.nn.functional.silu(g.detach())).abs()
+        grads, ref = torch.autograd.grad(h, leaves, c), torch.autograd.grad(hw, want, c.double(), retain_graph=True)
+        beyond = (du > 65520).any(1)  # (up to there a number rounds to 65504)
+        assert beyond.any() if scale == 1.0 else not (du > 65504).any()
+        assert torch.equal(~grads[0].isfinite().all(1), beyond)
+        dx, rx = grads[0][~beyond].double(), ref[0][~beyond]
+        assert (dx - rx).norm() <= 4 * 2.0**-11 * rx.norm()
+        if scale < 1:
+            for d, r in zip(grads[1:], ref[1:]):
+                inside = r.abs() < 65504  # (the gradients themselves are fp16)
+                assert (d.double() - r)[inside].norm() <= 4 * 2.0**-11 * r[inside].norm()
+
+
+def test_graphs_of_a_call():
+    x, tx, wg, wu, gh, gth = _inputs(20, 64, 48, "bf16", 14)
+    x.requires_grad_(), wg.requires_grad_()
+    h = gated_linear(x, wg, wg)  # one weight for both: its gradient is the sum
+    (dw,) = torch.autograd.grad(h, wg, gh, retain_graph=True)
+    w = wg.detach().double().requires_grad_()
+    p = x.detach().double() @ w.T
+    (ref,) = torch.autograd.grad(torch.nn.functional.silu(p) * p, w, gh.double())
+    assert (dw.double() - ref).norm() <= 2 * 4 * 2.0**-8 * ref.norm()
+    first, second = (torch.autograd.grad(h, x, gh, retain_graph=True)[0] for _ in range(2))
+    assert torch.equal(first, second)
+    torch.autograd.grad(h, x, gh)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(h, x, gh)
+    h = gated_linear(x, wg, wu)
+    with torch.no_grad():
+        wg.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(h, x, gh)
+
+
+def test_a_tangent_that_is_zero():
+    """torch hands some zero tangents over as a shape without memory."""
+    x, _, wg, wu, _, _ = _inputs(20, 64, 48, "bf16", 15)
+    with torch.autograd.forward_ad.dual_level():
+        zero = torch._efficientzerotensor(x.shape, dtype=x.dtype, device=x.device)
+        h, th = torch.autograd.forward_ad.unpack_dual(gated_linear(torch.autograd.forward_ad.make_dual(x, zero), wg, wu))
+    assert torch.equal(h, gated_linear(x, wg, wu)) and not th.any()
+
+
 def test_another_stream_and_captured_graphs():
     x, tx, wg, wu, gh, gth = _inputs(260, 100, 204, "bf16", 8)  # K = 100: copies in the workspace
     want = _run(x, tx, wg, wu, gh, gth, "silu", "jvp_bwd")
