@@ -82,7 +82,7 @@ std::vector<Tensor> launch_rotary(std::vector<Tensor> xs, const std::vector<Orde
     auto launch = rotary_module().attr("_launch");
     for (size_t i = 0; i < xs.size(); ++i)
       if (xs[i].defined())
-        ys[i] = launch(xs[i], freq, or_none(positions), turn.offset, turn.interleaved,
+        ys[i] = launch(primal_of(xs[i]), freq, or_none(positions), turn.offset, turn.interleaved,
                        turn.amplitude, turn.transposed).cast<Tensor>();
     return ys;
   }
@@ -204,10 +204,8 @@ py::object rotary(const Tensor& q_in, const std::optional<Tensor>& k_in, const T
   std::vector<Tensor> xs{q_, k_, q_._fw_grad(0), k_.defined() ? k_._fw_grad(0) : Tensor()};
   if (level >= 0 && !xs[2].defined() && !xs[3].defined()) return py::none();
   // Primals and tangents are taken off the transform's wrappers, the call runs one level down, and the results become dual again.
+  // (Inside a forward-AD level the primals stay dual: the kernels read their memory, the graph has their edges.)
   for (Tensor& x : xs) x = at_level_below(x, level);
-  if (level < 0)
-    for (int i = 0; i < 2; ++i)
-      if (xs[2 + i].defined()) xs[i] = xs[i]._fw_primal(0);
   const Tensor freq = unwrap(freq_in), positions = positions_in ? unwrap(*positions_in) : Tensor();
   for (const Tensor& x : xs)
     if (x.defined() && is_wrapped(x)) return py::none();
@@ -274,7 +272,7 @@ GatedOut launch_gated_fwd(const Tensor& x, const Tensor& tx, const Tensor& wg, c
     py::gil_scoped_acquire gil;
     NoFunctorch nf;
     at::AutoGradMode no_grad(false);
-    py::tuple out = gated_module().attr("_launch_fwd")(x, or_none(tx), wg, wu, activation, keep);
+    py::tuple out = gated_module().attr("_launch_fwd")(primal_of(x), or_none(tx), wg, wu, activation, keep);
     r.h = from_python(out[0]), r.th = from_python(out[1]), r.kept = from_python(out[2]);
     return r;
   }
@@ -475,7 +473,6 @@ py::object gated(const Tensor& x_in, const Tensor& wg_in, const Tensor& wu_in, i
   // (inside torch.func.jvp the function may use the weights as they are, or wrapped at its level without a tangent)
   x = at_level_below(x, level), tx = at_level_below(tx, level);
   const Tensor wg = at_level_below(wg_in, level), wu = at_level_below(wu_in, level);
-  if (level < 0 && tx.defined()) x = x._fw_primal(0);
   for (const Tensor* t : std::initializer_list<const Tensor*>{&x, &tx, &wg, &wu})
     if (t->defined() && is_wrapped(*t)) return py::none();
   if (!gated_acceptable(x, wg, wu)) return py::none();
