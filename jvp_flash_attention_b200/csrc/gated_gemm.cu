@@ -26,8 +26,8 @@ namespace tc5 {
 namespace {
 
 constexpr int kPairThreads = 384;
-template <typename T>
-constexpr int kPairStages = sizeof(T) == 4 ? 5 : 6;  // (fp32: more room for what warps write through)
+template <typename T, int KIND>
+constexpr int kPairStages = sizeof(T) == 4 || KIND == kPairGated ? 5 : 6;  // (5: more room for what warps write through)
 constexpr int kStageBytes = 32768;  // of a CTA: A 128 x 64, B 128 x 64
 constexpr int kExchangeBytes = 32768;  // 4 pairs of warps x two directions x 2 x 16 features x 32 rows
 constexpr int kMinPieceSteps = 4, kMinSavedSteps = 24;
@@ -112,29 +112,57 @@ __device__ __forceinline__ Item item_at(const PairArgs& p, int i) {
   return r;
 }
 
-// N entries of each of 32 rows (a lane has a row) of a row-major matrix, from column c on, through the warp's own shared memory: lanes that
-// write at once write next to each other.
+// Results leave through the warp's own shared memory, 32 rows (a lane has a row) of N entries, so that lanes that write at once write next to
+// each other.  put: 16 entries of a lane's row, from entry `first` on.
 template <typename T, int N>
-__device__ __forceinline__ void write_rows(T* out, const PairArgs& p, int row0, int c, int lane, uint8_t* mine, const float (&v)[N]) {
-  constexpr int E = 16 / sizeof(T), U = N / E, pitch = N * sizeof(T) + 16;
-  __syncwarp();
+constexpr int kRowsBytes = 32 * (N * (int)sizeof(T) + 16);
+template <typename T, int N>
+__device__ __forceinline__ void put(uint8_t* mine, int lane, int first, const float (&v)[16]) {
+  constexpr int E = 16 / sizeof(T), pitch = N * sizeof(T) + 16;
 #pragma unroll
-  for (int k = 0; k < U; ++k) {
+  for (int k = 0; k < 16 / E; ++k) {
     uint4 x;
     if constexpr (sizeof(T) == 4)
       x = make_uint4(__float_as_uint(v[k * 4]), __float_as_uint(v[k * 4 + 1]), __float_as_uint(v[k * 4 + 2]), __float_as_uint(v[k * 4 + 3]));
     else
       x = make_uint4(Elem<T>::pack(v[k * 8], v[k * 8 + 1]), Elem<T>::pack(v[k * 8 + 2], v[k * 8 + 3]),
                      Elem<T>::pack(v[k * 8 + 4], v[k * 8 + 5]), Elem<T>::pack(v[k * 8 + 6], v[k * 8 + 7]));
-    *reinterpret_cast<uint4*>(mine + lane * pitch + k * 16) = x;
+    *reinterpret_cast<uint4*>(mine + lane * pitch + first * sizeof(T) + k * 16) = x;
   }
-  __syncwarp();
-  if (p.aligned) {
+}
+// ... and from there to a row-major matrix, from its column c on: whole 16-byte pieces, or rows that begin anywhere.
+template <typename T, int N, int M>
+__device__ __forceinline__ void write_pieces(T* out, const PairArgs& p, int row0, int c, int lane, const uint8_t* mine) {
+  constexpr int E = 16 / sizeof(T), U = M / E, pitch = N * sizeof(T) + 16;
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int r = (i * 32 + lane) / U, k = (i * 32 + lane) % U;
-      if (row0 + r < p.rows && c + k * E < p.cols)
-        *reinterpret_cast<uint4*>(out + (size_t)(row0 + r) * p.cols + c + k * E) = *reinterpret_cast<const uint4*>(mine + r * pitch + k * 16);
+  for (int i = 0; i < U; ++i) {
+    const int r = (i * 32 + lane) / U, k = (i * 32 + lane) % U;
+    if (row0 + r < p.rows && c + k * E < p.cols)
+      *reinterpret_cast<uint4*>(out + (size_t)(row0 + r) * p.cols + c + k * E) = *reinterpret_cast<const uint4*>(mine + r * pitch + k * 16);
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void write_entries(T* out, const PairArgs& p, int row0, int c, int lane, const uint8_t* mine) {
+  constexpr int pitch = N * sizeof(T) + 16;
+  if constexpr (sizeof(T) == 2) {
+    // Two at a time where a word begins; the lane that has none of a row beginning between words, its ends.
+    uint16_t* const base = reinterpret_cast<uint16_t*>(out);
+#pragma unroll 4
+    for (int i = 0; i < N / 2; ++i) {
+      const int r = (i * 32 + lane) / (N / 2), k = (i * 32 + lane) % (N / 2) * 2;
+      const size_t at = (size_t)(row0 + r) * p.cols + c;
+      const uint16_t* const e = reinterpret_cast<const uint16_t*>(mine + r * pitch);
+      if (row0 + r >= p.rows) continue;
+      const int odd = (int)((reinterpret_cast<uintptr_t>(base) / 2 + at) & 1);
+      if (!odd || k + 2 < N) {
+        if (c + k + odd + 1 < p.cols)
+          *reinterpret_cast<uint32_t*>(base + at + k + odd) = e[k + odd] | (uint32_t)e[k + odd + 1] << 16;
+        else if (c + k + odd < p.cols)
+          base[at + k + odd] = e[k + odd];
+      } else {
+        if (c < p.cols) base[at] = e[0];
+        if (c + N - 1 < p.cols) base[at + N - 1] = e[N - 1];
+      }
     }
   } else {
 #pragma unroll 4
@@ -144,11 +172,20 @@ __device__ __forceinline__ void write_rows(T* out, const PairArgs& p, int row0, 
     }
   }
 }
+template <typename T, int N>
+__device__ __forceinline__ void write_rows(T* out, const PairArgs& p, int row0, int c, int lane, const uint8_t* mine) {
+  __syncwarp();
+  if (p.aligned)
+    write_pieces<T, N, N>(out, p, row0, c, lane, mine);
+  else
+    write_entries<T, N>(out, p, row0, c, lane, mine);
+  __syncwarp();
+}
 
-// The gate, for 16 features from c on of 32 rows: h (and th), and what a backward reads.
+// The gate, for 16 features from c on of 32 rows: what a backward reads, h in place of g and th in place of tg.
 template <typename T, bool DUAL>
-__device__ __forceinline__ void finish_gated(const PairArgs& p, int row0, int c, int lane, uint8_t* mine, float (&g)[16],
-                                             float (&u)[16], float (&tg)[16], float (&tu)[16]) {
+__device__ __forceinline__ void finish_gated(const PairArgs& p, int row0, int c, int lane, float (&g)[16], float (&u)[16], float (&tg)[16],
+                                             float (&tu)[16]) {
   constexpr bool EXACT = sizeof(T) == 4;
   constexpr int N = 16;
   if (p.kept && row0 < p.rows && c < p.cols) {
@@ -168,8 +205,14 @@ __device__ __forceinline__ void finish_gated(const PairArgs& p, int row0, int c,
       g[j] = y.a * u[j];
     }
   });
-  write_rows<T, N>(static_cast<T*>(p.h), p, row0, c, lane, mine, g);
-  if constexpr (DUAL) write_rows<T, N>(static_cast<T*>(p.th), p, row0, c, lane, mine, tg);
+}
+// h and th of finish_gated on their way out.
+template <typename T>
+__device__ __forceinline__ void write_dual(const PairArgs& p, int row0, int c, int lane, uint8_t* mine, const float (&h)[16], const float (&th)[16]) {
+  put<T, 16>(mine, lane, 0, h);
+  write_rows<T, 16>(static_cast<T*>(p.h), p, row0, c, lane, mine);
+  put<T, 16>(mine, lane, 0, th);
+  write_rows<T, 16>(static_cast<T*>(p.th), p, row0, c, lane, mine);
 }
 
 // A thread's b-th 16 sums of its piece.
@@ -188,15 +231,18 @@ struct Operand<float> {
   static constexpr bool kParts = true;
 };
 
+// Entries of a row that a warp has room for.
 template <typename T, int KIND>
-constexpr int kThroughBytes = KIND == kPairGatedDual ? kExchangeBytes : 8 * 32 * (32 * (int)sizeof(T) + 16);
+constexpr int kAtOnce = KIND == kPairGated && sizeof(T) == 2 ? 64 : 32;
+template <typename T, int KIND>
+constexpr int kThroughBytes = KIND == kPairGatedDual ? kExchangeBytes : 8 * kRowsBytes<T, kAtOnce<T, KIND>>;
 
 template <typename T, int KIND>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     pair_kernel(const __grid_constant__ PairArgs p, const __grid_constant__ PairMaps maps) {
   constexpr bool GATED = KIND <= kPairGatedDual, DUAL = KIND == kPairGatedDual, A_MN = KIND == kPairDw, B_MN = KIND >= kPairDx;
   constexpr bool PARTS = Operand<T>::kParts;
-  constexpr int STAGES = kPairStages<T>;
+  constexpr int STAGES = kPairStages<T, KIND>, AT_ONCE = kAtOnce<T, KIND>;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
   uint8_t* through = smem + STAGES * kStageBytes;  // for the warps that write
@@ -308,7 +354,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   } else if (warp >= 4) {
     const int e = warp - 4, q = warp & 3, half = e >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
-    uint8_t* const mine = through + (DUAL ? ((half * 2 + (q & 1)) * 2 + (q >> 1)) * 4096 : e * 32 * (32 * (int)sizeof(T) + 16));
+    uint8_t* const mine = through + (DUAL ? ((half * 2 + (q & 1)) * 2 + (q >> 1)) * 4096 : e * kRowsBytes<T, AT_ONCE>);
     int acc = 0;
     bool ok = !refused;
     for (int i = cluster; i < p.items; i += clusters) {
@@ -409,7 +455,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
               g[j] = tg[j], u[j] = tu[j], tg[j] = x, tu[j] = y;
             }
           }
-          finish_gated<T, true>(p, row0, it.nt * 128 + half * 64 + b * 32 + (tangent ? 16 : 0), lane, mine, g, u, tg, tu);
+          const int c = it.nt * 128 + half * 64 + b * 32 + (tangent ? 16 : 0);
+          finish_gated<T, true>(p, row0, c, lane, g, u, tg, tu);
+          write_dual<T>(p, row0, c, lane, mine, g, tg);
         }
       } else if constexpr (GATED) {
 #pragma unroll 1
@@ -418,16 +466,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           take16(b * 16, g);
           take16(64 + b * 16, u);
           taken(b == 3);
-          finish_gated<T, false>(p, row0, it.nt * 128 + half * 64 + b * 16, lane, mine, g, u, g, u);
+          // Whole pieces leave 32 entries at a time; rows that begin anywhere 64, whole lines of which most sectors are (fp16 M3990 K1024
+          // F2731: 55 -> 49 us; whole pieces of F2736 42 by 32, 44 by 64).
+          const int span = p.aligned ? 32 : AT_ONCE, c = it.nt * 128 + half * 64 + b * 16, first = b * 16 % span;
+          finish_gated<T, false>(p, row0, c, lane, g, u, g, u);
+          put<T, AT_ONCE>(mine, lane, first, g);
+          if (first + 16 == span) {
+            __syncwarp();
+            if (p.aligned)
+              write_pieces<T, AT_ONCE, 32>(static_cast<T*>(p.h), p, row0, c - first, lane, mine);
+            else
+              write_entries<T, AT_ONCE>(static_cast<T*>(p.h), p, row0, c - first, lane, mine);
+            __syncwarp();
+          }
         }
       } else {
 #pragma unroll 1
         for (int b = 0; b < 4; ++b) {
-          float v[32];
-          take16(b * 32, reinterpret_cast<float(&)[16]>(v[0]));
-          take16(b * 32 + 16, reinterpret_cast<float(&)[16]>(v[16]));
+          float v[16], w[16];
+          take16(b * 32, v);
+          take16(b * 32 + 16, w);
           taken(b == 3);
-          write_rows<T, 32>(static_cast<T*>(p.out[group]), p, row0, it.nt * 256 + half * 128 + b * 32, lane, mine, v);
+          put<T, 32>(mine, lane, 0, v);
+          put<T, 32>(mine, lane, 16, w);
+          write_rows<T, 32>(static_cast<T*>(p.out[group]), p, row0, it.nt * 256 + half * 128 + b * 32, lane, mine);
         }
       }
       ++acc;
@@ -456,7 +518,7 @@ template <typename T, int KIND>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ PairArgs p) {
   constexpr bool GATED = KIND <= kPairGatedDual, DUAL = KIND == kPairGatedDual;
   constexpr int kBlocks = GATED ? 4 : 8, kQ = DUAL ? 2 : 4;  // tasks: tile, rank, half, q, block
-  constexpr int kBytes = 32 * (16 * sizeof(T) + 16);
+  constexpr int kBytes = kRowsBytes<T, 16>;
   __shared__ __align__(16) uint8_t through[kJoinWarps * kBytes];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int task = blockIdx.x * kJoinWarps + warp;
@@ -490,14 +552,18 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
     if constexpr (DUAL) {
       add_up(q + 2, b, tg);
       add_up(q + 2, b + 4, tu);
-      finish_gated<T, true>(p, row0, c, lane, mine, g, u, tg, tu);
+      finish_gated<T, true>(p, row0, c, lane, g, u, tg, tu);
+      write_dual<T>(p, row0, c, lane, mine, g, tg);
     } else {
-      finish_gated<T, false>(p, row0, c, lane, mine, g, u, g, u);
+      finish_gated<T, false>(p, row0, c, lane, g, u, g, u);
+      put<T, 16>(mine, lane, 0, g);
+      write_rows<T, 16>(static_cast<T*>(p.h), p, row0, c, lane, mine);
     }
   } else {
     float v[16];
     add_up(q, b, v);
-    write_rows<T, 16>(static_cast<T*>(p.out[group]), p, row0, c, lane, mine, v);
+    put<T, 16>(mine, lane, 0, v);
+    write_rows<T, 16>(static_cast<T*>(p.out[group]), p, row0, c, lane, mine);
   }
 }
 
@@ -510,7 +576,7 @@ int launched(const char* what) {
 
 template <typename T, int KIND>
 int launch_kind(const PairArgs& p, const PairMaps& maps, cudaStream_t s) {
-  constexpr size_t smem = kPairStages<T> * kStageBytes + kThroughBytes<T, KIND> + sizeof(PairBarriers) + 1024;
+  constexpr size_t smem = kPairStages<T, KIND> * kStageBytes + kThroughBytes<T, KIND> + sizeof(PairBarriers) + 1024;
   static_assert(smem <= 232448, "shared memory of a CTA");
   auto kern = pair_kernel<T, KIND>;
   static SmemOptIn opt_in;
