@@ -376,3 +376,58 @@ def test_a_transformer_block_under_one_jvp():
     for a, b in zip(*out):
         # five operators and three library products in a row, each within 1e-5 of its largest entry, and their gradients
         assert (a.double() - b).norm() <= 1e-4 * b.norm()
+
+
+def test_a_captured_training_step():
+    """Rotary in front of the gated projection, value, tangent and gradients, captured once and replayed on other inputs."""
+    side = torch.cuda.Stream()  # (the legacy stream's graph nodes cannot be captured)
+    g = torch.Generator(device=DEV).manual_seed(16)
+    r = lambda *s: torch.randn(*s, generator=g, device=DEV).to(torch.bfloat16)  # noqa: E731
+    q, tq, c, ct = r(2, 3, 50, 64), r(2, 3, 50, 64), r(2, 3, 50, 136), r(2, 3, 50, 136)
+    wg, wu = (r(136, 64) / 8).requires_grad_(), (r(136, 64) / 8).requires_grad_()
+    w = rot.rotary_frequencies(64, device=DEV)
+    leaves = [q.requires_grad_(), tq.requires_grad_(), wg, wu]
+
+    def step():
+        h, th = torch.func.jvp(lambda x: gated_linear(rot.rotary(x, None, w), wg, wu), (q,), (tq,))
+        return [h.detach(), th.detach(), *torch.autograd.grad((h, th), leaves, (c, ct))]
+
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = step()
+        with torch.no_grad():
+            q.copy_(r(*q.shape)), c.copy_(r(*c.shape))
+        graph.replay()
+        first = [t.clone() for t in got]
+        want = step()
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) and torch.equal(a, x) for a, b, x in zip(got, want, first))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("M", [5, 700])
+@pytest.mark.parametrize("step", ["fwd_bwd", "jvp_bwd"])
+def test_a_replay_behind_a_launch_that_gave_up(M, dt, step):
+    """With the status word set (from the host, as a thread that gives up a wait would) replayed kernels write NaN and end; cleared, they are
+    themselves again.  K = 264, F = 2600: of 700 rows dw's tiles are cut, and joined."""
+    args = _inputs(M, 264, 2600, dt, 17)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = _run(*args, "silu", step)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = _run(*args, "silu", step)
+        for code in (9, 0):
+            _lib.device_status_inject(code)
+            try:
+                graph.replay()
+                side.synchronize()
+            finally:
+                assert _lib.device_status(clear=True) == code
+            for name, y in got.items():
+                assert y.isnan().all() if code else torch.equal(y, want[name]), (code, name)
