@@ -4,11 +4,13 @@
 //   dg = gh a' u + gth (a'' tg u + a' tu),  du = gh a + gth a' tg,  dtg = gth a' u,  dtu = gth a,
 // bound by memory (12 bytes an entry for the value of a 16-bit tensor: gh, 3 each for g and u, dg, du), then a product over the features for dx and dtx, and one over
 // the rows for dwg and dwu.  Tangents are further rows of the first (dx beside dtx, the weights shared) and further depth of the second.
+// The pass, measured on a B200: bf16 M8192 F11008 171 us = 6.3 TB/s, with tangents (24 bytes an entry) M8192 F2736 86 us = 6.2; rows that are no whole
+// pieces, fp16 M3990 F2731, 24.5 us instead of 20.5.
 //
 // Up to 128 rows (value and tangent together) the forward and dx are the kernels of gated_few.cu.
 //
 // Operands go to the tensor cores by TMA, which takes rows of whole 16-byte pieces; others are copied once into the workspace with padded
-// rows.  fp32 operands become three planes of bf16 parts there (f32_tc5_common.cuh).
+// rows.  fp32 operands become three planes of bf16 parts there (f32_tc5_common.cuh): both weights of K4096 F11008 152 us = 5.9 TB/s.
 #include <algorithm>
 #include <initializer_list>
 

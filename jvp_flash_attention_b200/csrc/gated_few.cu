@@ -11,6 +11,10 @@
 // (a copy of the parts in memory would be written and read again, four times the bytes).  The tensor cores round towards zero at every
 // step of 16, so those warps take the sums up in registers every 4 k-blocks, while the next go to another accumulator; and the five lesser
 // products of parts have accumulators of their own, where what is rounded away is that much smaller.
+//
+// Bound by memory, the weights read once.  Measured on a B200: one row of bf16 K4096 F11008 35 us = 5.2 TB/s, 32 rows 39, 100 rows 46; 24 rows with
+// tangent of fp16 K1024 F2736 9.4 us (two CTAs of 108 KB of stages an SM; one of 216 KB: 55 and 14.9 us).  fp32 one row of K4096 F11008
+// 148 us = 2.4 TB/s: five rounds of CTAs that each begin and end, and 24 products and a splitting to a k-block.
 #include "gated_common.cuh"
 
 namespace jvpfa {
