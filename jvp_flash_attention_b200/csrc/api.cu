@@ -200,6 +200,8 @@ int check_bwd_request(const jvpfa_bwd_args* a) {
 static int check_gated(int dtype, int M, int K, int F, int activation) {
   if (dtype != JVPFA_BF16 && dtype != JVPFA_FP16 && dtype != JVPFA_FP32) return JVPFA_ERR_DTYPE;
   if (M < 1 || K < 1 || F < 1) return JVPFA_ERR_SHAPE;
+  constexpr int kMost = 2147483647 - 4096;  // rows and columns of the last tile are counted in 32 bits
+  if (M > kMost || K > kMost || F > kMost) return JVPFA_ERR_TOO_LARGE;
   if (activation < JVPFA_ACT_SILU || activation > JVPFA_ACT_GELU_TANH) return JVPFA_ERR_UNSUPPORTED;
   return JVPFA_OK;
 }

@@ -14,19 +14,13 @@ struct Activated {
   float a, d1, d2;
 };
 // sigmoid(x) and sigmoid(-x), each with its own relative precision: neither is one minus the other.
+// (exp(-|x|) cannot overflow: gates of any size have their limits, and NaN stays NaN.)
 template <bool EXACT>
 __device__ __forceinline__ void sigmoids(float x, float& s, float& r) {
-  if constexpr (EXACT) {
-    const float e = expf(-fabsf(x)), big = 1.f / (1.f + e), small = e * big;
-    s = x >= 0.f ? big : small;
-    r = x >= 0.f ? small : big;
-  } else {
-    float y = x;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(-80.f));  // exp(80) and its reciprocal are normal numbers
-    const float e = fast_exp(-y);
-    s = __fdividef(1.f, 1.f + e);
-    r = e * s;
-  }
+  const float e = EXACT ? expf(-fabsf(x)) : fast_exp(-fabsf(x));
+  const float big = EXACT ? 1.f / (1.f + e) : __fdividef(1.f, 1.f + e), small = e * big;
+  s = x >= 0.f ? big : small;
+  r = x >= 0.f ? small : big;
 }
 template <int KIND, bool EXACT>
 __device__ __forceinline__ Activated activate(float g) {

@@ -153,7 +153,9 @@ int launch_rotary(const jvpfa_rotary_args& a, cudaStream_t s) {
   for (int t = 0; t < a.n_tensors; ++t) {
     const jvpfa_rotary_tensor& x = a.t[t];
     all |= (reinterpret_cast<uint64_t>(x.x) | reinterpret_cast<uint64_t>(x.y)) / size;
-    for (int d = 0; d < 3; ++d) all |= (uint64_t)x.x_stride[d] | (uint64_t)x.y_stride[d];
+    const bool counts[3] = {a.B > 1, x.H > 1, a.L > 1};  // (the stride of a single entry is nothing's)
+    for (int d = 0; d < 3; ++d)
+      if (counts[d]) all |= (uint64_t)x.x_stride[d] | (uint64_t)x.y_stride[d];
   }
   if (a.dtype == JVPFA_FP32) return all % 4 == 0 ? launch<float, 4>(a, s) : launch<float, 1>(a, s);
   const bool bf16 = a.dtype == JVPFA_BF16;

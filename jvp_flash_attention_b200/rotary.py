@@ -47,8 +47,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str | No
         return w / factor
     if scaling not in ("ramp", "bands"):
         raise ValueError("scaling is None, 'linear', 'base', 'ramp' or 'bands'")
-    if not quick > slow > 0:
-        raise ValueError("quick has to be above slow, and slow positive")
+    if not quick > slow > 0 or not base > 1:
+        raise ValueError("quick has to be above slow, slow positive and base above 1")
     if scaling == "bands":
         keep = (original_length * w / (2 * math.pi) - slow) / (quick - slow)
     else:

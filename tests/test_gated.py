@@ -175,7 +175,7 @@ def _bwd_args(**kw):
 def test_the_c_entries_refuse():
     lib = _lib.load()
     assert lib.jvpfa_gated_fwd(None, None) == -1 and lib.jvpfa_gated_bwd(None, None) == -1
-    common = [(-7, dict(struct_size=4)), (-3, dict(dtype=3)), (-2, dict(M=0)), (-2, dict(K=0)), (-2, dict(F=0)), (-9, dict(activation=4)),
+    common = [(-7, dict(struct_size=4)), (-3, dict(dtype=3)), (-2, dict(M=0)), (-10, dict(M=2**31 - 1)), (-10, dict(F=2**31 - 4000)), (-2, dict(K=0)), (-2, dict(F=0)), (-9, dict(activation=4)),
               (-9, dict(activation=-1)), (-1, dict(x=None)), (-1, dict(wg=None)), (-1, dict(wu=None)), (-8, dict(x=257)), (-2, dict(x_stride=-8))]
     for want, kw in common + [(-1, dict(h=None)), (-8, dict(h=264)), (-1, dict(tx=256)), (-1, dict(th=256)), (-8, dict(kept=264)),
                               (-1, dict(x=258)), (-1, dict(dtype=2))]:  # the last two need a workspace

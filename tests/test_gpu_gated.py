@@ -201,6 +201,25 @@ def test_far_arguments(name, dt):
     _check(got, x, tx, wg, wu, g, g, ACTIVATIONS[name])
 
 
+@pytest.mark.parametrize("name", list(ACTIVATIONS))
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_arguments_at_the_end_of_the_range(name, dt):
+    """Gates of +-1e12 and (but for the tanh form, whose cube is not finite there) +-1e30: a and a' have their limits, 0 and g, 0 and 1; for the sigmoid 0
+    and 1, 0 and 0."""
+    x = torch.zeros(4, 8, device=DEV, dtype=DT[dt])
+    far = 1e12 if name == "gelu_tanh" else 1e30
+    x[:, 0] = torch.tensor([-1e12, 1e12, -far, far], device=DEV)
+    x[:, 1] = 1
+    w = torch.zeros(2, 64, 8, device=DEV, dtype=DT[dt])
+    w[0, :, 0], w[1, :, 1] = 1, 1
+    tx = torch.zeros_like(x)
+    tx[:, 0] = 1
+    h, th = torch.func.jvp(lambda v: gated_linear(v, w[0], w[1], name), (x,), (tx,))
+    up = torch.tensor([0.0, 1.0, 0.0, 1.0], device=DEV)[:, None].expand(4, 64).to(DT[dt])
+    assert torch.equal(h, up if name == "sigmoid" else up * x[:, :1].clamp_min(0))
+    assert torch.equal(th, torch.zeros_like(up) if name == "sigmoid" else up)
+
+
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])
 def test_nan_and_infinite_entries_stay_in_their_rows(dt):
     x, tx, wg, wu, gh, _ = _inputs(300, 64, 200, dt, 5)

@@ -110,7 +110,8 @@ def test_frequencies(rd):
 
 
 @pytest.mark.parametrize("bad", [dict(rotary_dim=3), dict(rotary_dim=-2), dict(rotary_dim=8, base=0.0), dict(rotary_dim=8, factor=-1.0),
-                                 dict(rotary_dim=8, scaling="other"), dict(rotary_dim=8, scaling="ramp", quick=1.0, slow=2.0)])
+                                 dict(rotary_dim=8, scaling="other"), dict(rotary_dim=8, scaling="ramp", quick=1.0, slow=2.0),
+                                 dict(rotary_dim=8, scaling="ramp", base=1.0)])
 def test_frequencies_that_are_refused(bad):
     with pytest.raises(ValueError):
         rot.rotary_frequencies(**bad)
