@@ -26,8 +26,6 @@ struct Piece;
 template <>
 struct Piece<16> { using type = uint4; };
 template <>
-struct Piece<8> { using type = uint2; };
-template <>
 struct Piece<4> { using type = uint32_t; };
 template <>
 struct Piece<2> { using type = uint16_t; };

@@ -215,12 +215,12 @@ class _GatedGrad(Function):
 
 
 class _GatedDualGrad(Function):
-    """(dx, dtx, dwg, dwu) of <gh, h> + <gth, th>."""
+    """(dx, dtx, dwg, dwu) of <gth, th>."""
 
     @staticmethod
-    def forward(x, tx, w_gate, w_up, kept, gh, gth, activation):
-        tensors = [None if t is None else _unwrap(t) for t in (x, tx, w_gate, w_up, kept, gh, gth)]
-        return _launch_bwd(*tensors, activation, True, True, True)
+    def forward(x, tx, w_gate, w_up, kept, gth, activation):
+        x, tx, w_gate, w_up, kept, gth = (_unwrap(t) for t in (x, tx, w_gate, w_up, kept, gth))
+        return _launch_bwd(x, tx, w_gate, w_up, kept, None, gth, activation, True, True, True)
 
     @staticmethod
     def setup_context(ctx, inputs, outputs):
@@ -232,8 +232,12 @@ class _GatedDualGrad(Function):
 
 
 def _backward_under_functorch(x, tx, w_gate, w_up, kept, gh, gth, activation):
-    """The native layer's backward where a cotangent is a tensor of a functorch transform: Functions take part in it."""
+    """The native layer's backward where a cotangent is a tensor of a functorch transform: Functions take part in it, the part through h in one
+    that can be differentiated again."""
+    dx = dtx = dwg = dwu = None
     if gth is not None:
-        return _GatedDualGrad.apply(x, tx, w_gate, w_up, kept, gh, gth, activation)
-    dx, dwg, dwu = _GatedGrad.apply(x, tx, w_gate, w_up, kept, gh, activation)
-    return dx, None, dwg, dwu
+        dx, dtx, dwg, dwu = _GatedDualGrad.apply(x, tx, w_gate, w_up, kept, gth, activation)
+    if gh is not None:
+        part = _GatedGrad.apply(x, tx, w_gate, w_up, kept, gh, activation)
+        dx, dwg, dwu = part if dx is None else (a + b for a, b in zip((dx, dwg, dwu), part))
+    return dx, dtx, dwg, dwu

@@ -101,6 +101,32 @@ def test_nested_transforms_take_the_general_route(cpu_kernels):
                                torch.func.grad(lambda a: (torch.func.grad(plain)(a) * tx).sum())(x))
 
 
+@pytest.mark.parametrize("outputs", ["h", "both"])
+def test_a_functorch_transform_of_the_cotangent(cpu_kernels, monkeypatch, outputs):
+    """d/dc <dx(c), v> of a graph built outside the transform is th along v; through the tangent it is refused."""
+    def plain(launch):
+        def run(*args):
+            with torch.no_grad(), _lib.native().NoFunctorch():
+                return launch(*(gated._unwrap(t).detach() if isinstance(t, torch.Tensor) else t for t in args))
+        return run
+
+    monkeypatch.setattr(gated, "_launch_fwd", plain(formulas.launch_gated_fwd))
+    monkeypatch.setattr(gated, "_launch_bwd", plain(formulas.launch_gated_bwd))
+    x, tx, wg, wu, gh, gth = _inputs(11)
+    v = _inputs(12)[0]
+    x.requires_grad_()
+    if outputs == "h":
+        outs = (gated_linear(x, wg, wu),)
+    else:
+        outs = torch.func.jvp(lambda a: gated_linear(a, wg, wu), (x,), (tx,))
+    grad = lambda cots: torch.autograd.grad(outs, x, cots, retain_graph=True, create_graph=True)[0]  # noqa: E731
+    got = torch.func.grad(lambda c: (grad((c, gth)[:len(outs)]) * v).sum())(gh)
+    torch.testing.assert_close(got, formulas.gated_fwd(x.detach(), v, wg, wu, 0)[1])
+    if outputs == "both":
+        with pytest.raises(RuntimeError, match="cannot be differentiated a second time"):
+            torch.func.grad(lambda c: (grad((gh, c)) * v).sum())(gth)
+
+
 def test_only_what_is_asked_for_is_computed(cpu_kernels):
     x, tx, wg, wu, gh, gth = _inputs(6)
     gated_linear(x, wg, wu)

@@ -85,7 +85,16 @@ def test_nested_transforms_take_the_general_route(cpu_turn):
     torch.testing.assert_close(t, formulas.turn(6 * y * ty, W, transposed=True))
 
 
-def test_the_order_of_memory_is_kept(cpu_turn):
+def test_a_functorch_transform_of_the_cotangent(cpu_turn):
+    """A graph built outside the transform: the gradient is linear in its cotangent."""
+    q, k = _qk(11)
+    g, v, u = _qk(12)[0], _qk(13)[0], _qk(14)[1]
+    yq, yk = rot.rotary(q.requires_grad_(), k.requires_grad_(), W)
+    vjp = lambda c: torch.autograd.grad((yq, yk), q, (c, u), retain_graph=True, create_graph=True)[0]  # noqa: E731
+    torch.testing.assert_close(torch.func.grad(lambda c: (vjp(c) * v).sum())(g), formulas.turn(v, W))
+
+
+def test_nothing_to_turn(cpu_turn):
     assert rot.rotary(_qk(8)[0], None, W[:0]).shape == (B, H, L, D)
 
 
