@@ -179,7 +179,8 @@ struct FewArgs {
   const void *wg, *wu;       // fp32: read as they are
   int64_t wg_stride, wu_stride;
   bool pieces;               // ... and in whole 16-byte pieces
-  int padded, kblocks, steps, tiles, cluster, stages, tmem_columns;
+  int padded, kblocks, steps, tiles, stages, tmem_columns;
+  int first, whole, cluster;  // tiles from `first` on; those of whole rounds, one CTA each; CTAs of each of the others
   void *out[2], *h, *th;
   uint8_t* kept;
   int activation;

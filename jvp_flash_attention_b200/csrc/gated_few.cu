@@ -28,7 +28,6 @@ constexpr int kFewThreads = sizeof(T) == 4 ? 640 : 384;
 constexpr int kSplitThreads = 512, kUnits = 1024 / kSplitThreads;  // fp32: a k-block's 1024 pieces of eight entries
 constexpr int kAbortFewFull = 18, kAbortFewEmpty = 19, kAbortFewAcc = 20, kAbortFewAccEmpty = 21;
 constexpr int kTakeUp = 4;   // fp32: k-blocks between two looks at the accumulators
-constexpr int kFewOpen = 6;    // fp32: what beginning and ending a CTA's share costs, in k-blocks
 constexpr int kTile = 16384;  // 128 x 64 weights, 16 bits
 
 struct FewBarriers {
@@ -135,7 +134,7 @@ __global__ void __launch_bounds__(kFewThreads<T>, 1) few_kernel(const __grid_con
   const int stage_bytes = PARTS * (kTile + rows_bytes);  // weights, then rows, part by part
   FewBarriers& bar = *reinterpret_cast<FewBarriers*>(smem + p.stages * stage_bytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = p.cluster > 1 ? (int)few_rank() : 0, tile = (int)blockIdx.x / p.cluster;
+  const int rank = p.cluster > 1 ? (int)few_rank() : 0, tile = p.first + (int)blockIdx.x / p.cluster;
   const int begin = (int)((long long)p.steps * rank / p.cluster), end = (int)((long long)p.steps * (rank + 1) / p.cluster);
 
   if (threadIdx.x == 0) {
@@ -362,10 +361,8 @@ __global__ void __launch_bounds__(kFewThreads<T>, 1) few_kernel(const __grid_con
   }
 }
 
-template <typename T, int KIND, bool BIG = false>
-int launch_kind(const FewArgs& p, const FewMaps& maps, cudaStream_t s) {
-  if constexpr (sizeof(T) == 4 && !BIG)
-    if (p.padded * p.groups > 64) return launch_kind<T, KIND, true>(p, maps, s);
+template <typename T, int KIND, bool BIG>
+int launch_tiles(const FewArgs& p, const FewMaps& maps, cudaStream_t s) {
   constexpr int PARTS = FewOperand<T>::kParts;
   const size_t smem = (size_t)p.stages * PARTS * (kTile + p.padded * p.groups * 128) + sizeof(FewBarriers) + 1024;
   auto kern = few_kernel<T, KIND, BIG>;
@@ -389,6 +386,20 @@ int launch_kind(const FewArgs& p, const FewMaps& maps, cudaStream_t s) {
   return JVPFA_ERR_CUDA;
 }
 
+template <typename T, int KIND>
+int launch_kind(const FewArgs& planned, const FewMaps& maps, cudaStream_t s) {
+  auto launch = [&](int first, int tiles, int cluster) {
+    FewArgs p = planned;
+    p.first = first, p.tiles = tiles, p.cluster = cluster;
+    if constexpr (sizeof(T) == 4)
+      if (p.padded * p.groups > 64) return launch_tiles<T, KIND, true>(p, maps, s);
+    return launch_tiles<T, KIND, false>(p, maps, s);
+  };
+  int rc = planned.whole ? launch(0, planned.whole, 1) : JVPFA_OK;
+  if (!rc && planned.tiles > planned.whole) rc = launch(planned.whole, planned.tiles - planned.whole, planned.cluster);
+  return rc;
+}
+
 }  // namespace
 
 bool plan_few(int dtype, int kind, FewArgs& p) {
@@ -404,18 +415,14 @@ bool plan_few(int dtype, int kind, FewArgs& p) {
   // fp32: one CTA an SM, whose registers hold what is under way; else two, of some 100 KB of stages each
   const int stage = parts * (kTile + N * 128), room = parts > 1 ? 224 * 1024 : 108 * 1024;
   p.stages = room / stage < 8 ? room / stage : 8;
-  // CTAs of a tile.  16 bits: as many as find room at once, for memory sets the pace whoever asks for what.  fp32, where a CTA has an SM
-  // to itself and splitting costs as much as loading: so many that the SMs' rounds are the shortest, in k-blocks.
+  // CTAs of a tile: as many as find room at once.  fp32, where a CTA has an SM to itself: tiles by whole rounds of the SMs first, in a launch of
+  // their own, so that a last round of few does not take as long as one of all.
+  const int at_once = parts > 1 ? device_sms() : 2 * device_sms();
+  p.first = 0;
+  p.whole = parts > 1 ? p.tiles / at_once * at_once : 0;
+  const int rest = p.tiles - p.whole;
   p.cluster = 1;
-  if (parts == 1) {
-    while (p.cluster < 8 && p.tiles * 2 * p.cluster <= 2 * device_sms() && 4 * p.cluster <= p.steps) p.cluster *= 2;
-  } else {
-    long long best = -1;
-    for (int c = 1; c <= 8 && (c == 1 || 2 * c <= p.steps); c *= 2) {
-      const long long rounds = ((long long)p.tiles * c + device_sms() - 1) / device_sms(), blocks = rounds * ((p.steps + c - 1) / c + kFewOpen);
-      if (best < 0 || blocks < best) best = blocks, p.cluster = c;
-    }
-  }
+  while (p.cluster < 8 && rest * 2 * p.cluster <= at_once && 4 * p.cluster <= p.steps) p.cluster *= 2;
   p.tmem_columns = 32;
   while (p.tmem_columns < (parts > 1 ? 4 : 1) * N) p.tmem_columns *= 2;
   return true;
