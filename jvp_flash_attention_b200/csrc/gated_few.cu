@@ -14,7 +14,7 @@
 //
 // Bound by memory, the weights read once.  Measured on a B200: one row of bf16 K4096 F11008 35 us = 5.2 TB/s, 32 rows 39, 100 rows 46; 24 rows with
 // tangent of fp16 K1024 F2736 9.4 us (two CTAs of 108 KB of stages an SM; one of 216 KB: 55 and 14.9 us).  fp32 one row of K4096 F11008
-// 148 us = 2.4 TB/s: five rounds of CTAs that each begin and end, and 24 products and a splitting to a k-block.
+// 106 us = 3.4 TB/s, 100 rows 120: 24 products and a splitting to a k-block keep the shared-memory port busy (all tiles cut alike, in five rounds: 148).
 #include "gated_common.cuh"
 
 namespace jvpfa {

@@ -352,9 +352,10 @@ GatedGrads launch_gated_bwd(const Tensor& x, const Tensor& tx, const Tensor& wg,
   return r;
 }
 
-// (dx, dwg, dwu) of <gh, h> as a node that can be differentiated once more, along x: with v the incoming gradient of dx,
-//   d<dx, v>/d(x, wg, wu) = d<th(x; v), gh>/d(x, wg, wu)   and   d<dx, v>/d(gh) = th(x; v),
-// one value-and-tangent forward and one backward through the tangent.
+// (dx, dwg, dwu) of <gh, h> as a node that can be differentiated once more: with v the incoming gradients,
+//   d<(dx, dwg, dwu), v>/d(x, wg, wu) = d<th(x, wg, wu; v), gh>/d(x, wg, wu)   and   d<(dx, dwg, dwu), v>/d(gh) = th(x, wg, wu; v),
+// one value-and-tangent forward and one backward through the tangent (of operands side by side, which the Python module makes, where the
+// weights' gradients are differentiated).
 struct GatedGradNode : public Node {
   int activation;
   SavedVariable x, wg, wu, gh;
@@ -362,21 +363,29 @@ struct GatedGradNode : public Node {
   variable_list apply(variable_list&& v) override {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(4);
-    if (v[1].defined() || v[2].defined())
-      throw std::runtime_error("the gradients of gated_linear with respect to its weights cannot be differentiated a second time");
-    if (!v[0].defined()) return out;
-    if (is_wrapped(v[0])) throw std::runtime_error("gated_linear cannot be differentiated a second time under a functorch transform");
+    if (!v[0].defined() && !v[1].defined() && !v[2].defined()) return out;
+    for (const Tensor& t : v)
+      if (t.defined() && is_wrapped(t)) throw std::runtime_error("gated_linear cannot be differentiated a second time under a functorch transform");
     const Tensor x_ = x.unpack(), wg_ = wg.unpack(), wu_ = wu.unpack(), gh_ = gh.unpack();
-    const Tensor xp = unwrap(x_), wgp = unwrap(wg_), wup = unwrap(wu_), t = unwrap(v[0]);
+    const Tensor xp = unwrap(x_), wgp = unwrap(wg_), wup = unwrap(wu_);
     const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1) || task_should_compute_output(2);
-    const GatedOut f = launch_gated_fwd(xp, t, wgp, wup, activation, need_x || need_w);
-    if (need_x || need_w) {
-      const GatedGrads g = launch_gated_bwd(xp, t, wgp, wup, f.kept, Tensor(), unwrap(gh_), activation, need_x, false, need_w);
-      out[0] = g.dx, out[1] = g.dwg, out[2] = g.dwu;
+    if (v[1].defined() || v[2].defined()) {
+      py::gil_scoped_acquire gil;
+      NoFunctorch nf;
+      at::AutoGradMode no_grad(false);
+      py::tuple h = gated_module().attr("_second")(xp, wgp, wup, unwrap(gh_), or_none(v[0]), or_none(v[1]), or_none(v[2]), activation);
+      for (int i = 0; i < 4; ++i)
+        if (task_should_compute_output(i)) out[i] = from_python(h[i]);
+    } else {
+      const GatedOut f = launch_gated_fwd(xp, v[0], wgp, wup, activation, need_x || need_w);
+      if (need_x || need_w) {
+        const GatedGrads g = launch_gated_bwd(xp, v[0], wgp, wup, f.kept, Tensor(), unwrap(gh_), activation, need_x, false, need_w);
+        out[0] = g.dx, out[1] = g.dwg, out[2] = g.dwu;
+      }
+      if (task_should_compute_output(3)) out[3] = f.th;
     }
-    if (task_should_compute_output(3)) out[3] = f.th;
     if (at::GradMode::is_enabled())
-      attach_refusal("gated_linear cannot be differentiated a third time", {&out[0], &out[1], &out[2], &out[3]}, x_, wg_, wu_, gh_, v[0]);
+      attach_refusal("gated_linear cannot be differentiated a third time", {&out[0], &out[1], &out[2], &out[3]}, x_, wg_, wu_, gh_, v[0], v[1], v[2]);
     return out;
   }
   void release_variables() override {

@@ -3,7 +3,7 @@ products, the activation and the gate.
 
 ``gated_linear`` is to such a block what ``JVPAttn.fwd_dual`` is to attention: where x carries a tangent (``torch.func.jvp``, forward-AD
 dual tensors) value and tangent come from one launch, and the gradient goes through both, to x, its tangent and the weights.  The
-gradient of the value can be differentiated once more along x (Hessian-vector products, gradient penalties).  What follows in a block,
+gradient of the value can be differentiated once more (Hessian-vector products, gradient penalties).  What follows in a block,
 the product with the narrowing weights, is ``torch.nn.functional.linear``.  No upstream counterpart: upstream leaves it to the model.
 """
 from __future__ import annotations
@@ -33,7 +33,8 @@ def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, activation: str = "sil
     cotangents are rounded to x's type, so where one passes float16's 65504 the gradients of its row are not finite.  float32 is multiplied as three bfloat16 parts, about 1e-6 relative,
     whatever ``set_fp32_precision`` says of attention; an infinite entry gives NaN in its row.  Results are the same from run to run.
 
-    The weights have no tangents, and their gradients cannot be differentiated again: both are refused.
+    Tangents of the weights, and a second differentiation of their gradients, run on operands side by side, ``[tx | x]`` and ``[w | tw]``,
+    at twice the depth; the gradient through the tangent output cannot be differentiated again.
     """
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation is one of {', '.join(ACTIVATIONS)}; got {activation!r}")
@@ -45,6 +46,11 @@ def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, activation: str = "sil
         out = _lib.native().gated(x, w_gate, w_up, act)
         if out is not None:
             return out
+        if any(fwAD.unpack_dual(w).tangent is not None for w in (w_gate, w_up)):
+            _check(x, w_gate, w_up)
+            (x, tx), (w_gate, t_gate), (w_up, t_up) = (fwAD.unpack_dual(t) for t in (x, w_gate, w_up))
+            x, tx, w_gate, w_up = _side_by_side(x, tx, w_gate, t_gate, w_up, t_up)
+            return gated_linear(fwAD.make_dual(x, tx), w_gate, w_up, activation)
     _check(x, w_gate, w_up)
     return _Gated.apply(x, w_gate, w_up, act)[0]
 
@@ -64,9 +70,29 @@ def _check(x, w_gate, w_up) -> None:
             raise TypeError(f"x, w_gate and w_up must have one dtype, got {x.dtype} and {t.dtype}")
         if t.device != x.device:
             raise ValueError(f"x, w_gate and w_up must be on one device, got {x.device} and {t.device}")
-    if any(fwAD.unpack_dual(w).tangent is not None for w in (w_gate, w_up)):
-        raise NotImplementedError("gated_linear has no tangent with respect to its weights")
     _require_cuda(x, w_gate, w_up)
+
+
+def _side_by_side(x, tx, w_gate, t_gate, w_up, t_up):
+    """Operands of twice the width with the same value and, in the tangent, the weights' part as well:
+    ``[x | 0] [w | tw]^T = x w^T`` and ``[tx | x] [w | tw]^T = tx w^T + x tw^T``."""
+    or_zero = lambda t, like: torch.zeros_like(like) if t is None else t.to(like.dtype)  # noqa: E731
+    cat = lambda a, b: torch.cat((a, b), -1)  # noqa: E731
+    return (cat(x, torch.zeros_like(x)), cat(or_zero(tx, x), x), cat(w_gate, or_zero(t_gate, w_gate)), cat(w_up, or_zero(t_up, w_up)))
+
+
+def _second(x, w_gate, w_up, gh, vx, v_gate, v_up, activation):
+    """The gradients of <(dx, dwg, dwu), (vx, v_gate, v_up)> with respect to x, w_gate, w_up and gh, where (dx, dwg, dwu) are those of <gh, h>: of
+    <gh, th> for the tangents v, and th itself."""
+    K = x.shape[-1]
+    if v_gate is None and v_up is None:
+        _, th, kept = _launch_fwd(x, vx, w_gate, w_up, activation, True)
+        dx, _, dwg, dwu = _launch_bwd(x, vx, w_gate, w_up, kept, None, gh, activation, True, False, True)
+        return dx, dwg, dwu, th
+    wide = _side_by_side(x, vx, w_gate, v_gate, w_up, v_up)
+    _, th, kept = _launch_fwd(*wide, activation, True)
+    dx, dtx, dwg, dwu = _launch_bwd(*wide, kept, None, gh, activation, True, True, True)
+    return dx[..., :K] + dtx[..., K:], dwg[:, :K], dwu[:, :K], th
 
 
 # ---- the general route (functorch transforms other than a lone torch.func.jvp) --------------------------------------------
@@ -147,9 +173,9 @@ class _Gated(Function):
 
     @staticmethod
     def jvp(ctx, tx, t_gate, t_up, *_):
-        if t_gate is not None or t_up is not None:
-            raise NotImplementedError("gated_linear has no tangent with respect to its weights")
         x, w_gate, w_up = ctx.saved_tensors
+        if t_gate is not None or t_up is not None:
+            x, tx, w_gate, w_up = _side_by_side(x, tx, w_gate, t_gate, w_up, t_up)
         return (None if tx is None else _GatedTangent.apply(x, tx.to(x.dtype), w_gate, w_up, ctx.activation)[0]), None
 
     @staticmethod
@@ -185,7 +211,7 @@ class _GatedTangent(Function):
 
 
 class _GatedGrad(Function):
-    """(dx, dwg, dwu) of <gh, h>, differentiable once more along x (see GatedGradNode in csrc/native_block.cpp).  ``tx``: of the forward that
+    """(dx, dwg, dwu) of <gh, h>, differentiable once more.  ``tx``: of the forward that
     left ``kept``, or None."""
 
     @staticmethod
@@ -203,14 +229,10 @@ class _GatedGrad(Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, vx, v_gate, v_up):
-        if v_gate is not None or v_up is not None:
-            raise RuntimeError("the gradients of gated_linear with respect to its weights cannot be differentiated a second time")
-        if vx is None:
+        if vx is None and v_gate is None and v_up is None:
             return (None,) * 7
-        x, w_gate, w_up, gh = (_unwrap(t) for t in ctx.saved_tensors)
-        vx = _unwrap(vx).to(x.dtype)
-        _, th, kept = _launch_fwd(x, vx, w_gate, w_up, ctx.activation, True)
-        dx, _, dwg, dwu = _launch_bwd(x, vx, w_gate, w_up, kept, None, gh, ctx.activation, True, False, True)
+        tensors = [None if t is None else _unwrap(t) for t in (*ctx.saved_tensors, vx, v_gate, v_up)]
+        dx, dwg, dwu, th = _second(*tensors, ctx.activation)
         return dx, None, dwg, dwu, None, th, None
 
 

@@ -61,7 +61,7 @@ def test_values_tangents_and_gradients(cpu_kernels, route, name, through):
 def test_gradients_against_differences(cpu_kernels, name):
     x, _, wg, wu, _, _ = _inputs(2)
     torch.autograd.gradcheck(lambda *a: gated_linear(*a, name), tuple(t.requires_grad_() for t in (x, wg, wu)))
-    torch.autograd.gradgradcheck(lambda v: gated_linear(v, wg.detach(), wu.detach(), name), (x,))
+    torch.autograd.gradgradcheck(lambda *a: gated_linear(*a, name), (x, wg, wu))
 
 
 def test_a_gradient_penalty_reaches_the_weights(cpu_kernels):
@@ -76,12 +76,28 @@ def test_a_gradient_penalty_reaches_the_weights(cpu_kernels):
         torch.testing.assert_close(a, b)
 
 
+@pytest.mark.parametrize("wanted", ["xg", "g", "u", "xgu"])
+def test_second_derivatives_through_the_weights(cpu_kernels, wanted):
+    """Hessian-vector products of a loss with respect to x and the weights, whichever of them the product's vector lies along."""
+    x, tx, wg, wu, gh, _ = _inputs(3)
+    leaves = [t.requires_grad_() for t in (x, wg, wu)]
+    along = [t for t, name in zip(leaves, "xgu") if name in wanted]
+    vectors = [torch.randn(t.shape, generator=torch.Generator().manual_seed(i), dtype=t.dtype) for i, t in enumerate(along)]
+    out = []
+    for f in (gated_linear, _plain("silu")):
+        grads = torch.autograd.grad((f(*leaves) * gh).tanh().sum(), along, create_graph=True)
+        out.append(torch.autograd.grad(grads, leaves, vectors))
+    for a, b in zip(*out):
+        torch.testing.assert_close(a, b)
+
+
 def test_what_cannot_be_differentiated_says_so(cpu_kernels):
     x, tx, wg, wu, gh, gth = _inputs(4)
     leaves = [t.requires_grad_() for t in (x, wg, wu)]
     dx, dw = torch.autograd.grad(gated_linear(*leaves), (x, wg), gh, create_graph=True)
-    with pytest.raises(RuntimeError, match="cannot be differentiated a second time"):
-        torch.autograd.grad(dw.sum(), x, retain_graph=True)
+    (h,) = torch.autograd.grad((dw**2).sum() + (dx**2).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="third time"):
+        torch.autograd.grad(h.sum(), x)
     h, th = torch.func.jvp(lambda v: gated_linear(v, wg, wu), (x,), (tx,))
     (dx,) = torch.autograd.grad(th, x, gth, create_graph=True, retain_graph=True)
     with pytest.raises(RuntimeError, match="cannot be differentiated a second time"):
@@ -89,6 +105,39 @@ def test_what_cannot_be_differentiated_says_so(cpu_kernels):
     # ... but the part through h can
     (dx,) = torch.autograd.grad(h, x, gh, create_graph=True)
     torch.autograd.grad(dx.sum(), x)
+
+
+@pytest.mark.parametrize("route", ["func", "fwad", "nested"])
+@pytest.mark.parametrize("given", ["g", "u", "xg", "xgu"])
+def test_tangents_of_the_weights(cpu_kernels, route, given):
+    x, _, wg, wu, gh, gth = _inputs(13)
+    primals = [t.requires_grad_() for t in (x, wg, wu)]
+    tangents = [torch.randn(t.shape, generator=torch.Generator().manual_seed(i), dtype=t.dtype).requires_grad_(n in given)
+                for i, (t, n) in enumerate(zip(primals, "xgu"))]
+    at = [i for i, n in enumerate("xgu") if n in given]
+    leaves = primals + [tangents[i] for i in at]
+    out = []
+    for f in (gated_linear, _plain("silu")):
+        def along(*some):
+            args = list(primals)
+            for i, t in zip(at, some):
+                args[i] = t
+            return f(*args)
+
+        p, t = tuple(primals[i] for i in at), tuple(tangents[i] for i in at)
+        if route == "nested":
+            def value(*some):
+                return torch.func.vjp(along, *some)[0]
+
+            y, ty = torch.func.jvp(value, p, t)
+        elif route == "func":
+            y, ty = torch.func.jvp(along, p, t)
+        else:
+            with fwAD.dual_level():
+                y, ty = fwAD.unpack_dual(along(*(fwAD.make_dual(a, b) for a, b in zip(p, t))))
+        out.append((y, ty, *torch.autograd.grad((y, ty), leaves, (gh, gth))))
+    for a, b in zip(*out):
+        torch.testing.assert_close(a, b)
 
 
 def test_nested_transforms_take_the_general_route(cpu_kernels):
@@ -163,10 +212,6 @@ def test_refusals(cpu_kernels):
                         (ValueError, (x[..., 0:0], wg[:, :0], wu[:, :0]))]:
         with pytest.raises(error):
             gated_linear(*args)
-    with fwAD.dual_level(), pytest.raises(NotImplementedError, match="no tangent with respect to its weights"):
-        gated_linear(x, fwAD.make_dual(wg, wu), wu)
-    with pytest.raises(NotImplementedError, match="no tangent with respect to its weights"):
-        torch.func.jvp(lambda w: gated_linear(x, w, wu), (wg,), (wu,))
 
 
 def test_no_cpu_fallback():

@@ -311,6 +311,30 @@ def test_a_tangent_that_is_zero():
     assert torch.equal(h, gated_linear(x, wg, wu)) and not th.any()
 
 
+@pytest.mark.parametrize("M", [90, 400])
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_tangents_and_second_derivatives_of_the_weights(M, dt):
+    """Against torch in float64.  Operands side by side are twice as wide, else these are the launches of the other tests: fp32 within 1e-5 of the
+    norm (second derivatives: two gradients in a row, 2e-5), bf16 within e for values and 4 e for each gradient on the way."""
+    x, tx, wg, wu, gh, gth = _inputs(M, 72, 136, dt, 18)
+    tg, tu = (torch.randn_like(w) * 0.3 * 72**-0.5 for w in (wg, wu))
+    e = 1e-5 if dt == "fp32" else 2.0**-8
+    out = []
+    for own in (True, False):
+        cast = (lambda t: t) if own else (lambda t: t.double())
+        f = gated_linear if own else lambda v, a, b: torch.nn.functional.silu(v @ a.T) * (v @ b.T)
+        leaves = [cast(t).detach().requires_grad_() for t in (x, wg, wu)]
+        tangents = [cast(t).detach().requires_grad_() for t in (tx, tg, tu)]
+        h, th = torch.func.jvp(f, tuple(leaves), tuple(tangents))
+        first = torch.autograd.grad((h, th), leaves + tangents, (cast(gh), cast(gth)))
+        grads = torch.autograd.grad(f(*leaves), leaves, cast(gh), create_graph=True)
+        second = torch.autograd.grad(grads, leaves, tangents)
+        out.append([h, th, *first, *second])
+    for i, (a, b) in enumerate(zip(*out)):
+        most = e * (1 if i < 2 else (1 if dt == "fp32" else 4) * (1 if i < 8 else 2))
+        assert (a.double() - b).norm() <= most * b.norm(), (i, ((a.double() - b).norm() / b.norm()).item())
+
+
 def test_another_stream_and_captured_graphs():
     x, tx, wg, wu, gh, gth = _inputs(260, 100, 204, "bf16", 8)  # K = 100: copies in the workspace
     want = _run(x, tx, wg, wu, gh, gth, "silu", "jvp_bwd")
