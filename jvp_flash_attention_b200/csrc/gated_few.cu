@@ -7,7 +7,7 @@
 // A cluster of 1 to 8 CTAs shares a tile, a part of the depth each, so that all SMs have a part of the weights under way also where there are few
 // tiles; the parts' sums meet in the CTAs' shared memory and are added in their order, each CTA finishing a part of the tile.
 //
-// fp32 weights are read once, as they are: eight warps load them, split them into three bf16 parts and lay these down for the tensor cores
+// fp32 weights are read once, as they are: 16 warps load them, split them into three bf16 parts and lay these down for the tensor cores
 // (a copy of the parts in memory would be written and read again, four times the bytes).  The tensor cores round towards zero at every
 // step of 16, so those warps take the sums up in registers every 4 k-blocks, while the next go to another accumulator; and the five lesser
 // products of parts have accumulators of their own, where what is rounded away is that much smaller.

@@ -36,7 +36,7 @@ constexpr int kPairStages = sizeof(T) == 4 || KIND == kPairGated ? 5 : 6;  // (5
 constexpr int kStageBytes = 32768;  // of a CTA: A 128 x 64, B 128 x 64
 constexpr int kExchangeBytes = 32768;  // 4 pairs of warps x two directions x 2 x 16 features x 32 rows
 constexpr int kMinPieceSteps = 4;
-constexpr int kMinSavedSteps = 24;  // 7 us: a join's launch and its way through memory take 5 to 7
+constexpr int kMinSavedSteps = 24, kMinSavedGated = 36;  // 7 us: a join's launch and its way through memory take 5 to 7, with the gate 6 to 10
 constexpr int kAbortPairFull = 14, kAbortPairEmpty = 15, kAbortPairAcc = 16, kAbortPairAccEmpty = 17;
 
 struct PairBarriers {
@@ -655,7 +655,7 @@ int plan_pair(int dtype, int kind, PairArgs& p) {
     if (cut > 1) {
       const int piece = (p.steps + cut - 1) / cut;
       cut = (p.steps + piece - 1) / piece;
-      if (cut > 1 && p.steps - piece >= kMinSavedSteps) {
+      if (cut > 1 && p.steps - piece >= (gated ? kMinSavedGated : kMinSavedSteps)) {
         p.whole = (int)tiles - rest;
         p.cut = cut, p.piece = piece;
         p.items = p.whole + rest * cut;

@@ -40,6 +40,7 @@ def _check(got, x, tx, wg, wu, gh, gth, kind):
     a, a1, a2 = (t.abs() for t in formulas.activation(kind, g))
     dx, dtx, dwg, dwu = formulas.gated_bwd(x, tx, wg, wu, g, u, tg, tu, gh, gth, kind) if gh is not None or gth is not None else (None,) * 4
     k = _sum_error(x.shape[1], dtype)
+    tiny = torch.finfo(dtype).smallest_normal * e  # half the spacing of the smallest numbers, which cotangents of fp16 reach
     zero = torch.zeros_like(g)
     Eg, Eu = k * (x.abs() @ wg.abs().T), k * (x.abs() @ wu.abs().T)
     act = eta * (1 + g.abs())
@@ -62,8 +63,9 @@ def _check(got, x, tx, wg, wu, gh, gth, kind):
             Edu = Edu + GTH * (a2 * TG * Eg + a1 * Etg + act * TG)
             mdg, mdu = mdg + GTH * (a2 * TG * U + a1 * TU), mdu + GTH * a1 * TG
             mdtg, mdtu = GTH * a1 * U, GTH * a
-            Edtg, Edtu = GTH * (a2 * U * Eg + a1 * Eu + act * U) + (e + 2.0**-22) * mdtg, GTH * (a1 * Eg + act) + (e + 2.0**-22) * mdtu
-        Edg, Edu = Edg + (e + 2.0**-21) * mdg, Edu + (e + 2.0**-21) * mdu
+            Edtg, Edtu = (GTH * (a2 * U * Eg + a1 * Eu + act * U) + (e + 2.0**-22) * mdtg + tiny,
+                          GTH * (a1 * Eg + act) + (e + 2.0**-22) * mdtu + tiny)
+        Edg, Edu = Edg + (e + 2.0**-21) * mdg + tiny, Edu + (e + 2.0**-21) * mdu + tiny
         f, m = _sum_error(2 * g.shape[1], dtype), _sum_error(x.shape[0] * (2 if gth is not None else 1), dtype)
         WG, WU, X = wg.abs(), wu.abs(), x.abs()
         bounds["dx"] = (Edg + f * mdg) @ WG + (Edu + f * mdu) @ WU
