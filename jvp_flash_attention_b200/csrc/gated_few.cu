@@ -412,9 +412,6 @@ bool plan_few(int dtype, int kind, FewArgs& p) {
   p.kblocks = (depth + 63) / 64;
   p.steps = kind == kFewGated ? p.kblocks : 2 * p.kblocks;
   p.tiles = kind == kFewGated ? (p.features + 63) / 64 : (p.width + 127) / 128;
-  // fp32: one CTA an SM, whose registers hold what is under way; else two, of some 100 KB of stages each
-  const int stage = parts * (kTile + N * 128), room = parts > 1 ? 224 * 1024 : 108 * 1024;
-  p.stages = room / stage < 8 ? room / stage : 8;
   // CTAs of a tile: as many as find room at once.  fp32, where a CTA has an SM to itself: tiles by whole rounds of the SMs first, in a launch of
   // their own, so that a last round of few does not take as long as one of all.
   const int at_once = parts > 1 ? device_sms() : 2 * device_sms();
@@ -423,6 +420,11 @@ bool plan_few(int dtype, int kind, FewArgs& p) {
   const int rest = p.tiles - p.whole;
   p.cluster = 1;
   while (p.cluster < 8 && rest * 2 * p.cluster <= at_once && 4 * p.cluster <= p.steps) p.cluster *= 2;
+  // Room for stages: fp32 one CTA an SM, whose registers hold what is under way; else two CTAs, or three where two do not take all tiles in one round
+  // (4 rows of bf16 K4096 F20000 73 -> 60 us; of F11008 35 -> 37).  The sums take the stages' place at the end.
+  const int stage = parts * (kTile + N * 128), room = parts > 1 ? 224 * 1024 : p.tiles > 2 * device_sms() ? 74 * 1024 : 108 * 1024;
+  p.stages = room / stage < 8 ? room / stage : 8;
+  if (p.stages * stage < N * 512) return false;
   p.tmem_columns = 32;
   while (p.tmem_columns < (parts > 1 ? 4 : 1) * N) p.tmem_columns *= 2;
   return true;
