@@ -405,7 +405,8 @@ int jvpfa_rotary(const jvpfa_rotary_args* args, void* stream);
  *
  * Sums are held in 32 bits.  g, u, tg, tu are kept for the backward in a form of the library's own (24 bits an entry, 32 for JVPFA_FP32);
  * dg, du, dtg, dtu are rounded to the tensors' type.
- * JVPFA_FP32 multiplies three bf16 parts of every entry (error ~1e-6 relative).  x, tx, wg, wu have contiguous columns and row
+ * JVPFA_FP32 multiplies three bf16 parts of every entry (error ~1e-6 relative).  In 16 bits a sum has at most 2^26 terms (dx and dtx, their
+ * two products together; dwg and dwu, value and tangent together), else JVPFA_ERR_TOO_LARGE.  x, tx, wg, wu have contiguous columns and row
  * strides in elements; all other tensors are row-major and 16-byte aligned.  While the status word of jvpfa_device_status is set, whatever the
  * type, the calls answer JVPFA_ERR_DEVICE_STATUS, and launches that are queued or replayed write NaN.
  */

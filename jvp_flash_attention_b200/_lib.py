@@ -383,7 +383,7 @@ _native = None
 
 
 def native():
-    """The native call layer (``_native.so``, csrc/native.cpp); raises if it has not been built."""
+    """The native call layer (``_native.so``, csrc/native*.cpp); raises if it has not been built."""
     global _native
     if _native is None:
         load()

@@ -117,7 +117,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         r = subprocess.run(_native_cmd(), capture_output=True, text=True)
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
-            raise RuntimeError("g++ failed for native.cpp")
+            raise RuntimeError("g++ failed for native*.cpp")
         NATIVE_STAMP.write_text(_native_with())
     return LIB
 

@@ -190,6 +190,7 @@ struct FewArgs {
 bool plan_few(int dtype, int kind, FewArgs& p);
 int launch_few(int dtype, int kind, const FewArgs& p, const FewMaps& maps, cudaStream_t s);
 int device_sms();  // of the current device
+constexpr int kMaxSteps = 1 << 20;  // k-blocks of one sum on the tensor cores
 // The map of a (planes of) row-major matrix: boxes of 64 columns x box_rows rows.
 bool encode_matrix(CUtensorMap* m, int dtype, const void* ptr, int rows, int cols, int64_t stride, int planes, int box_rows);
 

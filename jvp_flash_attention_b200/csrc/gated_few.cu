@@ -410,6 +410,7 @@ bool plan_few(int dtype, int kind, FewArgs& p) {
   if (N > 128) return false;
   const int depth = kind == kFewGated ? p.width : p.features;
   p.kblocks = (depth + 63) / 64;
+  if (p.kblocks > kMaxSteps / 2) return false;
   p.steps = kind == kFewGated ? p.kblocks : 2 * p.kblocks;
   p.tiles = kind == kFewGated ? (p.features + 63) / 64 : (p.width + 127) / 128;
   // CTAs of a tile: as many as find room at once.  fp32, where a CTA has an SM to itself: tiles by whole rounds of the SMs first, in a launch of

@@ -637,6 +637,8 @@ int plan_pair(int dtype, int kind, PairArgs& p) {
   const long long tiles = (long long)p.groups * p.tiles_m * p.tiles_n;
   // (what a CTA counts, k-blocks of its tiles and tiles of a band, stays in 32 bits)
   if (steps > 2147483647LL || tiles > 2147483647LL - 1024 || steps * (tiles / 64 + 1) > 2147483647LL) return JVPFA_ERR_TOO_LARGE;
+  // A tile's sum is one wait of the warps that write it, and waits are bounded: 2^20 k-blocks (67 million rows for dw) take some 0.4 seconds.
+  if (dtype != JVPFA_FP32 && steps > kMaxSteps) return JVPFA_ERR_TOO_LARGE;
   p.steps = (int)steps;
   p.chunk = dtype == JVPFA_FP32 ? 4 : p.steps;
   // 74 tiles at once read band + 74 / band panels of their operands.  8 is the fewest, and best for the backward's, whose panels are as deep as the

@@ -272,5 +272,6 @@ def test_workspaces():
     assert bwd(M=0) == 0
     # tiles whose depth is worth cutting: 2 x 28 672 of the contraction, two rows of 16 tiles, 2 pieces each of 256 x 256 sums
     assert bwd(M=300, K=4096, F=28672, x_stride=4096, wg_stride=4096, wu_stride=4096) == 2 * 300 * 28672 * 2 + 32 * 2 * 256 * 256 * 4
+    assert bwd(M=2**26 + 64, dx=None, dwg=256, dwu=256) == 0 < bwd(M=2**26, dx=None, dwg=256, dwu=256)  # sums of more k-blocks than a wait lasts
     kept = lib.jvpfa_gated_kept_bytes
     assert kept(0, 1, 1, 0) == 2 * 1024 * 3 and kept(2, 33, 40, 1) == 4 * 4 * 1024 * 4 and kept(3, 1, 1, 0) == kept(0, 0, 1, 0) == 0
