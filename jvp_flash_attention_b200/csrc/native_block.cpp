@@ -149,11 +149,23 @@ struct RotaryNode : public Node {
       }
       plain[i] = g;
     }
-    variable_list out = launch_rotary(plain, orders, f, p, back);
+    variable_list out = turned_again(plain, f, p, back);
+    // A cotangent that is dual, inside a forward-AD level: so is its gradient.
+    std::vector<Tensor> tangents(grads.size());
+    for (size_t i = 0; i < grads.size(); ++i)
+      if (plain[i].defined()) tangents[i] = as_tangent(grads[i]._fw_grad(0), plain[i]);
+    tangents = turned_again(tangents, f, p, back);
+    for (size_t i = 0; i < out.size(); ++i)
+      if (tangents[i].defined()) out[i]._set_fw_grad(tangents[i], /*level=*/0, /*is_inplace_op=*/false);
+    return out;
+  }
+  // xs turned, with a node behind those that need one.
+  std::vector<Tensor> turned_again(const std::vector<Tensor>& xs, const Tensor& f, const Tensor& p, const Turn& back) const {
+    std::vector<Tensor> out = launch_rotary(xs, orders, f, p, back);
     std::vector<int> again;
     for (size_t i = 0; i < out.size(); ++i)
-      if (out[i].defined() && torch::autograd::compute_requires_grad(plain[i])) again.push_back((int)i);
-    connect(plain, out, again, f, p, back, orders);
+      if (out[i].defined() && torch::autograd::compute_requires_grad(xs[i])) again.push_back((int)i);
+    connect(xs, out, again, f, p, back, orders);
     return out;
   }
   void release_variables() override {

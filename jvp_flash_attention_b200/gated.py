@@ -34,7 +34,8 @@ def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, activation: str = "sil
     whatever ``set_fp32_precision`` says of attention; an infinite entry gives NaN in its row.  Results are the same from run to run.
 
     Tangents of the weights, and a second differentiation of their gradients, run on operands side by side, ``[tx | x]`` and ``[w | tw]``,
-    at twice the depth; the gradient through the tangent output cannot be differentiated again.
+    at twice the depth (where a weight's tangent is not finite, neither is the value there); the gradient through the tangent output cannot
+    be differentiated again.  Gradients that are taken inside a forward-AD level are those of the primals and carry no tangent, as attention's.
     """
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation is one of {', '.join(ACTIVATIONS)}; got {activation!r}")

@@ -94,6 +94,22 @@ def test_a_functorch_transform_of_the_cotangent(cpu_turn):
     torch.testing.assert_close(torch.func.grad(lambda c: (vjp(c) * v).sum())(g), formulas.turn(v, W))
 
 
+def test_the_gradient_of_a_dual_cotangent_is_dual(cpu_turn):
+    """Forward over reverse inside a forward-AD level; the gradient and its tangent can be differentiated in turn."""
+    q, k, tq, tk = _qk(15, 4)
+    v = _qk(16)[0]
+    leaves = [x.requires_grad_() for x in (q, k, tq, tk)]
+    out = []
+    for f in (lambda a, b: rot.rotary(a, b, W, offset=3), lambda a, b: (formulas.turn(a, W, None, 3), formulas.turn(b, W, None, 3))):
+        with fwAD.dual_level():
+            yq, yk = f(fwAD.make_dual(q, tq), fwAD.make_dual(k, tk))
+            (g,) = torch.autograd.grad((yq**3).sum() + (yk**2).sum(), q, create_graph=True)
+            g, tg = fwAD.unpack_dual(g)
+            out.append((g, tg, *torch.autograd.grad((g * v).sum() + (tg * v).sum(), (q, tq))))
+    for a, b in zip(*out):
+        torch.testing.assert_close(a, b)
+
+
 def test_nothing_to_turn(cpu_turn):
     assert rot.rotary(_qk(8)[0], None, W[:0]).shape == (B, H, L, D)
 
