@@ -3,6 +3,7 @@
 // are handed back to the Python modules' _launch functions (the CPU suite puts its formulas there); what this layer declines (bad
 // arguments, transforms other than a lone torch.func.jvp) returns None and is served by the Python modules' Functions.
 #include <algorithm>
+#include <limits>
 #include <mutex>
 
 #include "native_common.h"
@@ -364,6 +365,23 @@ GatedGrads launch_gated_bwd(const Tensor& x, const Tensor& tx, const Tensor& wg,
   return r;
 }
 
+constexpr const char* kThird = "gated_linear cannot be differentiated a third time";
+constexpr const char* kThroughTangent = "the gradient through the tangent output of gated_linear cannot be differentiated a second time";
+
+// Inside a forward-AD level: a tensor's tangent, if it has one, and one put on a gradient.
+Tensor tangent_of(const Tensor& t) { return t.defined() ? t._fw_grad(0) : Tensor(); }
+void set_tangent(Tensor& t, const Tensor& tangent) {
+  if (t.defined() && tangent.defined()) t._set_fw_grad(tangent, /*level=*/0, /*is_inplace_op=*/false);
+}
+// In place of a tangent that takes a third derivative, which there is no formula for: NaN, since none would be read as zero.  (The gradient
+// itself is right, and who does not ask for its tangent loses nothing.)
+Tensor unknown_like(const Tensor& t) {
+  if (!t.defined()) return t;
+  at::AutoDispatchBelowADInplaceOrView below;
+  at::AutoGradMode no_grad(false);
+  return at::full_like(t, std::numeric_limits<double>::quiet_NaN());
+}
+
 // (dx, dwg, dwu) of <gh, h> as a node that can be differentiated once more: with v the incoming gradients,
 //   d<(dx, dwg, dwu), v>/d(x, wg, wu) = d<th(x, wg, wu; v), gh>/d(x, wg, wu)   and   d<(dx, dwg, dwu), v>/d(gh) = th(x, wg, wu; v),
 // one value-and-tangent forward and one backward through the tangent (of operands side by side, which the Python module makes, where the
@@ -371,6 +389,23 @@ GatedGrads launch_gated_bwd(const Tensor& x, const Tensor& tx, const Tensor& wg,
 struct GatedGradNode : public Node {
   int activation;
   SavedVariable x, wg, wu, gh;
+
+  // One behind e's gradients.
+  static void connect(GatedGrads& e, int activation, const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& gh) {
+    auto node = std::shared_ptr<GatedGradNode>(new GatedGradNode(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x, wg, wu, gh));
+    node->activation = activation;
+    node->x = SavedVariable(x, false);
+    node->wg = SavedVariable(wg, false);
+    node->wu = SavedVariable(wu, false);
+    node->gh = SavedVariable(gh, false);
+    for (Tensor* t : {&e.dx, &e.dwg, &e.dwu}) {
+      if (t->defined())
+        torch::autograd::set_history(*t, node);
+      else
+        node->add_input_metadata(Node::undefined_input());
+    }
+  }
 
   variable_list apply(variable_list&& v) override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -397,7 +432,7 @@ struct GatedGradNode : public Node {
       if (task_should_compute_output(3)) out[3] = f.th;
     }
     if (at::GradMode::is_enabled())
-      attach_refusal("gated_linear cannot be differentiated a third time", {&out[0], &out[1], &out[2], &out[3]}, x_, wg_, wu_, gh_, v[0], v[1], v[2]);
+      attach_refusal(kThird, {&out[0], &out[1], &out[2], &out[3]}, x_, wg_, wu_, gh_, v[0], v[1], v[2]);
     return out;
   }
   void release_variables() override {
@@ -410,6 +445,7 @@ struct GatedGradNode : public Node {
 // The node of a call: outputs h (0) and, with a tangent, th (1); edges to x, wg, wu and, with a tangent, tx.
 struct GatedNode : public Node {
   int activation;
+  bool side_by_side;  // operands of twice the width, [x | 0], [tx | x] and [w | tw] (the Python module's, for tangents of the weights)
   SavedVariable x, tx, wg, wu, kept;
 
   variable_list apply(variable_list&& grads) override {
@@ -417,7 +453,7 @@ struct GatedNode : public Node {
     variable_list out(num_outputs());
     const Tensor gh = primal_of(grads[0]), gth = grads.size() > 1 ? primal_of(grads[1]) : Tensor();
     if (!gh.defined() && !gth.defined()) return out;
-    const Tensor x_ = primal_of(x.unpack()), wg_ = primal_of(wg.unpack()), wu_ = primal_of(wu.unpack());
+    const Tensor x_dual = x.unpack(), x_ = primal_of(x_dual), wg_ = primal_of(wg.unpack()), wu_ = primal_of(wu.unpack());
     const Tensor xp = unwrap(x_), wgp = unwrap(wg_), wup = unwrap(wu_);
     const Tensor tx_ = num_outputs() > 3 ? tx.unpack() : Tensor(), txp = unwrap(tx_), kept_ = unwrap(kept.unpack());
     const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1) || task_should_compute_output(2);
@@ -436,37 +472,57 @@ struct GatedNode : public Node {
     GatedGrads d;
     if (gth.defined()) {
       d = launch_gated_bwd(xp, txp, wgp, wup, kept_, again ? Tensor() : gh, gth, activation, need_x, need_tx, need_w);
-      if (again)
-        attach_refusal("the gradient through the tangent output of gated_linear cannot be differentiated a second time",
-                       {&d.dx, &d.dtx, &d.dwg, &d.dwu}, x_, wg_, wu_, tx_, gth);
+      if (again) attach_refusal(kThroughTangent, {&d.dx, &d.dtx, &d.dwg, &d.dwu}, x_, wg_, wu_, tx_, gth);
     }
     if (gh.defined() && (again || !gth.defined())) {
       GatedGrads e = launch_gated_bwd(xp, txp, wgp, wup, kept_, gh, Tensor(), activation, need_x, false, need_w);
-      if (again) {
-        auto node = std::shared_ptr<GatedGradNode>(new GatedGradNode(), torch::autograd::deleteNode);
-        node->set_next_edges(torch::autograd::collect_next_edges(x_, wg_, wu_, gh));
-        node->activation = activation;
-        node->x = SavedVariable(x_, false);
-        node->wg = SavedVariable(wg_, false);
-        node->wu = SavedVariable(wu_, false);
-        node->gh = SavedVariable(gh, false);
-        for (Tensor* t : {&e.dx, &e.dwg, &e.dwu}) {
-          if (t->defined())
-            torch::autograd::set_history(*t, node);
-          else
-            node->add_input_metadata(Node::undefined_input());
-        }
-      }
+      if (again) GatedGradNode::connect(e, activation, x_, wg_, wu_, gh);
       auto add = [](Tensor& to, const Tensor& t) {
         if (t.defined()) to = to.defined() ? to + t : t;
       };
       add(d.dx, e.dx), add(d.dwg, e.dwg), add(d.dwu, e.dwu);
+    }
+    // Inside a forward-AD level gradients are dual.
+    const Tensor tgh = tangent_of(grads[0]), tgth = grads.size() > 1 ? tangent_of(grads[1]) : Tensor();
+    const bool along = tangent_of(x_dual).defined();  // x moves along tx
+    if (along || tgh.defined() || tgth.defined()) {
+      GatedGrads t;
+      if (along && gth.defined()) {
+        t = {unknown_like(d.dx), unknown_like(d.dtx), unknown_like(d.dwg), unknown_like(d.dwu)};
+      } else if (along) {
+        t = along_tx(xp, txp, wgp, wup, kept_, gh, as_tangent(tgh, gh), need_x, need_w);
+        if (again) attach_refusal(kThird, {&t.dx, &t.dwg, &t.dwu}, x_, wg_, wu_, tx_, gh, tgh);
+      } else {  // linear in the cotangents
+        const Tensor ch = as_tangent(tgh, gh), cth = as_tangent(tgth, gth);
+        t = launch_gated_bwd(xp, txp, wgp, wup, kept_, ch, cth, activation, need_x, need_tx, need_w);
+        if (again && cth.defined())
+          attach_refusal(kThroughTangent, {&t.dx, &t.dtx, &t.dwg, &t.dwu}, x_, wg_, wu_, tx_, ch, cth);
+        else if (again)
+          GatedGradNode::connect(t, activation, x_, wg_, wu_, ch);
+      }
+      set_tangent(d.dx, t.dx), set_tangent(d.dtx, t.dtx), set_tangent(d.dwg, t.dwg), set_tangent(d.dwu, t.dwu);
     }
     out[0] = d.dx;
     if (task_should_compute_output(1)) out[1] = d.dwg;
     if (task_should_compute_output(2)) out[2] = d.dwu;
     if (need_tx) out[3] = d.dtx;
     return out;
+  }
+  // The tangents of the gradients (dx, dwg, dwu) of <gh, h>, x moving along tx and gh along tgh: by the symmetry of second derivatives the
+  // gradients of <tgh, h> + <gh, th>, from the projections that the forward kept.
+  GatedGrads along_tx(const Tensor& xp, const Tensor& txp, const Tensor& wgp, const Tensor& wup, const Tensor& kept_, const Tensor& gh,
+                      const Tensor& tgh, bool need_x, bool need_w) const {
+    GatedGrads t = launch_gated_bwd(xp, txp, wgp, wup, kept_, tgh, gh, activation, need_x, need_x && side_by_side, need_w);
+    if (!side_by_side) return t;
+    // Operands side by side: what is wanted of x is both halves' sum (the weights move as well), and h does not depend on what stands for
+    // the tangents.
+    at::AutoDispatchBelowADInplaceOrView below;
+    at::AutoGradMode no_grad(false);
+    const int64_t K = xp.size(-1) / 2;
+    auto with_zeros = [](const Tensor& y) { return at::cat({y, at::zeros_like(y)}, -1); };
+    if (need_x) t.dx = with_zeros(t.dx.narrow(-1, 0, K) + t.dtx.narrow(-1, K, K)), t.dtx = Tensor();
+    if (need_w) t.dwg = with_zeros(t.dwg.narrow(-1, 0, K)), t.dwu = with_zeros(t.dwu.narrow(-1, 0, K));
+    return t;
   }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -486,7 +542,7 @@ bool gated_acceptable(const Tensor& x, const Tensor& wg, const Tensor& wu) {
 }
 
 // None: not a case for this path; the caller takes its general route.
-py::object gated(const Tensor& x_in, const Tensor& wg_in, const Tensor& wu_in, int activation) {
+py::object gated(const Tensor& x_in, const Tensor& wg_in, const Tensor& wu_in, int activation, bool side_by_side) {
   const int64_t level = jvp_level();
   if (level == -2 || wg_in._fw_grad(0).defined() || wu_in._fw_grad(0).defined()) return py::none();
   Tensor x = x_in, tx = x._fw_grad(0);
@@ -512,6 +568,7 @@ py::object gated(const Tensor& x_in, const Tensor& wg_in, const Tensor& wu_in, i
     auto node = std::shared_ptr<GatedNode>(new GatedNode(), torch::autograd::deleteNode);
     node->set_next_edges(tx.defined() ? torch::autograd::collect_next_edges(x, wg, wu, tx) : torch::autograd::collect_next_edges(x, wg, wu));
     node->activation = activation;
+    node->side_by_side = side_by_side;
     node->x = SavedVariable(x, false);
     node->wg = SavedVariable(wg, false);
     node->wu = SavedVariable(wu, false);
@@ -533,5 +590,5 @@ py::object gated(const Tensor& x_in, const Tensor& wg_in, const Tensor& wu_in, i
 void bind_block(py::module_& m) {
   m.def("rotary", &rotary, py::arg("q"), py::arg("k").none(true), py::arg("inv_freq"), py::arg("positions").none(true), py::arg("offset"),
         py::arg("interleaved"), py::arg("amplitude"));
-  m.def("gated", &gated);
+  m.def("gated", &gated, py::arg("x"), py::arg("w_gate"), py::arg("w_up"), py::arg("activation"), py::arg("side_by_side") = false);
 }

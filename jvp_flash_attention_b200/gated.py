@@ -35,7 +35,9 @@ def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, activation: str = "sil
 
     Tangents of the weights, and a second differentiation of their gradients, run on operands side by side, ``[tx | x]`` and ``[w | tw]``,
     at twice the depth (where a weight's tangent is not finite, neither is the value there); the gradient through the tangent output cannot
-    be differentiated again.  Gradients that are taken inside a forward-AD level are those of the primals and carry no tangent, as attention's.
+    be differentiated again.  Gradients that are taken inside a forward-AD level carry their tangents (Hessian-vector products), which is a
+    further backward: take them behind the level where only they are wanted.  The tangent of one through the tangent output would be a third
+    derivative; it is NaN.
     """
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation is one of {', '.join(ACTIVATIONS)}; got {activation!r}")
@@ -49,9 +51,10 @@ def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, activation: str = "sil
             return out
         if any(fwAD.unpack_dual(w).tangent is not None for w in (w_gate, w_up)):
             _check(x, w_gate, w_up)
-            (x, tx), (w_gate, t_gate), (w_up, t_up) = (fwAD.unpack_dual(t) for t in (x, w_gate, w_up))
-            x, tx, w_gate, w_up = _side_by_side(x, tx, w_gate, t_gate, w_up, t_up)
-            return gated_linear(fwAD.make_dual(x, tx), w_gate, w_up, activation)
+            xs, txs, *ws = _side_by_side(*(t for operand in (x, w_gate, w_up) for t in fwAD.unpack_dual(operand)))
+            out = _lib.native().gated(fwAD.make_dual(xs, txs), *ws, act, side_by_side=True)
+            if out is not None:
+                return out
     _check(x, w_gate, w_up)
     return _Gated.apply(x, w_gate, w_up, act)[0]
 

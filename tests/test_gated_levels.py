@@ -1,0 +1,128 @@
+"""CPU tests of gated_linear's gradients where forward mode goes over them: inside a forward-AD level and under functorch transforms.
+Launches go to the formulas (tests/_block_formulas.py), and what they add up to is held against torch's differentiation of the plain form."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+import jvp_flash_attention_b200.gated as gated
+from jvp_flash_attention_b200 import _lib
+from jvp_flash_attention_b200.gated import ACTIVATIONS, gated_linear
+from tests import _block_formulas as formulas
+
+
+def _in_memory(launch):
+    """The launch as the GPU's is: it reads what is in the tensors' memory, whatever transforms they belong to."""
+    def run(*args):
+        with torch.no_grad(), _lib.native().NoFunctorch():
+            plain = [fwAD.unpack_dual(gated._unwrap(t)).primal.detach() if isinstance(t, torch.Tensor) else t for t in args]
+            assert not any(isinstance(t, torch.Tensor) and t._is_zerotensor() for t in plain)
+            return launch(*plain)
+    return run
+
+
+@pytest.fixture(autouse=True)
+def cpu_kernels(monkeypatch):
+    monkeypatch.setattr(gated, "_launch_fwd", _in_memory(formulas.launch_gated_fwd))
+    monkeypatch.setattr(gated, "_launch_bwd", _in_memory(formulas.launch_gated_bwd))
+    monkeypatch.setattr(gated, "_require_cuda", lambda *a: None)
+
+
+def _inputs(seed, k=4, f=3):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)  # noqa: E731
+    return {"x": r(2, 5, k), "wg": r(f, k), "wu": r(f, k), "tx": r(2, 5, k), "tg": r(f, k), "tu": r(f, k), "gh": r(2, 5, f), "tgh": r(2, 5, f),
+            "wd": r(k, f)}
+
+
+def _plain(name):
+    act = lambda g: formulas.activation(ACTIVATIONS[name], g)[0]  # noqa: E731  (elementary operations, which torch differentiates in any order)
+    return lambda x, wg, wu: act(x @ wg.T) * (x @ wu.T)
+
+
+def _forward_over_reverse(loss, primals, tangents):
+    """(gradients, their tangents), by torch."""
+    return torch.func.jvp(lambda *a: torch.func.grad(loss, argnums=tuple(range(len(primals))))(*a), tuple(primals), tuple(tangents))
+
+
+@pytest.mark.parametrize("name", list(ACTIVATIONS))
+@pytest.mark.parametrize("given", ["x", "g", "xgu"])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("create_graph", [False, True])
+def test_gradients_inside_a_level_carry_their_tangents(name, given, residual, create_graph):
+    i = _inputs(1)
+    primals = [i[n].requires_grad_() for n in ("x", "wg", "wu")]
+    tangents = [t if n in given else torch.zeros_like(t) for n, t in zip("xgu", (i["tx"], i["tg"], i["tu"]))]
+    block = lambda f: lambda x, wg, wu: ((x + f(x, wg, wu) @ i["wd"].T if residual else f(x, wg, wu)) ** 3).sum()  # noqa: E731
+    want, moving = _forward_over_reverse(block(_plain(name)), [p.detach() for p in primals], tangents)
+    with fwAD.dual_level():
+        duals = [fwAD.make_dual(p, t) if n in given else p for n, p, t in zip("xgu", primals, tangents)]
+        y = block(lambda *a: gated_linear(*a, name))(*duals)
+        grads = torch.autograd.grad(y, primals, create_graph=create_graph)
+        for d, w, m in zip(grads, want, moving):
+            d, t = fwAD.unpack_dual(d)
+            torch.testing.assert_close(d, w)
+            torch.testing.assert_close(t, m)
+
+
+def test_a_cotangent_that_alone_is_dual():
+    """The gradient is linear in it; with a graph, its tangent can be differentiated as the gradient can."""
+    i = _inputs(2)
+    leaves = [i[n].requires_grad_() for n in ("x", "wg", "wu", "gh", "tgh")]
+    out = []
+    for f in (gated_linear, _plain("silu")):
+        y = f(*leaves[:3])
+        with fwAD.dual_level():
+            if f is gated_linear:
+                grads = torch.autograd.grad(y, leaves[:3], fwAD.make_dual(leaves[3], leaves[4]), create_graph=True)
+                pairs = [tuple(fwAD.unpack_dual(d)) for d in grads]
+            else:
+                pairs = list(zip(*(torch.autograd.grad(y, leaves[:3], c, create_graph=True) for c in leaves[3:])))
+        flat = [t for p in pairs for t in p]
+        out.append([*flat, *torch.autograd.grad(sum((t**2).sum() for t in flat), leaves)])
+    for a, b in zip(*out):
+        torch.testing.assert_close(a, b)
+
+
+def test_dual_cotangents_of_a_graph_with_a_tangent():
+    """A call under torch.func.jvp, whose graph is walked later with dual cotangents of both outputs."""
+    i = _inputs(3)
+    leaves = [i[n].requires_grad_() for n in ("x", "wg", "wu", "tx")]
+    both = torch.func.jvp(lambda v: gated_linear(v, leaves[1], leaves[2]), (leaves[0],), (leaves[3],))
+    cots, tangents = (i["gh"], i["tgh"]), (i["tgh"] * 2, i["gh"] - 1)
+    want = [torch.autograd.grad(both, leaves, c, retain_graph=True) for c in (cots, tangents)]
+    with fwAD.dual_level():
+        got = torch.autograd.grad(both, leaves, [fwAD.make_dual(c, t) for c, t in zip(cots, tangents)], retain_graph=True)
+        for d, w, t in zip(got, *want):
+            d, td = fwAD.unpack_dual(d)
+            torch.testing.assert_close(d, w)
+            torch.testing.assert_close(td, t)
+
+
+@pytest.mark.parametrize("through", ["t", "both"])
+def test_a_third_derivative_is_nan_and_the_gradient_right(through):
+    i = _inputs(4)
+    leaves = [i[n].requires_grad_() for n in ("x", "wg", "wu")]
+    cots = [i["gh"], i["tgh"]][through == "t":]
+    out = []
+    for inside in (False, True):
+        with fwAD.dual_level():
+            both = tuple(fwAD.unpack_dual(gated_linear(fwAD.make_dual(leaves[0], i["tx"]), *leaves[1:])))[through == "t":]
+            if inside:
+                duals = [fwAD.unpack_dual(d) for d in torch.autograd.grad(both, leaves, cots)]
+                assert all(d.tangent.isnan().all() for d in duals)
+                out.append([d.primal for d in duals])
+        if not inside:
+            out.append(torch.autograd.grad(both, leaves, cots))
+    for a, b in zip(*out):
+        torch.testing.assert_close(a, b)
+
+
+def test_a_tangent_of_a_gradient_is_not_differentiated_again():
+    i = _inputs(5)
+    x = i["x"].requires_grad_()
+    with fwAD.dual_level():
+        (d,) = torch.autograd.grad((gated_linear(fwAD.make_dual(x, i["tx"]), i["wg"], i["wu"]) ** 2).sum(), x, create_graph=True)
+        d, td = fwAD.unpack_dual(d)
+        with pytest.raises(RuntimeError, match="third time"):
+            torch.autograd.grad(td.sum(), x, retain_graph=True)
+        torch.autograd.grad(d.sum(), x)

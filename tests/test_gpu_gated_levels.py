@@ -1,0 +1,51 @@
+"""GPU tests of gated_linear's gradients where forward mode goes over them, inside a forward-AD level and under functorch transforms.
+Bounds as in test_gpu_gated.py: the launches are the same, with other cotangents."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+from jvp_flash_attention_b200 import _lib
+from jvp_flash_attention_b200.gated import ACTIVATIONS, gated_linear
+from tests import _block_formulas as formulas
+from tests.test_gpu_gated import _check, _inputs
+
+pytestmark = pytest.mark.gpu
+
+
+def _plain(name):
+    return lambda x, wg, wu: formulas.activation(ACTIVATIONS[name], x @ wg.T)[0] * (x @ wu.T)
+
+
+@pytest.mark.parametrize("name", list(ACTIVATIONS))
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("M,K,F", [(90, 72, 136), (400, 128, 130)])
+def test_gradients_inside_a_level_carry_their_tangents(name, dt, M, K, F):
+    """By the symmetry of second derivatives the tangents are the gradients of <tgh, h> + <gh, th>."""
+    x, tx, wg, wu, gh, tgh = _inputs(M, K, F, dt, 31)
+    leaves = [t.requires_grad_() for t in (x, wg, wu)]
+    with fwAD.dual_level():
+        h = gated_linear(fwAD.make_dual(x, tx), wg, wu, name)
+        pairs = [fwAD.unpack_dual(d) for d in torch.autograd.grad(h, leaves, fwAD.make_dual(gh, tgh))]
+        first, second = (dict(zip(("dx", "dwg", "dwu"), ts)) for ts in zip(*pairs))
+    _check({k: v.detach() for k, v in first.items()}, x, None, wg, wu, gh, None, ACTIVATIONS[name])
+    _check({k: v.detach() for k, v in second.items()}, x, tx, wg, wu, tgh, gh, ACTIVATIONS[name])
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("M", [90, 400])
+def test_and_those_of_the_weights(dt, M):
+    """Against torch in float64.  An entry of x's is the rounded sum of two that are rounded: two gradients' bounds of the norm."""
+    x, tx, wg, wu, gh, tgh = _inputs(M, 72, 136, dt, 32)
+    tg, tu = (torch.randn(w.shape, generator=torch.Generator(device=w.device).manual_seed(7), device=w.device).to(w.dtype) * 0.3 * 72**-0.5
+              for w in (wg, wu))
+    leaves = [t.requires_grad_() for t in (x, wg, wu)]
+    with fwAD.dual_level():
+        h = gated_linear(*(fwAD.make_dual(p, t) for p, t in zip(leaves, (tx, tg, tu))))
+        pairs = [fwAD.unpack_dual(d) for d in torch.autograd.grad(h, leaves, fwAD.make_dual(gh, tgh))]
+        got = [t.detach() for p in zip(*pairs) for t in p]
+    gradient = lambda x, wg, wu, c: torch.func.vjp(_plain("silu"), x, wg, wu)[1](c)  # noqa: E731
+    want = torch.func.jvp(gradient, tuple(t.detach().double() for t in (x, wg, wu, gh)), tuple(t.double() for t in (tx, tg, tu, tgh)))
+    most = 2e-5 if dt == "fp32" else 8 * 2.0**-8
+    for a, b in zip(got, [t for p in want for t in p]):
+        assert (a.double() - b).norm() <= most * b.norm()
