@@ -371,7 +371,9 @@ constexpr const char* kThroughTangent = "the gradient through the tangent output
 // Inside a forward-AD level: a tensor's tangent, if it has one, and one put on a gradient.
 Tensor tangent_of(const Tensor& t) { return t.defined() ? t._fw_grad(0) : Tensor(); }
 void set_tangent(Tensor& t, const Tensor& tangent) {
-  if (t.defined() && tangent.defined()) t._set_fw_grad(tangent, /*level=*/0, /*is_inplace_op=*/false);
+  if (!t.defined() || !tangent.defined()) return;
+  if (t.is_view()) t = t.clone(at::MemoryFormat::Contiguous);  // (a view's would have to be one of its base's)
+  t._set_fw_grad(tangent, /*level=*/0, /*is_inplace_op=*/false);
 }
 // In place of a tangent that takes a third derivative, which there is no formula for: NaN, since none would be read as zero.  (The gradient
 // itself is right, and who does not ask for its tangent loses nothing.)
@@ -414,19 +416,34 @@ struct GatedGradNode : public Node {
     for (const Tensor& t : v)
       if (t.defined() && is_wrapped(t)) throw std::runtime_error("gated_linear cannot be differentiated a second time under a functorch transform");
     const Tensor x_ = x.unpack(), wg_ = wg.unpack(), wu_ = wu.unpack(), gh_ = gh.unpack();
-    const Tensor xp = unwrap(x_), wgp = unwrap(wg_), wup = unwrap(wu_);
+    variable_list plain, tangents;
+    for (const Tensor& t : v) plain.push_back(primal_of(t)), tangents.push_back(as_tangent(tangent_of(t), t));
+    out = along(plain, x_, wg_, wu_, gh_);
+    // Inside a forward-AD level: linear in v, and a third derivative where the operands move.
+    const bool moves = tangent_of(x_).defined() || tangent_of(gh_).defined();
+    if (moves) {
+      for (Tensor& t : out) set_tangent(t, unknown_like(t));
+    } else if (tangents[0].defined() || tangents[1].defined() || tangents[2].defined()) {
+      const variable_list t = along(tangents, x_, wg_, wu_, gh_);
+      for (int i = 0; i < 4; ++i) set_tangent(out[i], t[i]);
+    }
+    return out;
+  }
+  variable_list along(const variable_list& v, const Tensor& x_, const Tensor& wg_, const Tensor& wu_, const Tensor& gh_) {
+    variable_list out(4);
+    const Tensor xp = unwrap(primal_of(x_)), wgp = unwrap(wg_), wup = unwrap(wu_), ghp = unwrap(primal_of(gh_));
     const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1) || task_should_compute_output(2);
     if (v[1].defined() || v[2].defined()) {
       py::gil_scoped_acquire gil;
       NoFunctorch nf;
       at::AutoGradMode no_grad(false);
-      py::tuple h = gated_module().attr("_second")(xp, wgp, wup, unwrap(gh_), or_none(v[0]), or_none(v[1]), or_none(v[2]), activation);
+      py::tuple h = gated_module().attr("_second")(xp, wgp, wup, ghp, or_none(v[0]), or_none(v[1]), or_none(v[2]), activation);
       for (int i = 0; i < 4; ++i)
         if (task_should_compute_output(i)) out[i] = from_python(h[i]);
     } else {
       const GatedOut f = launch_gated_fwd(xp, v[0], wgp, wup, activation, need_x || need_w);
       if (need_x || need_w) {
-        const GatedGrads g = launch_gated_bwd(xp, v[0], wgp, wup, f.kept, Tensor(), unwrap(gh_), activation, need_x, false, need_w);
+        const GatedGrads g = launch_gated_bwd(xp, v[0], wgp, wup, f.kept, Tensor(), ghp, activation, need_x, false, need_w);
         out[0] = g.dx, out[1] = g.dwg, out[2] = g.dwu;
       }
       if (task_should_compute_output(3)) out[3] = f.th;
@@ -476,7 +493,7 @@ struct GatedNode : public Node {
     }
     if (gh.defined() && (again || !gth.defined())) {
       GatedGrads e = launch_gated_bwd(xp, txp, wgp, wup, kept_, gh, Tensor(), activation, need_x, false, need_w);
-      if (again) GatedGradNode::connect(e, activation, x_, wg_, wu_, gh);
+      if (again) GatedGradNode::connect(e, activation, x_dual, wg_, wu_, grads[0]);
       auto add = [](Tensor& to, const Tensor& t) {
         if (t.defined()) to = to.defined() ? to + t : t;
       };

@@ -126,3 +126,30 @@ def test_a_tangent_of_a_gradient_is_not_differentiated_again():
         with pytest.raises(RuntimeError, match="third time"):
             torch.autograd.grad(td.sum(), x, retain_graph=True)
         torch.autograd.grad(d.sum(), x)
+
+
+@pytest.mark.parametrize("wanted", ["x", "xgu"])
+def test_second_derivatives_inside_a_level(wanted):
+    """Linear in the vector they are taken along; a third derivative where the operands move, NaN beside what is right."""
+    i = _inputs(6)
+    leaves = [i[n].requires_grad_() for n in ("x", "wg", "wu", "gh")]
+    at = [n for n, k in enumerate("xgu") if k in wanted]
+    v, tv = [i[("tx", "tg", "tu")[k]] for k in at], [leaves[k].detach() for k in at]
+    want = []
+    for along in (v, tv):
+        grads = torch.autograd.grad(_plain("silu")(*leaves[:3]), [leaves[k] for k in at], leaves[3], create_graph=True)
+        want.append(torch.autograd.grad(grads, leaves, along))
+    with fwAD.dual_level():
+        grads = torch.autograd.grad(gated_linear(*leaves[:3]), [leaves[k] for k in at], leaves[3], create_graph=True)
+        got = torch.autograd.grad(grads, leaves, [fwAD.make_dual(a, b) for a, b in zip(v, tv)])
+        for d, w, m in zip(got, *want):
+            d, t = fwAD.unpack_dual(d)
+            torch.testing.assert_close(d, w)
+            torch.testing.assert_close(t, m)
+        moving = fwAD.make_dual(leaves[0], i["tx"])
+        grads = torch.autograd.grad(gated_linear(moving, *leaves[1:3]), [leaves[k] for k in at], leaves[3], create_graph=True)
+        got = torch.autograd.grad([fwAD.unpack_dual(d).primal for d in grads], leaves, v)
+        for d, w in zip(got, want[0]):
+            d, t = fwAD.unpack_dual(d)
+            torch.testing.assert_close(d, w)
+            assert t.isnan().all()
