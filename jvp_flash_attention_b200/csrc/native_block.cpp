@@ -476,9 +476,12 @@ struct GatedNode : public Node {
     const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1) || task_should_compute_output(2);
     const bool need_tx = num_outputs() > 3 && task_should_compute_output(3);
     if ((gh.defined() && is_wrapped(gh)) || (gth.defined() && is_wrapped(gth))) {
-      // the cotangents belong to a functorch transform, which differentiates Functions
+      // the cotangents belong to a functorch transform, which differentiates Functions (and takes their tangents along)
+      if (side_by_side && tangent_of(x_dual).defined())
+        throw std::runtime_error("inside a forward-AD level where gated_linear's weights have tangents, its gradient cannot be transformed");
       py::gil_scoped_acquire gil;
-      py::tuple d = gated_module().attr("_backward_under_functorch")(x_, or_none(tx_), wg_, wu_, kept_, or_none(gh), or_none(gth), activation);
+      py::tuple d = gated_module().attr("_backward_under_functorch")(x_dual, or_none(tx_), wg_, wu_, kept_, or_none(grads[0]),
+                                                                     or_none(grads.size() > 1 ? grads[1] : Tensor()), activation);
       const int at[] = {0, 3, 1, 2};  // of (dx, dtx, dwg, dwu) among the edges
       for (int i = 0; i < 4; ++i)
         if (at[i] < (int)out.size()) out[at[i]] = from_python(d[i]);

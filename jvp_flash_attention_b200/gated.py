@@ -20,6 +20,8 @@ from . import _lib
 from .jvp_attention import _JVP, _is_tracing, _peek_functorch, _require_cuda, _unwrap
 
 ACTIVATIONS = {"silu": 0, "sigmoid": 1, "gelu": 2, "gelu_tanh": 3}  # jvpfa_activation
+_THIRD = "gated_linear cannot be differentiated a third time"
+_THROUGH_TANGENT = "the gradient through the tangent output of gated_linear cannot be differentiated a second time"
 
 
 def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, activation: str = "silu") -> Tensor:
@@ -85,17 +87,18 @@ def _side_by_side(x, tx, w_gate, t_gate, w_up, t_up):
     return (cat(x, torch.zeros_like(x)), cat(or_zero(tx, x), x), cat(w_gate, or_zero(t_gate, w_gate)), cat(w_up, or_zero(t_up, w_up)))
 
 
-def _second(x, w_gate, w_up, gh, vx, v_gate, v_up, activation):
+def _second(x, w_gate, w_up, gh, vx, v_gate, v_up, activation, tgh=None):
     """The gradients of <(dx, dwg, dwu), (vx, v_gate, v_up)> with respect to x, w_gate, w_up and gh, where (dx, dwg, dwu) are those of <gh, h>: of
-    <gh, th> for the tangents v, and th itself."""
+    <gh, th> for the tangents v, and th itself.  The first three are also (dx, dwg, dwu)'s tangent along v, and with ``tgh``, which adds those of
+    <tgh, h>, along v and gh's tangent."""
     K = x.shape[-1]
     if v_gate is None and v_up is None:
         _, th, kept = _launch_fwd(x, vx, w_gate, w_up, activation, True)
-        dx, _, dwg, dwu = _launch_bwd(x, vx, w_gate, w_up, kept, None, gh, activation, True, False, True)
+        dx, _, dwg, dwu = _launch_bwd(x, vx, w_gate, w_up, kept, tgh, gh, activation, True, False, True)
         return dx, dwg, dwu, th
     wide = _side_by_side(x, vx, w_gate, v_gate, w_up, v_up)
     _, th, kept = _launch_fwd(*wide, activation, True)
-    dx, dtx, dwg, dwu = _launch_bwd(*wide, kept, None, gh, activation, True, True, True)
+    dx, dtx, dwg, dwu = _launch_bwd(*wide, kept, tgh, gh, activation, True, True, True)
     return dx[..., :K] + dtx[..., K:], dwg[:, :K], dwu[:, :K], th
 
 
@@ -186,8 +189,8 @@ class _Gated(Function):
     def backward(ctx, gh, *_):
         if gh is None:
             return None, None, None, None
-        x, w_gate, w_up, kept = (fwAD.unpack_dual(t).primal for t in ctx.saved_tensors)
-        return (*_GatedGrad.apply(x, None, w_gate, w_up, kept, fwAD.unpack_dual(gh).primal, ctx.activation), None)
+        x, w_gate, w_up, kept = ctx.saved_tensors
+        return (*_GatedGrad.apply(x, None, w_gate, w_up, kept, gh, ctx.activation), None)
 
 
 class _GatedTangent(Function):
@@ -206,17 +209,16 @@ class _GatedTangent(Function):
         ctx.set_materialize_grads(False)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gth, *_):
         if gth is None:
             return (None,) * 5
-        tensors = (_unwrap(t) for t in ctx.saved_tensors)
-        return (*_launch_bwd(*tensors, None, _unwrap(gth), ctx.activation, True, True, True), None)
+        dx, dtx, dwg, dwu = _GatedDualGrad.apply(*ctx.saved_tensors, gth, ctx.activation)
+        return dx, dtx, dwg, dwu, None
 
 
 class _GatedGrad(Function):
-    """(dx, dwg, dwu) of <gh, h>, differentiable once more.  ``tx``: of the forward that
-    left ``kept``, or None."""
+    """(dx, dwg, dwu) of <gh, h>, differentiable once more, in either direction.  ``tx``: of the forward that left ``kept``, or
+    None."""
 
     @staticmethod
     def forward(x, tx, w_gate, w_up, kept, gh, activation):
@@ -226,9 +228,17 @@ class _GatedGrad(Function):
 
     @staticmethod
     def setup_context(ctx, inputs, outputs):
-        x, _, w_gate, w_up, _, gh, ctx.activation = inputs
+        x, tx, w_gate, w_up, kept, gh, ctx.activation = inputs
         ctx.save_for_backward(x, w_gate, w_up, gh)
+        ctx.save_for_forward(x, tx, w_gate, w_up, kept, gh)
         ctx.set_materialize_grads(False)
+
+    @staticmethod
+    def jvp(ctx, vx, _, v_gate, v_up, __, tgh, ___):
+        x, tx, w_gate, w_up, kept, gh = ctx.saved_tensors
+        if vx is None and v_gate is None and v_up is None:  # linear in gh
+            return _GatedGrad.apply(x, tx, w_gate, w_up, kept, tgh, ctx.activation)
+        return _GatedGradTangent.apply(x, w_gate, w_up, gh, vx, v_gate, v_up, tgh, ctx.activation)
 
     @staticmethod
     @once_differentiable
@@ -238,6 +248,23 @@ class _GatedGrad(Function):
         tensors = [None if t is None else _unwrap(t) for t in (*ctx.saved_tensors, vx, v_gate, v_up)]
         dx, dwg, dwu, th = _second(*tensors, ctx.activation)
         return dx, None, dwg, dwu, None, th, None
+
+
+class _GatedGradTangent(Function):
+    """The tangents of (dx, dwg, dwu) of <gh, h>."""
+
+    @staticmethod
+    def forward(x, w_gate, w_up, gh, vx, v_gate, v_up, tgh, activation):
+        x, w_gate, w_up, gh, vx, v_gate, v_up, tgh = (None if t is None else _unwrap(t) for t in (x, w_gate, w_up, gh, vx, v_gate, v_up, tgh))
+        return _second(x, w_gate, w_up, gh, vx, v_gate, v_up, activation, tgh)[:3]
+
+    @staticmethod
+    def setup_context(ctx, inputs, outputs):
+        pass
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(_THIRD)
 
 
 class _GatedDualGrad(Function):
@@ -250,11 +277,19 @@ class _GatedDualGrad(Function):
 
     @staticmethod
     def setup_context(ctx, inputs, outputs):
-        pass
+        *tensors, ctx.activation = inputs
+        ctx.save_for_forward(*tensors[:-1])
+        ctx.set_materialize_grads(False)
+
+    @staticmethod
+    def jvp(ctx, vx, vtx, v_gate, v_up, _, tgth, __):
+        if vx is None and vtx is None and v_gate is None and v_up is None:  # linear in gth
+            return _GatedDualGrad.apply(*ctx.saved_tensors, tgth, ctx.activation)
+        return tuple(torch.full_like(t, torch.nan) for t in ctx.saved_tensors[:4])  # a third derivative, as the native layer's
 
     @staticmethod
     def backward(ctx, *grads):
-        raise RuntimeError("the gradient through the tangent output of gated_linear cannot be differentiated a second time")
+        raise RuntimeError(_THROUGH_TANGENT)
 
 
 def _backward_under_functorch(x, tx, w_gate, w_up, kept, gh, gth, activation):

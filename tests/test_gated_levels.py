@@ -153,3 +153,76 @@ def test_second_derivatives_inside_a_level(wanted):
             d, t = fwAD.unpack_dual(d)
             torch.testing.assert_close(d, w)
             assert t.isnan().all()
+
+
+@pytest.mark.parametrize("given", ["x", "g", "xgu"])
+@pytest.mark.parametrize("name", list(ACTIVATIONS))
+def test_torch_func_jvp_of_torch_func_grad(name, given):
+    i = _inputs(7)
+    at = [n for n, k in enumerate("xgu") if k in given]
+    primals, tangents = [i[n] for n in ("x", "wg", "wu")], [i[n] for n in ("tx", "tg", "tu")]
+
+    def loss(f):
+        def run(*some):
+            args = list(primals)
+            for k, t in zip(at, some):
+                args[k] = t
+            return ((args[0] + f(*args) @ i["wd"].T) ** 3).sum()
+        return run
+
+    got, want = (_forward_over_reverse(loss(f), [primals[k] for k in at], [tangents[k] for k in at])
+                 for f in (lambda *a: gated_linear(*a, name), _plain(name)))
+    for a, b in zip((*got[0], *got[1]), (*want[0], *want[1])):
+        torch.testing.assert_close(a, b)
+
+
+def test_torch_func_jvp_of_a_vjp():
+    """The gradient is linear in the cotangent, whether the graph is torch.func's or an ordinary one."""
+    i = _inputs(8)
+    _, vjp = torch.func.vjp(lambda *a: gated_linear(*a), i["x"], i["wg"], i["wu"])
+    want = [torch.func.vjp(_plain("silu"), i["x"], i["wg"], i["wu"])[1](c) for c in (i["gh"], i["tgh"])]
+    for a, b in zip(torch.func.jvp(vjp, (i["gh"],), (i["tgh"],)), want):
+        for d, w in zip(a, b):
+            torch.testing.assert_close(d, w)
+
+
+def test_torch_func_jvp_of_a_vjp_through_the_tangent():
+    i = _inputs(12)
+    along = lambda x, wg: torch.func.jvp(lambda v: gated_linear(v, wg, i["wu"]), (x,), (i["tx"],))  # noqa: E731
+    _, vjp = torch.func.vjp(along, i["x"], i["wg"])
+    cots, tangents = (i["gh"], i["tgh"]), (i["tgh"] - 1, i["gh"])
+    for a, b in zip(torch.func.jvp(vjp, (cots,), (tangents,)), (vjp(cots), vjp(tangents))):
+        for d, w in zip(a, b):
+            torch.testing.assert_close(d, w)
+    with pytest.raises(RuntimeError, match="cannot be differentiated a second time"):
+        torch.func.grad(lambda x: torch.func.grad(lambda v: along(v, i["wg"])[1].sum())(x).sum())(i["x"])
+
+
+@pytest.mark.parametrize("outputs", ["h", "t", "both"])
+def test_torch_func_jvp_of_the_cotangents_of_an_ordinary_graph(outputs):
+    i = _inputs(10)
+    leaves = [i[n].requires_grad_() for n in ("x", "tx", "wg", "wu")]
+    pick = {"h": [0], "t": [1], "both": [0, 1]}[outputs]
+    graph = torch.func.jvp(lambda v: gated_linear(v, *leaves[2:]), tuple(leaves[:1]), tuple(leaves[1:2]))
+    grads = lambda *c: torch.autograd.grad([graph[k] for k in pick], leaves[::2], c, retain_graph=True)  # noqa: E731
+    cots, tangents = (tuple(([i["gh"], i["tgh"]] if n == 0 else [i["tgh"] - 1, i["gh"]])[k] for k in pick) for n in (0, 1))
+    for a, b in zip(torch.func.jvp(grads, cots, tangents), (grads(*cots), grads(*tangents))):
+        for d, w in zip(a, b):
+            torch.testing.assert_close(d, w)
+
+
+def test_torch_func_grad_of_dual_tensors():
+    i = _inputs(11)
+    loss = lambda f: lambda v: (f(v, i["wg"], i["wu"]) ** 3).sum()  # noqa: E731
+    want = _forward_over_reverse(loss(_plain("silu")), [i["x"]], [i["tx"]])
+    with fwAD.dual_level():
+        got = fwAD.unpack_dual(torch.func.grad(loss(gated_linear))(fwAD.make_dual(i["x"], i["tx"])))
+        for a, (b,) in zip(got, want):
+            torch.testing.assert_close(a, b)
+
+
+def test_its_tangent_cannot_be_differentiated_a_third_time():
+    i = _inputs(9)
+    hvp = lambda x: torch.func.jvp(torch.func.grad(lambda v: (gated_linear(v, i["wg"], i["wu"]) ** 2).sum()), (x,), (i["tx"],))[1].sum()  # noqa: E731
+    with pytest.raises(RuntimeError, match="third time"):
+        torch.func.grad(hvp)(i["x"])

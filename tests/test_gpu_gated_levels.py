@@ -49,3 +49,19 @@ def test_and_those_of_the_weights(dt, M):
     most = 2e-5 if dt == "fp32" else 8 * 2.0**-8
     for a, b in zip(got, [t for p in want for t in p]):
         assert (a.double() - b).norm() <= most * b.norm()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_torch_func_jvp_of_a_vjp(dt):
+    """Forward over reverse under functorch, x and the weights moving, and the cotangent alone."""
+    x, tx, wg, wu, gh, tgh = _inputs(150, 72, 136, dt, 33)
+    gradient = lambda x, c: torch.func.vjp(lambda v: gated_linear(v, wg, wu), x)[1](c)[0]  # noqa: E731
+    dx, tdx = torch.func.jvp(gradient, (x, gh), (tx, tgh))
+    _check({"dx": dx}, x, None, wg, wu, gh, None, 0)
+    _check({"dx": tdx}, x, tx, wg, wu, tgh, gh, 0)
+    _, tdx = torch.func.jvp(lambda c: gradient(x, c), (gh,), (tgh,))
+    _check({"dx": tdx}, x, None, wg, wu, tgh, None, 0)
+    moving = lambda f: torch.func.jvp(lambda w, c: torch.func.vjp(lambda v: f(x.to(w.dtype), v, wu.to(w.dtype)), w)[1](c)[0],  # noqa: E731
+                                      *(tuple(t if f is gated_linear else t.double() for t in ts) for ts in ((wg, gh), (wu, tgh))))
+    for a, b in zip(moving(gated_linear), moving(_plain("silu"))):
+        assert (a.double() - b).norm() <= (2e-5 if dt == "fp32" else 8 * 2.0**-8) * b.norm()
