@@ -41,12 +41,18 @@ py::object dual(Tensor value, Tensor tangent, int64_t level) {
   value._set_fw_grad(tangent, /*level=*/0, /*is_inplace_op=*/false);
   return py::cast(value);
 }
-// The tangent in its value's type, and in memory (torch keeps some that are zero as a shape alone).
+// The tensor in memory: torch keeps some zeros as a shape alone.
+Tensor in_memory(const Tensor& t) {
+  if (!t.defined() || !t._is_zerotensor()) return t;
+  NoFunctorch nf;
+  return at::zeros(t.sizes(), t.options().requires_grad(false));
+}
+// The tangent in its value's type, and in memory.
 Tensor as_tangent(const Tensor& t, const Tensor& x) {
   if (!t.defined()) return t;
+  const Tensor y = in_memory(t);
   NoFunctorch nf;
-  if (t._is_zerotensor()) return at::zeros(t.sizes(), x.options().requires_grad(false));
-  return t.scalar_type() == x.scalar_type() ? t : t.to(x.scalar_type());
+  return y.scalar_type() == x.scalar_type() ? y : y.to(x.scalar_type());
 }
 
 // ---- rotary --------------------------------------------------------------------------------------------------------------
@@ -106,7 +112,7 @@ std::vector<Tensor> launch_rotary(std::vector<Tensor> xs, const std::vector<Orde
   }
   for (size_t i = 0; i < xs.size(); ++i) {
     if (!xs[i].defined()) continue;
-    Tensor x = xs[i];
+    Tensor x = xs[i] = in_memory(xs[i]);
     if (x.stride(3) != 1 && x.size(3) != 1) {
       NoFunctorch nf;
       at::AutoDispatchBelowADInplaceOrView below;
@@ -259,7 +265,8 @@ struct GatedGrads {
 Tensor from_python(const py::handle& o) { return o.is_none() ? Tensor() : o.cast<Tensor>(); }
 
 // (rows, K) with contiguous columns.
-Tensor as_rows(const Tensor& x) {
+Tensor as_rows(const Tensor& x_) {
+  const Tensor x = in_memory(x_);
   if (!x.defined() || (x.dim() == 2 && x.stride(1) == 1)) return x;
   NoFunctorch nf;
   at::AutoDispatchBelowADInplaceOrView below;
@@ -268,7 +275,8 @@ Tensor as_rows(const Tensor& x) {
   return r.stride(1) == 1 ? r : r.contiguous();
 }
 // Row-major, on a 16-byte boundary, of the type of `like`.
-Tensor as_dense(const Tensor& x, const Tensor& like) {
+Tensor as_dense(const Tensor& x_, const Tensor& like) {
+  const Tensor x = in_memory(x_);
   if (!x.defined()) return x;
   const bool aligned = (reinterpret_cast<uintptr_t>(x.const_data_ptr()) & 15u) == 0;
   if (x.is_contiguous() && aligned && x.scalar_type() == like.scalar_type()) return x;

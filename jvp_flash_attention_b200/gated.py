@@ -18,6 +18,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .jvp_attention import _JVP, _is_tracing, _peek_functorch, _require_cuda, _unwrap
+from .rotary import _in_memory
 
 ACTIVATIONS = {"silu": 0, "sigmoid": 1, "gelu": 2, "gelu_tanh": 3}  # jvpfa_activation
 _THIRD = "gated_linear cannot be differentiated a third time"
@@ -124,7 +125,7 @@ def _launch_bwd(x, tx, w_gate, w_up, kept, gh, gth, activation, need_x, need_tx,
     F, K = w_gate.shape
     x2, wg, wu = _rows(x), _rows(w_gate), _rows(w_up)
     tx2 = _rows(tx) if gth is not None else None
-    gh, gth = (None if c is None else c.to(x.dtype).contiguous() for c in (gh, gth))
+    gh, gth = (None if c is None else _in_memory(c).to(x.dtype).contiguous() for c in (gh, gth))
     make = torch.empty if x.numel() else torch.zeros
     out = [make(shape, device=x.device, dtype=x.dtype) if wanted else None
            for wanted, shape in ((need_x, x.shape), (need_tx and gth is not None, x.shape), (need_w, (F, K)), (need_w, (F, K)))]
@@ -139,6 +140,7 @@ def _launch_bwd(x, tx, w_gate, w_up, kept, gh, gth, activation, need_x, need_tx,
 
 
 def _rows(t):
+    t = _in_memory(t)
     t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 else t.contiguous()
 

@@ -119,8 +119,14 @@ def _check(q, k, inv_freq, positions) -> None:
     _require_cuda(q)
 
 
+def _in_memory(t):
+    """The plain tensor in memory: torch keeps some zeros as a shape alone."""
+    return torch.zeros(t.shape, dtype=t.dtype, device=t.device) if t._is_zerotensor() else t
+
+
 def _launch(x, inv_freq, positions, offset, interleaved, amplitude, transposed):
     """Runs jvpfa_rotary on one plain tensor and returns the result."""
+    x = _in_memory(x)
     if x.stride(-1) != 1:
         x = x.contiguous()
     y = torch.empty_like(x)
