@@ -125,7 +125,7 @@ def _launch_bwd(x, tx, w_gate, w_up, kept, gh, gth, activation, need_x, need_tx,
     F, K = w_gate.shape
     x2, wg, wu = _rows(x), _rows(w_gate), _rows(w_up)
     tx2 = _rows(tx) if gth is not None else None
-    gh, gth = (None if c is None else _in_memory(c).to(x.dtype).contiguous() for c in (gh, gth))
+    gh, gth = (None if c is None else _dense(c, x.dtype) for c in (gh, gth))
     make = torch.empty if x.numel() else torch.zeros
     out = [make(shape, device=x.device, dtype=x.dtype) if wanted else None
            for wanted, shape in ((need_x, x.shape), (need_tx and gth is not None, x.shape), (need_w, (F, K)), (need_w, (F, K)))]
@@ -143,6 +143,12 @@ def _rows(t):
     t = _in_memory(t)
     t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 else t.contiguous()
+
+
+def _dense(t, dtype):
+    """Row-major and on a 16-byte boundary, where the entry wants a cotangent (a slice of a longer one begins anywhere)."""
+    t = _in_memory(t).to(dtype).contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
 
 
 def _describe(a, x, tx, wg, wu, activation):

@@ -65,3 +65,22 @@ def test_torch_func_jvp_of_a_vjp(dt):
                                       *(tuple(t if f is gated_linear else t.double() for t in ts) for ts in ((wg, gh), (wu, tgh))))
     for a, b in zip(moving(gated_linear), moving(_plain("silu"))):
         assert (a.double() - b).norm() <= (2e-5 if dt == "fp32" else 8 * 2.0**-8) * b.norm()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_cotangents_that_begin_between_16_byte_pieces(dt):
+    """Of a loss that concatenates something in front of h, where rows of F = 37 end anywhere: torch.func.grad, and a second derivative through
+    the weights, which reads the first one's cotangent."""
+    x, _, wg, wu, gh, _ = _inputs(21, 72, 37, dt, 34)
+    front = torch.randn(3, 37, device=x.device).to(x.dtype)
+    c = torch.cat((front, gh)) * 2
+    behind = lambda f: lambda v, w: torch.cat((front.to(v.dtype), f(v, w, wu.to(v.dtype))))  # noqa: E731
+    got = torch.func.grad(lambda v, w: (behind(gated_linear)(v, w) * c).sum(), argnums=(0, 1))(x, wg)
+    _check(dict(zip(("dx", "dwg"), got)), x, None, wg, wu, c[3:], None, 0)
+    second = []
+    for f in (gated_linear, _plain("silu")):
+        leaves = [(t if f is gated_linear else t.double()).detach().requires_grad_() for t in (x, wg)]
+        (dw,) = torch.autograd.grad(behind(f)(*leaves), leaves[1], c.to(leaves[0].dtype), create_graph=True)
+        second.append(torch.autograd.grad(dw, leaves, wu.to(dw.dtype)))
+    for a, b in zip(*second):
+        assert (a.double() - b).norm() <= (2e-5 if dt == "fp32" else 8 * 2.0**-8) * b.norm()
