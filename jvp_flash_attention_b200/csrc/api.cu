@@ -397,13 +397,16 @@ int64_t jvpfa_gated_kept_bytes(int dtype, int32_t M, int32_t F, int tangent) {
 }
 
 int64_t jvpfa_gated_fwd_workspace(const jvpfa_gated_fwd_args* a) {
-  return validate_gated_fwd(a) == JVPFA_OK ? gated_fwd_workspace(*a) : 0;
+  int64_t bytes = 0;
+  return validate_gated_fwd(a) == JVPFA_OK && plan_gated_fwd(*a, &bytes) == JVPFA_OK ? bytes : 0;
 }
 
 int jvpfa_gated_fwd(const jvpfa_gated_fwd_args* a, void* stream) {
   int rc = validate_gated_fwd(a);
   if (rc) return rc;
-  const int64_t need = gated_fwd_workspace(*a);
+  int64_t need = 0;
+  rc = plan_gated_fwd(*a, &need);  // (a call that is too large has no workspace that one could ask for)
+  if (rc) return rc;
   if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return JVPFA_ERR_NULL;
   rc = check_arch();
   if (rc) return rc;
@@ -412,13 +415,16 @@ int jvpfa_gated_fwd(const jvpfa_gated_fwd_args* a, void* stream) {
 }
 
 int64_t jvpfa_gated_bwd_workspace(const jvpfa_gated_bwd_args* a) {
-  return validate_gated_bwd(a) == JVPFA_OK ? gated_bwd_workspace(*a) : 0;
+  int64_t bytes = 0;
+  return validate_gated_bwd(a) == JVPFA_OK && plan_gated_bwd(*a, &bytes) == JVPFA_OK ? bytes : 0;
 }
 
 int jvpfa_gated_bwd(const jvpfa_gated_bwd_args* a, void* stream) {
   int rc = validate_gated_bwd(a);
   if (rc) return rc;
-  const int64_t need = gated_bwd_workspace(*a);
+  int64_t need = 0;
+  rc = plan_gated_bwd(*a, &need);  // (a call that is too large has no workspace that one could ask for)
+  if (rc) return rc;
   if (!a->workspace || a->workspace_bytes < need) return JVPFA_ERR_NULL;
   rc = check_arch();
   if (rc) return rc;

@@ -614,9 +614,9 @@ int launch_mask_tiles(const jvpfa_mask_tiles_args& a, cudaStream_t stream);
 int launch_pad_bias(const jvpfa_pad_bias_args& a, cudaStream_t stream);
 int launch_rotary(const jvpfa_rotary_args& a, cudaStream_t stream);
 int64_t gated_kept_bytes(int dtype, int64_t M, int64_t F, bool tangent);
-int64_t gated_fwd_workspace(const jvpfa_gated_fwd_args& a);
+int plan_gated_fwd(const jvpfa_gated_fwd_args& a, int64_t* workspace);  // a status, and the bytes of scratch
 int launch_gated_fwd(const jvpfa_gated_fwd_args& a, cudaStream_t stream);
-int64_t gated_bwd_workspace(const jvpfa_gated_bwd_args& a);
+int plan_gated_bwd(const jvpfa_gated_bwd_args& a, int64_t* workspace);  // a status, and the bytes of scratch
 int launch_gated_bwd(const jvpfa_gated_bwd_args& a, cudaStream_t stream);
 int launch_fwd_tc5(const jvpfa_fwd_args& a, cudaStream_t stream);
 bool fwd_tc5_eligible(const jvpfa_fwd_args& a);

@@ -363,13 +363,15 @@ void few_weights(const Args& a, Plan& plan, FewMaps& maps, bool& ok) {
 }  // namespace
 
 int64_t gated_kept_bytes(int dtype, int64_t M, int64_t F, bool tangent) { return kept_bytes(dtype, M, F, tangent); }
-int64_t gated_fwd_workspace(const jvpfa_gated_fwd_args& a) {
+int plan_gated_fwd(const jvpfa_gated_fwd_args& a, int64_t* workspace) {
   const FwdPlan plan(a);
-  return plan.rc ? 0 : plan.bytes;
+  *workspace = plan.bytes;
+  return plan.rc;
 }
-int64_t gated_bwd_workspace(const jvpfa_gated_bwd_args& a) {
+int plan_gated_bwd(const jvpfa_gated_bwd_args& a, int64_t* workspace) {
   const BwdPlan plan(a);
-  return plan.rc ? 0 : plan.bytes;
+  *workspace = plan.bytes;
+  return plan.rc;
 }
 
 int launch_gated_fwd(const jvpfa_gated_fwd_args& a, cudaStream_t s) {
