@@ -14,7 +14,7 @@ struct Activated {
   float a, d1, d2;
 };
 // sigmoid(x) and sigmoid(-x), each with its own relative precision: neither is one minus the other.
-// (exp(-|x|) cannot overflow: gates of any size have their limits, and NaN stays NaN.)
+// (exp(-|x|) cannot overflow, and NaN stays NaN.)
 template <bool EXACT>
 __device__ __forceinline__ void sigmoids(float x, float& s, float& r) {
   const float e = EXACT ? expf(-fabsf(x)) : fast_exp(-fabsf(x));
@@ -22,6 +22,9 @@ __device__ __forceinline__ void sigmoids(float x, float& s, float& r) {
   s = x >= 0.f ? big : small;
   r = x >= 0.f ? small : big;
 }
+// What a decaying factor multiplies: the gate itself up to 32, where that factor has long been zero (gelu: exp(-512); its tanh form: below
+// exp(-2000)).  Powers of the gate stay finite, so that zero times one is zero: all finite gates have the limits of a, a' and a''.
+__device__ __forceinline__ float within(float g) { return fminf(fmaxf(g, -32.f), 32.f); }
 template <int KIND, bool EXACT>
 __device__ __forceinline__ Activated activate(float g) {
   Activated y;
@@ -36,14 +39,15 @@ __device__ __forceinline__ Activated activate(float g) {
     }
   } else if constexpr (KIND == JVPFA_ACT_GELU) {
     const float p = normcdff(g), d = 0.3989422804014327f * (EXACT ? expf(-0.5f * g * g) : fast_exp(-0.5f * g * g));
-    y.a = g * p, y.d1 = p + g * d, y.d2 = d * (2.f - g * g);
+    const float w = within(g);
+    y.a = g * p, y.d1 = p + w * d, y.d2 = d * (2.f - w * w);
   } else {
     // 0.5 (1 + tanh z) = sigmoid(2 z), z = c (g + c3 g^3)
     constexpr float c = 0.7978845608028654f, c3 = 0.044715f;
     float s, r;
     sigmoids<EXACT>(2.f * c * (g + c3 * g * g * g), s, r);
-    const float z1 = 2.f * c * (1.f + 3.f * c3 * g * g), z2 = 12.f * c * c3 * g, d = s * r;
-    y.a = g * s, y.d1 = s + g * d * z1, y.d2 = d * (2.f * z1 + g * (z2 + (r - s) * z1 * z1));
+    const float w = within(g), z1 = 2.f * c * (1.f + 3.f * c3 * w * w), z2 = 12.f * c * c3 * w, d = s * r;
+    y.a = g * s, y.d1 = s + w * d * z1, y.d2 = d * (2.f * z1 + w * (z2 + (r - s) * z1 * z1));
   }
   return y;
 }

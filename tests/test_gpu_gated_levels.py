@@ -7,7 +7,7 @@ import torch.autograd.forward_ad as fwAD
 from jvp_flash_attention_b200 import _lib
 from jvp_flash_attention_b200.gated import ACTIVATIONS, gated_linear
 from tests import _block_formulas as formulas
-from tests.test_gpu_gated import _check, _inputs
+from tests.test_gpu_gated import _check, _inputs, _run
 
 pytestmark = pytest.mark.gpu
 
@@ -84,3 +84,32 @@ def test_cotangents_that_begin_between_16_byte_pieces(dt):
         second.append(torch.autograd.grad(dw, leaves, wu.to(dw.dtype)))
     for a, b in zip(*second):
         assert (a.double() - b).norm() <= (2e-5 if dt == "fp32" else 8 * 2.0**-8) * b.norm()
+
+
+@pytest.mark.parametrize("name", list(ACTIVATIONS))
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("M", [10, 200])
+def test_second_derivatives_of_far_gates(name, dt, M):
+    """Gates of 40.7 to 1e36 to either side, with u = 1, tg = 1, tu = 0 and gth = 1: the cotangents are dg = a'', du = dtg = a', dtu = a, whose sums over 64
+    features or M rows are finite (the largest, in dwu, below 2 M 1e36), and a'' and a' have their limits, 0 and 0 or 1.
+
+    They are off by no more than (2 + |g|) exp(-|g|), which falls: 42.7 exp(-40.7) = 9.1e-17 < 2^-53 for a' and a'', and with the factor |g| that dwg
+    has from x, 3.7e-15 < 2^-47.  Next to 1 that is nothing; beside 0 the sums are off by 64 or M of it."""
+    K, F = 8, 64
+    x, _, wg, wu, _, gth = _inputs(M, K, F, dt, 35)
+    far = 10.0 ** torch.linspace(1.61, 36, M // 2, device=x.device)
+    with torch.no_grad():
+        for t in (x, wg, wu):
+            t.zero_()
+        x[:, 0], x[:, 1], wg[:, 0], wu[:, 1] = torch.cat((far, -far)).to(x.dtype), 1, 1, 1
+        tx = torch.zeros_like(x)
+        tx[:, 0] = 1
+    got = _run(x, tx, wg, wu, None, torch.ones_like(gth), name, "jvp_bwd_t")
+    _check(got, x, tx, wg, wu, None, torch.ones_like(gth), ACTIVATIONS[name])
+    up = (x[:, 0] > 0).to(x.dtype) * (name != "sigmoid")
+    near = lambda y, limit, off: torch.testing.assert_close(y, limit, rtol=0, atol=off)  # noqa: E731
+    near(got["th"], up[:, None].expand(M, F), 2.0**-53)
+    near(got["dx"][:, 0], torch.zeros_like(up), 64 * 2.0**-53)
+    near(got["dx"][:, 1], 64 * up, 64 * 2.0**-53)
+    near(got["dtx"][:, 0], 64 * up, 64 * 2.0**-53)
+    near(got["dwg"][:, 0], up.sum().expand(F), M * 2.0**-47)
