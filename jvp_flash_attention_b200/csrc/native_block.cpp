@@ -478,6 +478,9 @@ struct GatedNode : public Node {
     variable_list out(num_outputs());
     const Tensor gh = primal_of(grads[0]), gth = grads.size() > 1 ? primal_of(grads[1]) : Tensor();
     if (!gh.defined() && !gth.defined()) return out;
+    for (const Tensor& g : grads)
+      TORCH_CHECK_NOT_IMPLEMENTED(!g.defined() || !g.key_set().has(c10::DispatchKey::Batched),
+                                  "gated_linear has no rule for torch.autograd.grad(is_grads_batched=True)");
     const Tensor x_dual = x.unpack(), x_ = primal_of(x_dual), wg_ = primal_of(wg.unpack()), wu_ = primal_of(wu.unpack());
     const Tensor xp = unwrap(x_), wgp = unwrap(wg_), wup = unwrap(wu_);
     const Tensor tx_ = num_outputs() > 3 ? tx.unpack() : Tensor(), txp = unwrap(tx_), kept_ = unwrap(kept.unpack());

@@ -22,6 +22,7 @@ from .rotary import _in_memory
 
 ACTIVATIONS = {"silu": 0, "sigmoid": 1, "gelu": 2, "gelu_tanh": 3}  # jvpfa_activation
 _THIRD = "gated_linear cannot be differentiated a third time"
+_ALONG_TANGENT = "the tangent output of gated_linear cannot be differentiated by a further forward transform"
 _THROUGH_TANGENT = "the gradient through the tangent output of gated_linear cannot be differentiated a second time"
 
 
@@ -40,7 +41,8 @@ def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, activation: str = "sil
     at twice the depth (where a weight's tangent is not finite, neither is the value there); the gradient through the tangent output cannot
     be differentiated again.  Gradients that are taken inside a forward-AD level carry their tangents (Hessian-vector products), which is a
     further backward: take them behind the level where only they are wanted.  The tangent of one through the tangent output would be a third
-    derivative; it is NaN.
+    derivative; it is NaN.  Under ``torch.func`` ``jvp``, ``vjp`` and ``grad`` nest as far as that goes; ``jvp`` of ``jvp`` and ``vmap`` (so
+    ``jacfwd``, ``jacrev`` and ``hessian``) are refused, and batched cotangents of ``torch.autograd.grad``.
     """
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation is one of {', '.join(ACTIVATIONS)}; got {activation!r}")
@@ -170,7 +172,16 @@ def _run(a, x, entry):
     _lib.check(_lib._launch(x, getattr(lib, entry), a), entry)
 
 
-class _Gated(Function):
+class _Operator(Function):
+    """A launch as torch.autograd and torch.func's jvp, vjp and grad see it."""
+
+    @staticmethod
+    def vmap(info, in_dims, *args):
+        raise NotImplementedError("gated_linear has no rule for torch.func.vmap (nor for jacfwd, jacrev and hessian, which are made of it): "
+                                  "the rows of x are a batch already")
+
+
+class _Gated(_Operator):
     """h, and what its backward reads."""
 
     @staticmethod
@@ -201,7 +212,7 @@ class _Gated(Function):
         return (*_GatedGrad.apply(x, None, w_gate, w_up, kept, gh, ctx.activation), None)
 
 
-class _GatedTangent(Function):
+class _GatedTangent(_Operator):
     """th, differentiable once with respect to x, its tangent and the weights."""
 
     @staticmethod
@@ -217,6 +228,10 @@ class _GatedTangent(Function):
         ctx.set_materialize_grads(False)
 
     @staticmethod
+    def jvp(ctx, *tangents):
+        raise RuntimeError(_ALONG_TANGENT)
+
+    @staticmethod
     def backward(ctx, gth, *_):
         if gth is None:
             return (None,) * 5
@@ -224,7 +239,7 @@ class _GatedTangent(Function):
         return dx, dtx, dwg, dwu, None
 
 
-class _GatedGrad(Function):
+class _GatedGrad(_Operator):
     """(dx, dwg, dwu) of <gh, h>, differentiable once more, in either direction.  ``tx``: of the forward that left ``kept``, or
     None."""
 
@@ -258,7 +273,7 @@ class _GatedGrad(Function):
         return dx, None, dwg, dwu, None, th, None
 
 
-class _GatedGradTangent(Function):
+class _GatedGradTangent(_Operator):
     """The tangents of (dx, dwg, dwu) of <gh, h>."""
 
     @staticmethod
@@ -271,11 +286,15 @@ class _GatedGradTangent(Function):
         pass
 
     @staticmethod
+    def jvp(ctx, *tangents):
+        raise RuntimeError(_THIRD)
+
+    @staticmethod
     def backward(ctx, *grads):
         raise RuntimeError(_THIRD)
 
 
-class _GatedDualGrad(Function):
+class _GatedDualGrad(_Operator):
     """(dx, dtx, dwg, dwu) of <gth, th>."""
 
     @staticmethod

@@ -226,3 +226,25 @@ def test_its_tangent_cannot_be_differentiated_a_third_time():
     hvp = lambda x: torch.func.jvp(torch.func.grad(lambda v: (gated_linear(v, i["wg"], i["wu"]) ** 2).sum()), (x,), (i["tx"],))[1].sum()  # noqa: E731
     with pytest.raises(RuntimeError, match="third time"):
         torch.func.grad(hvp)(i["x"])
+
+
+def test_transforms_that_are_refused():
+    i = _inputs(13)
+    f = lambda x: gated_linear(x, i["wg"], i["wu"])  # noqa: E731
+    along = lambda x: torch.func.jvp(f, (x,), (i["tx"],))[1]  # noqa: E731
+    with pytest.raises(RuntimeError, match="by a further forward transform"):
+        torch.func.jvp(along, (i["x"],), (i["tx"],))
+    grad = torch.func.grad(lambda x: (f(x) ** 2).sum())
+    with pytest.raises(RuntimeError, match="by a further forward transform|third time"):
+        torch.func.jvp(lambda x: torch.func.jvp(grad, (x,), (i["tx"],))[1], (i["x"],), (i["tx"],))
+    for call in (lambda: torch.func.vmap(f)(i["x"]), lambda: torch.func.vmap(grad)(i["x"]), lambda: torch.func.jacfwd(f)(i["x"]),
+                 lambda: torch.func.jacrev(f)(i["x"]), lambda: torch.func.hessian(lambda x: f(x).sum())(i["x"]),
+                 lambda: torch.func.vmap(lambda w: gated_linear(i["x"], w, i["wu"]))(torch.stack((i["wg"], i["wu"])))):
+        with pytest.raises(NotImplementedError, match="gated_linear has no rule for torch.func.vmap"):
+            call()
+    x = i["x"].requires_grad_()
+    h = f(x)
+    with pytest.raises(NotImplementedError, match="gated_linear has no rule for torch.func.vmap"):  # an ordinary graph
+        torch.func.vmap(lambda c: torch.autograd.grad(h, x, c, retain_graph=True)[0])(torch.stack((i["gh"], i["tgh"])))
+    with pytest.raises(NotImplementedError, match="gated_linear has no rule for .*is_grads_batched"):
+        torch.autograd.grad(h, x, torch.stack((i["gh"], i["tgh"])), is_grads_batched=True)
