@@ -25,6 +25,8 @@ namespace {
 // Warps 0: TMA, 1: products, 2: TMEM, from 4 on: fp32 weights, results
 template <typename T>
 constexpr int kFewThreads = sizeof(T) == 4 ? 640 : 384;
+template <typename T>
+constexpr int kFewResident = sizeof(T) == 4 ? 1 : 3;  // CTAs that plan_few counts on an SM's registers for: 56 a thread in 16 bits
 constexpr int kSplitThreads = 512, kUnits = 1024 / kSplitThreads;  // fp32: a k-block's 1024 pieces of eight entries
 constexpr int kAbortFewFull = 18, kAbortFewEmpty = 19, kAbortFewAcc = 20, kAbortFewAccEmpty = 21;
 constexpr int kTakeUp = 4;   // fp32: k-blocks between two looks at the accumulators
@@ -125,7 +127,7 @@ struct Piece8 {
 
 // BIG: more than 64 columns (fp32: a thread holds 32 sums, and has one k-block less under way).
 template <typename T, int KIND, bool BIG>
-__global__ void __launch_bounds__(kFewThreads<T>, 1) few_kernel(const __grid_constant__ FewArgs p, const __grid_constant__ FewMaps maps) {
+__global__ void __launch_bounds__(kFewThreads<T>, kFewResident<T>) few_kernel(const __grid_constant__ FewArgs p, const __grid_constant__ FewMaps maps) {
   constexpr int PARTS = FewOperand<T>::kParts;
   constexpr bool SPLIT = PARTS > 1, GATED = KIND == kFewGated;
   extern __shared__ uint8_t raw[];
