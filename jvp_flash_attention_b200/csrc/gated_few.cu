@@ -423,9 +423,13 @@ bool plan_few(int dtype, int kind, FewArgs& p) {
   const int rest = p.tiles - p.whole;
   p.cluster = 1;
   while (p.cluster < 8 && rest * 2 * p.cluster <= at_once && 4 * p.cluster <= p.steps) p.cluster *= 2;
-  // Room for stages: fp32 one CTA an SM, whose registers hold what is under way; else two CTAs, or three where two do not take all tiles in one round
-  // (4 rows of bf16 K4096 F20000 73 -> 60 us; of F11008 35 -> 37).  The sums take the stages' place at the end.
-  const int stage = parts * (kTile + N * 128), room = parts > 1 ? 224 * 1024 : p.tiles > 2 * device_sms() ? 74 * 1024 : 108 * 1024;
+  // Room for stages: fp32 one CTA an SM, whose registers hold what is under way; else two CTAs, or three, with less under way each, where they take
+  // the tiles in fewer rounds.  us of bf16 K2048 with two and with three, 1 row / 32 / 100, values and tangents alike: F11008 (172 tiles) 19.2, 20.5, 26.1
+  // and 20.2, 22.6, 30.6; F20000 (313) 40.4, 43.0, 49.0 and 31.4, 32.7, 38.5; F28672 (448, two rounds of either) 43.2, 45.8, 55.0 and 47.2, 51.4, 66.7;
+  // F40000 (625) 63.3, 68.0, 79.4 and 55.1, 60.3, 73.0; dx of K40960 F1024 (320) 38.7, 42.2, 54.3 and 26.7, 29.6, 42.9.  The sums take the stages' place
+  // at the end.
+  const auto rounds = [&](int ctas) { return (p.tiles + ctas * device_sms() - 1) / (ctas * device_sms()); };
+  const int stage = parts * (kTile + N * 128), room = parts > 1 ? 224 * 1024 : rounds(3) < rounds(2) ? 74 * 1024 : 108 * 1024;
   p.stages = room / stage < 8 ? room / stage : 8;
   if (p.stages * stage < N * 512) return false;
   p.tmem_columns = 32;
