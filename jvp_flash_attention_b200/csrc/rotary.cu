@@ -5,7 +5,7 @@
 //
 // Angles.  position * frequency passes 10^6 radians in long contexts, where 32 bits leave no digit of the fraction of a turn that
 // counts.  The product is formed in 64 bits as turns, its fraction is exact there, and only that is rounded to 32 bits
-// (at most 2^-25 turns, 1.9e-7 radians) for sincospif.
+// (by at most 2^-26 turns, 9.4e-8 radians, as the fraction is within half a turn) for sincospif.
 //
 // What bounds it: memory, each tensor read and written once.  A thread takes the pairs of one row's 2 * 16 bytes and goes through
 // several heads with the same cosines, so that their cost (a few 64-bit products, some 25 instructions for each pair) is shared.

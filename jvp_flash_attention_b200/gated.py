@@ -33,14 +33,16 @@ def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, activation: str = "sil
     bfloat16, float16 or float32, of one type and device.  ``activation``: ``"silu"``, ``"sigmoid"``, ``"gelu"`` (exact) or ``"gelu_tanh"``.
     Rows of whole 16-byte pieces (K a multiple of 8) are read in place, others, and float32, through a copy.
 
-    Sums are in 32 bits, and the result is rounded once.  For a backward the projections are kept in 24 bits an entry (float32: 32); their
-    cotangents are rounded to x's type, so where one passes float16's 65504 the gradients of its row are not finite.  float32 is multiplied as three bfloat16 parts, about 1e-6 relative,
-    whatever ``set_fp32_precision`` says of attention; an infinite entry gives NaN in its row.  Results are the same from run to run.
+    Sums are in 32 bits (16-bit types': the tensor cores' accumulators, which round towards zero every 16 terms), activations of 16-bit types within
+    ``2**-17 (1 + |g|)``, and the result is rounded once.  For a backward the projections are kept in 24 bits an entry (float32: 32); their
+    cotangents are rounded to x's type, so where one passes float16's 65504 the gradients of its row are not finite.  float32 is multiplied as
+    three bfloat16 parts, about 1e-6 relative, whatever ``set_fp32_precision`` says of attention; an infinite entry gives NaN in its row.  Results
+    are the same from run to run.
 
     Tangents of the weights, and a second differentiation of their gradients, run on operands side by side, ``[tx | x]`` and ``[w | tw]``,
     at twice the depth (where a weight's tangent is not finite, neither is the value there); the gradient through the tangent output cannot
-    be differentiated again.  Gradients that are taken inside a forward-AD level carry their tangents (Hessian-vector products), which is a
-    further backward: take them behind the level where only they are wanted.  The tangent of one through the tangent output would be a third
+    be differentiated again.  Gradients that are taken inside a forward-AD level carry their tangents (Hessian-vector products; attention's do
+    not), which is a further backward: take them behind the level where only they are wanted.  The tangent of one through the tangent output would be a third
     derivative; it is NaN.  Under ``torch.func`` ``jvp``, ``vjp`` and ``grad`` nest as far as that goes; ``jvp`` of ``jvp`` and ``vmap`` (so
     ``jacfwd``, ``jacrev`` and ``hessian``) are refused, and batched cotangents of ``torch.autograd.grad``.
     """
