@@ -14,7 +14,6 @@ import torch
 import torch.autograd.forward_ad as fwAD
 from torch import Tensor
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .jvp_attention import _JVP, _is_tracing, _peek_functorch, _require_cuda, _unwrap
@@ -183,6 +182,13 @@ class _Operator(Function):
                                   "the rows of x are a batch already")
 
 
+def _unknown(like, message):
+    """Tangents that take a third derivative: refused where a transform asks for them, NaN inside a forward-AD level (as the native layer's)."""
+    if _peek_functorch() is not None:
+        raise RuntimeError(message)
+    return tuple(torch.full_like(t, torch.nan) for t in like)
+
+
 class _Gated(_Operator):
     """h, and what its backward reads."""
 
@@ -266,13 +272,35 @@ class _GatedGrad(_Operator):
         return _GatedGradTangent.apply(x, w_gate, w_up, gh, vx, v_gate, v_up, tgh, ctx.activation)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, vx, v_gate, v_up):
         if vx is None and v_gate is None and v_up is None:
             return (None,) * 7
-        tensors = [None if t is None else _unwrap(t) for t in (*ctx.saved_tensors, vx, v_gate, v_up)]
-        dx, dwg, dwu, th = _second(*tensors, ctx.activation)
+        dx, dwg, dwu, th = _GatedSecond.apply(*ctx.saved_tensors, vx, v_gate, v_up, ctx.activation)
         return dx, None, dwg, dwu, None, th, None
+
+
+class _GatedSecond(_Operator):
+    """``_second``: differentiable in the tangents v, which it is linear in, and forward only."""
+
+    @staticmethod
+    def forward(x, w_gate, w_up, gh, vx, v_gate, v_up, activation):
+        return _second(*(None if t is None else _unwrap(t) for t in (x, w_gate, w_up, gh, vx, v_gate, v_up)), activation)
+
+    @staticmethod
+    def setup_context(ctx, inputs, outputs):
+        *tensors, ctx.activation = inputs
+        ctx.save_for_forward(*tensors[:4])
+        ctx.set_materialize_grads(False)
+
+    @staticmethod
+    def jvp(ctx, tx, t_gate, t_up, tgh, vx, v_gate, v_up, _):
+        if tx is None and t_gate is None and t_up is None and tgh is None:
+            return _GatedSecond.apply(*ctx.saved_tensors, vx, v_gate, v_up, ctx.activation)
+        return _unknown(ctx.saved_tensors, _THIRD)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(_THIRD)
 
 
 class _GatedGradTangent(_Operator):
@@ -314,7 +342,7 @@ class _GatedDualGrad(_Operator):
     def jvp(ctx, vx, vtx, v_gate, v_up, _, tgth, __):
         if vx is None and vtx is None and v_gate is None and v_up is None:  # linear in gth
             return _GatedDualGrad.apply(*ctx.saved_tensors, tgth, ctx.activation)
-        return tuple(torch.full_like(t, torch.nan) for t in ctx.saved_tensors[:4])  # a third derivative, as the native layer's
+        return _unknown(ctx.saved_tensors[:4], _THROUGH_TANGENT)
 
     @staticmethod
     def backward(ctx, *grads):

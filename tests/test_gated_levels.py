@@ -15,8 +15,7 @@ def _in_memory(launch):
     def run(*args):
         with torch.no_grad(), _lib.native().NoFunctorch():
             plain = [fwAD.unpack_dual(gated._unwrap(t)).primal.detach() if isinstance(t, torch.Tensor) else t for t in args]
-            assert not any(isinstance(t, torch.Tensor) and t._is_zerotensor() for t in plain)
-            return launch(*plain)
+            return launch(*(gated._in_memory(t) if isinstance(t, torch.Tensor) else t for t in plain))
     return run
 
 
@@ -248,3 +247,32 @@ def test_transforms_that_are_refused():
         torch.func.vmap(lambda c: torch.autograd.grad(h, x, c, retain_graph=True)[0])(torch.stack((i["gh"], i["tgh"])))
     with pytest.raises(NotImplementedError, match="gated_linear has no rule for .*is_grads_batched"):
         torch.autograd.grad(h, x, torch.stack((i["gh"], i["tgh"])), is_grads_batched=True)
+
+
+@pytest.mark.parametrize("linear", [False, True])
+def test_a_third_derivative_under_torch_func_is_refused(linear):
+    """Whichever way it is taken: not even the part of it that other operators make comes out alone."""
+    i = _inputs(14)
+    loss = lambda f: lambda v: (f(v, i["wg"], i["wu"]) * i["gh"]).sum() if linear else (f(v, i["wg"], i["wu"]) ** 2).sum()  # noqa: E731
+    along = lambda f: lambda x: (f(x) * i["tx"]).sum()  # noqa: E731
+    twice = lambda f: torch.func.grad(along(torch.func.grad(loss(f))))  # noqa: E731
+    torch.testing.assert_close(twice(gated_linear)(i["x"]), twice(_plain("silu"))(i["x"]))
+    for third in (lambda: torch.func.grad(along(twice(gated_linear)))(i["x"]), lambda: torch.func.jvp(twice(gated_linear), (i["x"],), (i["tx"],))):
+        with pytest.raises(RuntimeError, match="third time"):
+            third()
+    # linear in the vector of a second derivative
+    pulled = [torch.func.vjp(torch.func.grad(loss(f)), i["x"])[1] for f in (gated_linear, _plain("silu"))]
+    for a, b in zip(*(torch.func.jvp(lambda v: p(v)[0], (i["tx"],), (i["x"],)) for p in pulled)):
+        torch.testing.assert_close(a, b)
+    with fwAD.dual_level():
+        d, t = fwAD.unpack_dual(twice(gated_linear)(fwAD.make_dual(i["x"], i["tx"])))
+        torch.testing.assert_close(d, twice(_plain("silu"))(i["x"]))
+        assert t.isnan().all()
+
+
+def test_reverse_over_forward_under_torch_func():
+    i = _inputs(15)
+    for loss in (lambda h: (h * i["gh"]).sum(), lambda h: (h**2).sum()):
+        got, want = (torch.func.grad(lambda x: torch.func.jvp(lambda v: loss(f(v, i["wg"], i["wu"])), (x,), (i["tx"],))[1])(i["x"])
+                     for f in (gated_linear, _plain("silu")))
+        torch.testing.assert_close(got, want)
