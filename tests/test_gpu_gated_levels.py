@@ -113,3 +113,19 @@ def test_second_derivatives_of_far_gates(name, dt, M):
     near(got["dx"][:, 1], 64 * up, 64 * 2.0**-53)
     near(got["dtx"][:, 0], 64 * up, 64 * 2.0**-53)
     near(got["dwg"][:, 0], up.sum().expand(F), M * 2.0**-47)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_nested_reverse_transforms(dt):
+    """torch.func.grad of torch.func.grad, against torch in float64: two gradients' bounds of the norm.  A third derivative is refused."""
+    x, tx, wg, wu, gh, _ = _inputs(140, 72, 136, dt, 36)
+
+    def hvp(f, x, tx, wg, wu, gh):
+        first = torch.func.grad(lambda v: (f(v, wg, wu) * gh).sum())
+        return torch.func.grad(lambda v: (first(v) * tx).sum())(x)
+
+    want = hvp(_plain("silu"), *(t.double() for t in (x, tx, wg, wu, gh)))
+    got = hvp(gated_linear, x, tx, wg, wu, gh)
+    assert (got.double() - want).norm() <= (2e-5 if dt == "fp32" else 8 * 2.0**-8) * want.norm()
+    with pytest.raises(RuntimeError, match="third time"):
+        torch.func.grad(lambda v: (hvp(gated_linear, v, tx, wg, wu, gh) * tx).sum())(x)
