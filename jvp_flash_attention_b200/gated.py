@@ -40,10 +40,10 @@ def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, activation: str = "sil
 
     Tangents of the weights, and a second differentiation of their gradients, run on operands side by side, ``[tx | x]`` and ``[w | tw]``,
     at twice the depth (where a weight's tangent is not finite, neither is the value there); the gradient through the tangent output cannot
-    be differentiated again.  Gradients that are taken inside a forward-AD level carry their tangents (Hessian-vector products; attention's do
-    not), which is a further backward: take them behind the level where only they are wanted.  The tangent of one through the tangent output would be a third
-    derivative; it is NaN.  Under ``torch.func`` ``jvp``, ``vjp`` and ``grad`` nest as far as that goes; ``jvp`` of ``jvp`` and ``vmap`` (so
-    ``jacfwd``, ``jacrev`` and ``hessian``) are refused, and batched cotangents of ``torch.autograd.grad``.
+    be differentiated again.  Gradients that are taken inside a forward-AD level carry their tangents (Hessian-vector products; attention's
+    do not), which is a further backward: take them behind the level where only they are wanted.  The tangent of one through the tangent
+    output would be a third derivative; it is NaN.  Under ``torch.func`` ``jvp``, ``vjp`` and ``grad`` nest as far as that goes; ``jvp`` of
+    ``jvp`` and ``vmap`` (so ``jacfwd``, ``jacrev`` and ``hessian``) are refused, and batched cotangents of ``torch.autograd.grad``.
     """
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation is one of {', '.join(ACTIVATIONS)}; got {activation!r}")
