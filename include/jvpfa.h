@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define JVPFA_VERSION 104 /* major*100 + minor; 101: fields after the last of 100 in four structs; 102: workspace in two; 103: kv_len_host in two; 104: jvpfa_rotary, jvpfa_gated_fwd, jvpfa_gated_bwd */
+#define JVPFA_VERSION 105 /* major*100 + minor; 101: fields after the last of 100 in four structs; 102: workspace in two; 103: kv_len_host in two; 104: jvpfa_rotary, jvpfa_gated_fwd, jvpfa_gated_bwd; 105: jvpfa_norm_fwd, jvpfa_norm_bwd */
 
 typedef enum {
   JVPFA_OK = 0,
@@ -456,6 +456,56 @@ typedef struct {
 
 int jvpfa_gated_bwd(const jvpfa_gated_bwd_args* args, void* stream);
 int64_t jvpfa_gated_bwd_workspace(const jvpfa_gated_bwd_args* args);
+
+/*
+ * jvpfa_norm_fwd, jvpfa_norm_bwd -- the norm in front of a block and the residual sum behind one, in one pass, value and tangent, and the
+ * gradients through both.  No upstream counterpart.
+ *
+ *   r = x + alpha gate post_weight * N_post(y)        (x itself without y; N_post(y) = y without a norm of y)
+ *   n = N(r) weight (1 + scale) + bias (1 + scale) + shift
+ *   N(x) = (x - m) / sqrt(mean((x - m)^2) + eps) over the C entries of a row, m their mean (JVPFA_NORM_LAYER) or 0 (JVPFA_NORM_RMS)
+ *
+ * and tr, tn along tangents of x, y and any of the vectors.  The vectors have C entries; a grouped one has a row for each `group_rows`
+ * successive rows of x (M is a multiple of it), the others one for all.  An absent vector (v NULL) is 1, of bias, scale and shift 0.
+ * All arithmetic is in 32 bits; every result is rounded once (n is the norm of the r that was not rounded).  Rows have at most
+ * JVPFA_NORM_MAX_WIDTH entries.  x, tx, y, ty have contiguous columns and row strides in entries; vectors have contiguous entries;
+ * r, tr, n, tn and what the backward reads and writes of them are row-major.  Addresses are multiples of an entry.
+ */
+#define JVPFA_NORM_MAX_WIDTH 16384
+typedef enum { JVPFA_NORM_NONE = 0, JVPFA_NORM_RMS = 1, JVPFA_NORM_LAYER = 2 } jvpfa_norm_kind;
+typedef enum { JVPFA_VEC_WEIGHT = 0, JVPFA_VEC_BIAS = 1, JVPFA_VEC_SCALE = 2, JVPFA_VEC_SHIFT = 3, JVPFA_VEC_GATE = 4, JVPFA_VEC_POST_WEIGHT = 5 } jvpfa_norm_vector;
+typedef struct {
+  const void *v, *tv;         /* tv NULL: no tangent; never without v */
+  int64_t stride, tv_stride;  /* entries from one group's to the next (grouped ones) */
+  int32_t grouped;
+} jvpfa_norm_vec;
+
+typedef struct {
+  int32_t struct_size; /* sizeof(jvpfa_norm_args) */
+  int32_t dtype;       /* of x, y and the results: JVPFA_BF16, JVPFA_FP16 or JVPFA_FP32 */
+  int32_t vec_dtype;   /* of the vectors: dtype or JVPFA_FP32 */
+  int32_t M, C, group_rows;
+  int32_t kind, post;  /* jvpfa_norm_kind of r (NONE: no n) and of y */
+  float alpha, eps;
+  const void *x, *tx, *y, *ty; /* y NULL: no sum; tangents NULL: zero */
+  int64_t x_stride, tx_stride, y_stride, ty_stride;
+  jvpfa_norm_vec vec[6];       /* by jvpfa_norm_vector */
+  int32_t dual;                /* form tangents, respectively take their cotangents */
+  /* forward */
+  void *r, *tr;                /* with y; tr iff dual */
+  void *n, *tn;                /* unless kind is NONE; tn iff dual */
+  float* stats;                /* NULL, or for the backward: 8 M values, 16-byte aligned */
+  /* backward: stats as the forward with these operands (and dual) left them */
+  const void *gr, *gtr, *gn, *gtn; /* cotangents; NULL: zero */
+  void *dx, *dtx, *dy, *dty;       /* NULL: not wanted; dtx, dty only with dual */
+  void *d[6], *dt[6];              /* gradients of the vectors, of vec_dtype, row-major, one row or one a group; NULL: not wanted */
+  void* workspace;                 /* jvpfa_norm_bwd_workspace() bytes of scratch, 16-byte aligned (0: NULL) */
+  int64_t workspace_bytes;
+} jvpfa_norm_args;
+
+int jvpfa_norm_fwd(const jvpfa_norm_args* args, void* stream);
+int jvpfa_norm_bwd(const jvpfa_norm_args* args, void* stream);
+int64_t jvpfa_norm_bwd_workspace(const jvpfa_norm_args* args);
 
 /* Human-readable text for a jvpfa_status (static storage, never NULL). */
 const char* jvpfa_strerror(int status);

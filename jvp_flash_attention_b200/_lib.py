@@ -59,6 +59,9 @@ EXPORTS = (
     "jvpfa_gated_fwd_workspace",
     "jvpfa_gated_bwd",
     "jvpfa_gated_bwd_workspace",
+    "jvpfa_norm_fwd",
+    "jvpfa_norm_bwd",
+    "jvpfa_norm_bwd_workspace",
 )
 
 NOALLOC_MAX_ROWS = 524288  # JVPFA_NOALLOC_MAX_ROWS
@@ -317,6 +320,40 @@ class GatedBwdArgs(C.Structure):
     ]
 
 
+class NormVec(C.Structure):
+    _fields_ = [
+        ("v", C.c_void_p),
+        ("tv", C.c_void_p),
+        ("stride", C.c_int64),
+        ("tv_stride", C.c_int64),
+        ("grouped", C.c_int32),
+    ]
+
+
+class NormArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_int32),
+        ("dtype", C.c_int32),
+        ("vec_dtype", C.c_int32),
+        ("M", C.c_int32),
+        ("C", C.c_int32),
+        ("group_rows", C.c_int32),
+        ("kind", C.c_int32),
+        ("post", C.c_int32),
+        ("alpha", C.c_float),
+        ("eps", C.c_float),
+        *((name, C.c_void_p) for name in ("x", "tx", "y", "ty")),
+        *((name + "_stride", C.c_int64) for name in ("x", "tx", "y", "ty")),
+        ("vec", NormVec * 6),
+        ("dual", C.c_int32),
+        *((name, C.c_void_p) for name in ("r", "tr", "n", "tn", "stats", "gr", "gtr", "gn", "gtn", "dx", "dtx", "dy", "dty")),
+        ("d", C.c_void_p * 6),
+        ("dt", C.c_void_p * 6),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
+    ]
+
+
 _lib = None
 
 
@@ -375,6 +412,11 @@ def load() -> C.CDLL:
     lib.jvpfa_gated_bwd.restype = C.c_int
     lib.jvpfa_gated_bwd_workspace.argtypes = [C.POINTER(GatedBwdArgs)]
     lib.jvpfa_gated_bwd_workspace.restype = C.c_int64
+    for name in ("norm_fwd", "norm_bwd"):
+        entry = getattr(lib, "jvpfa_" + name)
+        entry.argtypes, entry.restype = [C.POINTER(NormArgs), C.c_void_p], C.c_int
+    lib.jvpfa_norm_bwd_workspace.argtypes = [C.POINTER(NormArgs)]
+    lib.jvpfa_norm_bwd_workspace.restype = C.c_int64
     _lib = lib
     return lib
 

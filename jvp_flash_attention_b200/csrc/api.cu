@@ -30,7 +30,7 @@ bool SmemOptIn::ensure(const void* kernel, size_t bytes) {
   return true;
 }
 
-static int check_arch() {
+int check_arch() {
   static thread_local int cached_dev = -1;
   static thread_local int cached_ok = 0;
   int dev = -1;

@@ -644,6 +644,7 @@ long long bwd_f32_tc5_workspace(const jvpfa_bwd_args& a);
 bool bwd_f32_tc5_eligible(const jvpfa_bwd_args& a);
 int launch_bwd_f32_tc5(const jvpfa_bwd_args& a, cudaStream_t stream);
 void set_last_cuda_error(cudaError_t e, const char* where);
+int check_arch();  // JVPFA_OK on a device that these kernels run on
 int check_pre_request(const jvpfa_pre_args* a);
 int check_bwd_request(const jvpfa_bwd_args* a);
 

@@ -735,4 +735,5 @@ PYBIND11_MODULE(_native, m) {
   m.def("set_impl", [](int v) { g_impl = v; });
   m.def("set_single_pass", [](bool v) { g_single_pass = v; });
   bind_block(m);
+  bind_norm(m);
 }

@@ -108,3 +108,5 @@ inline Tensor primal_of(const Tensor& x) {  // inside a forward-AD level the sav
 
 // The operators beside attention (native_block.cpp)
 void bind_block(py::module_& m);
+// The norms and residual sums (native_norm.cpp)
+void bind_norm(py::module_& m);
