@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define JVPFA_VERSION 105 /* major*100 + minor; 101: fields after the last of 100 in four structs; 102: workspace in two; 103: kv_len_host in two; 104: jvpfa_rotary, jvpfa_gated_fwd, jvpfa_gated_bwd; 105: jvpfa_norm_fwd, jvpfa_norm_bwd */
+#define JVPFA_VERSION 105 /* major*100 + minor; 101: fields after the last of 100 in four structs; 102: workspace in two; 103: kv_len_host in two; 104: jvpfa_rotary, jvpfa_gated_fwd, jvpfa_gated_bwd; 105: jvpfa_norm_fwd, jvpfa_norm_bwd, jvpfa_linear_fwd, jvpfa_linear_bwd, jvpfa_linear_step */
 
 typedef enum {
   JVPFA_OK = 0,
@@ -506,6 +506,64 @@ typedef struct {
 int jvpfa_norm_fwd(const jvpfa_norm_args* args, void* stream);
 int jvpfa_norm_bwd(const jvpfa_norm_args* args, void* stream);
 int64_t jvpfa_norm_bwd_workspace(const jvpfa_norm_args* args);
+
+/*
+ * jvpfa_linear_fwd, jvpfa_linear_bwd, jvpfa_linear_step -- causal linear attention with a decay for each head, value and tangent, the
+ * gradients through both, and its form for one more token.  No upstream counterpart.
+ *
+ *   S_t = exp(log_decay) S_{t-1} + k_t v_t^T,   o_t = scale S_t^T q_t          S: (D, E), S_{-1} = state (0 without one)
+ *
+ * q, k (and their tangents and gradients): (B, H, L, D); v, o: (B, H, L, E); any positive strides, entries contiguous; 1 <= D, E <= 128.
+ * Rows from lengths[b] on are not read, and their results are zero; state_out is the state behind row lengths[b] - 1.  States are
+ * (B, H, D, E) row-major, in 32 bits whatever the type, and so are all sums.  log_decay: H values, at most 0 in use (NULL: 0 for all;
+ * below -1e4 it counts as -1e4, which leaves a row its own key alone).
+ */
+typedef struct {
+  const void* p; /* NULL: absent (a tangent: zero) */
+  int64_t stride[3]; /* batch, head, row */
+} jvpfa_linear_tensor;
+
+typedef struct {
+  int32_t struct_size; /* sizeof(jvpfa_linear_args) */
+  int32_t dtype;       /* JVPFA_BF16, JVPFA_FP16 or JVPFA_FP32 */
+  int32_t B, H, L, D, E;
+  float scale;
+  int32_t dual; /* form tangents, respectively take their cotangents */
+  const float* log_decay;
+  const int32_t* lengths; /* B values (NULL: L for all; values outside [0, L] count as the nearer end) */
+  jvpfa_linear_tensor q, k, v, tq, tk, tv;
+  const float *state, *tstate;
+  /* forward */
+  jvpfa_linear_tensor o, to; /* written; to iff dual */
+  float *state_out, *tstate_out; /* NULL: not wanted */
+  /* backward */
+  jvpfa_linear_tensor go, gto;       /* NULL: zero */
+  const float *gstate, *gtstate;     /* cotangents of state_out, tstate_out */
+  jvpfa_linear_tensor dq, dk, dv, dtq, dtk, dtv; /* written; NULL: not wanted */
+  float *dstate, *dtstate;
+  void* workspace; /* jvpfa_linear_fwd_workspace() / _bwd_workspace() bytes, 16-byte aligned (0: NULL) */
+  int64_t workspace_bytes;
+} jvpfa_linear_args;
+
+int jvpfa_linear_fwd(const jvpfa_linear_args* args, void* stream);
+int64_t jvpfa_linear_fwd_workspace(const jvpfa_linear_args* args);
+int jvpfa_linear_bwd(const jvpfa_linear_args* args, void* stream);
+int64_t jvpfa_linear_bwd_workspace(const jvpfa_linear_args* args);
+
+typedef struct {
+  int32_t struct_size; /* sizeof(jvpfa_linear_step_args) */
+  int32_t dtype;
+  int32_t B, H, D, E;
+  float scale;
+  const float* log_decay;
+  const void *q, *k, *v; /* (B, H, D), (B, H, D), (B, H, E), entries contiguous */
+  void* o;               /* (B, H, E) row-major */
+  int64_t q_stride[2], k_stride[2], v_stride[2]; /* batch, head */
+  float* state;          /* (B, H, D, E), updated in place: D and E row-major, batches and heads anywhere but not twice */
+  int64_t state_stride[2];
+} jvpfa_linear_step_args;
+
+int jvpfa_linear_step(const jvpfa_linear_step_args* args, void* stream);
 
 /* Human-readable text for a jvpfa_status (static storage, never NULL). */
 const char* jvpfa_strerror(int status);

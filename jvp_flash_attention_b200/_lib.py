@@ -62,6 +62,11 @@ EXPORTS = (
     "jvpfa_norm_fwd",
     "jvpfa_norm_bwd",
     "jvpfa_norm_bwd_workspace",
+    "jvpfa_linear_fwd",
+    "jvpfa_linear_fwd_workspace",
+    "jvpfa_linear_bwd",
+    "jvpfa_linear_bwd_workspace",
+    "jvpfa_linear_step",
 )
 
 NOALLOC_MAX_ROWS = 524288  # JVPFA_NOALLOC_MAX_ROWS
@@ -354,6 +359,47 @@ class NormArgs(C.Structure):
     ]
 
 
+class LinearTensor(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("stride", C.c_int64 * 3)]
+
+
+class LinearArgs(C.Structure):
+    _fields_ = [
+        *((name, C.c_int32) for name in ("struct_size", "dtype", "B", "H", "L", "D", "E")),
+        ("scale", C.c_float),
+        ("dual", C.c_int32),
+        ("log_decay", C.c_void_p),
+        ("lengths", C.c_void_p),
+        *((name, LinearTensor) for name in ("q", "k", "v", "tq", "tk", "tv")),
+        ("state", C.c_void_p),
+        ("tstate", C.c_void_p),
+        ("o", LinearTensor),
+        ("to", LinearTensor),
+        ("state_out", C.c_void_p),
+        ("tstate_out", C.c_void_p),
+        ("go", LinearTensor),
+        ("gto", LinearTensor),
+        ("gstate", C.c_void_p),
+        ("gtstate", C.c_void_p),
+        *((name, LinearTensor) for name in ("dq", "dk", "dv", "dtq", "dtk", "dtv")),
+        ("dstate", C.c_void_p),
+        ("dtstate", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
+    ]
+
+
+class LinearStepArgs(C.Structure):
+    _fields_ = [
+        *((name, C.c_int32) for name in ("struct_size", "dtype", "B", "H", "D", "E")),
+        ("scale", C.c_float),
+        *((name, C.c_void_p) for name in ("log_decay", "q", "k", "v", "o")),
+        *((name, C.c_int64 * 2) for name in ("q_stride", "k_stride", "v_stride")),
+        ("state", C.c_void_p),
+        ("state_stride", C.c_int64 * 2),
+    ]
+
+
 _lib = None
 
 
@@ -412,11 +458,13 @@ def load() -> C.CDLL:
     lib.jvpfa_gated_bwd.restype = C.c_int
     lib.jvpfa_gated_bwd_workspace.argtypes = [C.POINTER(GatedBwdArgs)]
     lib.jvpfa_gated_bwd_workspace.restype = C.c_int64
-    for name in ("norm_fwd", "norm_bwd"):
+    for name, args in (("norm_fwd", NormArgs), ("norm_bwd", NormArgs), ("linear_fwd", LinearArgs), ("linear_bwd", LinearArgs),
+                       ("linear_step", LinearStepArgs)):
         entry = getattr(lib, "jvpfa_" + name)
-        entry.argtypes, entry.restype = [C.POINTER(NormArgs), C.c_void_p], C.c_int
-    lib.jvpfa_norm_bwd_workspace.argtypes = [C.POINTER(NormArgs)]
-    lib.jvpfa_norm_bwd_workspace.restype = C.c_int64
+        entry.argtypes, entry.restype = [C.POINTER(args), C.c_void_p], C.c_int
+    for name, args in (("norm_bwd", NormArgs), ("linear_fwd", LinearArgs), ("linear_bwd", LinearArgs)):
+        entry = getattr(lib, f"jvpfa_{name}_workspace")
+        entry.argtypes, entry.restype = [C.POINTER(args)], C.c_int64
     _lib = lib
     return lib
 

@@ -1,0 +1,305 @@
+// Entries of linear attention: argument checks, the cut of long sequences into segments, the launches that the outputs and gradients are made
+// of, and the form for one more token.
+#include "linear_common.cuh"
+
+namespace jvpfa {
+namespace linear {
+
+template <typename T, bool OUT>
+int launch_scan(const Scan& s, cudaStream_t stream);
+
+namespace {
+
+template <bool OUT>
+int launch_of_type(const Scan& s, cudaStream_t stream) {
+  if (s.dtype == JVPFA_FP32) return launch_scan<float, OUT>(s, stream);
+  return s.dtype == JVPFA_BF16 ? launch_scan<__nv_bfloat16, OUT>(s, stream) : launch_scan<__half, OUT>(s, stream);
+}
+
+// The states that the segments begin with, from those that each one's own rows leave: one entry of M a thread, segment after segment.
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Scan p) {
+  const int size = p.D * p.E, head = blockIdx.x, b = head / p.H, h = head - b * p.H;
+  const int n = length_of(p.lengths, b, p.L);
+  const double w = decay_of(p.log_decay, h);
+  for (int i = blockIdx.y * 256 + threadIdx.x; i < size; i += gridDim.y * 256) {
+    const long long given = (long long)head * size + i / p.E * p.first_stride[0] + i % p.E * p.first_stride[1];
+    for (int which = 0; which < (p.dual ? 2 : 1); ++which) {
+      const float* first = which ? p.tfirst : p.first;
+      float* at = (which ? p.tstates : p.states) + (long long)head * p.segments * size + i;
+      float x = first ? p.first_scale * first[given] : 0.f;
+      for (int s = 0; s < p.segments; ++s, at += size) {
+        const float own = s + 1 < p.segments ? *at : 0.f;
+        *at = x;
+        const int rows = max(0, min(n - s * p.segment, p.segment)) + (s == 0 ? p.ahead - 1 : 0);
+        x = fmaf(x, (float)expm1(w * rows), x) + own;
+      }
+    }
+  }
+}
+
+// Rows of a segment and segments (1: no workspace).
+void cut(Scan& s) {
+  // CTAs that SMs hold by their shared memory, 2 or 3; segments of at least 4 chunks, and as many as there is room for at once
+  const int heads = s.B * s.H, room = kSMs * 2;
+  int segments = room / heads, most = s.L / 256;
+  if (segments > most) segments = most;
+  if (segments > 64) segments = 64;
+  s.segments = 1, s.segment = s.L;
+  if (segments < 2) return;
+  s.segment = ((s.L + segments - 1) / segments + 63) / 64 * 64;
+  s.segments = (s.L + s.segment - 1) / s.segment;
+}
+
+int launch(const Scan& s, cudaStream_t stream) {
+  if (s.segments > 1) {
+    const int rc = launch_of_type<false>(s, stream);
+    if (rc) return rc;
+    join_kernel<<<dim3((unsigned)(s.B * s.H), (unsigned)((s.D * s.E + 1023) / 1024)), 256, 0, stream>>>(s);
+  }
+  return launch_of_type<true>(s, stream);
+}
+
+// ---- one more token ------------------------------------------------------------------------------------------------------
+// S = l S + k v^T and o = scale S^T q, a CTA for `cols` columns of one head's state, V of them a thread.  Memory-bound: the state is read and
+// written once, in 16-byte pieces.
+constexpr int kStepThreads = 256;
+
+__device__ __forceinline__ float load_as(const void* p, long long at, int dtype) {
+  if (dtype == JVPFA_FP32) return static_cast<const float*>(p)[at];
+  return dtype == JVPFA_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at]) : __half2float(static_cast<const __half*>(p)[at]);
+}
+
+template <int V>
+__global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constant__ jvpfa_linear_step_args a, const int cols) {
+  __shared__ float sq[128], sk[128], part[kStepThreads * 4];
+  const int tid = threadIdx.x, b = blockIdx.x / a.H, h = blockIdx.x - b * a.H;
+  const int lanes = cols / V, row_step = kStepThreads / lanes;  // threads along a row, rows at once
+  const int row0 = tid / lanes, e = blockIdx.y * cols + tid % lanes * V;
+  const bool live = row0 < row_step && e < a.E;
+  for (int d = tid; d < a.D; d += kStepThreads) {
+    sq[d] = a.scale * load_as(a.q, b * a.q_stride[0] + h * a.q_stride[1] + d, a.dtype);
+    sk[d] = load_as(a.k, b * a.k_stride[0] + h * a.k_stride[1] + d, a.dtype);
+  }
+  const float down = (float)expm1((double)decay_of(a.log_decay, h));
+  float v[V], o[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    v[i] = live ? load_as(a.v, b * a.v_stride[0] + h * a.v_stride[1] + e + i, a.dtype) : 0.f;
+    o[i] = 0.f;
+  }
+  __syncthreads();
+  float* state = a.state + b * a.state_stride[0] + h * a.state_stride[1] + e;
+  if (live) {
+    constexpr int AHEAD = 8;
+    for (int d0 = row0; d0 < a.D; d0 += AHEAD * row_step) {
+      float s[AHEAD][V];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const int d = d0 + j * row_step;
+        if (d >= a.D) break;
+        if constexpr (V == 4) {
+          const float4 x = *reinterpret_cast<const float4*>(state + (long long)d * a.E);
+          s[j][0] = x.x, s[j][1] = x.y, s[j][2] = x.z, s[j][3] = x.w;
+        } else {
+          s[j][0] = state[(long long)d * a.E];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const int d = d0 + j * row_step;
+        if (d >= a.D) break;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          s[j][i] = fmaf(s[j][i], down, s[j][i]) + sk[d] * v[i];
+          o[i] += sq[d] * s[j][i];
+        }
+        if constexpr (V == 4)
+          *reinterpret_cast<float4*>(state + (long long)d * a.E) = make_float4(s[j][0], s[j][1], s[j][2], s[j][3]);
+        else
+          state[(long long)d * a.E] = s[j][0];
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) part[tid * V + i] = o[i];
+  __syncthreads();
+  // part: [row0][column of the CTA]
+  for (int c = tid; c < cols; c += kStepThreads) {
+    const int col = blockIdx.y * cols + c;
+    if (col >= a.E) continue;
+    float s = 0.f;
+    for (int r = 0; r < row_step; ++r) s += part[(r * lanes + c / V) * V + c % V];
+    const long long at = ((long long)b * a.H + h) * a.E + col;
+    if (a.dtype == JVPFA_FP32)
+      static_cast<float*>(a.o)[at] = s;
+    else if (a.dtype == JVPFA_BF16)
+      static_cast<__nv_bfloat16*>(a.o)[at] = __float2bfloat16_rn(s);
+    else
+      static_cast<__half*>(a.o)[at] = __float2half_rn(s);
+  }
+}
+
+// ---- checks --------------------------------------------------------------------------------------------------------------
+bool bad_dtype(int dtype) { return dtype != JVPFA_BF16 && dtype != JVPFA_FP16 && dtype != JVPFA_FP32; }
+
+int check(const jvpfa_linear_args* a, bool backward) {
+  if (!a) return JVPFA_ERR_NULL;
+  if (a->struct_size != (int32_t)sizeof(jvpfa_linear_args)) return JVPFA_ERR_STRUCT;
+  if (bad_dtype(a->dtype)) return JVPFA_ERR_DTYPE;
+  if (a->B < 1 || a->H < 1 || a->L < 1 || a->D < 1 || a->E < 1 || a->D > 128 || a->E > 128) return JVPFA_ERR_SHAPE;
+  if ((long long)a->B * a->H > (1 << 24)) return JVPFA_ERR_TOO_LARGE;
+  if (!(a->scale == a->scale) || (backward && a->scale == 0.f && (a->gstate || a->gtstate))) return JVPFA_ERR_UNSUPPORTED;
+  if (!a->q.p || !a->k.p || !a->v.p) return JVPFA_ERR_NULL;
+  if (!a->dual && (a->tq.p || a->tk.p || a->tv.p || a->tstate || a->to.p || a->tstate_out || a->gto.p || a->gtstate || a->dtq.p || a->dtk.p || a->dtv.p || a->dtstate))
+    return JVPFA_ERR_NULL;
+  if (!backward && (!a->o.p || (a->dual && !a->to.p))) return JVPFA_ERR_NULL;
+  if (backward && !a->state && a->dstate) return JVPFA_ERR_NULL;
+  const uintptr_t size = a->dtype == JVPFA_FP32 ? 4 : 2;
+  for (const jvpfa_linear_tensor* x : {&a->q, &a->k, &a->v, &a->tq, &a->tk, &a->tv, &a->o, &a->to, &a->go, &a->gto, &a->dq, &a->dk, &a->dv, &a->dtq, &a->dtk, &a->dtv}) {
+    if (!x->p) continue;
+    if (reinterpret_cast<uintptr_t>(x->p) % size) return JVPFA_ERR_ALIGN;
+    for (int64_t st : x->stride)
+      if (st < 0) return JVPFA_ERR_SHAPE;
+  }
+  for (const void* p : {(const void*)a->state, (const void*)a->tstate, (const void*)a->state_out, (const void*)a->tstate_out, (const void*)a->gstate,
+                        (const void*)a->gtstate, (const void*)a->dstate, (const void*)a->dtstate, (const void*)a->log_decay, (const void*)a->lengths})
+    if (reinterpret_cast<uintptr_t>(p) % 4) return JVPFA_ERR_ALIGN;
+  return JVPFA_OK;
+}
+
+// A scan with the call's sizes; D and E are those of its a and c.
+Scan scan_of(const jvpfa_linear_args& a, int D, int E) {
+  Scan s{};
+  s.dtype = a.dtype, s.B = a.B, s.H = a.H, s.L = a.L, s.D = D, s.E = E;
+  s.scale = a.scale, s.dual = a.dual != 0;
+  s.log_decay = a.log_decay, s.lengths = a.lengths;
+  s.first_scale = s.last_scale = 1.f, s.ahead = 1;
+  s.first_stride[0] = s.last_stride[0] = E, s.first_stride[1] = s.last_stride[1] = 1;
+  cut(s);
+  return s;
+}
+void give_workspace(Scan& s, void* workspace) {
+  s.states = static_cast<float*>(workspace);
+  s.tstates = s.states + (size_t)s.B * s.H * s.segments * s.D * s.E;
+}
+int64_t workspace_bytes(const jvpfa_linear_args& a) { return state_bytes(scan_of(a, a.D, a.E)) * (a.dual ? 2 : 1); }
+
+}  // namespace
+}  // namespace linear
+}  // namespace jvpfa
+
+using namespace jvpfa;
+
+extern "C" {
+
+int64_t jvpfa_linear_fwd_workspace(const jvpfa_linear_args* a) { return linear::check(a, false) == JVPFA_OK ? linear::workspace_bytes(*a) : 0; }
+int64_t jvpfa_linear_bwd_workspace(const jvpfa_linear_args* a) { return linear::check(a, true) == JVPFA_OK ? linear::workspace_bytes(*a) : 0; }
+
+int jvpfa_linear_fwd(const jvpfa_linear_args* a, void* stream) {
+  int rc = linear::check(a, false);
+  if (rc) return rc;
+  const int64_t need = linear::workspace_bytes(*a);
+  if (need && (!a->workspace || a->workspace_bytes < need)) return JVPFA_ERR_NULL;
+  if (reinterpret_cast<uintptr_t>(a->workspace) % 16) return JVPFA_ERR_ALIGN;
+  rc = check_arch();
+  if (rc) return rc;
+  linear::Scan s = linear::scan_of(*a, a->D, a->E);
+  s.a = a->q, s.b = a->k, s.c = a->v, s.ta = a->tq, s.tb = a->tk, s.tc = a->tv, s.out = a->o, s.tout = a->to;
+  s.first = a->state, s.tfirst = a->tstate, s.last = a->state_out, s.tlast = a->tstate_out;
+  linear::give_workspace(s, a->workspace);
+  return linear::launch(s, static_cast<cudaStream_t>(stream));
+}
+
+int jvpfa_linear_bwd(const jvpfa_linear_args* a, void* stream) {
+  int rc = linear::check(a, true);
+  if (rc) return rc;
+  const int64_t need = linear::workspace_bytes(*a);
+  if (need && (!a->workspace || a->workspace_bytes < need)) return JVPFA_ERR_NULL;
+  if (reinterpret_cast<uintptr_t>(a->workspace) % 16) return JVPFA_ERR_ALIGN;
+  rc = check_arch();
+  if (rc) return rc;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // With tangents the maps' value has gto for its cotangent and gives the tangents' gradients, and their tangent has go and gives the others.
+  const bool dual = a->dual != 0;
+  const jvpfa_linear_tensor none{}, &g = dual ? a->gto : a->go, &tg = dual ? a->go : none;
+  auto value = [&](const jvpfa_linear_tensor& d, const jvpfa_linear_tensor& dt) -> const jvpfa_linear_tensor& { return dual ? dt : d; };
+  auto tangent = [&](const jvpfa_linear_tensor& d) -> const jvpfa_linear_tensor& { return dual ? d : none; };
+  if (a->dq.p || a->dtq.p) {
+    linear::Scan s = linear::scan_of(*a, a->E, a->D);
+    s.a = g, s.ta = tg, s.b = a->v, s.tb = a->tv, s.c = a->k, s.tc = a->tk;
+    s.out = value(a->dq, a->dtq), s.tout = tangent(a->dq);
+    s.first = a->state, s.tfirst = a->tstate, s.first_stride[0] = 1, s.first_stride[1] = a->E;
+    linear::give_workspace(s, a->workspace);
+    rc = linear::launch(s, st);
+    if (rc) return rc;
+  }
+  // Backwards, M begins with the cotangent of the last state, which the scale does not go with.
+  const float* first = dual ? a->gtstate : a->gstate;
+  const float* tfirst = dual ? a->gstate : nullptr;
+  const float unscaled = first || tfirst ? 1.f / a->scale : 1.f;
+  if (a->dk.p || a->dtk.p || a->dstate || a->dtstate) {
+    linear::Scan s = linear::scan_of(*a, a->E, a->D);
+    s.reversed = true, s.ahead = 0, s.last_ahead = 1, s.first_scale = unscaled, s.last_scale = a->scale;
+    s.a = a->v, s.ta = a->tv, s.b = g, s.tb = tg, s.c = a->q, s.tc = a->tq;
+    s.out = value(a->dk, a->dtk), s.tout = tangent(a->dk);
+    s.first = first, s.tfirst = tfirst, s.first_stride[0] = 1, s.first_stride[1] = a->E;
+    s.last = dual ? a->dtstate : a->dstate, s.tlast = dual ? a->dstate : nullptr, s.last_stride[0] = 1, s.last_stride[1] = a->E;
+    linear::give_workspace(s, a->workspace);
+    rc = linear::launch(s, st);
+    if (rc) return rc;
+  }
+  if (a->dv.p || a->dtv.p) {
+    linear::Scan s = linear::scan_of(*a, a->D, a->E);
+    s.reversed = true, s.ahead = 0, s.first_scale = unscaled;
+    s.a = a->k, s.ta = a->tk, s.b = a->q, s.tb = a->tq, s.c = g, s.tc = tg;
+    s.out = value(a->dv, a->dtv), s.tout = tangent(a->dv);
+    s.first = first, s.tfirst = tfirst;
+    linear::give_workspace(s, a->workspace);
+    rc = linear::launch(s, st);
+    if (rc) return rc;
+  }
+  return JVPFA_OK;
+}
+
+int jvpfa_linear_step(const jvpfa_linear_step_args* a, void* stream) {
+  if (!a) return JVPFA_ERR_NULL;
+  if (a->struct_size != (int32_t)sizeof(jvpfa_linear_step_args)) return JVPFA_ERR_STRUCT;
+  if (linear::bad_dtype(a->dtype)) return JVPFA_ERR_DTYPE;
+  if (a->B < 1 || a->H < 1 || a->D < 1 || a->E < 1 || a->D > 128 || a->E > 128) return JVPFA_ERR_SHAPE;
+  if ((long long)a->B * a->H > (1 << 24)) return JVPFA_ERR_TOO_LARGE;
+  if (!a->q || !a->k || !a->v || !a->o || !a->state) return JVPFA_ERR_NULL;
+  const uintptr_t size = a->dtype == JVPFA_FP32 ? 4 : 2;
+  for (const void* p : {a->q, a->k, a->v, (const void*)a->o})
+    if (reinterpret_cast<uintptr_t>(p) % size) return JVPFA_ERR_ALIGN;
+  if (reinterpret_cast<uintptr_t>(a->state) % 4 || reinterpret_cast<uintptr_t>(a->log_decay) % 4) return JVPFA_ERR_ALIGN;
+  for (const int64_t* st : {a->q_stride, a->k_stride, a->v_stride, a->state_stride})
+    if (st[0] < 0 || st[1] < 0) return JVPFA_ERR_SHAPE;
+  // two heads of one state would race
+  const int64_t one = (int64_t)a->D * a->E;
+  const int64_t sb = a->state_stride[0], sh = a->state_stride[1];
+  if ((a->H > 1 && sh < one) || (a->B > 1 && sb < one) || (a->B > 1 && a->H > 1 && (sb > sh ? sb < (a->H - 1) * sh + one : sh < (a->B - 1) * sb + one)))
+    return JVPFA_ERR_SHAPE;
+  const int rc = check_arch();
+  if (rc) return rc;
+  uint64_t all = reinterpret_cast<uint64_t>(a->state) | (uint64_t)a->E * 4;
+  if (a->B > 1) all |= (uint64_t)sb * 4;
+  if (a->H > 1) all |= (uint64_t)sh * 4;
+  const bool wide = all % 16 == 0;
+  // columns of a CTA: all, or 32 where the heads do not fill the SMs
+  const int padded = (a->E + 3) / 4 * 4;
+  const int cols = a->B * a->H < linear::kSMs && padded > 32 ? 32 : padded;
+  const dim3 grid((unsigned)(a->B * a->H), (unsigned)((a->E + cols - 1) / cols));
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (wide)
+    linear::step_kernel<4><<<grid, linear::kStepThreads, 0, s>>>(*a, cols);
+  else
+    linear::step_kernel<1><<<grid, linear::kStepThreads, 0, s>>>(*a, cols);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) {
+    set_last_cuda_error(e, "step_kernel");
+    return JVPFA_ERR_CUDA;
+  }
+  return JVPFA_OK;
+}
+
+}  // extern "C"

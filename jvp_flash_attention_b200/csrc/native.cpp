@@ -736,4 +736,5 @@ PYBIND11_MODULE(_native, m) {
   m.def("set_single_pass", [](bool v) { g_single_pass = v; });
   bind_block(m);
   bind_norm(m);
+  bind_linear(m);
 }

@@ -56,20 +56,6 @@ Tensor as_tangent(const Tensor& t, const Tensor& x) {
 }
 
 // ---- rotary --------------------------------------------------------------------------------------------------------------
-// The order of a tensor's dimensions in memory, the widest first (the last one stays innermost).
-using Order = std::array<int, 4>;
-Order order_of(const Tensor& x) {
-  Order o{0, 1, 2, 3};
-  std::stable_sort(o.begin(), o.begin() + 3, [&](int a, int b) { return x.stride(a) > x.stride(b); });
-  return o;
-}
-Tensor empty_in_order(at::IntArrayRef sizes, const Order& o, at::ScalarType dtype, at::Device device) {
-  std::array<int64_t, 4> st;
-  int64_t n = 1;
-  for (int d = 3; d >= 0; --d) st[o[d]] = n, n *= std::max<int64_t>(sizes[o[d]], 1);
-  return Tensor(at::detail::empty_strided_cuda(sizes, st, dtype, device));
-}
-
 struct Turn {
   int64_t offset;
   bool interleaved, transposed;

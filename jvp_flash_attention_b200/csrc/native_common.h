@@ -14,6 +14,8 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
+#include <array>
 #include <atomic>
 #include <memory>
 #include <optional>
@@ -100,6 +102,20 @@ void attach_refusal(const char* message, std::initializer_list<Tensor*> outs, co
     if (t->defined()) torch::autograd::set_history(*t, node);
 }
 
+// The order of a tensor's dimensions in memory, the widest first (the last one stays innermost).
+using Order = std::array<int, 4>;
+inline Order order_of(const Tensor& x) {
+  Order o{0, 1, 2, 3};
+  std::stable_sort(o.begin(), o.begin() + 3, [&](int a, int b) { return x.stride(a) > x.stride(b); });
+  return o;
+}
+inline Tensor empty_in_order(at::IntArrayRef sizes, const Order& o, at::ScalarType dtype, at::Device device) {
+  std::array<int64_t, 4> st;
+  int64_t n = 1;
+  for (int d = 3; d >= 0; --d) st[o[d]] = n, n *= std::max<int64_t>(sizes[o[d]], 1);
+  return Tensor(at::detail::empty_strided_cuda(sizes, st, dtype, device));
+}
+
 inline Tensor primal_of(const Tensor& x) {  // inside a forward-AD level the saved tensors are still dual
   return x.defined() && x._fw_grad(0).defined() ? x._fw_primal(0) : x;
 }
@@ -110,3 +126,5 @@ inline Tensor primal_of(const Tensor& x) {  // inside a forward-AD level the sav
 void bind_block(py::module_& m);
 // The norms and residual sums (native_norm.cpp)
 void bind_norm(py::module_& m);
+// Linear attention (native_linear.cpp)
+void bind_linear(py::module_& m);
