@@ -10,40 +10,52 @@ int launch_scan(const Scan& s, cudaStream_t stream);
 
 namespace {
 
+constexpr int kMostSegments = 128;
+
 template <bool OUT>
 int launch_of_type(const Scan& s, cudaStream_t stream) {
   if (s.dtype == JVPFA_FP32) return launch_scan<float, OUT>(s, stream);
-  return s.dtype == JVPFA_BF16 ? launch_scan<__nv_bfloat16, OUT>(s, stream) : launch_scan<__half, OUT>(s, stream);
+  return s.dtype == JVPFA_BF16 ? launch_chunks(s, OUT, stream) : launch_scan<__half, OUT>(s, stream);
 }
 
-// The states that the segments begin with, from those that each one's own rows leave: one entry of M a thread, segment after segment.
+// The states that the segments begin with, from those that each one's own rows leave: one entry of M a thread, segment after segment.  (Its place
+// in the states goes over all of them, whatever their order; where the given state is.)
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Scan p) {
+  __shared__ float down[kMostSegments];
   const int size = p.D * p.E, head = blockIdx.x, b = head / p.H, h = head - b * p.H;
   const int n = length_of(p.lengths, b, p.L);
   const double w = decay_of(p.log_decay, h);
-  for (int i = blockIdx.y * 256 + threadIdx.x; i < size; i += gridDim.y * 256) {
-    const long long given = (long long)head * size + i / p.E * p.first_stride[0] + i % p.E * p.first_stride[1];
-    for (int which = 0; which < (p.dual ? 2 : 1); ++which) {
-      const float* first = which ? p.tfirst : p.first;
-      float* at = (which ? p.tstates : p.states) + (long long)head * p.segments * size + i;
-      float x = first ? p.first_scale * first[given] : 0.f;
-      for (int s = 0; s < p.segments; ++s, at += size) {
-        const float own = s + 1 < p.segments ? *at : 0.f;
-        *at = x;
-        const int rows = max(0, min(n - s * p.segment, p.segment)) + (s == 0 ? p.ahead - 1 : 0);
-        x = fmaf(x, (float)expm1(w * rows), x) + own;
-      }
+  for (int s = threadIdx.x; s < p.segments; s += 256) {
+    const int rows = max(0, min(n - s * p.segment, p.segment)) + (s == 0 ? p.ahead - 1 : 0);
+    down[s] = (float)expm1(w * rows);
+  }
+  __syncthreads();
+  const int i = blockIdx.y * 256 + threadIdx.x;
+  if (i >= size) return;
+  const int d = i / p.E, e = i - d * p.E;
+  const long long given = (long long)head * size + d * p.first_stride[0] + e * p.first_stride[1];
+  for (int which = 0; which < (p.dual ? 2 : 1); ++which) {
+    const float* first = which ? p.tfirst : p.first;
+    float* at = (which ? p.tstates : p.states) + (long long)head * p.segments * size + d * p.state_stride[0] + e * p.state_stride[1];
+    float x = first ? p.first_scale * first[given] : 0.f;
+    float own = at[0];
+    for (int s = 0; s < p.segments; ++s, at += size) {
+      const float next = s + 2 < p.segments ? at[size] : 0.f;  // (the last one's is nobody's)
+      *at = x;
+      x = fmaf(x, down[s], x) + own;
+      own = next;
     }
   }
 }
 
 // Rows of a segment and segments (1: no workspace).
 void cut(Scan& s) {
-  // CTAs that SMs hold by their shared memory, 2 or 3; segments of at least 4 chunks, and as many as there is room for at once
-  const int heads = s.B * s.H, room = kSMs * 2;
-  int segments = room / heads, most = s.L / 256;
+  // As many CTAs as SMs hold at once, and no segment below 128 rows
+  const int heads = s.B * s.H, width = s.D > s.E ? s.D : s.E;
+  const int room = kSMs * (width <= 64 ? (s.dual ? 2 : 3) : s.dual || s.dtype == JVPFA_FP32 ? 1 : 2);
+  int segments = room / heads, most = s.L / 128;
   if (segments > most) segments = most;
-  if (segments > 64) segments = 64;
+  if (segments > kMostSegments) segments = kMostSegments;
   s.segments = 1, s.segment = s.L;
   if (segments < 2) return;
   s.segment = ((s.L + segments - 1) / segments + 63) / 64 * 64;
@@ -54,7 +66,7 @@ int launch(const Scan& s, cudaStream_t stream) {
   if (s.segments > 1) {
     const int rc = launch_of_type<false>(s, stream);
     if (rc) return rc;
-    join_kernel<<<dim3((unsigned)(s.B * s.H), (unsigned)((s.D * s.E + 1023) / 1024)), 256, 0, stream>>>(s);
+    join_kernel<<<dim3((unsigned)(s.B * s.H), (unsigned)((s.D * s.E + 255) / 256)), 256, 0, stream>>>(s);
   }
   return launch_of_type<true>(s, stream);
 }
@@ -174,7 +186,7 @@ Scan scan_of(const jvpfa_linear_args& a, int D, int E) {
   s.scale = a.scale, s.dual = a.dual != 0;
   s.log_decay = a.log_decay, s.lengths = a.lengths;
   s.first_scale = s.last_scale = 1.f, s.ahead = 1;
-  s.first_stride[0] = s.last_stride[0] = E, s.first_stride[1] = s.last_stride[1] = 1;
+  s.first_stride[0] = s.last_stride[0] = s.state_stride[0] = E, s.first_stride[1] = s.last_stride[1] = s.state_stride[1] = 1;
   cut(s);
   return s;
 }

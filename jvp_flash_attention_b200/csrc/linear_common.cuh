@@ -31,10 +31,14 @@ struct Scan {
   float first_scale, last_scale;
   int ahead;       // the first row sees `first` l^ahead times
   int last_ahead;  // ... and `last` is M's behind the last row l^last_ahead times
-  // a head's rows are cut into `segments` of `segment` rows; their states in the workspace, [head][segment][D * E], value and tangent apart
+  // a head's rows are cut into `segments` of `segment` rows; their states in the workspace, [head][segment][D * E], value and tangent apart,
+  // entry (d, e) at d * state_stride[0] + e * state_stride[1]
   int segments, segment;
   float *states, *tstates;
+  long long state_stride[2];
 };
+
+int launch_chunks(const Scan& s, bool outputs, cudaStream_t stream);  // bfloat16 (linear_chunk.cu)
 
 inline long long state_bytes(const Scan& s) { return s.segments > 1 ? 4ll * s.B * s.H * s.segments * s.D * s.E : 0; }
 

@@ -1,5 +1,5 @@
-// The map of linear_common.cuh on TF32 instructions, for every type: entries of 16-bit types are TF32 numbers as they are, float32 ones and
-// what is formed in 32 bits are split in two (common.cuh).
+// The map of linear_common.cuh on TF32 instructions, for float16 and float32: entries of float16 are TF32 numbers as they are (and what is
+// formed of them in 32 bits may pass float16's range), float32 ones and what is formed in 32 bits are split in two (common.cuh).
 //
 // A CTA takes a segment of one head's rows, chunk by chunk.  Warp w keeps columns 16 w .. 16 w + 15 of M in registers, transposed (rows of the
 // accumulator are columns of M), which as it stands is the second operand of a M.  The weighted products of a chunk go through shared
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(2 * DT) scan_kernel(const __grid_constant__ Sc
     float x = 0.f, y = 0.f;
     if (OUT && d < p.D && e < p.E) {
       if (p.segments > 1) {
-        const long long at = ((long long)head * p.segments + segment) * size + (long long)d * p.E + e;
+        const long long at = ((long long)head * p.segments + segment) * size + d * p.state_stride[0] + e * p.state_stride[1];
         x = p.states[at];
         if (DUAL) y = p.tstates[at];
       } else {
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(2 * DT) scan_kernel(const __grid_constant__ Sc
   if constexpr (!OUT) {
     each([&](int i, int j, int d, int e) {
       if (d >= p.D || e >= p.E) return;
-      const long long at = ((long long)head * p.segments + segment) * size + (long long)d * p.E + e;
+      const long long at = ((long long)head * p.segments + segment) * size + d * p.state_stride[0] + e * p.state_stride[1];
       p.states[at] = M[i][j];
       if (DUAL) p.tstates[at] = tM[i][j];
     });
