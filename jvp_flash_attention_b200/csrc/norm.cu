@@ -13,7 +13,7 @@ int launch_fwd(const jvpfa_norm_args& a, cudaStream_t s);
 
 namespace {
 
-constexpr int kCols = 16, kLanes = 16;  // of a CTA that adds up parts: its columns, and how many take turns with the slices
+constexpr int kCols = 32, kLanes = 8;  // of a CTA that adds up parts: its columns, and how many take turns with the slices
 constexpr int kMostChunks = 64;         // of groups, each by CTAs of its own
 
 struct Totals {
@@ -49,6 +49,7 @@ __global__ void __launch_bounds__(kCols * kLanes) norm_parts_kernel(const __grid
   for (long long group = g0; group < g1; ++group) {
     float p[kParts] = {};
     if (live)
+#pragma unroll 4
       for (int slice = lane; slice < cut.slices; slice += kLanes) {
         const float* from = static_cast<const float*>(a.workspace) + (group * cut.slices + slice) * cut.n_parts * (long long)a.C + col;
 #pragma unroll
@@ -151,14 +152,12 @@ struct Plan {
   int64_t parts_bytes, bytes;
 };
 
-// Parts of a group's rows: as many as there are CTAs for, with at least 8 rows each, so that the parts stay a fraction of what is read.
+// Parts of a group's rows: one for each SM, with at least 4 rows each.
 Plan plan_bwd(const jvpfa_norm_args& a) {
   Plan p{};
   p.cut.groups = a.M / a.group_rows;
-  const int resident_ctas = a.C <= 1024 ? 4 : a.C <= 2048 ? 2 : 1;
-  const int most = a.C <= 256 ? 2048 : kSMs * resident_ctas;
-  int slices = most / p.cut.groups;
-  if (slices > a.group_rows / 8) slices = a.group_rows / 8;
+  int slices = kSMs / p.cut.groups;
+  if (slices > a.group_rows / 4) slices = a.group_rows / 4;
   p.cut.slices = slices < 1 ? 1 : slices;
   auto wants = [&](int i) { return a.d[i] || a.dt[i]; };
   if (wants(JVPFA_VEC_WEIGHT) || wants(JVPFA_VEC_SCALE)) p.cut.parts |= 1u << PG;

@@ -2,9 +2,9 @@
 //
 // A row is formed again from the operands and the four statistics of each norm that the forward kept, in 32 bits as there, so no result that
 // was rounded is read.  Two sums over the row's threads (five values each with tangents, two without) are all that its entries exchange.  The
-// vectors' gradients are sums over rows: each thread adds up its columns' in registers while its CTA goes through successive rows of one
-// group, and leaves them in the workspace; a second launch adds these parts in a fixed order.
-// What bounds it: memory, each tensor read and written once, and the parts.
+// vectors' gradients are sums over rows: each thread adds up its columns' in registers while its CTA, one on each SM and several rows at once, goes
+// through a part of one group's rows, and leaves them in the workspace; a second launch adds these parts in a fixed order.
+// What bounds it: memory, each tensor read and written once; with tangents and a residual sum the registers (170 of a thread, 12 warps).
 #pragma once
 #include "norm_common.cuh"
 
@@ -20,44 +20,37 @@ struct Cut {
   int n_parts;
 };
 
-template <typename T, int V, int NC, bool TAN, bool HASY, bool HASN>
-__global__ void __launch_bounds__(kAtMost) norm_bwd_kernel(const __grid_constant__ jvpfa_norm_args a, const Wide wide, const int threads, const Cut cut) {
-  constexpr int E = V * NC, ET = TAN ? E : 1;
-  __shared__ float sums[512];
-  const int team = threads == 32 ? (int)threadIdx.x >> 5 : 0, teams = (int)blockDim.x / threads;
-  const int tid = threads == 32 ? (int)threadIdx.x & 31 : (int)threadIdx.x;
-  RowSum row_sum{sums, threads / 32};
-  const long long workers = (long long)gridDim.x * teams, me = (long long)blockIdx.x * teams + team;
+template <typename T, int NC, Way WAY, bool TAN, bool HASY, bool HASN, int BOUND>
+__global__ void __launch_bounds__(BOUND) norm_bwd_kernel(const __grid_constant__ jvpfa_norm_args a, const Wide wide, const Layout lay, const bool aligned, const Cut cut) {
+  constexpr int V = 16 / (int)sizeof(T), E = V * NC, ET = TAN ? E : 1, SIDES = TAN ? 2 : 1;
+  constexpr int TENSORS = SIDES * ((HASY ? 3 : 1) + (HASN ? 1 : 0));
+  extern __shared__ __align__(16) unsigned char smem[];
+  const Team team{(int)threadIdx.x / lay.threads, lay.threads, (int)threadIdx.x % lay.threads};
+  unsigned char* mine = smem + team.index * lay.team_bytes;
+  RowSum row_sum{reinterpret_cast<float*>(mine), team};
+  unsigned char* ring = mine + kSumFloats * 4;
+  unsigned char* outs = ring + lay.depth * TENSORS * lay.slot;
+  float* shared_parts = reinterpret_cast<float*>(smem + lay.teams * lay.team_bytes);
+  const Rows<T, NC, WAY> rows{a.C, a.M, team, aligned};
+  // x, tx, gn, gtn, y, ty, gr, gtr, as far as there are any of them
+  Source sources[TENSORS];
+  int n_sources = 0;
+  auto source = [&](const void* p, long long stride) { sources[n_sources++] = Source{p, stride}; };
+  source(a.x, a.x_stride);
+  if (TAN) source(a.tx, a.tx_stride);
+  if (HASN) source(a.gn, a.C);
+  if (HASN && TAN) source(a.gtn, a.C);
+  if (HASY) source(a.y, a.y_stride);
+  if (HASY && TAN) source(a.ty, a.ty_stride);
+  if (HASY) source(a.gr, a.C);
+  if (HASY && TAN) source(a.gtr, a.C);
   const float by = 1.f / a.C;
   const bool layer = a.kind == JVPFA_NORM_LAYER, post_layer = a.post == JVPFA_NORM_LAYER, post = a.post != JVPFA_NORM_NONE;
-  bool live[NC];
-  int col[NC];
-#pragma unroll
-  for (int j = 0; j < NC; ++j) col[j] = (j * threads + tid) * V, live[j] = col[j] < a.C;
-  auto get = [&](float* to, const void* p, long long at) {  // a row's entries; zeros for an absent tensor and behind the end
-#pragma unroll
-    for (int j = 0; j < NC; ++j) {
-      if (p && live[j]) {
-        const Pack<T, V> x = load_pack<T, V>(static_cast<const T*>(p) + at + col[j]);
-#pragma unroll
-        for (int i = 0; i < V; ++i) to[j * V + i] = Elem<T>::to_float(x.e[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) to[j * V + i] = 0.f;
-      }
-    }
-  };
-  auto put = [&](void* p, long long at, const float* x) {
-    if (!p) return;
-#pragma unroll
-    for (int j = 0; j < NC; ++j)
-      if (live[j]) store_floats<T, V>(static_cast<T*>(p) + at + col[j], x + j * V);
-  };
 
-  for (long long unit = me; unit < (long long)cut.groups * cut.slices; unit += workers) {
+  for (long long unit = blockIdx.x; unit < (long long)cut.groups * cut.slices; unit += gridDim.x) {
     const long long group = unit / cut.slices;
     const int slice = (int)(unit - group * cut.slices);
-    const int first = (int)(group * a.group_rows + (long long)a.group_rows * slice / cut.slices);
+    const int first = (int)(group * a.group_rows + (long long)a.group_rows * slice / cut.slices) + team.index;
     const int end = (int)(group * a.group_rows + (long long)a.group_rows * (slice + 1) / cut.slices);
     float pG[HASN ? E : 1], pO[HASN ? E : 1], pE[HASY ? E : 1], ptG[HASN ? ET : 1], ptO[HASN ? ET : 1], ptE[HASY ? ET : 1];
 #pragma unroll
@@ -67,31 +60,64 @@ __global__ void __launch_bounds__(kAtMost) norm_bwd_kernel(const __grid_constant
       if (HASN && TAN) ptG[e] = ptO[e] = 0.f;
       if (HASY && TAN) ptE[e] = 0.f;
     }
-    for (int row = first; row < end; ++row) {
-      const long long at = (long long)row * a.C;
+    auto fetch = [&](int k) {  // the team's k-th row
+      const int row = first + k * lay.teams;
+      if (row < end) {
+        unsigned char* to = ring + k % lay.depth * TENSORS * lay.slot;
+#pragma unroll
+        for (int i = 0; i < TENSORS; ++i) rows.fetch(to + i * lay.slot, sources[i], row);
+      }
+      cp_async_commit();
+    };
+    if (WAY != DIRECT)
+      for (int k = 0; k < lay.depth; ++k) fetch(k);
+    for (int row = first, k = 0; row < end; row += lay.teams, ++k) {
       float r[E], tr[ET], m[HASY ? E : 1], tm[HASY ? ET : 1], Eg[HASY ? E : 1], tE[HASY ? ET : 1];
-      float dr[E], dtr[ET];
-      get(r, a.x, row * a.x_stride);
-      if (TAN) get(tr, a.tx, row * a.tx_stride);
-      if (HASY) get(m, a.y, row * a.y_stride);
-      if (HASY && TAN) get(tm, a.ty, row * a.ty_stride);
-      float g[HASN ? E : 1], h[HASN ? ET : 1];
-      if (HASN) get(g, a.gn, at);
-      if (HASN && TAN) get(h, a.gtn, at);
-      get(dr, HASY ? a.gr : nullptr, at);
-      if (TAN) get(dtr, HASY ? a.gtr : nullptr, at);
+      float dr[E], dtr[ET], g[HASN ? E : 1], h[HASN ? ET : 1];
+      if (WAY != DIRECT) wait_rows(lay.depth);
+      if (WAY == RAGGED) team.sync();
+      {
+        const unsigned char* from = ring + k % lay.depth * TENSORS * lay.slot;
+        int at = 0;
+        auto get = [&](float* to) {
+          Pieces<T, NC> raw;
+          rows.read(raw, from + at * lay.slot, sources[at], row);
+          ++at;
+#pragma unroll
+          for (int j = 0; j < NC; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) to[j * V + i] = raw.at(j, i);
+        };
+        get(r);
+        if (TAN) get(tr);
+        if (HASN) get(g);
+        if (HASN && TAN) get(h);
+        if (HASY) get(m);
+        if (HASY && TAN) get(tm);
+        if (HASY) get(dr);
+        if (HASY && TAN) get(dtr);
+      }
+      if constexpr (!HASY) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          dr[e] = 0.f;
+          if (TAN) dtr[e] = 0.f;
+        }
+      }
+      if (WAY == RAGGED) team.sync();
+      if (WAY != DIRECT) fetch(k + lay.depth);
       const float4* st = reinterpret_cast<const float4*>(a.stats) + 2ll * row;
       const float4 sy = st[0], sr = st[1];  // mean, 1 / deviation, the tangent's mean, mean(n tangent)
       if (HASY) {
 #pragma unroll
         for (int j = 0; j < NC; ++j)
-          if (live[j]) gate_of<T, V, TAN>(a, wide, group, col[j], Eg + j * V, tE + (TAN ? j * V : 0));
+          if (rows.on(j, 0)) gate_of<T, V, TAN>(a, wide, group, rows.piece(j) * V, Eg + j * V, tE + (TAN ? j * V : 0));
 #pragma unroll
         for (int j = 0; j < NC; ++j)
 #pragma unroll
           for (int i = 0; i < V; ++i) {
             const int e = j * V + i;
-            if (!live[j]) {
+            if (!rows.on(j, i)) {
               Eg[e] = 0.f;
               if (TAN) tE[e] = 0.f;
               continue;
@@ -110,25 +136,25 @@ __global__ void __launch_bounds__(kAtMost) norm_bwd_kernel(const __grid_constant
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
           float G[V], O[V], tG[V], tO[V];
-          if (!live[j]) {
+          if (!rows.on(j, 0)) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
               const int e = j * V + i;
-              r[e] = g[e] = 0.f;
-              if (TAN) tr[e] = h[e] = 0.f;
+              r[e] = 0.f;
+              if (TAN) tr[e] = 0.f;
             }
-            continue;
+            continue;  // (g and h are zero there)
           }
-          gain_of<T, V, TAN>(a, wide, group, col[j], G, O, tG, tO);
+          gain_of<T, V, TAN>(a, wide, group, rows.piece(j) * V, G, O, tG, tO);
 #pragma unroll
           for (int i = 0; i < V; ++i) {
             const int e = j * V + i;
-            const float n = (r[e] - sr.x) * sr.y;
+            const float n = rows.on(j, i) ? (r[e] - sr.x) * sr.y : 0.f;
             r[e] = n;
             pO[e] += g[e];
             pG[e] += g[e] * n;
             if (TAN) {
-              const float tn = sr.y * (tr[e] - sr.z - n * sr.w);
+              const float tn = rows.on(j, i) ? sr.y * (tr[e] - sr.z - n * sr.w) : 0.f;
               tr[e] = tn;
               ptO[e] += h[e], ptG[e] += h[e] * n, pG[e] += h[e] * tn;
               const float gh = h[e] * G[i];
@@ -158,8 +184,8 @@ __global__ void __launch_bounds__(kAtMost) norm_bwd_kernel(const __grid_constant
           }
         }
       }
-      put(a.dx, at, dr);
-      if (TAN) put(a.dtx, at, dtr);
+      rows.write(a.dx, row, dr, outs);
+      if (TAN) rows.write(a.dtx, row, dtr, outs + lay.slot);
       if (HASY) {
         float s[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -196,37 +222,52 @@ __global__ void __launch_bounds__(kAtMost) norm_bwd_kernel(const __grid_constant
             }
           }
         }
-        put(a.dy, at, dr);
-        if (TAN) put(a.dty, at, dtr);
+        rows.write(a.dy, row, dr, outs + SIDES * lay.slot);
+        if (TAN) rows.write(a.dty, row, dtr, outs + 3 * lay.slot);
       }
     }
     if (cut.parts) {
       float* to = static_cast<float*>(a.workspace) + unit * cut.n_parts * (long long)a.C;
-      auto leave = [&](int part, const float* x) {
-        if (!(cut.parts >> part & 1)) return;
+      // the rows of a CTA one after the other, through shared memory
+      for (int turn = 0; turn < lay.teams; ++turn) {
+        if (turn == team.index) {
+          int part = 0;
+          auto leave = [&](Part which, const float* x) {
+            if (!(cut.parts >> which & 1)) return;
+            const bool last = turn == lay.teams - 1;
 #pragma unroll
-        for (int j = 0; j < NC; ++j)
-          if (live[j])
+            for (int j = 0; j < NC; ++j)
 #pragma unroll
-            for (int i = 0; i < V; ++i) to[col[j] + i] = x[j * V + i];
-        to += a.C;
-      };
-      if (HASN) leave(PG, pG), leave(PO, pO);
-      if (HASY) leave(PE, pE);
-      if (HASN && TAN) leave(PtG, ptG), leave(PtO, ptO);
-      if (HASY && TAN) leave(PtE, ptE);
+              for (int i = 0; i < V; ++i) {
+                if (!rows.on(j, i)) continue;
+                const int col = rows.piece(j) * V + i;
+                const float sum = turn ? shared_parts[part * a.C + col] + x[j * V + i] : x[j * V + i];
+                (last ? to : shared_parts)[part * a.C + col] = sum;
+              }
+            ++part;
+          };
+          if (HASN) leave(PG, pG), leave(PO, pO);
+          if (HASY) leave(PE, pE);
+          if (HASN && TAN) leave(PtG, ptG), leave(PtO, ptO);
+          if (HASY && TAN) leave(PtE, ptE);
+        }
+        if (lay.teams > 1) __syncthreads();
+      }
     }
+    cp_async_wait<0>();  // (groups without rows)
   }
 }
 
-template <typename T, int V, int NC, bool TAN, bool HASY, bool HASN>
-int launch_bwd(const jvpfa_norm_args& a, const Cut& cut, cudaStream_t s) {
-  const auto kernel = norm_bwd_kernel<T, V, NC, TAN, HASY, HASN>;
-  static int known[33] = {};
-  const int threads = (a.C + V * NC * 32 - 1) / (V * NC * 32) * 32;
-  const int cta = threads == 32 ? 128 : threads, teams = cta / threads;
-  const long long units = ((long long)cut.groups * cut.slices + teams - 1) / teams, most = (long long)kSMs * resident(kernel, cta, known);
-  kernel<<<(unsigned)(units < most ? units : most), cta, 0, s>>>(a, wide_vectors(a), threads, cut);
+template <typename T, int NC, Way WAY, bool TAN, bool HASY, bool HASN, int BOUND>
+int launch_bwd(const jvpfa_norm_args& a, const Cut& cut, bool aligned, cudaStream_t s) {
+  const auto kernel = norm_bwd_kernel<T, NC, WAY, TAN, HASY, HASN, BOUND>;
+  static SmemOptIn opt;
+  const int sides = TAN ? 2 : 1;
+  const Layout lay = layout_of(a, WAY, 16 / (int)sizeof(T) * NC, BOUND, sides * ((HASY ? 3 : 1) + (HASN ? 1 : 0)), sides * (HASY ? 2 : 1), cut.n_parts);
+  if (lay.depth < 1) return JVPFA_ERR_UNSUPPORTED;
+  if (!opt.ensure(reinterpret_cast<const void*>(kernel), 225 * 1024)) return JVPFA_ERR_CUDA;
+  const long long units = (long long)cut.groups * cut.slices, most = kSMs * (lay.bytes < 110 * 1024 && 2 * lay.threads * lay.teams <= BOUND ? 2 : 1);
+  kernel<<<(unsigned)(units < most ? units : most), lay.threads * lay.teams, lay.bytes, s>>>(a, wide_vectors(a), lay, aligned, cut);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {
     set_last_cuda_error(e, "norm_bwd_kernel");
@@ -235,19 +276,27 @@ int launch_bwd(const jvpfa_norm_args& a, const Cut& cut, cudaStream_t s) {
   return JVPFA_OK;
 }
 
-template <typename T, int V, int NC>
-int launch_bwd(const jvpfa_norm_args& a, const Cut& c, cudaStream_t s) {
+template <typename T, int NC, Way WAY, int BOUND>
+int launch_bwd(const jvpfa_norm_args& a, const Cut& c, bool al, cudaStream_t s) {
   const bool y = a.y != nullptr, n = a.kind != JVPFA_NORM_NONE;
-  if (a.dual) return y ? (n ? launch_bwd<T, V, NC, true, true, true>(a, c, s) : launch_bwd<T, V, NC, true, true, false>(a, c, s)) : launch_bwd<T, V, NC, true, false, true>(a, c, s);
-  return y ? (n ? launch_bwd<T, V, NC, false, true, true>(a, c, s) : launch_bwd<T, V, NC, false, true, false>(a, c, s)) : launch_bwd<T, V, NC, false, false, true>(a, c, s);
+  // with tangents a row's threads have 170 registers where it takes at most 384 of them
+  if (a.dual)
+    return !y ? launch_bwd<T, NC, WAY, true, false, true, BOUND>(a, c, al, s)
+           : n ? launch_bwd<T, NC, WAY, true, true, true, BOUND>(a, c, al, s) : launch_bwd<T, NC, WAY, true, true, false, BOUND>(a, c, al, s);
+  return !y ? launch_bwd<T, NC, WAY, false, false, true, 512>(a, c, al, s)
+         : n ? launch_bwd<T, NC, WAY, false, true, true, 512>(a, c, al, s) : launch_bwd<T, NC, WAY, false, true, false, 512>(a, c, al, s);
 }
 
+// As the forward's, and for what does not fit in shared memory.
 template <typename T>
 int launch_bwd(const jvpfa_norm_args& a, const Cut& c, cudaStream_t s) {
   constexpr int V = 16 / (int)sizeof(T);
-  if (vector_entries(a) == 1) return a.C <= 16 * kAtMost ? launch_bwd<T, 1, 16>(a, c, s) : launch_bwd<T, 1, 32>(a, c, s);
-  if (a.C <= 8 * kAtMost) return launch_bwd<T, V, 8 / V>(a, c, s);
-  return a.C <= 16 * kAtMost ? launch_bwd<T, V, 16 / V>(a, c, s) : launch_bwd<T, V, 32 / V>(a, c, s);
+  const bool aligned = aligned_rows(a);
+  if (a.C <= 8 * 384) return aligned ? launch_bwd<T, 8 / V, ALIGNED, 384>(a, c, true, s) : launch_bwd<T, 8 / V, RAGGED, 384>(a, c, false, s);
+  if (a.C <= 4096) return aligned ? launch_bwd<T, 8 / V, ALIGNED, 512>(a, c, true, s) : launch_bwd<T, 8 / V, RAGGED, 512>(a, c, false, s);
+  if constexpr (sizeof(T) == 2)
+    if (a.C <= 8192 && aligned) return launch_bwd<T, 16 / V, ALIGNED, 512>(a, c, true, s);
+  return launch_bwd<T, 32 / V, DIRECT, 512>(a, c, aligned, s);
 }
 
 }  // namespace norms
