@@ -30,7 +30,11 @@ __global__ void __launch_bounds__(BOUND) norm_bwd_kernel(const __grid_constant__
   RowSum row_sum{reinterpret_cast<float*>(mine), team};
   unsigned char* ring = mine + kSumFloats * 4;
   unsigned char* outs = ring + lay.depth * TENSORS * lay.slot;
-  float* shared_parts = reinterpret_cast<float*>(smem + lay.teams * lay.team_bytes);
+  // the vectors of the group in work, put together: E, tE, G, tG
+  constexpr int VECTORS = SIDES * ((HASY ? 1 : 0) + (HASN ? 1 : 0));
+  float* vectors = reinterpret_cast<float*>(smem + lay.teams * lay.team_bytes);
+  const int padded = (a.C + V - 1) / V * V;
+  float* shared_parts = vectors + VECTORS * padded;
   const Rows<T, NC, WAY> rows{a.C, a.M, team, aligned};
   // x, tx, gn, gtn, y, ty, gr, gtr, as far as there are any of them
   Source sources[TENSORS];
@@ -60,28 +64,45 @@ __global__ void __launch_bounds__(BOUND) norm_bwd_kernel(const __grid_constant__
       if (HASN && TAN) ptG[e] = ptO[e] = 0.f;
       if (HASY && TAN) ptE[e] = 0.f;
     }
-    auto fetch = [&](int k) {  // the team's k-th row
-      const int row = first + k * lay.teams;
+    // (everybody has read the vectors of the unit before: its sums are behind a barrier where several rows share the CTA)
+    if (WAY != DIRECT) {
+      if (lay.teams == 1 || !cut.parts) __syncthreads();
+      for (int col = threadIdx.x * V; col < a.C; col += blockDim.x * V) {
+        float x[4][V];
+        float O[V], tO[V];
+        if (HASY) gate_of<T, V, TAN>(a, wide, group, col, x[0], x[1]);
+        if (HASN) gain_of<T, V, TAN>(a, wide, group, col, x[HASY ? SIDES : 0], O, x[HASY ? 3 : 1], tO);
+#pragma unroll
+        for (int k = 0; k < VECTORS; ++k)
+#pragma unroll
+          for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(rows.place(vectors + k * padded, col / V, i)) = make_float4(x[k][i], x[k][i + 1], x[k][i + 2], x[k][i + 3]);
+      }
+      __syncthreads();
+    }
+    // piece j of one of them
+    auto vector = [&](float* to, int which, int j) { rows.vector(to, vectors + which * padded, j); };
+    auto fetch = [&](unsigned char* to, int row) {
       if (row < end) {
-        unsigned char* to = ring + k % lay.depth * TENSORS * lay.slot;
 #pragma unroll
         for (int i = 0; i < TENSORS; ++i) rows.fetch(to + i * lay.slot, sources[i], row);
       }
       cp_async_commit();
     };
     if (WAY != DIRECT)
-      for (int k = 0; k < lay.depth; ++k) fetch(k);
-    for (int row = first, k = 0; row < end; row += lay.teams, ++k) {
+      for (int k = 0; k < lay.depth; ++k) fetch(ring + k * TENSORS * lay.slot, first + k * lay.teams);
+    unsigned char* slot = ring;
+    const float4* stats = reinterpret_cast<const float4*>(a.stats);
+    float4 next_y = first < end ? stats[2ll * first] : float4{}, next_r = first < end ? stats[2ll * first + 1] : float4{};
+    for (int row = first; row < end; row += lay.teams) {
       float r[E], tr[ET], m[HASY ? E : 1], tm[HASY ? ET : 1], Eg[HASY ? E : 1], tE[HASY ? ET : 1];
       float dr[E], dtr[ET], g[HASN ? E : 1], h[HASN ? ET : 1];
       if (WAY != DIRECT) wait_rows(lay.depth);
       if (WAY == RAGGED) team.sync();
       {
-        const unsigned char* from = ring + k % lay.depth * TENSORS * lay.slot;
         int at = 0;
         auto get = [&](float* to) {
           Pieces<T, NC> raw;
-          rows.read(raw, from + at * lay.slot, sources[at], row);
+          rows.read(raw, slot + at * lay.slot, sources[at], row);
           ++at;
 #pragma unroll
           for (int j = 0; j < NC; ++j)
@@ -105,13 +126,24 @@ __global__ void __launch_bounds__(BOUND) norm_bwd_kernel(const __grid_constant__
         }
       }
       if (WAY == RAGGED) team.sync();
-      if (WAY != DIRECT) fetch(k + lay.depth);
-      const float4* st = reinterpret_cast<const float4*>(a.stats) + 2ll * row;
-      const float4 sy = st[0], sr = st[1];  // mean, 1 / deviation, the tangent's mean, mean(n tangent)
+      if (WAY != DIRECT) {
+        fetch(slot, row + lay.depth * lay.teams);
+        slot += TENSORS * lay.slot;
+        if (slot == outs) slot = ring;
+      }
+      const float4 sy = next_y, sr = next_r;  // mean, 1 / deviation, the tangent's mean, mean(n tangent)
+      if (row + lay.teams < end) next_y = stats[2ll * (row + lay.teams)], next_r = stats[2ll * (row + lay.teams) + 1];
       if (HASY) {
 #pragma unroll
         for (int j = 0; j < NC; ++j)
-          if (rows.on(j, 0)) gate_of<T, V, TAN>(a, wide, group, rows.piece(j) * V, Eg + j * V, tE + (TAN ? j * V : 0));
+          if (rows.on(j, 0)) {
+            if (WAY == DIRECT) {
+              gate_of<T, V, TAN>(a, wide, group, rows.piece(j) * V, Eg + j * V, tE + (TAN ? j * V : 0));
+            } else {
+              vector(Eg + j * V, 0, j);
+              if (TAN) vector(tE + (TAN ? j * V : 0), 1, j);
+            }
+          }
 #pragma unroll
         for (int j = 0; j < NC; ++j)
 #pragma unroll
@@ -145,7 +177,12 @@ __global__ void __launch_bounds__(BOUND) norm_bwd_kernel(const __grid_constant__
             }
             continue;  // (g and h are zero there)
           }
-          gain_of<T, V, TAN>(a, wide, group, rows.piece(j) * V, G, O, tG, tO);
+          if (WAY == DIRECT) {
+            gain_of<T, V, TAN>(a, wide, group, rows.piece(j) * V, G, O, tG, tO);
+          } else {
+            vector(G, HASY ? SIDES : 0, j);
+            if (TAN) vector(tG, HASY ? 3 : 1, j);
+          }
 #pragma unroll
           for (int i = 0; i < V; ++i) {
             const int e = j * V + i;
@@ -258,15 +295,19 @@ __global__ void __launch_bounds__(BOUND) norm_bwd_kernel(const __grid_constant__
   }
 }
 
-template <typename T, int NC, Way WAY, bool TAN, bool HASY, bool HASN, int BOUND>
+constexpr int kDoesNotFit = 1;
+
+template <typename T, int E, Way WAY, bool TAN, bool HASY, bool HASN, int BOUND>
 int launch_bwd(const jvpfa_norm_args& a, const Cut& cut, bool aligned, cudaStream_t s) {
+  constexpr int NC = E * (int)sizeof(T) / 16, SIDES = TAN ? 2 : 1;
   const auto kernel = norm_bwd_kernel<T, NC, WAY, TAN, HASY, HASN, BOUND>;
   static SmemOptIn opt;
-  const int sides = TAN ? 2 : 1;
-  const Layout lay = layout_of(a, WAY, 16 / (int)sizeof(T) * NC, BOUND, sides * ((HASY ? 3 : 1) + (HASN ? 1 : 0)), sides * (HASY ? 2 : 1), cut.n_parts);
-  if (lay.depth < 1) return JVPFA_ERR_UNSUPPORTED;
+  static int registers = 0;
+  const Layout lay = layout_of(a, WAY, E, BOUND, registers_of(kernel, registers), SIDES * ((HASY ? 3 : 1) + (HASN ? 1 : 0)), SIDES * (HASY ? 2 : 1), cut.n_parts,
+                               WAY == DIRECT ? 0 : SIDES * ((HASY ? 1 : 0) + (HASN ? 1 : 0)));
+  if (lay.depth < 1) return kDoesNotFit;
   if (!opt.ensure(reinterpret_cast<const void*>(kernel), 225 * 1024)) return JVPFA_ERR_CUDA;
-  const long long units = (long long)cut.groups * cut.slices, most = kSMs * (lay.bytes < 110 * 1024 && 2 * lay.threads * lay.teams <= BOUND ? 2 : 1);
+  const long long units = (long long)cut.groups * cut.slices, most = kSMs * lay.ctas;
   kernel<<<(unsigned)(units < most ? units : most), lay.threads * lay.teams, lay.bytes, s>>>(a, wide_vectors(a), lay, aligned, cut);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {
@@ -276,27 +317,37 @@ int launch_bwd(const jvpfa_norm_args& a, const Cut& cut, bool aligned, cudaStrea
   return JVPFA_OK;
 }
 
-template <typename T, int NC, Way WAY, int BOUND>
+// Entries of a thread: 8 with tangents or with the sum and its norm, else 16 of rows that give them to a whole warp; threads have 170 registers
+// with 16 entries or tangents, where a row takes at most 384 of them, else 128.  (us at 8 / 16 entries, 512 threads / 16 and 384: the norm of
+// fp16 3990 x 2731 rows 58 / 46 / 43, bf16 8192 x 4096 with sum and both norms 121 / 165 / 149, where 16 entries and their sums leave the
+// registers or, with 384 threads, one row in work on an SM.)
+template <typename T, Way WAY, bool TAN, bool HASY, bool HASN>
 int launch_bwd(const jvpfa_norm_args& a, const Cut& c, bool al, cudaStream_t s) {
-  const bool y = a.y != nullptr, n = a.kind != JVPFA_NORM_NONE;
-  // with tangents a row's threads have 170 registers where it takes at most 384 of them
-  if (a.dual)
-    return !y ? launch_bwd<T, NC, WAY, true, false, true, BOUND>(a, c, al, s)
-           : n ? launch_bwd<T, NC, WAY, true, true, true, BOUND>(a, c, al, s) : launch_bwd<T, NC, WAY, true, true, false, BOUND>(a, c, al, s);
-  return !y ? launch_bwd<T, NC, WAY, false, false, true, 512>(a, c, al, s)
-         : n ? launch_bwd<T, NC, WAY, false, true, true, 512>(a, c, al, s) : launch_bwd<T, NC, WAY, false, true, false, 512>(a, c, al, s);
+  if constexpr (WAY == DIRECT) {
+    return launch_bwd<T, 32, WAY, TAN, HASY, HASN, 512>(a, c, al, s);
+  } else if constexpr (TAN) {
+    if (a.C <= 8 * 384) return launch_bwd<T, 8, WAY, TAN, HASY, HASN, 384>(a, c, al, s);
+    return a.C <= 4096 ? launch_bwd<T, 8, WAY, TAN, HASY, HASN, 512>(a, c, al, s) : kDoesNotFit;
+  } else {
+    if (a.C <= 256 || (HASY && HASN && a.C <= 4096)) return launch_bwd<T, 8, WAY, TAN, HASY, HASN, 512>(a, c, al, s);
+    if (a.C <= 16 * 384) return launch_bwd<T, 16, WAY, TAN, HASY, HASN, 384>(a, c, al, s);
+    return a.C <= 8192 ? launch_bwd<T, 16, WAY, TAN, HASY, HASN, 512>(a, c, al, s) : kDoesNotFit;
+  }
 }
 
-// As the forward's, and for what does not fit in shared memory.
+template <typename T, Way WAY>
+int launch_bwd(const jvpfa_norm_args& a, const Cut& c, bool al, cudaStream_t s) {
+  const bool y = a.y != nullptr, n = a.kind != JVPFA_NORM_NONE;
+  if (a.dual)
+    return !y ? launch_bwd<T, WAY, true, false, true>(a, c, al, s) : n ? launch_bwd<T, WAY, true, true, true>(a, c, al, s) : launch_bwd<T, WAY, true, true, false>(a, c, al, s);
+  return !y ? launch_bwd<T, WAY, false, false, true>(a, c, al, s) : n ? launch_bwd<T, WAY, false, true, true>(a, c, al, s) : launch_bwd<T, WAY, false, true, false>(a, c, al, s);
+}
+
 template <typename T>
 int launch_bwd(const jvpfa_norm_args& a, const Cut& c, cudaStream_t s) {
-  constexpr int V = 16 / (int)sizeof(T);
   const bool aligned = aligned_rows(a);
-  if (a.C <= 8 * 384) return aligned ? launch_bwd<T, 8 / V, ALIGNED, 384>(a, c, true, s) : launch_bwd<T, 8 / V, RAGGED, 384>(a, c, false, s);
-  if (a.C <= 4096) return aligned ? launch_bwd<T, 8 / V, ALIGNED, 512>(a, c, true, s) : launch_bwd<T, 8 / V, RAGGED, 512>(a, c, false, s);
-  if constexpr (sizeof(T) == 2)
-    if (a.C <= 8192 && aligned) return launch_bwd<T, 16 / V, ALIGNED, 512>(a, c, true, s);
-  return launch_bwd<T, 32 / V, DIRECT, 512>(a, c, aligned, s);
+  const int rc = aligned ? launch_bwd<T, ALIGNED>(a, c, true, s) : launch_bwd<T, RAGGED>(a, c, false, s);
+  return rc == kDoesNotFit ? launch_bwd<T, DIRECT>(a, c, aligned, s) : rc;
 }
 
 }  // namespace norms

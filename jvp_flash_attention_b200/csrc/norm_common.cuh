@@ -184,18 +184,17 @@ struct RowSum {
     }
     float* b = buf + turn * 128;
     turn ^= 1;
-    if (lane % kStride == 0) b[(team.tid >> 5) * 8 + which] = v[0];
+    if (lane % kStride == 0) b[(team.tid >> 5) * P + which] = v[0];
     team.sync();
+    // lane: value lane % P of warps lane / P, lane / P + 32 / P, ...
+    float sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) x[k] = 0.f;
-    for (int i = 0; i < warps; ++i) {
-      const float4 lo = *reinterpret_cast<const float4*>(b + i * 8);
-      x[0] += lo.x;
-      if constexpr (K > 1) x[1] += lo.y;
-      if constexpr (K > 2) x[2] += lo.z;
-      if constexpr (K > 3) x[3] += lo.w;
-      if constexpr (K > 4) x[4] += b[i * 8 + 4];
-    }
+    for (int i = 0; i < 16 * P; i += 32)
+      if (i + lane < warps * P) sum += b[i + lane];
+#pragma unroll
+    for (int o = P; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+#pragma unroll
+    for (int k = 0; k < K; ++k) x[k] = __shfl_sync(0xffffffffu, sum, k);
   }
 };
 constexpr int kSumFloats = 256;  // of a row's RowSum
@@ -331,6 +330,15 @@ struct Rows {
       }
     }
   }
+  // A vector of 32 bits in shared memory: four entries of each piece, then the next four of each, so that neighbours read neighbouring 16 bytes.
+  __device__ __forceinline__ float* place(float* vector, int piece_, int i) const { return vector + (i / 4 * ((C + V - 1) / V) + piece_) * 4; }
+  __device__ __forceinline__ void vector(float* to, float* from, int j) const {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(place(from, piece(j), i));
+      to[i] = x.x, to[i + 1] = x.y, to[i + 2] = x.z, to[i + 3] = x.w;
+    }
+  }
   // x: V entries of each piece.  RAGGED ones go through `slot`, which nobody may still be reading.
   __device__ __forceinline__ void write(void* p, int row, const float* x, unsigned char* slot) const {
     if (!p) return;
@@ -393,30 +401,49 @@ __device__ __forceinline__ void wait_rows(int depth) {  // for the oldest of `de
     cp_async_wait<3>();
 }
 
-// How a launch is laid out: threads of a row, rows of a CTA at once, rows ahead, the shared memory of a row and of a CTA.
+// How a launch is laid out: threads of a row, rows of a CTA at once, rows ahead, the shared memory of a row and of a CTA, CTAs of an SM.
 struct Layout {
-  int threads, teams, depth, slot, team_bytes, bytes;
+  int threads, teams, depth, slot, team_bytes, bytes, ctas;
 };
-// `tensors` read and `written`; `parts` of a CTA's sums where several rows share it.  Where no row fits, depth is 0.
-inline Layout layout_of(const jvpfa_norm_args& a, Way way, int entries, int most_threads, int tensors, int written, int parts) {
+// `tensors` read and `written`; `parts` of a CTA's sums where several rows share it; `vectors` of 32 bits that it keeps.  Where no row fits, depth is 0.
+// As many rows at once as the registers allow: a row alone waits for its sums most of the time.
+inline Layout layout_of(const jvpfa_norm_args& a, Way way, int entries, int most_threads, int registers, int tensors, int written, int parts, int vectors) {
   const int size = a.dtype == JVPFA_FP32 ? 4 : 2;
   Layout l;
   l.threads = (a.C + entries * 32 - 1) / (entries * 32) * 32;
   l.slot = way == DIRECT ? 0 : (a.C * size + 15) / 16 * 16 + (way == RAGGED ? 32 : 0);
-  const int rows = (a.M + kSMs - 1) / kSMs;
+  const int of_sm = (a.M + kSMs - 1) / kSMs, rows = of_sm < a.group_rows ? of_sm : a.group_rows;
   l.teams = most_threads / l.threads;
   if (l.teams > 15) l.teams = 15;  // (16 barriers, one of them the CTA's)
   if (l.teams > rows) l.teams = rows;
   if (l.teams < 1) l.teams = 1;
-  const int room = 225 * 1024;
   for (;; --l.teams) {
-    for (l.depth = way == DIRECT ? 1 : kMostDepth; l.depth >= 1; --l.depth) {
-      l.team_bytes = kSumFloats * 4 + (l.depth * tensors + (way == RAGGED ? written : 0)) * l.slot;
-      l.bytes = l.teams * l.team_bytes + (l.teams > 1 ? parts * a.C * 4 : 0);
-      if (l.bytes <= room) return l;
-    }
+    l.ctas = 65536 / ((registers + 7) / 8 * 8 * l.threads * l.teams);
+    if (l.ctas > (of_sm + l.teams - 1) / l.teams) l.ctas = (of_sm + l.teams - 1) / l.teams;
+    if (l.ctas > 16) l.ctas = 16;
+    if (l.ctas < 1) l.ctas = 1;
+    for (; l.ctas >= 1; --l.ctas)
+      for (l.depth = way == DIRECT ? 1 : kMostDepth; l.depth >= 1; --l.depth) {
+        l.team_bytes = kSumFloats * 4 + (l.depth * tensors + (way == RAGGED ? written : 0)) * l.slot;
+        l.bytes = l.teams * l.team_bytes + ((l.teams > 1 ? parts : 0) + vectors) * ((a.C + 7) / 8 * 8) * 4;
+        if (l.bytes + 1024 <= 226 * 1024 / l.ctas) return l;
+      }
     if (l.teams == 1) return l;
   }
+}
+
+// A kernel's registers, asked for once.
+template <typename K>
+int registers_of(K kernel, int& known) {
+  int n = __atomic_load_n(&known, __ATOMIC_RELAXED);
+  if (n) return n;
+  cudaFuncAttributes at;
+  if (cudaFuncGetAttributes(&at, reinterpret_cast<const void*>(kernel)) != cudaSuccess) {
+    cudaGetLastError();
+    return 128;
+  }
+  __atomic_store_n(&known, at.numRegs, __ATOMIC_RELAXED);
+  return at.numRegs;
 }
 
 // Whether all rows begin on 16 bytes and are whole pieces of 16.
