@@ -541,9 +541,16 @@ typedef struct {
   const float *gstate, *gtstate;     /* cotangents of state_out, tstate_out */
   jvpfa_linear_tensor dq, dk, dv, dtq, dtk, dtv; /* written; NULL: not wanted */
   float *dstate, *dtstate;
+  /* states inside the sequences, which the forward leaves for the backward: jvpfa_linear_kept_bytes() bytes, 16-byte aligned, or NULL.  In the
+   * backward kept_dual says whether the forward that left them had tangents. */
+  void* kept;
+  int32_t kept_dual;
   void* workspace; /* jvpfa_linear_fwd_workspace() / _bwd_workspace() bytes, 16-byte aligned (0: NULL) */
   int64_t workspace_bytes;
 } jvpfa_linear_args;
+
+/* Bytes of jvpfa_linear_args.kept for a forward with these sizes, type and dual (0: none are needed); host logic. */
+int64_t jvpfa_linear_kept_bytes(const jvpfa_linear_args* args);
 
 int jvpfa_linear_fwd(const jvpfa_linear_args* args, void* stream);
 int64_t jvpfa_linear_fwd_workspace(const jvpfa_linear_args* args);

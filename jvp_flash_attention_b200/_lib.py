@@ -66,6 +66,7 @@ EXPORTS = (
     "jvpfa_linear_fwd_workspace",
     "jvpfa_linear_bwd",
     "jvpfa_linear_bwd_workspace",
+    "jvpfa_linear_kept_bytes",
     "jvpfa_linear_step",
 )
 
@@ -384,6 +385,8 @@ class LinearArgs(C.Structure):
         *((name, LinearTensor) for name in ("dq", "dk", "dv", "dtq", "dtk", "dtv")),
         ("dstate", C.c_void_p),
         ("dtstate", C.c_void_p),
+        ("kept", C.c_void_p),
+        ("kept_dual", C.c_int32),
         ("workspace", C.c_void_p),
         ("workspace_bytes", C.c_int64),
     ]
@@ -462,8 +465,9 @@ def load() -> C.CDLL:
                        ("linear_step", LinearStepArgs)):
         entry = getattr(lib, "jvpfa_" + name)
         entry.argtypes, entry.restype = [C.POINTER(args), C.c_void_p], C.c_int
-    for name, args in (("norm_bwd", NormArgs), ("linear_fwd", LinearArgs), ("linear_bwd", LinearArgs)):
-        entry = getattr(lib, f"jvpfa_{name}_workspace")
+    for name, args in (("norm_bwd_workspace", NormArgs), ("linear_fwd_workspace", LinearArgs), ("linear_bwd_workspace", LinearArgs),
+                       ("linear_kept_bytes", LinearArgs)):
+        entry = getattr(lib, "jvpfa_" + name)
         entry.argtypes, entry.restype = [C.POINTER(args)], C.c_int64
     _lib = lib
     return lib

@@ -50,20 +50,28 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Scan 
 
 // Rows of a segment and segments (1: no workspace).
 void cut(Scan& s) {
-  // As many CTAs as SMs hold at once, and no segment below 128 rows
+  // Rounds of as many CTAs as SMs hold at once, in units of a whole head's time, and the states that each segment costs, about 1/250 of that; no
+  // segment below 128 rows.  (bf16 B4 H16 L8192 D128, 296 at once: 4 segments, 256 CTAs, 1.75 ms forward and backward; 9 segments 1.62.)
   const int heads = s.B * s.H, width = s.D > s.E ? s.D : s.E;
   const int room = kSMs * (width <= 64 ? (s.dual ? 2 : 3) : s.dual || s.dtype == JVPFA_FP32 ? 1 : 2);
-  int segments = room / heads, most = s.L / 128;
-  if (segments > most) segments = most;
-  if (segments > kMostSegments) segments = kMostSegments;
+  int most = s.L / 128;
+  if (most > kMostSegments) most = kMostSegments;
+  int segments = 1;
+  double least = 1e30;
+  for (int n = 1; n <= most || n == 1; ++n) {
+    const long long rounds = ((long long)heads * n + room - 1) / room;
+    const double cost = (double)rounds / n + 0.004 * n;
+    if (cost < least) least = cost, segments = n;
+  }
   s.segments = 1, s.segment = s.L;
   if (segments < 2) return;
   s.segment = ((s.L + segments - 1) / segments + 63) / 64 * 64;
   s.segments = (s.L + s.segment - 1) / s.segment;
 }
 
-int launch(const Scan& s, cudaStream_t stream) {
-  if (s.segments > 1) {
+// `found`: the segments' states are there already.
+int launch(const Scan& s, cudaStream_t stream, bool found = false) {
+  if (s.segments > 1 && !found) {
     const int rc = launch_of_type<false>(s, stream);
     if (rc) return rc;
     join_kernel<<<dim3((unsigned)(s.B * s.H), (unsigned)((s.D * s.E + 255) / 256)), 256, 0, stream>>>(s);
@@ -154,12 +162,16 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constan
 // ---- checks --------------------------------------------------------------------------------------------------------------
 bool bad_dtype(int dtype) { return dtype != JVPFA_BF16 && dtype != JVPFA_FP16 && dtype != JVPFA_FP32; }
 
+int bad_sizes(const jvpfa_linear_args& a) {
+  if (bad_dtype(a.dtype)) return JVPFA_ERR_DTYPE;
+  if (a.B < 1 || a.H < 1 || a.L < 1 || a.D < 1 || a.E < 1 || a.D > 128 || a.E > 128) return JVPFA_ERR_SHAPE;
+  return (long long)a.B * a.H > (1 << 24) ? JVPFA_ERR_TOO_LARGE : JVPFA_OK;
+}
+
 int check(const jvpfa_linear_args* a, bool backward) {
   if (!a) return JVPFA_ERR_NULL;
   if (a->struct_size != (int32_t)sizeof(jvpfa_linear_args)) return JVPFA_ERR_STRUCT;
-  if (bad_dtype(a->dtype)) return JVPFA_ERR_DTYPE;
-  if (a->B < 1 || a->H < 1 || a->L < 1 || a->D < 1 || a->E < 1 || a->D > 128 || a->E > 128) return JVPFA_ERR_SHAPE;
-  if ((long long)a->B * a->H > (1 << 24)) return JVPFA_ERR_TOO_LARGE;
+  if (const int rc = bad_sizes(*a)) return rc;
   if (!(a->scale == a->scale) || (backward && a->scale == 0.f && (a->gstate || a->gtstate))) return JVPFA_ERR_UNSUPPORTED;
   if (!a->q.p || !a->k.p || !a->v.p) return JVPFA_ERR_NULL;
   if (!a->dual && (a->tq.p || a->tk.p || a->tv.p || a->tstate || a->to.p || a->tstate_out || a->gto.p || a->gtstate || a->dtq.p || a->dtk.p || a->dtv.p || a->dtstate))
@@ -179,22 +191,28 @@ int check(const jvpfa_linear_args* a, bool backward) {
   return JVPFA_OK;
 }
 
-// A scan with the call's sizes; D and E are those of its a and c.
-Scan scan_of(const jvpfa_linear_args& a, int D, int E) {
+// A scan with the call's sizes; D and E are those of its a and c.  cut_dual: cut as a call with tangents, or without, is.
+Scan scan_of(const jvpfa_linear_args& a, int D, int E, bool cut_dual) {
   Scan s{};
   s.dtype = a.dtype, s.B = a.B, s.H = a.H, s.L = a.L, s.D = D, s.E = E;
   s.scale = a.scale, s.dual = a.dual != 0;
   s.log_decay = a.log_decay, s.lengths = a.lengths;
   s.first_scale = s.last_scale = 1.f, s.ahead = 1;
   s.first_stride[0] = s.last_stride[0] = s.state_stride[0] = E, s.first_stride[1] = s.last_stride[1] = s.state_stride[1] = 1;
+  s.dual = cut_dual;
   cut(s);
+  s.dual = a.dual != 0;
   return s;
 }
-void give_workspace(Scan& s, void* workspace) {
-  s.states = static_cast<float*>(workspace);
+// Where the segments' states are; `transposed`: as those of the map with b and c changed for one another.
+void put_states(Scan& s, void* at, bool transposed = false) {
+  s.states = static_cast<float*>(at);
   s.tstates = s.states + (size_t)s.B * s.H * s.segments * s.D * s.E;
+  if (transposed) s.state_stride[0] = 1, s.state_stride[1] = s.D;
 }
-int64_t workspace_bytes(const jvpfa_linear_args& a) { return state_bytes(scan_of(a, a.D, a.E)) * (a.dual ? 2 : 1); }
+int64_t states_of(const jvpfa_linear_args& a) { return state_bytes(scan_of(a, a.D, a.E, a.dual != 0)) * (a.dual ? 2 : 1); }
+// What the forward needs is nothing where it keeps its states.
+int64_t workspace_bytes(const jvpfa_linear_args& a, bool backward) { return !backward && a.kept ? 0 : states_of(a); }
 
 }  // namespace
 }  // namespace linear
@@ -204,30 +222,35 @@ using namespace jvpfa;
 
 extern "C" {
 
-int64_t jvpfa_linear_fwd_workspace(const jvpfa_linear_args* a) { return linear::check(a, false) == JVPFA_OK ? linear::workspace_bytes(*a) : 0; }
-int64_t jvpfa_linear_bwd_workspace(const jvpfa_linear_args* a) { return linear::check(a, true) == JVPFA_OK ? linear::workspace_bytes(*a) : 0; }
+int64_t jvpfa_linear_fwd_workspace(const jvpfa_linear_args* a) { return linear::check(a, false) == JVPFA_OK ? linear::workspace_bytes(*a, false) : 0; }
+int64_t jvpfa_linear_bwd_workspace(const jvpfa_linear_args* a) { return linear::check(a, true) == JVPFA_OK ? linear::workspace_bytes(*a, true) : 0; }
+int64_t jvpfa_linear_kept_bytes(const jvpfa_linear_args* a) {
+  if (!a || a->struct_size != (int32_t)sizeof(jvpfa_linear_args) || linear::bad_sizes(*a) != JVPFA_OK) return 0;
+  return linear::states_of(*a);
+}
 
 int jvpfa_linear_fwd(const jvpfa_linear_args* a, void* stream) {
   int rc = linear::check(a, false);
   if (rc) return rc;
-  const int64_t need = linear::workspace_bytes(*a);
+  const int64_t need = linear::workspace_bytes(*a, false);
   if (need && (!a->workspace || a->workspace_bytes < need)) return JVPFA_ERR_NULL;
-  if (reinterpret_cast<uintptr_t>(a->workspace) % 16) return JVPFA_ERR_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(a->workspace) | reinterpret_cast<uintptr_t>(a->kept)) % 16) return JVPFA_ERR_ALIGN;
   rc = check_arch();
   if (rc) return rc;
-  linear::Scan s = linear::scan_of(*a, a->D, a->E);
+  linear::Scan s = linear::scan_of(*a, a->D, a->E, a->dual != 0);
   s.a = a->q, s.b = a->k, s.c = a->v, s.ta = a->tq, s.tb = a->tk, s.tc = a->tv, s.out = a->o, s.tout = a->to;
   s.first = a->state, s.tfirst = a->tstate, s.last = a->state_out, s.tlast = a->tstate_out;
-  linear::give_workspace(s, a->workspace);
+  linear::put_states(s, a->kept ? a->kept : a->workspace);
   return linear::launch(s, static_cast<cudaStream_t>(stream));
 }
 
 int jvpfa_linear_bwd(const jvpfa_linear_args* a, void* stream) {
   int rc = linear::check(a, true);
   if (rc) return rc;
-  const int64_t need = linear::workspace_bytes(*a);
+  const int64_t need = linear::workspace_bytes(*a, true);
   if (need && (!a->workspace || a->workspace_bytes < need)) return JVPFA_ERR_NULL;
-  if (reinterpret_cast<uintptr_t>(a->workspace) % 16) return JVPFA_ERR_ALIGN;
+  if (a->kept && a->dual && !a->kept_dual) return JVPFA_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(a->workspace) | reinterpret_cast<uintptr_t>(a->kept)) % 16) return JVPFA_ERR_ALIGN;
   rc = check_arch();
   if (rc) return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -237,37 +260,38 @@ int jvpfa_linear_bwd(const jvpfa_linear_args* a, void* stream) {
   auto value = [&](const jvpfa_linear_tensor& d, const jvpfa_linear_tensor& dt) -> const jvpfa_linear_tensor& { return dual ? dt : d; };
   auto tangent = [&](const jvpfa_linear_tensor& d) -> const jvpfa_linear_tensor& { return dual ? d : none; };
   if (a->dq.p || a->dtq.p) {
-    linear::Scan s = linear::scan_of(*a, a->E, a->D);
+    linear::Scan s = linear::scan_of(*a, a->E, a->D, a->kept ? a->kept_dual != 0 : dual);
     s.a = g, s.ta = tg, s.b = a->v, s.tb = a->tv, s.c = a->k, s.tc = a->tk;
     s.out = value(a->dq, a->dtq), s.tout = tangent(a->dq);
     s.first = a->state, s.tfirst = a->tstate, s.first_stride[0] = 1, s.first_stride[1] = a->E;
-    linear::give_workspace(s, a->workspace);
-    rc = linear::launch(s, st);
+    linear::put_states(s, a->kept ? a->kept : a->workspace, a->kept != nullptr);  // (the forward's are those of (k, v))
+    rc = linear::launch(s, st, a->kept != nullptr);
     if (rc) return rc;
   }
   // Backwards, M begins with the cotangent of the last state, which the scale does not go with.
   const float* first = dual ? a->gtstate : a->gstate;
   const float* tfirst = dual ? a->gstate : nullptr;
   const float unscaled = first || tfirst ? 1.f / a->scale : 1.f;
-  if (a->dk.p || a->dtk.p || a->dstate || a->dtstate) {
-    linear::Scan s = linear::scan_of(*a, a->E, a->D);
+  const bool keys = a->dk.p || a->dtk.p || a->dstate || a->dtstate;
+  if (keys) {
+    linear::Scan s = linear::scan_of(*a, a->E, a->D, dual);
     s.reversed = true, s.ahead = 0, s.last_ahead = 1, s.first_scale = unscaled, s.last_scale = a->scale;
     s.a = a->v, s.ta = a->tv, s.b = g, s.tb = tg, s.c = a->q, s.tc = a->tq;
     s.out = value(a->dk, a->dtk), s.tout = tangent(a->dk);
     s.first = first, s.tfirst = tfirst, s.first_stride[0] = 1, s.first_stride[1] = a->E;
     s.last = dual ? a->dtstate : a->dstate, s.tlast = dual ? a->dstate : nullptr, s.last_stride[0] = 1, s.last_stride[1] = a->E;
-    linear::give_workspace(s, a->workspace);
+    linear::put_states(s, a->workspace);
     rc = linear::launch(s, st);
     if (rc) return rc;
   }
   if (a->dv.p || a->dtv.p) {
-    linear::Scan s = linear::scan_of(*a, a->D, a->E);
+    linear::Scan s = linear::scan_of(*a, a->D, a->E, dual);
     s.reversed = true, s.ahead = 0, s.first_scale = unscaled;
     s.a = a->k, s.ta = a->tk, s.b = a->q, s.tb = a->tq, s.c = g, s.tc = tg;
     s.out = value(a->dv, a->dtv), s.tout = tangent(a->dv);
     s.first = first, s.tfirst = tfirst;
-    linear::give_workspace(s, a->workspace);
-    rc = linear::launch(s, st);
+    linear::put_states(s, a->workspace, keys);  // (the keys' are those of (go, q))
+    rc = linear::launch(s, st, keys);
     if (rc) return rc;
   }
   return JVPFA_OK;

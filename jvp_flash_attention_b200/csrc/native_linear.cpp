@@ -91,6 +91,11 @@ struct LinearOp : ModuleOp {
     put(c.a.o, r.y[0]);
     c.a.state_out = out(r.y[1]);
     if (dual) put(c.a.to, r.ty[0]), c.a.tstate_out = out(r.ty[1]);
+    if (want_kept) {
+      const int64_t bytes = jvpfa_linear_kept_bytes(&c.a);
+      r.kept = empty({bytes}, at::kByte, q.device());
+      if (bytes > 0) c.a.kept = r.kept.data_ptr();
+    }
     const Tensor w = workspace(c, jvpfa_linear_fwd_workspace(&c.a), q);
     check_status(jvpfa_linear_fwd(&c.a, c10::cuda::getCurrentCUDAStream(q.get_device()).stream()), "jvpfa_linear_fwd");
     return r;
@@ -127,6 +132,7 @@ struct LinearOp : ModuleOp {
       const Tensor& t = d[i < 3 ? i : kOperands + i - 3];
       if (t.defined() && (i < 3 || dual)) put(*to[i], t);
     }
+    if (kept.defined() && kept.numel() > 0) c.a.kept = const_cast<void*>(kept.const_data_ptr()), c.a.kept_dual = any_defined(tx);
     c.a.dstate = out(d[kState]);
     if (dual) c.a.dtstate = out(d[kOperands + kState]);
     const Tensor w = workspace(c, jvpfa_linear_bwd_workspace(&c.a), q);

@@ -135,7 +135,7 @@ def _check_step(q, k, v, log_decay, scale, state) -> None:
 
 def _launch_fwd(x, tx, extras, options, keep):
     y, ty, kept = _lib.native().linear_launch_fwd(x, tx, extras, options, keep)
-    return y, ty, x[0].new_empty(0) if kept is None else kept
+    return y, ty, x[0].new_empty(0) if kept is None else kept  # (without rows nothing is kept)
 
 
 def _launch_bwd(x, tx, extras, kept, g, gt, options, want):
@@ -143,5 +143,4 @@ def _launch_bwd(x, tx, extras, kept, g, gt, options, want):
 
 
 def _backward_under_functorch(x, tx, extras, kept, g, gt, options):
-    kept = x[0].new_empty(0) if kept is None else kept
     return _dual.backward_under_functorch(sys.modules[__name__], x, tx, extras, kept, g, gt, options)
