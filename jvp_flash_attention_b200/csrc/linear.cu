@@ -38,12 +38,16 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Scan 
     const float* first = which ? p.tfirst : p.first;
     float* at = (which ? p.tstates : p.states) + (long long)head * p.segments * size + d * p.state_stride[0] + e * p.state_stride[1];
     float x = first ? p.first_scale * first[given] : 0.f;
-    float own = at[0];
-    for (int s = 0; s < p.segments; ++s, at += size) {
-      const float next = s + 2 < p.segments ? at[size] : 0.f;  // (the last one's is nobody's)
-      *at = x;
-      x = fmaf(x, down[s], x) + own;
-      own = next;
+    for (int s0 = 0; s0 < p.segments; s0 += 8, at += 8ll * size) {  // eight loads under way at once
+      float own[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) own[k] = s0 + k + 1 < p.segments ? at[(long long)k * size] : 0.f;  // (the last one's is nobody's)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (s0 + k >= p.segments) break;
+        at[(long long)k * size] = x;
+        x = fmaf(x, down[s0 + k], x) + own[k];
+      }
     }
   }
 }

@@ -48,31 +48,34 @@ __device__ __forceinline__ void split(float x, float y, uint32_t (&part)[PARTS])
 // absent tensor.
 template <int DT, int NT>
 __device__ __forceinline__ void stage(T* to, const jvpfa_linear_tensor& x, long long head, int width, int row0, int rows, int n, bool back, bool wide) {
-  constexpr int LD = DT + 8, PIECES = DT / 8;
-  const T* from = static_cast<const T*>(x.p) + head;
-#pragma unroll
-  for (int k = 0; k < CH * PIECES / NT; ++k) {
-    const int i = k * NT + threadIdx.x, r = i / PIECES, col = i % PIECES * 8;
-    const long long at = (long long)(back ? n - 1 - row0 - r : row0 + r) * x.stride[2] + col;
-    T* d = to + r * LD + col;
-    if (!x.p || r >= rows || col >= width) {
+  // (a loop of few instructions: the kernels' code is long, and what does not fit the instruction caches waits)
+  constexpr int LD = DT + 8, PIECES = DT / 8, AT_ONCE = NT / PIECES;
+  static_assert(AT_ONCE == 16, "four rows of a thread");
+  const int col = threadIdx.x % PIECES * 8, r0 = threadIdx.x / PIECES;
+  const T* from = static_cast<const T*>(x.p) + head + (long long)(back ? n - 1 - row0 - r0 : row0 + r0) * x.stride[2] + col;
+  const long long step = back ? -AT_ONCE * x.stride[2] : AT_ONCE * x.stride[2];
+  T* d = to + r0 * LD + col;
+  const int live = x.p && col < width ? rows : 0;
+#pragma unroll 1
+  for (int r = r0; r < CH; r += AT_ONCE, from += step, d += AT_ONCE * LD) {
+    if (r >= live) {
       *reinterpret_cast<uint4*>(d) = make_uint4(0, 0, 0, 0);
     } else if (wide) {
-      cp_async16(d, from + at, 16);
+      cp_async16(d, from, 16);
     } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) d[j] = col + j < width ? from[at + j] : Elem<T>::from_float(0.f);
+#pragma unroll 1
+      for (int j = 0; j < 8; ++j) d[j] = col + j < width ? from[j] : Elem<T>::from_float(0.f);
     }
   }
 }
 
+// Shared memory of a CTA: two tiles of b (and of its tangent), which a chunk reads to its end, and one of c and one of a, which are free behind the
+// products' barrier and take the next chunk's rows then; the products.  States alone: two tiles of b and c.
 template <int DT, bool DUAL, bool OUT>
 struct ChunkShape {
-  static constexpr int LD = DT + 8, NT = 2 * DT, TILES = (DUAL ? 2 : 1) * (OUT ? 3 : 2);
-  // Two stages where two CTAs or more still fit an SM, else one
-  static constexpr int STAGES = OUT && (DUAL || DT > 64) ? 1 : 2;
-  static constexpr int CTAS = DT == 32 ? (DUAL ? 3 : 4) : DT == 64 ? (DUAL ? 2 : 3) : DUAL ? 1 : 2;
-  static constexpr size_t bytes() { return sizeof(T) * (STAGES * (size_t)TILES * CH * LD + (OUT ? (DUAL ? 4 : 2) * (size_t)CH * LP : 0)); }
+  static constexpr int LD = DT + 8, NT = 2 * DT, SIDES = DUAL ? 2 : 1, TILE = CH * LD;
+  static constexpr int CTAS = DT == 32 ? (DUAL ? 2 : 4) : DT == 64 ? (DUAL ? 2 : 3) : DUAL ? 1 : 2;
+  static constexpr size_t bytes() { return sizeof(T) * SIDES * (4 * (size_t)TILE + (OUT ? 2 * (size_t)CH * LP : 0)); }
 };
 
 // OUT: the outputs, from the states that the segments begin with; else the states that their rows leave, from nothing.
@@ -82,8 +85,11 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
   constexpr int NT = S::NT, LD = S::LD, ND = DT / 8, KD = DT / 16, NW = DT / 16, SIDES = DUAL ? 2 : 1;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float power[CH + 2], less1[CH + 2];  // l^j and l^j - 1
-  T* tiles = reinterpret_cast<T*>(smem);           // of a stage: b, c (and their tangents), a (and its)
-  T* sP = tiles + S::STAGES * S::TILES * CH * LD;  // products in two parts, then their tangents
+  constexpr int TILE = S::TILE;
+  T* tiles_b = reinterpret_cast<T*>(smem);     // two times b and its tangent
+  T* tiles_c = tiles_b + 2 * SIDES * TILE;     // c and its tangent (states alone: two times)
+  T* tiles_a = tiles_c + SIDES * TILE;         // a and its tangent
+  T* sP = tiles_a + SIDES * TILE;              // products in two parts, then their tangents
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int segment = blockIdx.x % p.segments, head = blockIdx.x / p.segments, b = head / p.H, h = head - b * p.H;
   const int n = length_of(p.lengths, b, p.L), row_begin = segment * p.segment, row_end = min(n, row_begin + p.segment);
@@ -123,41 +129,48 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
   // The given state is l^ahead away from the first row, what the rows leave l^1.
   int shift = OUT && segment == 0 ? p.ahead - 1 : 0;
 
-  auto tile_of = [&](int stage_, int which) { return tiles + (stage_ * S::TILES + which) * CH * LD; };
-  auto fetch = [&](int stage_, int row0) {
+  auto fetch_b = [&](int half, int row0) {
     const int rows = min(CH, row_end - row0);
-    int k = 0;
-    stage<DT, NT>(tile_of(stage_, k++), p.b, of_head(p.b), p.D, row0, rows, n, p.reversed, wide & 1);
-    stage<DT, NT>(tile_of(stage_, k++), p.c, of_head(p.c), p.E, row0, rows, n, p.reversed, wide & 2);
-    if (DUAL) stage<DT, NT>(tile_of(stage_, k++), p.tb, of_head(p.tb), p.D, row0, rows, n, p.reversed, wide & 8);
-    if (DUAL) stage<DT, NT>(tile_of(stage_, k++), p.tc, of_head(p.tc), p.E, row0, rows, n, p.reversed, wide & 16);
-    if (OUT) stage<DT, NT>(tile_of(stage_, k++), p.a, of_head(p.a), p.D, row0, rows, n, p.reversed, wide & 4);
-    if (OUT && DUAL) stage<DT, NT>(tile_of(stage_, k++), p.ta, of_head(p.ta), p.D, row0, rows, n, p.reversed, wide & 32);
-    cp_async_commit();
+    T* to = tiles_b + half * SIDES * TILE;
+    stage<DT, NT>(to, p.b, of_head(p.b), p.D, row0, rows, n, p.reversed, wide & 1);
+    if (DUAL) stage<DT, NT>(to + TILE, p.tb, of_head(p.tb), p.D, row0, rows, n, p.reversed, wide & 8);
+  };
+  auto fetch_c = [&](int half, int row0) {
+    const int rows = min(CH, row_end - row0);
+    T* to = tiles_c + (OUT ? 0 : half * SIDES * TILE);
+    stage<DT, NT>(to, p.c, of_head(p.c), p.E, row0, rows, n, p.reversed, wide & 2);
+    if (DUAL) stage<DT, NT>(to + TILE, p.tc, of_head(p.tc), p.E, row0, rows, n, p.reversed, wide & 16);
+  };
+  auto fetch_a = [&](int row0) {
+    const int rows = min(CH, row_end - row0);
+    stage<DT, NT>(tiles_a, p.a, of_head(p.a), p.D, row0, rows, n, p.reversed, wide & 4);
+    if (DUAL) stage<DT, NT>(tiles_a + TILE, p.ta, of_head(p.ta), p.D, row0, rows, n, p.reversed, wide & 32);
   };
   // where a lane of ldmatrix reads: first operand and transposed second one (rows 0-7, 8-15, then columns 8-15), second one (columns 8-15, then rows 8-15)
   const int lane_row = lane & 15, lane_col = lane >> 4 << 3;
   const int lane_row_n = (lane & 7) + (lane >> 4 << 3), lane_col_n = lane >> 3 & 1 ? 8 : 0;
 
   int now = 0;
-  if (S::STAGES == 2 && row_begin < row_end) fetch(0, row_begin);
-  for (int row0 = row_begin; row0 < row_end; row0 += CH, shift = 0) {
+  if (row_begin < row_end) {
+    fetch_b(0, row_begin), fetch_c(0, row_begin);
+    if (OUT) fetch_a(row_begin);
+    cp_async_commit();
+  }
+  for (int row0 = row_begin; row0 < row_end; row0 += CH, shift = 0, now ^= 1) {
     const int rows = min(CH, row_end - row0);
-    if constexpr (S::STAGES == 2) {
-      cp_async_wait<0>();
-      __syncthreads();  // this chunk has arrived, the one before has been read
-      if (row0 + CH < row_end) fetch(now ^ 1, row0 + CH);
-    } else {
-      __syncthreads();
-      fetch(0, row0);
-      cp_async_wait<0>();
-      __syncthreads();
+    const bool more = row0 + CH < row_end;
+    cp_async_wait<0>();
+    __syncthreads();  // this chunk has arrived, the one before has been read
+    if (more) {
+      fetch_b(now ^ 1, row0 + CH);
+      if (!OUT) fetch_c(now ^ 1, row0 + CH);
+      cp_async_commit();
     }
-    const T *sB = tile_of(now, 0), *sC = tile_of(now, 1), *stB = tile_of(now, DUAL ? 2 : 0), *stC = tile_of(now, DUAL ? 3 : 1);
-    if (S::STAGES == 2) now ^= 1;
+    const T *sB = tiles_b + now * SIDES * TILE, *stB = sB + (SIDES - 1) * TILE;
+    const T *sC = tiles_c + (OUT ? 0 : now * SIDES * TILE), *stC = sC + (SIDES - 1) * TILE;
     uint32_t fc[SIDES][4][4];  // columns e0 .. e0 + 15 of c: 16 rows each; second operand's halves (0, 1) and (2, 3)
     if constexpr (OUT) {
-      const T *sA = tile_of(S::STAGES == 2 ? now ^ 1 : 0, DUAL ? 4 : 2), *stA = tile_of(0, DUAL ? 5 : 2);
+      const T *sA = tiles_a, *stA = tiles_a + (SIDES - 1) * TILE;
       // the chunk's products
 #pragma unroll 1
       for (int block = warp; block < 10; block += NW) {
@@ -206,23 +219,31 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
           for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int u = 0; u < 2; ++u) split(M[side][2 * k + u][2 * j], M[side][2 * k + u][2 * j + 1], m[side][j][u]);
+        // (an accumulator's next product is eight instructions away, or four with tangents)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t fa[4];
-          ldmatrix(fa, sA + (i * 16 + lane_row) * LD + k * 16 + lane_col);
+        for (int h2 = 0; h2 < 4; h2 += DUAL ? 2 : 4) {
+          constexpr int TILES_AT_ONCE = DUAL ? 2 : 4;
+          uint32_t fa[TILES_AT_ONCE][4];
+#pragma unroll
+          for (int i = 0; i < TILES_AT_ONCE; ++i) ldmatrix(fa[i], sA + ((h2 + i) * 16 + lane_row) * LD + k * 16 + lane_col);
 #pragma unroll
           for (int part = 1; part >= 0; --part)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              mma(acc[0][i][j], fa, m[0][j][0][part], m[0][j][1][part]);
-              if (DUAL) mma(acc[SIDES - 1][i][j], fa, m[SIDES - 1][j][0][part], m[SIDES - 1][j][1][part]);
-            }
+            for (int i = 0; i < TILES_AT_ONCE; ++i)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                mma(acc[0][h2 + i][j], fa[i], m[0][j][0][part], m[0][j][1][part]);
+                if (DUAL) mma(acc[SIDES - 1][h2 + i][j], fa[i], m[SIDES - 1][j][0][part], m[SIDES - 1][j][1][part]);
+              }
           if constexpr (DUAL) {
-            ldmatrix(fa, stA + (i * 16 + lane_row) * LD + k * 16 + lane_col);
+#pragma unroll
+            for (int i = 0; i < TILES_AT_ONCE; ++i) ldmatrix(fa[i], stA + ((h2 + i) * 16 + lane_row) * LD + k * 16 + lane_col);
 #pragma unroll
             for (int part = 1; part >= 0; --part)
 #pragma unroll
-              for (int j = 0; j < 2; ++j) mma(acc[1][i][j], fa, m[0][j][0][part], m[0][j][1][part]);
+              for (int i = 0; i < TILES_AT_ONCE; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) mma(acc[1][h2 + i][j], fa[i], m[0][j][0][part], m[0][j][1][part]);
           }
         }
       }
@@ -241,7 +262,11 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
         ldmatrix_t(fc[0][k], sC + (k * 16 + lane_row) * LD + e0 + lane_col);
         if (DUAL) ldmatrix_t(fc[SIDES - 1][k], stC + (k * 16 + lane_row) * LD + e0 + lane_col);
       }
-      __syncthreads();  // the products
+      __syncthreads();  // the products are there, and nobody reads a and c again
+      if (more) {
+        fetch_c(0, row0 + CH), fetch_a(row0 + CH);
+        cp_async_commit();
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (i * 16 >= rows) break;
