@@ -24,10 +24,10 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Scan 
   __shared__ float down[kMostSegments];
   const int size = p.D * p.E, head = blockIdx.x, b = head / p.H, h = head - b * p.H;
   const int n = length_of(p.lengths, b, p.L);
-  const double w = decay_of(p.log_decay, h);
+  const float w = decay_of(p.log_decay, h);
   for (int s = threadIdx.x; s < p.segments; s += 256) {
     const int rows = max(0, min(n - s * p.segment, p.segment)) + (s == 0 ? p.ahead - 1 : 0);
-    down[s] = (float)expm1(w * rows);
+    down[s] = expm1f(w * rows);
   }
   __syncthreads();
   const int i = blockIdx.y * 256 + threadIdx.x;
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constan
     sq[d] = a.scale * load_as(a.q, b * a.q_stride[0] + h * a.q_stride[1] + d, a.dtype);
     sk[d] = load_as(a.k, b * a.k_stride[0] + h * a.k_stride[1] + d, a.dtype);
   }
-  const float down = (float)expm1((double)decay_of(a.log_decay, h));
+  const float down = expm1f(decay_of(a.log_decay, h));
   float v[V], o[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {

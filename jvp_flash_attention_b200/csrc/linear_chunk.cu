@@ -96,8 +96,8 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
   if (!OUT && segment + 1 == p.segments) return;  // nobody begins with what the last one leaves
   const float w = decay_of(p.log_decay, h);
   for (int j = tid; j < CH + 2; j += NT) {
-    power[j] = (float)exp((double)w * j);
-    less1[j] = (float)expm1((double)w * j);
+    power[j] = expf(w * j);  // (in 64 bits a CTA would wait 2 us for them; what w * j loses is at most 2^-24 |w j| e^(w j) of a result)
+    less1[j] = expm1f(w * j);
   }
   auto of_head = [&](const jvpfa_linear_tensor& x) { return b * x.stride[0] + h * x.stride[1]; };
   const int e0 = warp * 16;
@@ -208,7 +208,118 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
             }
           }
       }
-      // what is before the chunk
+      // what is before the chunk, and its own rows
+      // 16 rows from i * 16 on, in accumulators
+      auto answer = [&](int i, const float (&tile)[SIDES][2][4]) {
+#pragma unroll
+        for (int side = 0; side < SIDES; ++side) {
+          const jvpfa_linear_tensor& x = side ? p.tout : p.out;
+          if (!x.p) continue;
+          T* out = static_cast<T*>(const_cast<void*>(x.p)) + of_head(x);
+          uint32_t v[4];  // (row g or g + 8, columns 0-7 or 8-15) of the tile, two entries
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) v[2 * u + j] = Elem<T>::pack(p.scale * tile[side][j][2 * u], p.scale * tile[side][j][2 * u + 1]);
+          auto row_of = [&](int r) { return (long long)(p.reversed ? n - 1 - row0 - r : row0 + r) * x.stride[2]; };
+          if (wide >> (6 + side) & 1) {
+            // four lanes hold two rows of 32 bytes, a word of each half row in each: they are turned so that each holds 16 successive bytes
+            uint32_t s;
+            s = __shfl_xor_sync(0xffffffffu, t & 1 ? v[0] : v[1], 1), (t & 1 ? v[0] : v[1]) = s;
+            s = __shfl_xor_sync(0xffffffffu, t & 1 ? v[2] : v[3], 1), (t & 1 ? v[2] : v[3]) = s;
+            s = __shfl_xor_sync(0xffffffffu, t & 2 ? v[0] : v[2], 2), (t & 2 ? v[0] : v[2]) = s;
+            s = __shfl_xor_sync(0xffffffffu, t & 2 ? v[1] : v[3], 2), (t & 2 ? v[1] : v[3]) = s;
+            const int r = i * 16 + g + (t >> 1) * 8, e = e0 + (t & 1) * 8;
+            if (r < rows && e < p.E) *reinterpret_cast<uint4*>(out + row_of(r) + e) = make_uint4(v[0], v[1], v[2], v[3]);
+          } else {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const int r = i * 16 + g + u * 8, e = e0 + j * 8 + 2 * t;
+                const __nv_bfloat162 two = *reinterpret_cast<const __nv_bfloat162*>(&v[2 * u + j]);
+                if (r < rows && e < p.E) out[row_of(r) + e] = two.x;
+                if (r < rows && e + 1 < p.E) out[row_of(r) + e + 1] = two.y;
+              }
+          }
+        }
+      };
+      if constexpr (DT <= 64) {
+        // M in two parts, once for all rows; then 16 rows after the other
+        uint32_t m[SIDES][KD][2][2][2];  // side, step, columns 0-7 or 8-15, rows 0-7 or 8-15, part
+#pragma unroll
+        for (int side = 0; side < SIDES; ++side)
+#pragma unroll
+          for (int k = 0; k < KD; ++k)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int u = 0; u < 2; ++u) split(M[side][2 * k + u][2 * j], M[side][2 * k + u][2 * j + 1], m[side][k][j][u]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          ldmatrix_t(fc[0][k], sC + (k * 16 + lane_row) * LD + e0 + lane_col);
+          if (DUAL) ldmatrix_t(fc[SIDES - 1][k], stC + (k * 16 + lane_row) * LD + e0 + lane_col);
+        }
+        __syncthreads();  // the products are there, and nobody reads c again
+        if (more) {
+          fetch_c(0, row0 + CH);
+          cp_async_commit();
+        }
+#pragma unroll 1
+        for (int i = 0; i * 16 < rows; ++i) {
+          float acc[SIDES][2][4] = {}, low_acc[2][4] = {};  // (two chains without tangents: an accumulator's next product is four instructions away)
+#pragma unroll
+          for (int k = 0; k < KD; ++k) {
+            uint32_t fa[4], fta[4];
+            ldmatrix(fa, sA + (i * 16 + lane_row) * LD + k * 16 + lane_col);
+            if (DUAL) ldmatrix(fta, stA + (i * 16 + lane_row) * LD + k * 16 + lane_col);
+#pragma unroll
+            for (int part = 1; part >= 0; --part)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                mma(!DUAL && part ? low_acc[j] : acc[0][j], fa, m[0][k][j][0][part], m[0][k][j][1][part]);
+                if (DUAL) mma(acc[SIDES - 1][j], fa, m[SIDES - 1][k][j][0][part], m[SIDES - 1][k][j][1][part]);
+                if (DUAL) mma(low_acc[j], fta, m[0][k][j][0][part], m[0][k][j][1][part]);
+              }
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float f = power[min(i * 16 + g + u * 8, rows - 1) + 1 + shift];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int v = 2 * u; v < 2 * u + 2; ++v) {
+                acc[SIDES - 1][j][v] = (acc[SIDES - 1][j][v] + low_acc[j][v]) * f;
+                if (DUAL) acc[0][j][v] *= f;
+              }
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (k > i) break;
+#pragma unroll
+            for (int part = 1; part >= 0; --part) {
+              uint32_t fp[4], ftp[4];
+              ldmatrix(fp, sP + part * CH * LP + (i * 16 + lane_row) * LP + k * 16 + lane_col);
+              if (DUAL) ldmatrix(ftp, sP + (2 + part) * CH * LP + (i * 16 + lane_row) * LP + k * 16 + lane_col);
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                mma(acc[0][j], fp, fc[0][k][2 * j], fc[0][k][2 * j + 1]);
+                if (DUAL) mma(acc[SIDES - 1][j], fp, fc[SIDES - 1][k][2 * j], fc[SIDES - 1][k][2 * j + 1]);
+              }
+              if constexpr (DUAL) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) mma(acc[1][j], ftp, fc[0][k][2 * j], fc[0][k][2 * j + 1]);
+              }
+            }
+          }
+          answer(i, acc);
+        }
+        __syncthreads();  // nobody reads a again
+        if (more) {
+          fetch_a(row0 + CH);
+          cp_async_commit();
+        }
+      } else {
       float acc[SIDES][4][2][4] = {};
 #pragma unroll
       for (int k = 0; k < KD; ++k) {
@@ -288,38 +399,15 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
             }
           }
         }
+        float tile[SIDES][2][4];
 #pragma unroll
-        for (int side = 0; side < SIDES; ++side) {
-          const jvpfa_linear_tensor& x = side ? p.tout : p.out;
-          if (!x.p) continue;
-          T* out = static_cast<T*>(const_cast<void*>(x.p)) + of_head(x);
-          uint32_t v[4];  // (row g or g + 8, columns 0-7 or 8-15) of the tile, two entries
+        for (int side = 0; side < SIDES; ++side)
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
+          for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) v[2 * u + j] = Elem<T>::pack(p.scale * acc[side][i][j][2 * u], p.scale * acc[side][i][j][2 * u + 1]);
-          auto row_of = [&](int r) { return (long long)(p.reversed ? n - 1 - row0 - r : row0 + r) * x.stride[2]; };
-          if (wide >> (6 + side) & 1) {
-            // four lanes hold two rows of 32 bytes, a word of each half row in each: they are turned so that each holds 16 successive bytes
-            uint32_t s;
-            s = __shfl_xor_sync(0xffffffffu, t & 1 ? v[0] : v[1], 1), (t & 1 ? v[0] : v[1]) = s;
-            s = __shfl_xor_sync(0xffffffffu, t & 1 ? v[2] : v[3], 1), (t & 1 ? v[2] : v[3]) = s;
-            s = __shfl_xor_sync(0xffffffffu, t & 2 ? v[0] : v[2], 2), (t & 2 ? v[0] : v[2]) = s;
-            s = __shfl_xor_sync(0xffffffffu, t & 2 ? v[1] : v[3], 2), (t & 2 ? v[1] : v[3]) = s;
-            const int r = i * 16 + g + (t >> 1) * 8, e = e0 + (t & 1) * 8;
-            if (r < rows && e < p.E) *reinterpret_cast<uint4*>(out + row_of(r) + e) = make_uint4(v[0], v[1], v[2], v[3]);
-          } else {
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const int r = i * 16 + g + u * 8, e = e0 + j * 8 + 2 * t;
-                const __nv_bfloat162 two = *reinterpret_cast<const __nv_bfloat162*>(&v[2 * u + j]);
-                if (r < rows && e < p.E) out[row_of(r) + e] = two.x;
-                if (r < rows && e + 1 < p.E) out[row_of(r) + e + 1] = two.y;
-              }
-          }
-        }
+            for (int v = 0; v < 4; ++v) tile[side][j][v] = acc[side][i][j][v];
+        answer(i, tile);
+      }
       }
     } else {
 #pragma unroll

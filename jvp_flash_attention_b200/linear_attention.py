@@ -36,7 +36,7 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor | None =
     Sums and states are in 32 bits.  Entries of 16-bit types are multiplied as they are, decayed ones and states in 22 bits or more, the
     products of q and k within a chunk of rows in 11 bits or more; float32 in 22 bits.  A NaN or an infinite entry reaches its own
     row, all later ones and those before it of its chunk.  Results are the same from run to run; last bits depend on how a
-    sequence is cut, so on B, H and L.
+    sequence is cut, so on B, H and L, and on whether there are tangents.
 
     The gradient goes to q, k, v and state, through values and tangents.  That of the values can be differentiated once more; that through the
     tangents cannot.  Gradients that are taken inside a forward-AD level carry their tangents, but for those through the tangent, which are
