@@ -19,12 +19,12 @@ namespace {
 using T = __nv_bfloat16;
 constexpr int CH = 64, LP = CH + 8;
 
-__device__ __forceinline__ void ldmatrix(uint32_t r[4], const T* p) {
-  const uint32_t a = (uint32_t)__cvta_generic_to_shared(p);
+// Addresses in shared memory are 32-bit numbers here: what is added to a lane's own is part of the instruction then.
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void ldmatrix(uint32_t r[4], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
-__device__ __forceinline__ void ldmatrix_t(uint32_t r[4], const T* p) {
-  const uint32_t a = (uint32_t)__cvta_generic_to_shared(p);
+__device__ __forceinline__ void ldmatrix_t(uint32_t r[4], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
 __device__ __forceinline__ void mma(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
@@ -40,7 +40,10 @@ __device__ __forceinline__ void split(float x, float y, uint32_t (&part)[PARTS])
 #pragma unroll
   for (int i = 0; i < PARTS; ++i) {
     part[i] = Elem<T>::pack(x, y);
-    if (i + 1 < PARTS) x -= low(part[i]), y -= high(part[i]);
+    if (i + 1 < PARTS) {
+      const float2 left = __ffma2_rn(make_float2(low(part[i]), high(part[i])), make_float2(-1.f, -1.f), make_float2(x, y));
+      x = left.x, y = left.y;
+    }
   }
 }
 
@@ -149,6 +152,10 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
   // where a lane of ldmatrix reads: first operand and transposed second one (rows 0-7, 8-15, then columns 8-15), second one (columns 8-15, then rows 8-15)
   const int lane_row = lane & 15, lane_col = lane >> 4 << 3;
   const int lane_row_n = (lane & 7) + (lane >> 4 << 3), lane_col_n = lane >> 3 & 1 ? 8 : 0;
+  constexpr uint32_t SZ = sizeof(T), ROWS16 = 16 * LD * SZ, P16 = 16 * LP * SZ, PART = CH * LP * SZ, SIDE = (SIDES - 1) * TILE * SZ;
+  const uint32_t at_first = (lane_row * LD + lane_col) * SZ;  // of a first operand, or a transposed second one
+  const uint32_t at_second = (lane_row_n * LD + lane_col_n) * SZ;
+  const uint32_t lane_a = shared_address(tiles_a) + at_first, lane_p = shared_address(sP) + (lane_row * LP + lane_col) * SZ;
 
   int now = 0;
   if (row_begin < row_end) {
@@ -166,11 +173,10 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
       if (!OUT) fetch_c(now ^ 1, row0 + CH);
       cp_async_commit();
     }
-    const T *sB = tiles_b + now * SIDES * TILE, *stB = sB + (SIDES - 1) * TILE;
-    const T *sC = tiles_c + (OUT ? 0 : now * SIDES * TILE), *stC = sC + (SIDES - 1) * TILE;
+    const uint32_t tile_b = shared_address(tiles_b + now * SIDES * TILE), lane_b = tile_b + at_first;
+    const uint32_t lane_c = shared_address(tiles_c + (OUT ? 0 : now * SIDES * TILE)) + at_first + e0 * SZ;
     uint32_t fc[SIDES][4][4];  // columns e0 .. e0 + 15 of c: 16 rows each; second operand's halves (0, 1) and (2, 3)
     if constexpr (OUT) {
-      const T *sA = tiles_a, *stA = tiles_a + (SIDES - 1) * TILE;
       // the chunk's products
 #pragma unroll 1
       for (int block = warp; block < 10; block += NW) {
@@ -180,13 +186,13 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
 #pragma unroll
           for (int k = 0; k < KD; ++k) {
             uint32_t fa[4], fb[4];
-            ldmatrix(fa, sA + (i * 16 + lane_row) * LD + k * 16 + lane_col);
-            ldmatrix(fb, sB + (j * 16 + lane_row_n) * LD + k * 16 + lane_col_n);
+            ldmatrix(fa, lane_a + i * ROWS16 + k * 32);
+            ldmatrix(fb, tile_b + at_second + j * ROWS16 + k * 32);
             mma(x[0][0], fa, fb[0], fb[1]), mma(x[0][1], fa, fb[2], fb[3]);
             if constexpr (DUAL) {
               uint32_t fta[4], ftb[4];
-              ldmatrix(fta, stA + (i * 16 + lane_row) * LD + k * 16 + lane_col);
-              ldmatrix(ftb, stB + (j * 16 + lane_row_n) * LD + k * 16 + lane_col_n);
+              ldmatrix(fta, lane_a + SIDE + i * ROWS16 + k * 32);
+              ldmatrix(ftb, tile_b + at_second + SIDE + j * ROWS16 + k * 32);
               mma(x[1][0], fta, fb[0], fb[1]), mma(x[1][1], fta, fb[2], fb[3]);
               mma(x[1][0], fa, ftb[0], ftb[1]), mma(x[1][1], fa, ftb[2], ftb[3]);
             }
@@ -257,8 +263,8 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
               for (int u = 0; u < 2; ++u) split(M[side][2 * k + u][2 * j], M[side][2 * k + u][2 * j + 1], m[side][k][j][u]);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          ldmatrix_t(fc[0][k], sC + (k * 16 + lane_row) * LD + e0 + lane_col);
-          if (DUAL) ldmatrix_t(fc[SIDES - 1][k], stC + (k * 16 + lane_row) * LD + e0 + lane_col);
+          ldmatrix_t(fc[0][k], lane_c + k * ROWS16);
+          if (DUAL) ldmatrix_t(fc[SIDES - 1][k], lane_c + SIDE + k * ROWS16);
         }
         __syncthreads();  // the products are there, and nobody reads c again
         if (more) {
@@ -271,8 +277,8 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
 #pragma unroll
           for (int k = 0; k < KD; ++k) {
             uint32_t fa[4], fta[4];
-            ldmatrix(fa, sA + (i * 16 + lane_row) * LD + k * 16 + lane_col);
-            if (DUAL) ldmatrix(fta, stA + (i * 16 + lane_row) * LD + k * 16 + lane_col);
+            ldmatrix(fa, lane_a + i * ROWS16 + k * 32);
+            if (DUAL) ldmatrix(fta, lane_a + SIDE + i * ROWS16 + k * 32);
 #pragma unroll
             for (int part = 1; part >= 0; --part)
 #pragma unroll
@@ -299,8 +305,8 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
 #pragma unroll
             for (int part = 1; part >= 0; --part) {
               uint32_t fp[4], ftp[4];
-              ldmatrix(fp, sP + part * CH * LP + (i * 16 + lane_row) * LP + k * 16 + lane_col);
-              if (DUAL) ldmatrix(ftp, sP + (2 + part) * CH * LP + (i * 16 + lane_row) * LP + k * 16 + lane_col);
+              ldmatrix(fp, lane_p + part * PART + i * P16 + k * 32);
+              if (DUAL) ldmatrix(ftp, lane_p + (2 + part) * PART + i * P16 + k * 32);
 #pragma unroll
               for (int j = 0; j < 2; ++j) {
                 mma(acc[0][j], fp, fc[0][k][2 * j], fc[0][k][2 * j + 1]);
@@ -336,7 +342,7 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
           constexpr int TILES_AT_ONCE = DUAL ? 2 : 4;
           uint32_t fa[TILES_AT_ONCE][4];
 #pragma unroll
-          for (int i = 0; i < TILES_AT_ONCE; ++i) ldmatrix(fa[i], sA + ((h2 + i) * 16 + lane_row) * LD + k * 16 + lane_col);
+          for (int i = 0; i < TILES_AT_ONCE; ++i) ldmatrix(fa[i], lane_a + (h2 + i) * ROWS16 + k * 32);
 #pragma unroll
           for (int part = 1; part >= 0; --part)
 #pragma unroll
@@ -348,7 +354,7 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
               }
           if constexpr (DUAL) {
 #pragma unroll
-            for (int i = 0; i < TILES_AT_ONCE; ++i) ldmatrix(fa[i], stA + ((h2 + i) * 16 + lane_row) * LD + k * 16 + lane_col);
+            for (int i = 0; i < TILES_AT_ONCE; ++i) ldmatrix(fa[i], lane_a + SIDE + (h2 + i) * ROWS16 + k * 32);
 #pragma unroll
             for (int part = 1; part >= 0; --part)
 #pragma unroll
@@ -370,8 +376,8 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
         }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        ldmatrix_t(fc[0][k], sC + (k * 16 + lane_row) * LD + e0 + lane_col);
-        if (DUAL) ldmatrix_t(fc[SIDES - 1][k], stC + (k * 16 + lane_row) * LD + e0 + lane_col);
+        ldmatrix_t(fc[0][k], lane_c + k * ROWS16);
+        if (DUAL) ldmatrix_t(fc[SIDES - 1][k], lane_c + SIDE + k * ROWS16);
       }
       __syncthreads();  // the products are there, and nobody reads a and c again
       if (more) {
@@ -386,14 +392,14 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
 #pragma unroll
           for (int part = 1; part >= 0; --part) {
             uint32_t fp[4];
-            ldmatrix(fp, sP + part * CH * LP + (i * 16 + lane_row) * LP + k * 16 + lane_col);
+            ldmatrix(fp, lane_p + part * PART + i * P16 + k * 32);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               mma(acc[0][i][j], fp, fc[0][k][2 * j], fc[0][k][2 * j + 1]);
               if (DUAL) mma(acc[SIDES - 1][i][j], fp, fc[SIDES - 1][k][2 * j], fc[SIDES - 1][k][2 * j + 1]);
             }
             if constexpr (DUAL) {
-              ldmatrix(fp, sP + (2 + part) * CH * LP + (i * 16 + lane_row) * LP + k * 16 + lane_col);
+              ldmatrix(fp, lane_p + (2 + part) * PART + i * P16 + k * 32);
 #pragma unroll
               for (int j = 0; j < 2; ++j) mma(acc[1][i][j], fp, fc[0][k][2 * j], fc[0][k][2 * j + 1]);
             }
@@ -412,8 +418,8 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        ldmatrix_t(fc[0][k], sC + (k * 16 + lane_row) * LD + e0 + lane_col);
-        if (DUAL) ldmatrix_t(fc[SIDES - 1][k], stC + (k * 16 + lane_row) * LD + e0 + lane_col);
+        ldmatrix_t(fc[0][k], lane_c + k * ROWS16);
+        if (DUAL) ldmatrix_t(fc[SIDES - 1][k], lane_c + SIDE + k * ROWS16);
       }
     }
     // M = l^rows M + sum of l^(rows - 1 - s) b_s c_s^T; the factor by its distance from 1, which keeps the digits of slow decays.  As a first operand the
@@ -430,7 +436,8 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const uint32_t x = fc[side][k][2 * j + u];
-            split(low(x) * w0, high(x) * w1, wc[side][k][2 * u + j]);
+            const float2 y = __fmul2_rn(make_float2(low(x), high(x)), make_float2(w0, w1));
+            split(y.x, y.y, wc[side][k][2 * u + j]);
           }
       }
     const float down = less1[rows + shift];
@@ -440,7 +447,7 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         uint32_t fb[4];
-        ldmatrix_t(fb, sB + (k * 16 + lane_row) * LD + d * 8 + lane_col);
+        ldmatrix_t(fb, lane_b + k * ROWS16 + d * 16);
 #pragma unroll
         for (int part = PARTS - 1; part >= 0; --part) {
           const uint32_t fa[4] = {wc[0][k][0][part], wc[0][k][1][part], wc[0][k][2][part], wc[0][k][3][part]};
@@ -451,7 +458,7 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
           }
         }
         if constexpr (DUAL) {
-          ldmatrix_t(fb, stB + (k * 16 + lane_row) * LD + d * 8 + lane_col);
+          ldmatrix_t(fb, lane_b + SIDE + k * ROWS16 + d * 16);
 #pragma unroll
           for (int part = PARTS - 1; part >= 0; --part) {
             const uint32_t fa[4] = {wc[0][k][0][part], wc[0][k][1][part], wc[0][k][2][part], wc[0][k][3][part]};
@@ -464,7 +471,12 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) M[side][d + u][j] = fmaf(M[side][d + u][j], down, M[side][d + u][j]) + x[side][u][j];
+          for (int j = 0; j < 4; j += 2) {
+            float* m = &M[side][d + u][j];
+            const float2 old = make_float2(m[0], m[1]);
+            const float2 sum = __fadd2_rn(__ffma2_rn(old, make_float2(down, down), old), make_float2(x[side][u][j], x[side][u][j + 1]));
+            m[0] = sum.x, m[1] = sum.y;
+          }
     }
   }
 
