@@ -468,7 +468,7 @@ int64_t jvpfa_gated_bwd_workspace(const jvpfa_gated_bwd_args* args);
  * and tr, tn along tangents of x, y and any of the vectors.  The vectors have C entries; a grouped one has a row for each `group_rows`
  * successive rows of x (M is a multiple of it), the others one for all.  An absent vector (v NULL) is 1, of bias, scale and shift 0.
  * All arithmetic is in 32 bits; every result is rounded once (n is the norm of the r that was not rounded).  Rows have at most
- * JVPFA_NORM_MAX_WIDTH entries.  x, tx, y, ty have contiguous columns and row strides in entries; vectors have contiguous entries;
+ * JVPFA_NORM_MAX_WIDTH entries, and there are at most 2^30 of them (else JVPFA_ERR_TOO_LARGE).  x, tx, y, ty have contiguous columns and row strides in entries; vectors have contiguous entries;
  * r, tr, n, tn and what the backward reads and writes of them are row-major.  Addresses are multiples of an entry.
  */
 #define JVPFA_NORM_MAX_WIDTH 16384

@@ -42,7 +42,10 @@ int launch_chunks(const Scan& s, bool outputs, cudaStream_t stream);  // bfloat1
 
 inline long long state_bytes(const Scan& s) { return s.segments > 1 ? 4ll * s.B * s.H * s.segments * s.D * s.E : 0; }
 
-__device__ __forceinline__ float decay_of(const float* log_decay, int h) { return log_decay ? fmaxf(log_decay[h], kLowest) : 0.f; }
+__device__ __forceinline__ float decay_of(const float* log_decay, int h) {
+  const float w = log_decay ? log_decay[h] : 0.f;
+  return w < kLowest ? kLowest : w;  // (a NaN stays one)
+}
 __device__ __forceinline__ int length_of(const int32_t* lengths, int b, int L) { return lengths ? min(max(lengths[b], 0), L) : L; }
 
 }  // namespace linear

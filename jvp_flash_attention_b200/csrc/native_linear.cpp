@@ -224,10 +224,10 @@ py::object step(const Tensor& q_, const Tensor& k_, const Tensor& v_, const std:
   for (int d = 0; d < 2; ++d)
     a.q_stride[d] = q.stride(d), a.k_stride[d] = k.stride(d), a.v_stride[d] = v.stride(d), a.state_stride[d] = state.stride(d);
   a.state = static_cast<float*>(state.data_ptr());
+  state.unsafeGetTensorImpl()->bump_version();  // (refuses what must not be written)
   const int rc = jvpfa_linear_step(&a, c10::cuda::getCurrentCUDAStream(q.get_device()).stream());
   if (rc == JVPFA_ERR_SHAPE) return py::none();  // states that share memory
   check_status(rc, "jvpfa_linear_step");
-  state.unsafeGetTensorImpl()->bump_version();
   return py::cast(o);
 }
 

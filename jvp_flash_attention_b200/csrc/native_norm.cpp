@@ -166,7 +166,7 @@ py::object norm(const std::vector<std::optional<Tensor>>& operands, int kind, in
   if (!in.ok || in.x.size() != kOperands) return py::none();
   const Tensor& x = in.x[kX];
   if (!x.defined() || x.dim() < 1 || (x.is_cuda() && dtype_of(x, false) < 0) || x.size(-1) < 1 || x.size(-1) > JVPFA_NORM_MAX_WIDTH ||
-      x.numel() / x.size(-1) > INT32_MAX)
+      x.numel() / x.size(-1) > (1 << 30))
     return py::none();
   const Tensor& y = in.x[kY];
   if (y.defined() && (y.sizes() != x.sizes() || y.scalar_type() != x.scalar_type() || y.device() != x.device())) return py::none();

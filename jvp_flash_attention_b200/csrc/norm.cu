@@ -13,7 +13,7 @@ int launch_fwd(const jvpfa_norm_args& a, cudaStream_t s);
 
 namespace {
 
-constexpr int kCols = 32, kLanes = 8;  // of a CTA that adds up parts: its columns, and how many take turns with the slices
+constexpr int kCols = 32, kLanes = 32;  // of a CTA that adds up parts: its columns, and how many take turns with the slices
 constexpr int kMostChunks = 64;         // of groups, each by CTAs of its own
 
 struct Totals {
@@ -44,6 +44,7 @@ __global__ void __launch_bounds__(kCols * kLanes) norm_parts_kernel(const __grid
   const int x = threadIdx.x % kCols, lane = threadIdx.x / kCols, col = blockIdx.x * kCols + x;
   const bool live = col < a.C;
   Totals t;
+#pragma unroll
   for (int i = 0; i < 6; ++i) t.d[i] = t.dt[i] = 0.f;
   const long long g0 = (long long)cut.groups * blockIdx.y / gridDim.y, g1 = (long long)cut.groups * (blockIdx.y + 1) / gridDim.y;
   for (long long group = g0; group < g1; ++group) {
@@ -113,6 +114,7 @@ int check(const jvpfa_norm_args* a, bool backward) {
   if (a->struct_size != (int32_t)sizeof(jvpfa_norm_args)) return JVPFA_ERR_STRUCT;
   if (a->dtype != JVPFA_BF16 && a->dtype != JVPFA_FP16 && a->dtype != JVPFA_FP32) return JVPFA_ERR_DTYPE;
   if (a->vec_dtype != a->dtype && a->vec_dtype != JVPFA_FP32) return JVPFA_ERR_DTYPE;
+  if (a->M > (1 << 30)) return JVPFA_ERR_TOO_LARGE;
   if (a->M < 1 || a->C < 1 || a->C > JVPFA_NORM_MAX_WIDTH || a->group_rows < 1 || a->M % a->group_rows) return JVPFA_ERR_SHAPE;
   if (a->kind < JVPFA_NORM_NONE || a->kind > JVPFA_NORM_LAYER || a->post < JVPFA_NORM_NONE || a->post > JVPFA_NORM_LAYER) return JVPFA_ERR_UNSUPPORTED;
   const bool y = a->y != nullptr, n = a->kind != JVPFA_NORM_NONE;

@@ -29,7 +29,8 @@ def norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, *,
 
     x: (..., C), bfloat16, float16 or float32, plain or dual, C up to 16384; rows that are 16-byte aligned are read 16 bytes at a time.
     weight, bias: (C,).  scale, shift: of a conditioned norm, (C,) or with x's leading dimensions up to some and ones behind, as (B, 1, C) for x
-    (B, L, C).  The vectors have one type, x's or float32.  All arithmetic is in 32 bits, and the result is rounded once.
+    (B, L, C).  The vectors have one type, x's or float32.  (A backward holds their sums in 32 bits, once for each group of rows that has vectors
+    of its own, or 148 times: where every row has, that is four bytes an entry of x for each of weight or scale, bias or shift, and gate.)  All arithmetic is in 32 bits, and the result is rounded once.
 
     The gradient goes to all operands, through the value and through the tangent.  That of the value can be differentiated once more; that through
     the tangent cannot.  Gradients that are taken inside a forward-AD level carry their tangents, but for those through the tangent, which are
@@ -78,8 +79,8 @@ def _apply(x, y, vectors, kind, post, alpha, eps, name):
 def _check(x, y, vectors, post) -> None:
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_WIDTH:
         raise ValueError(f"x must have the shape (..., C) with C from 1 to {MAX_WIDTH}, got {tuple(x.shape)}")
-    if x.numel() // x.shape[-1] >= 2**31:
-        raise ValueError("x must have less than 2**31 rows")
+    if x.numel() // x.shape[-1] > 2**30:
+        raise ValueError("x must have at most 2**30 rows")
     if y is not None and y.shape != x.shape:
         raise ValueError(f"x and y must have one shape, got {tuple(x.shape)} and {tuple(y.shape)}")
     if x.is_cuda and x.dtype not in _lib.DTYPE_ENUM:

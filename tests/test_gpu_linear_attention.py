@@ -182,6 +182,20 @@ def test_steps_that_are_refused():
             la.linear_attention_step(*args)
     with torch.no_grad():
         la.linear_attention_step(q, q, q, None, s.clone().requires_grad_())
+    with torch.inference_mode():
+        kept, other = s.clone(), s.clone()
+        o = la.linear_attention_step(q, q, q, None, kept)
+    assert torch.equal(o, la.linear_attention_step(q, q, q, None, other.clone())) and not torch.equal(kept, s)
+    before = kept.clone()
+    with pytest.raises(RuntimeError, match="[Ii]nference"):
+        la.linear_attention_step(q, q, q, None, kept)
+    assert torch.equal(kept, before)
+
+
+def test_a_decay_that_is_not_a_number_shows():
+    q = torch.randn(1, 2, 70, 16, device=DEV)
+    o = la.linear_attention(q, q, q, torch.tensor([float("nan"), -1.0], device=DEV))
+    assert not o[0, 0, 1:].isfinite().any() and o[0, 1].isfinite().all()
 
 
 @pytest.mark.parametrize("shape", [(0, 2, 5, 16), (2, 2, 0, 16), (2, 0, 5, 16)])

@@ -74,6 +74,9 @@ CASES = [
     ({"x", "y", "gate", "scale", "shift"}, (2, 3, 4104), (2, 1), "layer", None),
     (ALL, (2, 1, 16384), (2, 1), "layer", "rms"),
     ({"x", "y", "weight", "gate"}, (1, 3, 16383), None, "rms", None),
+    (ALL, (300, 5, 48), (300, 1), "layer", "rms"),  # more groups than SMs
+    ({"x", "y", "gate", "scale", "bias"}, (400, 72), (400,), "layer", "layer"),  # every row vectors of its own
+    ({"x", "weight", "shift"}, (150, 2, 1032), (150, 1), "rms", None),
 ]
 
 

@@ -184,7 +184,7 @@ def test_the_c_entries_refuse():
                 setattr(a, key, v)
         return entry(ctypes.byref(a), None) if entry is not lib.jvpfa_norm_bwd_workspace else entry(ctypes.byref(a))
 
-    both = [(-7, dict(struct_size=8)), (-3, dict(dtype=3)), (-3, dict(vec_dtype=1)), (-2, dict(M=0)), (-2, dict(C=0)), (-2, dict(C=16385)), (-2, dict(group_rows=3)),
+    both = [(-7, dict(struct_size=8)), (-3, dict(dtype=3)), (-3, dict(vec_dtype=1)), (-2, dict(M=0)), (-2, dict(C=0)), (-2, dict(C=16385)), (-10, dict(M=1 << 30 | 2)), (-2, dict(group_rows=3)),
             (-9, dict(kind=3)), (-9, dict(kind=0)), (-9, dict(post=1)), (-9, dict(ty=64)), (-1, dict(x=None)), (-1, dict(tx=64)), (-2, dict(x_stride=-8)),
             (-1, dict(vec={0: (None, 64)})), (-1, dict(vec={0: (64, 64)})), (-9, dict(vec={4: (64, None)})), (-8, dict(x=65)), (-8, dict(vec={1: (63, None)})), (-8, dict(stats=68))]
     forward = [(-1, dict(n=None)), (-1, dict(r=64)), (-1, dict(dual=1)), (-1, dict(y=64))]
