@@ -54,23 +54,20 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Scan 
 
 // Rows of a segment and segments (1: no workspace).
 void cut(Scan& s) {
-  // Rounds of as many CTAs as SMs hold at once, in units of a whole head's time, and the states that each segment costs, about 1/250 of that; no
-  // segment below 128 rows.  (bf16 B4 H16 L8192 D128, 296 at once: 4 segments, 256 CTAs, 1.75 ms forward and backward; 9 segments 1.62.)
-  const int heads = s.B * s.H, width = s.D > s.E ? s.D : s.E;
+  // Rounds of as many CTAs as SMs hold at once, each of a segment's rows, and the states that a segment costs, about 3/1000 of a sequence; no
+  // segment below 128 rows.  (us by segments: bf16 B4 H16 L2048 D64 with tangents and gradients, 296 CTAs at once, 4 / 6 / 8 / 11: 426 / 592 / 459 / 506;
+  // L8192 D128 forward and backward 4 / 8 / 9 / 16: 1584 / 1620 / 1552 / 1549; fp32 B2 H8 L1023 D128 with tangents, 148 at once, 4 / 6 / 8: 377 / 294 / 223.)
+  const int heads = s.B * s.H, width = s.D > s.E ? s.D : s.E, chunk = s.dtype == JVPFA_FP32 && width > 64 ? 32 : 64;
   const int room = kSMs * (width <= 64 ? (s.dual ? 2 : 3) : s.dual || s.dtype == JVPFA_FP32 ? 1 : 2);
-  int most = s.L / 128;
-  if (most > kMostSegments) most = kMostSegments;
-  int segments = 1;
-  double least = 1e30;
-  for (int n = 1; n <= most || n == 1; ++n) {
-    const long long rounds = ((long long)heads * n + room - 1) / room;
-    const double cost = (double)rounds / n + 0.004 * n;
-    if (cost < least) least = cost, segments = n;
-  }
   s.segments = 1, s.segment = s.L;
-  if (segments < 2) return;
-  s.segment = ((s.L + segments - 1) / segments + 63) / 64 * 64;
-  s.segments = (s.L + s.segment - 1) / s.segment;
+  double least = 1e30;
+  for (int n = 1; n <= kMostSegments; ++n) {
+    const int rows = ((s.L + n - 1) / n + chunk - 1) / chunk * chunk, segments = (s.L + rows - 1) / rows;
+    if (n > 1 && rows < 128) break;
+    const long long rounds = ((long long)heads * segments + room - 1) / room;
+    const double cost = (double)rounds * rows + 0.003 * s.L * segments;
+    if (cost < least) least = cost, s.segments = segments, s.segment = segments > 1 ? rows : s.L;
+  }
 }
 
 // `found`: the segments' states are there already.
