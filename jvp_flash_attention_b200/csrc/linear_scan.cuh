@@ -20,10 +20,6 @@ struct Part {
     else
       split_tf32(x, hi, lo);
   }
-  __device__ __forceinline__ void round(float x) {  // to 11 bits
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-    lo = 0u;
-  }
 };
 // x = a b, from nothing.
 __device__ __forceinline__ void mma_fresh(float x[4], const uint32_t a[4], const uint32_t b[2]) {
@@ -200,13 +196,7 @@ __global__ void __launch_bounds__(2 * DT) scan_kernel(const __grid_constant__ Sc
         for (int k = 0; k < r0 + 16; k += 8) {
           auto load_p = [&](Part<false>(&f)[4], const float* s) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float v = s[(r0 + g + (i & 1) * 8) * LP + k + t + (i >> 1) * 4];
-              if constexpr (X)
-                f[i].round(v);  // a 16-bit result: 11 bits of the products are more than it has, or as many
-              else
-                f[i].set(v);
-            }
+            for (int i = 0; i < 4; ++i) f[i].set(s[(r0 + g + (i & 1) * 8) * LP + k + t + (i >> 1) * 4]);
           };
           auto times = [&](float(&acc)[2][4], const Part<false>(&f)[4], const T* s) {
 #pragma unroll
@@ -214,12 +204,7 @@ __global__ void __launch_bounds__(2 * DT) scan_kernel(const __grid_constant__ Sc
               Part<X> fc[2];
 #pragma unroll
               for (int i = 0; i < 2; ++i) fc[i].set(Elem<T>::to_float(s[(k + t + i * 4) * LD + e0 + j * 8 + g]));
-              if constexpr (X) {
-                const uint32_t ah[4] = {f[0].hi, f[1].hi, f[2].hi, f[3].hi}, bh[2] = {fc[0].hi, fc[1].hi};
-                mma_1688_tf32(acc[j], ah, bh);
-              } else {
-                mul(acc[j], f, fc);
-              }
+              mul(acc[j], f, fc);
             }
           };
           Part<false> fp[4];

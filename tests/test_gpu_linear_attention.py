@@ -1,7 +1,7 @@
 """GPU tests of linear attention against its definition in float64.
 
 Bound of an entry: half a step of its type; 2^-11 of the sum of the magnitudes that it is made of for 16-bit types, whose weighted products of
-queries and keys may be rounded to 11 bits; and for sums in 32 bits, which the tensor cores truncate (2^-23 a step): at most three instructions
+queries and keys have 16 bits or more (and would do with 11); and for sums in 32 bits, which the tensor cores truncate (2^-23 a step): at most three instructions
 for every 8 rows or entries and 22 bits of each operand, (3 (L / 8 + D / 8 + 8) + 8) 2^-22 of that sum.  A gradient is such a map too; one through
 tangents is a sum of three."""
 import pytest
