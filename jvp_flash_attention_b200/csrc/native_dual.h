@@ -366,17 +366,14 @@ inline Tensors tensors_of(const py::handle& o) {
 // and whose Functions are that module's _backward_under_functorch(x, tx, extras, kept, g, gt, options) -> d.
 struct ModuleOp : DualOp {
   const char* module;
-  py::object options;
-  ~ModuleOp() override {
-    py::gil_scoped_acquire gil;
-    options = py::object();
-  }
+  // The Python module's form of what the operator was called with (made when it is needed: a graph holds nothing of Python's).
+  virtual py::tuple options() const = 0;
   py::object function(const char* name) const { return py::module_::import(module).attr(name); }
   DualOut python_forward(const Tensors& x, const Tensors& tx, const Tensors& extras, bool keep) const {
     py::gil_scoped_acquire gil;
     NoFunctorch nf;
     at::AutoGradMode no_grad(false);
-    py::tuple r = function("_launch_fwd")(list_of(map_tensors(x, primal_of)), list_of(tx), list_of(extras), options, keep);
+    py::tuple r = function("_launch_fwd")(list_of(map_tensors(x, primal_of)), list_of(tx), list_of(extras), options(), keep);
     return {tensors_of(r[0]), r[1].is_none() ? Tensors(outputs) : tensors_of(r[1]), tensor_of(r[2])};
   }
   Tensors python_backward(const Tensors& x, const Tensors& tx, const Tensors& extras, const Tensor& kept, const Tensors& g, const Tensors& gt,
@@ -384,12 +381,12 @@ struct ModuleOp : DualOp {
     py::gil_scoped_acquire gil;
     NoFunctorch nf;
     at::AutoGradMode no_grad(false);
-    return tensors_of(function("_launch_bwd")(list_of(x), list_of(tx), list_of(extras), none_or(kept), list_of(g), list_of(gt), options, want));
+    return tensors_of(function("_launch_bwd")(list_of(x), list_of(tx), list_of(extras), none_or(kept), list_of(g), list_of(gt), options(), want));
   }
   Tensors backward_under_functorch(const Tensors& x, const Tensors& tx, const Tensors& extras, const Tensor& kept, const Tensors& g,
                                    const Tensors& gt) const override {
     py::gil_scoped_acquire gil;
-    return tensors_of(function("_backward_under_functorch")(list_of(x), list_of(tx), list_of(extras), none_or(kept), list_of(g), list_of(gt), options));
+    return tensors_of(function("_backward_under_functorch")(list_of(x), list_of(tx), list_of(extras), none_or(kept), list_of(g), list_of(gt), options()));
   }
 };
 

@@ -13,6 +13,7 @@ bool any_of(const std::vector<bool>& v) { return std::find(v.begin(), v.end(), t
 struct LinearOp : ModuleOp {
   double scale;
   bool want_state;
+  py::tuple options() const override { return py::make_tuple(scale, want_state, name); }
 
   struct Call {
     jvpfa_linear_args a{};
@@ -168,7 +169,6 @@ std::shared_ptr<LinearOp> operator_of(const py::tuple& options) {
   auto op = std::make_shared<LinearOp>();
   op->name = "linear_attention", op->outputs = 2, op->module = "jvp_flash_attention_b200.linear_attention";
   op->scale = options[0].cast<double>(), op->want_state = options[1].cast<bool>();
-  op->options = options;
   return op;
 }
 

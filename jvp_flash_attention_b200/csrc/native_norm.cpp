@@ -12,6 +12,7 @@ constexpr int kOperands = 8;
 struct NormOp : ModuleOp {
   int kind, post;
   double alpha, eps;
+  py::tuple options() const override { return py::make_tuple(kind, post, alpha, eps, name); }
 
   // Rows of a group, 0 where the vectors cannot be laid out so: their dimensions are x's from the first up to some, and 1 from there on.
   static int64_t group_rows(const Tensors& x, bool grouped[6]) {
@@ -183,7 +184,6 @@ py::object norm(const std::vector<std::optional<Tensor>>& operands, int kind, in
   op->name = which == "norm" ? "norm" : which == "residual" ? "residual" : "residual_norm";  // (it outlives the caller's text)
   op->outputs = 2, op->module = "jvp_flash_attention_b200.norms";
   op->kind = kind, op->post = post, op->alpha = alpha, op->eps = eps;
-  op->options = py::make_tuple(kind, post, alpha, eps, name);
   std::vector<py::object> r = apply_dual(op, in);
   return py::make_tuple(r[0], r[1]);
 }
@@ -192,7 +192,6 @@ std::shared_ptr<NormOp> operator_of(const py::tuple& options) {
   auto op = std::make_shared<NormOp>();
   op->name = "norm", op->outputs = 2, op->module = "jvp_flash_attention_b200.norms";
   op->kind = options[0].cast<int>(), op->post = options[1].cast<int>(), op->alpha = options[2].cast<double>(), op->eps = options[3].cast<double>();
-  op->options = options;
   return op;
 }
 
