@@ -15,7 +15,7 @@ constexpr int kMostSegments = 128;
 template <bool OUT>
 int launch_of_type(const Scan& s, cudaStream_t stream) {
   if (s.dtype == JVPFA_FP32) return launch_scan<float, OUT>(s, stream);
-  return s.dtype == JVPFA_BF16 ? launch_chunks(s, OUT, stream) : launch_scan<__half, OUT>(s, stream);
+  return s.dtype == JVPFA_BF16 ? launch_chunks<__nv_bfloat16>(s, OUT, stream) : launch_chunks<__half>(s, OUT, stream);
 }
 
 // The states that the segments begin with, from those that each one's own rows leave: one entry of M a thread, segment after segment.  (Its place
@@ -58,7 +58,7 @@ void cut(Scan& s) {
   // segment below 128 rows.  (us by segments: bf16 B4 H16 L2048 D64 with tangents and gradients, 296 CTAs at once, 4 / 6 / 8 / 11: 426 / 592 / 459 / 506;
   // L8192 D128 forward and backward 4 / 8 / 9 / 16: 1584 / 1620 / 1552 / 1549; fp32 B2 H8 L1023 D128 with tangents, 148 at once, 4 / 6 / 8: 377 / 294 / 223.)
   const int heads = s.B * s.H, width = s.D > s.E ? s.D : s.E, chunk = s.dtype == JVPFA_FP32 && width > 64 ? 32 : 64;
-  const int room = kSMs * (width <= 64 ? (s.dual ? 2 : 3) : s.dual || s.dtype == JVPFA_FP32 ? 1 : 2);
+  const int room = kSMs * (width <= 64 ? (s.dual ? 2 : 4) : s.dual || s.dtype == JVPFA_FP32 ? 1 : 2);
   s.segments = 1, s.segment = s.L;
   double least = 1e30;
   for (int n = 1; n <= kMostSegments; ++n) {

@@ -38,7 +38,8 @@ struct Scan {
   long long state_stride[2];
 };
 
-int launch_chunks(const Scan& s, bool outputs, cudaStream_t stream);  // bfloat16 (linear_chunk.cu)
+template <typename T>
+int launch_chunks(const Scan& s, bool outputs, cudaStream_t stream);  // 16-bit types (linear_chunk.cuh)
 
 inline long long state_bytes(const Scan& s) { return s.segments > 1 ? 4ll * s.B * s.H * s.segments * s.D * s.E : 0; }
 

@@ -1,5 +1,5 @@
-// The map of linear_common.cuh on TF32 instructions, for float16 and float32: entries of float16 are TF32 numbers as they are (and what is
-// formed of them in 32 bits may pass float16's range), float32 ones and what is formed in 32 bits are split in two (common.cuh).
+// The map of linear_common.cuh on TF32 instructions, for float32: entries and what is formed of them are split in two (common.cuh).  (Written for any
+// type: entries of 16-bit types are TF32 numbers as they are.)
 //
 // A CTA takes a segment of one head's rows, chunk by chunk.  Warp w keeps columns 16 w .. 16 w + 15 of M in registers, transposed (rows of the
 // accumulator are columns of M), which as it stands is the second operand of a M.  The weighted products of a chunk go through shared
@@ -306,8 +306,9 @@ __global__ void __launch_bounds__(2 * DT) scan_kernel(const __grid_constant__ Sc
       const jvpfa_linear_tensor& x = which ? p.tout : p.out;
       if (!x.p) continue;
       T* out = static_cast<T*>(const_cast<void*>(x.p)) + of_head(x);
-      const int from = max(n, row_begin), to = min(p.L, row_begin + p.segment);
-      for (long long i = tid; i < (long long)(to - from) * p.E; i += NT) out[(from + i / p.E) * x.stride[2] + i % p.E] = Elem<T>::from_float(0.f);
+      const int to = min(p.L, row_begin + p.segment);
+      for (int row = max(n, row_begin) + warp; row < to; row += NT / 32)
+        for (int e = lane; e < p.E; e += 32) out[row * x.stride[2] + e] = Elem<T>::from_float(0.f);
     }
     if (n == 0 ? segment == 0 : row_begin < n && row_begin + p.segment >= n) {
       const float f = n == 0 ? p.last_scale : p.last_scale * power[p.last_ahead];

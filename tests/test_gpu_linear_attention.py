@@ -1,7 +1,7 @@
 """GPU tests of linear attention against its definition in float64.
 
 Bound of an entry: half a step of its type; 2^-11 of the sum of the magnitudes that it is made of for 16-bit types, whose weighted products of
-queries and keys have 16 bits or more (and would do with 11); and for sums in 32 bits, which the tensor cores truncate (2^-23 a step): at most three instructions
+queries and keys, states and weighted values may have 11 bits (half a step of each, 2^-12, and two of them stand one behind the other); and for sums in 32 bits, which the tensor cores truncate (2^-23 a step): at most three instructions
 for every 8 rows or entries and 22 bits of each operand, (3 (L / 8 + D / 8 + 8) + 8) 2^-22 of that sum.  A gradient is such a map too; one through
 tangents is a sum of three."""
 import pytest
@@ -238,10 +238,47 @@ def test_streams_graphs_and_determinism():
     assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
-def test_nonfinite_entries_stay_in_their_head_and_column():
-    q, k, v = (torch.randn(2, 2, 200, 32, device=DEV) for _ in range(3))
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+def test_powers_of_two_go_through(dt):
+    """Operands and tangents times powers of two give results times powers of two, bit by bit, as long as nothing leaves the type's range."""
+    big = 1 if dt == "fp16" else 5
+    g = torch.Generator(device=DEV).manual_seed(8)
+    x = [_make(1, 3, 150, 64, DT[dt], "bhld", g).clamp_(-4, 4) for _ in range(3)]
+    tx = [_make(1, 3, 150, 64, DT[dt], "bhld", g, 0.25).clamp_(-1, 1) for _ in range(3)]
+    x, tx = ([torch.where(t.abs() < 2.0**-6, 0, t) for t in ts] for ts in (x, tx))  # (nothing subnormal below)
+    w = _decay("slow", 3)
+    f = lambda *a: la.linear_attention(*a, w, return_state=True)  # noqa: E731
+    y, ty = torch.func.jvp(f, tuple(x), tuple(tx))
+    a, b, c, d = 2.0 ** (-4 * big), 2.0 ** (3 * big), 2.0 ** (2 * big), 2.0 ** (-2 * big)
+    z, tz = torch.func.jvp(f, (x[0] * a, x[1] * b, x[2] * c), tuple(t * s * d for t, s in zip(tx, (a, b, c))))
+    assert torch.equal(z[1], y[1] * (b * c)) and torch.equal(tz[1], ty[1] * (b * c * d))
+    if dt != "fp16":  # (its small results are subnormal)
+        assert torch.equal(z[0], y[0] * (a * b * c)) and torch.equal(tz[0], ty[0] * (a * b * c * d))
+    else:
+        assert (z[0] - y[0] * (a * b * c)).abs().max() <= 2.0**-10 * y[0].abs().max() * (a * b * c)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+def test_rows_of_very_different_size(dt):
+    """A few rows 2^12 times the others, in one tile with them; values from 2^-20 on in a column."""
+    B, H, L, D = 1, 2, 200, 64
+    g = torch.Generator(device=DEV).manual_seed(9)
+    q, k, v = (_make(B, H, L, D, DT[dt], "bhld", g) for _ in range(3))
+    q[:, :, 37], k[:, :, 70:72], v[..., 5] = q[:, :, 37] * 2.0**8, k[:, :, 70:72] * 2.0**-12, v[..., 5] * 2.0**-12
+    args = ((_decay("slow", H), None), (D**-0.5, True, ""), False)
+    o, s = la.linear_attention(q, k, v, args[0][0], return_state=True)
+    want, _, _ = formulas.launch_fwd([q, k, v, None], [None] * 4, *args)
+    size, _, _ = formulas.launch_fwd([q.abs(), k.abs(), v.abs(), None], [None] * 4, *args)
+    _near(o, want[0], size[0], _bits(L, D) + 2.0**-11, "o")
+    _near(s, want[1], size[1], _bits(L, D), "state")
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("bad_value", [float("nan"), float("inf")])
+def test_nonfinite_entries_stay_in_their_head_and_column(bad_value, dt):
+    q, k, v = (torch.randn(2, 2, 200, 32, device=DEV).to(DT[dt]) for _ in range(3))
     want = la.linear_attention(q, k, v)
-    v[1, 0, 150, 3] = float("nan")
+    v[1, 0, 150, 3] = bad_value
     o = la.linear_attention(q, k, v)
     bad = ~o.isfinite()
     assert bad[1, 0, 150:, 3].all() and not bad[1, 0, :128].any() and not bad[0].any() and not bad[1, 1].any() and not bad[..., :3].any() and not bad[..., 4:].any()
