@@ -166,7 +166,7 @@ bool bad_dtype(int dtype) { return dtype != JVPFA_BF16 && dtype != JVPFA_FP16 &&
 int bad_sizes(const jvpfa_linear_args& a) {
   if (bad_dtype(a.dtype)) return JVPFA_ERR_DTYPE;
   if (a.B < 1 || a.H < 1 || a.L < 1 || a.D < 1 || a.E < 1 || a.D > 128 || a.E > 128) return JVPFA_ERR_SHAPE;
-  return (long long)a.B * a.H > (1 << 24) ? JVPFA_ERR_TOO_LARGE : JVPFA_OK;
+  return (long long)a.B * a.H > (1 << 24) || a.L > (1 << 30) ? JVPFA_ERR_TOO_LARGE : JVPFA_OK;  // (a chunk behind the last row is counted in 32 bits)
 }
 
 int check(const jvpfa_linear_args* a, bool backward) {

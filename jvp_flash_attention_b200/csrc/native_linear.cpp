@@ -155,7 +155,7 @@ bool linear_acceptable(const Tensors& x, const Tensors& extras) {
   for (int d = 0; d < 3; ++d)
     if (v.size(d) != q.size(d)) return false;
   const int64_t B = q.size(0), H = q.size(1), D = q.size(3), E = v.size(3);
-  if (D < 1 || E < 1 || D > 128 || E > 128 || q.size(2) > INT32_MAX || B * H > (1 << 24)) return false;
+  if (D < 1 || E < 1 || D > 128 || E > 128 || q.size(2) > (1 << 30) || B * H > (1 << 24)) return false;
   if (q.is_cuda() && dtype_of(q, false) < 0) return false;
   if (state.defined() && (state.dim() != 4 || state.size(0) != B || state.size(1) != H || state.size(2) != D || state.size(3) != E ||
                           (q.is_cuda() && state.scalar_type() != at::kFloat) || state.device() != q.device()))

@@ -35,7 +35,8 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor | None =
 
     Sums and states are in 32 bits.  Entries of 16-bit types are multiplied as they are (but for what is 2^-39 of the largest in its 64 rows); what is formed
     of them in 32 bits and multiplied again (decayed entries, states, the products of q and k within a chunk of rows) in 11 bits for bfloat16, which
-    has 8, and 22 for float16, float32 and the state that is answered.  A NaN or an infinite entry reaches its own
+    has 8, and 22 for float16, float32 and the state that is answered.  Where the largest entries of 64 rows (or a state's and a row's) have products beyond the range of
+    32 bits, a zero that meets them may become NaN in the 16-bit types.  A NaN or an infinite entry reaches its own
     row, all later ones and those before it of its chunk.  Results are the same from run to run; last bits depend on how a
     sequence is cut, so on B, H and L, and on whether there are tangents.
 
@@ -111,8 +112,8 @@ def _check(q, k, v, log_decay, scale, state, lengths) -> None:
         raise ValueError(f"q, k and v must have the shapes (B, H, L, D), (B, H, L, D) and (B, H, L, E); got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
     _check_scale(scale)
     B, H, L, D = q.shape
-    if L >= 2**31:
-        raise ValueError("sequences must have less than 2**31 rows")
+    if L > 2**30:
+        raise ValueError("sequences must have at most 2**30 rows")
     _check_operands(q, k, v, state, log_decay, B, H, D, v.shape[3])
     if lengths is not None:
         if lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,) or not lengths.is_contiguous():

@@ -151,6 +151,12 @@ def test_bad_arguments(cpu):
             call()
 
 
+def test_rows_are_counted_in_32_bits():
+    x = torch.ones(1, 1, 1, 1).expand(1, 1, 2**30 + 1, 1)
+    with pytest.raises(ValueError, match="at most 2\\*\\*30 rows"):
+        la.linear_attention(x, x, x)
+
+
 def test_no_cpu_fallback():
     x = torch.ones(1, 2, 3, 4)
     with pytest.raises(RuntimeError, match="runs only on CUDA tensors"):
@@ -177,7 +183,7 @@ def test_the_c_entries_refuse():
                 setattr(a, key, v)
         return entry(ctypes.byref(a), None)
 
-    both = [(-7, dict(struct_size=8)), (-3, dict(dtype=3)), (-2, dict(B=0)), (-2, dict(L=0)), (-2, dict(D=129)), (-2, dict(E=0)), (-10, dict(B=1 << 20, H=17)),
+    both = [(-7, dict(struct_size=8)), (-3, dict(dtype=3)), (-2, dict(B=0)), (-2, dict(L=0)), (-2, dict(D=129)), (-2, dict(E=0)), (-10, dict(B=1 << 20, H=17)), (-10, dict(L=2**30 + 1)),
             (-9, dict(scale=float("nan"))), (-1, dict(q=None)), (-1, dict(tq=64)), (-1, dict(tstate=64)), (-8, dict(k=65)), (-8, dict(state=66)), (-8, dict(lengths=66)),
             (-1, dict(L=4096))]
     for entry, more in ((lib.jvpfa_linear_fwd, [(-1, dict(o=None)), (-1, dict(dual=1))]), (lib.jvpfa_linear_bwd, [(-1, dict(dstate=64)), (-9, dict(scale=0.0, gstate=64))])):
