@@ -99,63 +99,66 @@ __device__ __forceinline__ void stage(T* to, const jvpfa_linear_tensor& x, long 
   }
 }
 
-// A thread's own pieces of a tile that has arrived: the largest finite magnitude (bits of a float), and all of them in float16, times 2^k.
-template <typename T, int DT, int NT>
-__device__ __forceinline__ uint32_t own_largest(const T* tile) {
+// A thread's own pieces of a tile that has arrived: their largest finite magnitude (bits of a float), and all of them in float16, times 2^k.
+constexpr int kOwn = CH / 16;
+template <typename T, int DT>
+__device__ __forceinline__ T* own_place(T* tile, int r) {
   constexpr int LD = DT + 8, PIECES = DT / 8;
+  return tile + (threadIdx.x / PIECES + r * 16) * LD + threadIdx.x % PIECES * 8;
+}
+template <typename T, int DT>
+__device__ __forceinline__ void own(uint4 (&v)[kOwn], T* tile) {
+#pragma unroll
+  for (int r = 0; r < kOwn; ++r) v[r] = *reinterpret_cast<const uint4*>(own_place<T, DT>(tile, r));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t largest_of(const uint4 (&v)[kOwn]) {
   using W = typename Two<T>::type;
-  const T* from = tile + threadIdx.x / PIECES * LD + threadIdx.x % PIECES * 8;
   W m;
   *reinterpret_cast<uint32_t*>(&m) = 0u;
 #pragma unroll
-  for (int r = 0; r < CH / 16; ++r) {
-    const uint4 v = *reinterpret_cast<const uint4*>(from + r * 16 * LD);
+  for (int r = 0; r < kOwn; ++r)
 #pragma unroll
-    for (const uint32_t w : {v.x, v.y, v.z, v.w}) m = __hmax2(m, __habs2(*reinterpret_cast<const W*>(&w)));  // (a NaN is passed over)
-  }
+    for (const uint32_t w : {v[r].x, v[r].y, v[r].z, v[r].w}) m = __hmax2(m, __habs2(*reinterpret_cast<const W*>(&w)));  // (a NaN is passed over)
   const float2 both = of_word<T>(*reinterpret_cast<const uint32_t*>(&m));
-  float x = fmaxf(both.x, both.y);
-  if (x > 3.4e38f || (std::is_same_v<T, __half> && x > 65504.f)) {  // infinite: the others' largest
-    x = 0.f;
-    for (int r = 0; r < CH / 16; ++r)
-      for (int j = 0; j < 8; ++j) {
-        const float y = fabsf(Elem<T>::to_float(from[r * 16 * LD + j]));
-        if (y > x && y < __int_as_float(0x7f800000)) x = y;
-      }
-  }
-  return __float_as_uint(x);
-}
-template <typename T, int DT, int NT>
-__device__ __forceinline__ void convert(T* tile, int k) {
-  constexpr int LD = DT + 8, PIECES = DT / 8;
-  T* from = tile + threadIdx.x / PIECES * LD + threadIdx.x % PIECES * 8;
-  const float2 by = make_float2(two_to(k), two_to(k));
+  uint32_t most = __float_as_uint(fmaxf(both.x, both.y));
+  if (most >= kInfinite) {  // the others' largest
+    most = 0;
 #pragma unroll
-  for (int r = 0; r < CH / 16; ++r) {
-    uint4* at = reinterpret_cast<uint4*>(from + r * 16 * LD);
-    const uint4 v = *at;
-    auto half_of = [&](uint32_t w) {
-      const float2 x = __fmul2_rn(of_word<T>(w), by);
-      return halves(x.x, x.y);
-    };
-    *at = make_uint4(half_of(v.x), half_of(v.y), half_of(v.z), half_of(v.w));
+    for (int r = 0; r < kOwn; ++r)
+#pragma unroll
+      for (const uint32_t w : {v[r].x, v[r].y, v[r].z, v[r].w}) most = larger_finite(larger_finite(most, of_word<T>(w).x), of_word<T>(w).y);
   }
+  return most;
+}
+template <typename T, int DT>
+__device__ __forceinline__ void convert(T* tile, const uint4 (&v)[kOwn], int k) {
+  const float2 by = make_float2(two_to(k), two_to(k));
+  auto half_of = [&](uint32_t w) {
+    const float2 x = __fmul2_rn(of_word<T>(w), by);
+    return halves(x.x, x.y);
+  };
+#pragma unroll
+  for (int r = 0; r < kOwn; ++r) *reinterpret_cast<uint4*>(own_place<T, DT>(tile, r)) = make_uint4(half_of(v[r].x), half_of(v[r].y), half_of(v[r].z), half_of(v[r].w));
 }
 
-// Shared memory of a CTA: two tiles of b (and of its tangent), which a chunk reads to its end, and one of c and one of a, which are free behind the
-// products' barrier and take the next chunk's rows then; the products.  States alone: two tiles of b and c.
-template <int DT, bool DUAL, bool OUT>
+// Shared memory of a CTA: two tiles of b (and of its tangent), which a chunk reads to its end, and of a where there is room, else one that takes the
+// next rows behind the chunk's end; one of c, which is free behind the products' barrier; the products.  States alone: two tiles of b and c.
+template <int DT, bool DUAL, bool OUT, int PP>
 struct ChunkShape {
   static constexpr int LD = DT + 8, NT = 2 * DT, SIDES = DUAL ? 2 : 1, TILE = CH * LD;
   static constexpr int CTAS = DT == 32 ? (DUAL ? 2 : 4) : DT == 64 ? (DUAL ? 2 : 4) : DUAL ? 1 : 2;
-  static constexpr size_t bytes(int parts) { return 2 * SIDES * (4 * (size_t)TILE + (OUT ? parts * (size_t)CH * LP : 0)); }
+  static constexpr size_t bytes_with(int tiles) { return 2 * SIDES * (tiles * (size_t)TILE + (OUT ? PP * (size_t)CH * LP : 0)); }
+  static constexpr bool fits(size_t bytes) { return bytes * CTAS <= 227 * 1024 - CTAS * 2048; }
+  static constexpr bool TWO_A = OUT && fits(bytes_with(5)), KEEP = DT <= 64;  // KEEP: a thread has registers for its pieces of all tiles
+  static constexpr size_t bytes = bytes_with(TWO_A ? 5 : 4);
 };
 
 // OUT: the outputs, from the states that the segments begin with; else the states that their rows leave, from nothing.  PP: parts of products and
 // of M, PW: of the weighted c.
 template <typename T, int DT, bool DUAL, bool OUT, int PP, int PW>
-__global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk_kernel(const __grid_constant__ Scan p, const uint32_t wide) {
-  using S = ChunkShape<DT, DUAL, OUT>;
+__global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT, PP>::CTAS) chunk_kernel(const __grid_constant__ Scan p, const uint32_t wide) {
+  using S = ChunkShape<DT, DUAL, OUT, PP>;
   constexpr int NT = S::NT, LD = S::LD, ND = DT / 8, KD = DT / 16, NW = DT / 16, SIDES = DUAL ? 2 : 1;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float power[CH + 2], less1[CH + 2];  // l^j and l^j - 1
@@ -164,8 +167,8 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
   constexpr int TILE = S::TILE;
   T* tiles_b = reinterpret_cast<T*>(smem);     // two times b and its tangent
   T* tiles_c = tiles_b + 2 * SIDES * TILE;     // c and its tangent (states alone: two times)
-  T* tiles_a = tiles_c + SIDES * TILE;         // a and its tangent
-  T* sP = tiles_a + SIDES * TILE;              // products in their parts, then their tangents
+  T* tiles_a = tiles_c + SIDES * TILE;         // a and its tangent, TWO_A: twice
+  T* sP = tiles_a + (S::TWO_A ? 2 : 1) * SIDES * TILE;  // products in their parts, then their tangents
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int segment = blockIdx.x % p.segments, head = blockIdx.x / p.segments, b = head / p.H, h = head - b * p.H;
   const int n = length_of(p.lengths, b, p.L), row_begin = segment * p.segment, row_end = min(n, row_begin + p.segment);
@@ -217,10 +220,11 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
     stage<T, DT, NT>(to, p.c, of_head(p.c), p.E, row0, rows, n, p.reversed, wide & 2);
     if (DUAL) stage<T, DT, NT>(to + TILE, p.tc, of_head(p.tc), p.E, row0, rows, n, p.reversed, wide & 16);
   };
-  auto fetch_a = [&](int row0) {
+  auto fetch_a = [&](int half, int row0) {
     const int rows = min(CH, row_end - row0);
-    stage<T, DT, NT>(tiles_a, p.a, of_head(p.a), p.D, row0, rows, n, p.reversed, wide & 4);
-    if (DUAL) stage<T, DT, NT>(tiles_a + TILE, p.ta, of_head(p.ta), p.D, row0, rows, n, p.reversed, wide & 32);
+    T* to = tiles_a + (S::TWO_A ? half * SIDES * TILE : 0);
+    stage<T, DT, NT>(to, p.a, of_head(p.a), p.D, row0, rows, n, p.reversed, wide & 4);
+    if (DUAL) stage<T, DT, NT>(to + TILE, p.ta, of_head(p.ta), p.D, row0, rows, n, p.reversed, wide & 32);
   };
   // where a lane of ldmatrix reads: first operand and transposed second one (rows 0-7, 8-15, then columns 8-15), second one (columns 8-15, then rows 8-15)
   const int lane_row = lane & 15, lane_col = lane >> 4 << 3;
@@ -228,12 +232,12 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
   constexpr uint32_t SZ = 2, ROWS16 = 16 * LD * SZ, P16 = 16 * LP * SZ, PART = CH * LP * SZ, SIDE = (SIDES - 1) * TILE * SZ;
   const uint32_t at_first = (lane_row * LD + lane_col) * SZ;  // of a first operand, or a transposed second one
   const uint32_t at_second = (lane_row_n * LD + lane_col_n) * SZ;
-  const uint32_t lane_a = shared_address(tiles_a) + at_first, lane_p = shared_address(sP) + (lane_row * LP + lane_col) * SZ;
+  const uint32_t lane_p = shared_address(sP) + (lane_row * LP + lane_col) * SZ;
 
   int now = 0;
   if (row_begin < row_end) {
     fetch_b(0, row_begin), fetch_c(0, row_begin);
-    if (OUT) fetch_a(row_begin);
+    if (OUT) fetch_a(0, row_begin);
     cp_async_commit();
   }
   for (int row0 = row_begin; row0 < row_end; row0 += CH, shift = 0, now ^= 1) {
@@ -242,18 +246,22 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
     cp_async_wait<0>();
     // b, its tangent, c, its tangent, a, its tangent
     T* const arrived[6] = {tiles_b + now * SIDES * TILE, tiles_b + now * SIDES * TILE + TILE, tiles_c + (OUT ? 0 : now * SIDES * TILE),
-                           tiles_c + (OUT ? 0 : now * SIDES * TILE) + TILE, tiles_a, tiles_a + TILE};
+                           tiles_c + (OUT ? 0 : now * SIDES * TILE) + TILE, tiles_a + (S::TWO_A ? now * SIDES * TILE : 0),
+                           tiles_a + (S::TWO_A ? now * SIDES * TILE : 0) + TILE};
     auto there = [&](int i) { return (DUAL || i % 2 == 0) && (OUT || i < 4); };
+    uint4 mine_of[6][kOwn];
 #pragma unroll
     for (int i = 0; i < 6; ++i) {
       if (!there(i)) continue;
-      const uint32_t m = __reduce_max_sync(0xffffffffu, own_largest<T, DT, NT>(arrived[i]));
+      own<T, DT>(mine_of[i], arrived[i]);
+      const uint32_t m = __reduce_max_sync(0xffffffffu, largest_of<T>(mine_of[i]));
       if (lane == 0) largest[i][warp] = m;
     }
     __syncthreads();  // the largest are there, and the chunk before has been read
     if (more) {
       fetch_b(now ^ 1, row0 + CH);
       if (!OUT) fetch_c(now ^ 1, row0 + CH);
+      if (S::TWO_A) fetch_a(now ^ 1, row0 + CH);
       cp_async_commit();
     }
     int room[6];
@@ -261,13 +269,15 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
     for (int i = 0; i < 6; ++i) {
       if (!there(i)) continue;
       room[i] = room_for(__reduce_max_sync(0xffffffffu, lane < NW ? largest[i][lane] : 0u));
-      convert<T, DT, NT>(arrived[i], room[i]);
+      if (!S::KEEP) own<T, DT>(mine_of[i], arrived[i]);
+      convert<T, DT>(arrived[i], mine_of[i], room[i]);
     }
     __syncthreads();  // everything is float16
     // what the tiles are in units of (1 of those that are zero, so that no zero meets an infinite unit)
     auto unit_of = [&](int i) { return there(i) ? two_to(-room[i]) : 0.f; };
     const float ub = unit_of(0), utb = unit_of(1), uc = unit_of(2), utc = unit_of(3), ua = unit_of(4), uta = unit_of(5);
     const uint32_t tile_b = shared_address(tiles_b + now * SIDES * TILE), lane_b = tile_b + at_first;
+    const uint32_t lane_a = shared_address(arrived[4]) + at_first;
     const uint32_t lane_c = shared_address(tiles_c + (OUT ? 0 : now * SIDES * TILE)) + at_first + e0 * SZ;
     uint32_t fc[SIDES][4][4];  // columns e0 .. e0 + 15 of c: 16 rows each; second operand's halves (0, 1) and (2, 3)
     if constexpr (OUT) {
@@ -482,10 +492,12 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT>::CTAS) chunk
         }
         answer(i, acc);
       }
-      __syncthreads();  // nobody reads a again
-      if (more) {
-        fetch_a(row0 + CH);
-        cp_async_commit();
+      if constexpr (!S::TWO_A) {
+        __syncthreads();  // nobody reads a again
+        if (more) {
+          fetch_a(0, row0 + CH);
+          cp_async_commit();
+        }
       }
     } else {
 #pragma unroll
@@ -588,14 +600,14 @@ int launch(const Scan& s, cudaStream_t stream) {
   static SmemOptIn opt;
   constexpr int PP = std::is_same_v<T, __half> ? 2 : 1;
   const auto kernel = chunk_kernel<T, DT, DUAL, OUT, PP, PW>;
-  constexpr size_t bytes = ChunkShape<DT, DUAL, OUT>::bytes(PP);
-  static_assert(bytes * ChunkShape<DT, DUAL, OUT>::CTAS <= 227 * 1024 - ChunkShape<DT, DUAL, OUT>::CTAS * 2048, "an SM's shared memory");
+  constexpr size_t bytes = ChunkShape<DT, DUAL, OUT, PP>::bytes;
+  static_assert(ChunkShape<DT, DUAL, OUT, PP>::fits(bytes), "an SM's shared memory");
   if (!opt.ensure(reinterpret_cast<const void*>(kernel), bytes)) return JVPFA_ERR_CUDA;
   uint32_t wide = 0;
   const jvpfa_linear_tensor* tensors[8] = {&s.b, &s.c, &s.a, &s.tb, &s.tc, &s.ta, &s.out, &s.tout};
   for (int i = 0; i < 8; ++i)
     if (wide_tensor<T>(*tensors[i], s, i % 3 == 1 || i >= 6 ? s.E : s.D)) wide |= 1u << i;
-  kernel<<<(unsigned)((long long)s.B * s.H * s.segments), ChunkShape<DT, DUAL, OUT>::NT, bytes, stream>>>(s, wide);
+  kernel<<<(unsigned)((long long)s.B * s.H * s.segments), ChunkShape<DT, DUAL, OUT, PP>::NT, bytes, stream>>>(s, wide);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {
     set_last_cuda_error(e, "chunk_kernel");
