@@ -5,17 +5,13 @@
 namespace jvpfa {
 namespace linear {
 
-template <typename T, bool OUT>
-int launch_scan(const Scan& s, cudaStream_t stream);
-
 namespace {
 
 constexpr int kMostSegments = 128;
 
-template <bool OUT>
-int launch_of_type(const Scan& s, cudaStream_t stream) {
-  if (s.dtype == JVPFA_FP32) return launch_scan<float, OUT>(s, stream);
-  return s.dtype == JVPFA_BF16 ? launch_chunks<__nv_bfloat16>(s, OUT, stream) : launch_chunks<__half>(s, OUT, stream);
+int launch_of_type(const Scan& s, bool outputs, cudaStream_t stream) {
+  if (s.dtype == JVPFA_FP32) return launch_scan(s, outputs, stream);
+  return s.dtype == JVPFA_BF16 ? launch_chunks<__nv_bfloat16>(s, outputs, stream) : launch_chunks<__half>(s, outputs, stream);
 }
 
 // The states that the segments begin with, from those that each one's own rows leave: one entry of M a thread, segment after segment.  (Its place
@@ -73,11 +69,11 @@ void cut(Scan& s) {
 // `found`: the segments' states are there already.
 int launch(const Scan& s, cudaStream_t stream, bool found = false) {
   if (s.segments > 1 && !found) {
-    const int rc = launch_of_type<false>(s, stream);
+    const int rc = launch_of_type(s, false, stream);
     if (rc) return rc;
     join_kernel<<<dim3((unsigned)(s.B * s.H), (unsigned)((s.D * s.E + 255) / 256)), 256, 0, stream>>>(s);
   }
-  return launch_of_type<true>(s, stream);
+  return launch_of_type(s, true, stream);
 }
 
 // ---- one more token ------------------------------------------------------------------------------------------------------

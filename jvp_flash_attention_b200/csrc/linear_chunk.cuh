@@ -586,15 +586,6 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT, PP>::CTAS) c
   }
 }
 
-template <typename T>
-bool wide_tensor(const jvpfa_linear_tensor& x, const Scan& s, int width) {
-  uint64_t all = (uint64_t)width * sizeof(T) | reinterpret_cast<uint64_t>(x.p);
-  const int counts[3] = {s.B, s.H, s.L};
-  for (int d = 0; d < 3; ++d)
-    if (counts[d] > 1) all |= (uint64_t)x.stride[d] * sizeof(T);
-  return all % 16 == 0;
-}
-
 template <typename T, int DT, bool DUAL, bool OUT, int PW>
 int launch(const Scan& s, cudaStream_t stream) {
   static SmemOptIn opt;

@@ -40,6 +40,17 @@ struct Scan {
 
 template <typename T>
 int launch_chunks(const Scan& s, bool outputs, cudaStream_t stream);  // 16-bit types (linear_chunk.cuh)
+int launch_scan(const Scan& s, bool outputs, cudaStream_t stream);    // float32 (linear_scan.cu)
+
+// Whether a tensor's rows are whole 16-byte pieces.
+template <typename T>
+bool wide_tensor(const jvpfa_linear_tensor& x, const Scan& s, int width) {
+  uint64_t all = (uint64_t)width * sizeof(T) | reinterpret_cast<uint64_t>(x.p);
+  const int counts[3] = {s.B, s.H, s.L};
+  for (int d = 0; d < 3; ++d)
+    if (counts[d] > 1) all |= (uint64_t)x.stride[d] * sizeof(T);
+  return all % 16 == 0;
+}
 
 inline long long state_bytes(const Scan& s) { return s.segments > 1 ? 4ll * s.B * s.H * s.segments * s.D * s.E : 0; }
 
