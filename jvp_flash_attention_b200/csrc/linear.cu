@@ -9,16 +9,20 @@ namespace {
 
 constexpr int kMostSegments = 128;
 
+template <int V>
+struct alignas(4 * V) Entries { float x[V]; };
+
 int launch_of_type(const Scan& s, bool outputs, cudaStream_t stream) {
   if (s.dtype == JVPFA_FP32) return launch_scan(s, outputs, stream);
   return s.dtype == JVPFA_BF16 ? launch_chunks<__nv_bfloat16>(s, outputs, stream) : launch_chunks<__half>(s, outputs, stream);
 }
 
-// The states that the segments begin with, from those that each one's own rows leave: one entry of M a thread, segment after segment.  (Its place
-// in the states goes over all of them, whatever their order; where the given state is.)
+// The states that the segments begin with, from those that each one's own rows leave, in place and segment after segment; V successive entries of M
+// a thread, value or tangent.  Memory-bound, though what it reads was just written and is in L2.
+template <int V>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Scan p) {
   __shared__ float down[kMostSegments];
-  const int size = p.D * p.E, head = blockIdx.x, b = head / p.H, h = head - b * p.H;
+  const int size = p.D * p.E, head = blockIdx.x, b = head / p.H, h = head - b * p.H, which = blockIdx.z;
   const int n = length_of(p.lengths, b, p.L);
   const float w = decay_of(p.log_decay, h);
   for (int s = threadIdx.x; s < p.segments; s += 256) {
@@ -26,23 +30,32 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Scan 
     down[s] = expm1f(w * rows);
   }
   __syncthreads();
-  const int i = blockIdx.y * 256 + threadIdx.x;
+  const int i = (blockIdx.y * 256 + threadIdx.x) * V;
   if (i >= size) return;
-  const int d = i / p.E, e = i - d * p.E;
-  const long long given = (long long)head * size + d * p.first_stride[0] + e * p.first_stride[1];
-  for (int which = 0; which < (p.dual ? 2 : 1); ++which) {
-    const float* first = which ? p.tfirst : p.first;
-    float* at = (which ? p.tstates : p.states) + (long long)head * p.segments * size + d * p.state_stride[0] + e * p.state_stride[1];
-    float x = first ? p.first_scale * first[given] : 0.f;
-    for (int s0 = 0; s0 < p.segments; s0 += 8, at += 8ll * size) {  // eight loads under way at once
-      float own[8];
+  float x[V];
+  const float* first = which ? p.tfirst : p.first;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) own[k] = s0 + k + 1 < p.segments ? at[(long long)k * size] : 0.f;  // (the last one's is nobody's)
+  for (int v = 0; v < V; ++v) {
+    const int d = (i + v) / p.E, e = i + v - d * p.E;
+    x[v] = first ? p.first_scale * first[(long long)head * size + d * p.first_stride[0] + e * p.first_stride[1]] : 0.f;
+  }
+  float* at = (which ? p.tstates : p.states) + (long long)head * p.segments * size + i;
+  constexpr int AHEAD = 8;  // loads under way at once
+  for (int s0 = 0; s0 < p.segments; s0 += AHEAD, at += AHEAD * (long long)size) {
+    Entries<V> own[AHEAD];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (s0 + k >= p.segments) break;
-        at[(long long)k * size] = x;
-        x = fmaf(x, down[s0 + k], x) + own[k];
+    for (int k = 0; k < AHEAD; ++k)
+      if (s0 + k + 1 < p.segments) own[k] = *reinterpret_cast<const Entries<V>*>(at + k * (long long)size);  // (the last one's is nobody's)
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      if (s0 + k >= p.segments) break;
+      Entries<V> begin;
+#pragma unroll
+      for (int v = 0; v < V; ++v) begin.x[v] = x[v];
+      *reinterpret_cast<Entries<V>*>(at + k * (long long)size) = begin;
+      if (s0 + k + 1 < p.segments) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) x[v] = fmaf(x[v], down[s0 + k], x[v]) + own[k].x[v];
       }
     }
   }
@@ -71,7 +84,13 @@ int launch(const Scan& s, cudaStream_t stream, bool found = false) {
   if (s.segments > 1 && !found) {
     const int rc = launch_of_type(s, false, stream);
     if (rc) return rc;
-    join_kernel<<<dim3((unsigned)(s.B * s.H), (unsigned)((s.D * s.E + 255) / 256)), 256, 0, stream>>>(s);
+    const bool wide = s.D * s.E % 4 == 0;  // (the workspace begins on 16 bytes)
+    const int each = wide ? 1024 : 256;
+    const dim3 grid((unsigned)(s.B * s.H), (unsigned)((s.D * s.E + each - 1) / each), s.dual ? 2 : 1);
+    if (wide)
+      join_kernel<4><<<grid, 256, 0, stream>>>(s);
+    else
+      join_kernel<1><<<grid, 256, 0, stream>>>(s);
   }
   return launch_of_type(s, true, stream);
 }
