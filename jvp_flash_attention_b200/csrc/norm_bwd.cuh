@@ -4,7 +4,8 @@
 // was rounded is read.  Two sums over the row's threads (five values each with tangents, two without) are all that its entries exchange.  The
 // vectors' gradients are sums over rows: each thread adds up its columns' in registers while its CTA, one on each SM and several rows at once, goes
 // through a part of one group's rows, and leaves them in the workspace; a second launch adds these parts in a fixed order.
-// What bounds it: memory, each tensor read and written once; with tangents and a residual sum the registers (170 of a thread, 12 warps).
+// What bounds it: memory, each tensor read and written once; with tangents and a residual sum the registers (170 of a thread, 12 warps).  bf16 8192 x 4096 with both norms 120 us (403 MB at 3.4 TB/s; issue slots
+// 57 % busy, a row at once on an SM); 8192 x 1024 with tangents the norm 36 and with the residual sum 73; fp16 3990 x 2731 43.
 #pragma once
 #include "norm_common.cuh"
 

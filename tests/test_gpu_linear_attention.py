@@ -57,6 +57,8 @@ CASES = [
     (2, 2, 1030, 128, 128, "bhld", "mixed", True, (1030, 300)),
     (1, 2, 2048, 40, 24, "blhd", None, False, None),
     (1, 2, 769, 128, 64, "blhd", "fast", True, (640,)),
+    (2, 2, 1400, 33, 7, "odd", "slow", True, (1400, 515)),
+    (1, 3, 2500, 5, 3, "bhld", "mixed", True, None),
 ]
 
 
