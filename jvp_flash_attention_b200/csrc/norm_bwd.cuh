@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(BOUND) norm_bwd_kernel(const __grid_constant__
   constexpr int VECTORS = SIDES * ((HASY ? 1 : 0) + (HASN ? 1 : 0));
   float* vectors = reinterpret_cast<float*>(smem + lay.teams * lay.team_bytes);
   const int padded = (a.C + V - 1) / V * V;
-  float* shared_parts = vectors + VECTORS * padded;
+  float* shared_parts = vectors + (WAY == DIRECT ? 0 : VECTORS * padded);  // (DIRECT ones read the vectors as they are)
   const Rows<T, NC, WAY> rows{a.C, a.M, team, aligned};
   // x, tx, gn, gtn, y, ty, gr, gtr, as far as there are any of them
   Source sources[TENSORS];

@@ -77,6 +77,8 @@ CASES = [
     (ALL, (300, 5, 48), (300, 1), "layer", "rms"),  # more groups than SMs
     ({"x", "y", "gate", "scale", "bias"}, (400, 72), (400,), "layer", "layer"),  # every row vectors of its own
     ({"x", "weight", "shift"}, (150, 2, 1032), (150, 1), "rms", None),
+    ({"x", "y", "post_weight"}, (600, 5710), None, None, "layer"),  # too wide for shared memory, several rows of a CTA at once
+    (ALL, (2, 300, 4104), (2, 1), "rms", "layer"),
 ]
 
 
