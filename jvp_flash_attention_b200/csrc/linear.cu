@@ -22,13 +22,13 @@ int launch_of_type(const Scan& s, bool outputs, cudaStream_t stream) {
 // segments, 38 MB read and written, 14 us (an entry a thread: 33).
 template <int V>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Scan p) {
-  __shared__ float down[kMostSegments];
+  __shared__ Down down[kMostSegments];
   const int size = p.D * p.E, head = blockIdx.x, b = head / p.H, h = head - b * p.H, which = blockIdx.z;
   const int n = length_of(p.lengths, b, p.L);
   const float w = decay_of(p.log_decay, h);
   for (int s = threadIdx.x; s < p.segments; s += 256) {
     const int rows = max(0, min(n - s * p.segment, p.segment)) + (s == 0 ? p.ahead - 1 : 0);
-    down[s] = expm1f(w * rows);
+    down[s] = down_of(expf(w * rows), expm1f(w * rows));
   }
   __syncthreads();
   const int i = (blockIdx.y * 256 + threadIdx.x) * V;
@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Scan 
       *reinterpret_cast<Entries<V>*>(at + k * (long long)size) = begin;
       if (s0 + k + 1 < p.segments) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) x[v] = fmaf(x[v], down[s0 + k], x[v]) + own[k].x[v];
+        for (int v = 0; v < V; ++v) x[v] = fmaf(x[v], down[s0 + k].by, fmaf(x[v], down[s0 + k].keep, own[k].x[v]));
       }
     }
   }
@@ -117,7 +117,8 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constan
     sq[d] = a.scale * load_as(a.q, b * a.q_stride[0] + h * a.q_stride[1] + d, a.dtype);
     sk[d] = load_as(a.k, b * a.k_stride[0] + h * a.k_stride[1] + d, a.dtype);
   }
-  const float down = expm1f(decay_of(a.log_decay, h));
+  const float w = decay_of(a.log_decay, h);
+  const Down down = down_of(expf(w), expm1f(w));
   float v[V], o[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -147,7 +148,7 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constan
         if (d >= a.D) break;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          s[j][i] = fmaf(s[j][i], down, s[j][i]) + sk[d] * v[i];
+          s[j][i] = fmaf(s[j][i], down.by, fmaf(s[j][i], down.keep, sk[d] * v[i]));
           o[i] += sq[d] * s[j][i];
         }
         if constexpr (V == 4)

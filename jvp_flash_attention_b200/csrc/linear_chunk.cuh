@@ -509,8 +509,7 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT, PP>::CTAS) c
         if (DUAL) ldmatrix_t(fc[SIDES - 1][k], lane_c + SIDE + k * ROWS16);
       }
     }
-    // M = l^rows M + sum of l^(rows - 1 - s) b_s c_s^T; the factor by its distance from 1, which keeps the digits of slow decays.  As a first operand the
-    // words of c are (0, 2, 1, 3).
+    // M = l^rows M + sum of l^(rows - 1 - s) b_s c_s^T.  As a first operand the words of c are (0, 2, 1, 3).
     uint32_t wc[SIDES][4][4][PW];
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -523,7 +522,7 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT, PP>::CTAS) c
 #pragma unroll
           for (int j = 0; j < 2; ++j) split(__fmul2_rn(of_halves(fc[side][k][2 * j + u]), by), wc[side][k][2 * u + j]);
       }
-    const float down = less1[rows + shift];
+    const Down down = down_of(power[rows + shift], less1[rows + shift]);
     const float f0 = uc * ub, f1 = utc * ub, f2 = uc * utb;
 #pragma unroll
     for (int d = 0; d < ND; d += 2) {
@@ -550,7 +549,7 @@ __global__ void __launch_bounds__(2 * DT, ChunkShape<DT, DUAL, OUT, PP>::CTAS) c
         for (int j = 0; j < 4; j += 2) {
           auto take_on = [&](float* to, float2 add) {
             const float2 old = make_float2(to[0], to[1]);
-            const float2 sum = __fadd2_rn(__ffma2_rn(old, make_float2(down, down), old), add);
+            const float2 sum = __ffma2_rn(old, make_float2(down.by, down.by), __ffma2_rn(old, make_float2(down.keep, down.keep), add));
             to[0] = sum.x, to[1] = sum.y;
           };
           take_on(&M[0][d + u][j], __fmul2_rn(make_float2(x[0][u][j], x[0][u][j + 1]), make_float2(f0, f0)));

@@ -58,6 +58,12 @@ __device__ __forceinline__ float decay_of(const float* log_decay, int h) {
   const float w = log_decay ? log_decay[h] : 0.f;
   return w < kLowest ? kLowest : w;  // (a NaN stays one)
 }
+// l^n as by + keep, keep 1 or 0: next to 1 by its distance from it, which keeps the digits of slow decays, else as it is, which keeps those of
+// what little is left.  M l^n + x is fma(M, by, fma(M, keep, x)).
+struct Down {
+  float by, keep;
+};
+__device__ __forceinline__ Down down_of(float power, float less1) { return less1 > -0.5f ? Down{less1, 1.f} : Down{power, 0.f}; }
 __device__ __forceinline__ int length_of(const int32_t* lengths, int b, int L) { return lengths ? min(max(lengths[b], 0), L) : L; }
 
 }  // namespace linear

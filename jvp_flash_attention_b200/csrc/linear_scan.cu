@@ -238,14 +238,14 @@ __global__ void __launch_bounds__(2 * DT) scan_kernel(const __grid_constant__ Sc
           }
       }
     }
-    // M = l^rows M + sum of l^(rows - 1 - s) b_s c_s^T; the factor by its distance from 1, which keeps the digits of slow decays
-    const float down = less1[rows + shift];
+    // M = l^rows M + sum of l^(rows - 1 - s) b_s c_s^T
+    const Down down = down_of(power[rows + shift], less1[rows + shift]);
 #pragma unroll
     for (int i = 0; i < ND; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        M[i][j] = fmaf(M[i][j], down, M[i][j]);
-        if (DUAL) tM[i][j] = fmaf(tM[i][j], down, tM[i][j]);
+        M[i][j] = fmaf(M[i][j], down.by, M[i][j] * down.keep);
+        if (DUAL) tM[i][j] = fmaf(tM[i][j], down.by, tM[i][j] * down.keep);
       }
     for (int k = 0; k < rows; k += 8) {
       auto load_c = [&](Part(&f)[4], const float* s) {

@@ -59,6 +59,8 @@ CASES = [
     (1, 2, 769, 128, 64, "blhd", "fast", True, (640,)),
     (2, 2, 1400, 33, 7, "odd", "slow", True, (1400, 515)),
     (1, 3, 2500, 5, 3, "bhld", "mixed", True, None),
+    (3, 4, 24, 32, 128, "blhd", "mixed", True, (3, 24, 10)),  # little is left of a given state
+    (2, 4, 6, 103, 107, "blhd", "mixed", True, (3, 6)),
 ]
 
 
@@ -116,6 +118,21 @@ def test_values_tangents_and_gradients(case, dual, dt):
             # (in the same form: with tangents the order of some sums is another one)
             o, s = torch.func.jvp(f, tuple(bad), tuple(tx))[0] if dual else f(*bad)
         assert torch.equal(o, y[0]) and torch.equal(s, y[1])
+
+
+def test_what_is_left_keeps_its_digits():
+    """Of a state alone, decayed row by row, over a whole sequence and over several segments of one."""
+    w = torch.tensor([-3.0, -9.0, -0.02, -1e-4], device=DEV)
+    s = torch.randn(1, 4, 64, 64, generator=torch.Generator(device=DEV).manual_seed(3), device=DEV)
+    for dt in DT.values():
+        zero = torch.zeros(1, 4, 1000, 64, device=DEV, dtype=dt)
+        token = s.clone()
+        la.linear_attention_step(zero[:, :, 0], zero[:, :, 0], zero[:, :, 0], w, token)
+        for n, got in [(1, token)] + [(n, la.linear_attention(zero[:, :, :n], zero[:, :, :n], zero[:, :, :n], w, state=s, return_state=True)[1]) for n in (1, 3, 9, 1000)]:
+            want = s.double() * (w.double() * n).exp()[:, None, None]
+            # an exponent's rounding and its function's, and a rounding for each of up to 16 chunks and 8 segments, all of them taken twice
+            rel = 2 * ((w.double() * n).abs()[:, None, None] + 2 + 2 * 24) * 2.0**-24
+            assert ((got.double() - want).abs() <= rel * want.abs() + 2.0**-126).all(), (dt, n)
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])
