@@ -68,7 +68,7 @@ void cut(Scan& s) {
   // segment below 128 rows.  (us by segments: bf16 B4 H16 L2048 D64 with tangents and gradients, 296 CTAs at once, 4 / 6 / 8 / 11: 426 / 592 / 459 / 506;
   // L8192 D128 forward and backward 4 / 8 / 9 / 16: 1584 / 1620 / 1552 / 1549; fp32 B2 H8 L1023 D128 with tangents, 148 at once, 4 / 6 / 8: 377 / 294 / 223.)
   const int heads = s.B * s.H, width = s.D > s.E ? s.D : s.E, chunk = s.dtype == JVPFA_FP32 && width > 64 ? 32 : 64;
-  const int room = kSMs * (width <= 64 ? (s.dual ? 2 : 4) : s.dual || s.dtype == JVPFA_FP32 ? 1 : 2);
+  const int room = kSMs * (width <= 64 ? (s.dual ? 2 : width <= 32 || s.dtype == JVPFA_FP32 ? 4 : 3) : s.dual || s.dtype == JVPFA_FP32 ? 1 : 2);
   s.segments = 1, s.segment = s.L;
   double least = 1e30;
   for (int n = 1; n <= kMostSegments; ++n) {

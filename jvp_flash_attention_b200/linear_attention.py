@@ -33,12 +33,12 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor | None =
     a row sees itself alone); no gradient.  ``sm_scale``: 1 / sqrt(D) by default.  ``state``: (B, H, D, E) float32, S before the first row, plain or
     dual.  ``lengths``: (B) int32, rows of each sequence; those behind are not read and their results are zero, and S is that behind the last one.
 
-    Sums and states are in 32 bits.  Entries of 16-bit types are multiplied as they are (but for what is 2^-39 of the largest in its 64 rows); what is formed
-    of them in 32 bits and multiplied again (decayed entries, states, the products of q and k within a chunk of rows) in 11 bits for bfloat16, which
-    has 8, and 22 for float16, float32 and the state that is answered.  Where the largest entries of 64 rows (or a state's and a row's) have products beyond the range of
-    32 bits, a zero that meets them may become NaN in the 16-bit types.  A NaN or an infinite entry reaches its own
+    Sums and states are in 32 bits.  Entries are multiplied as they are; what is formed of them in 32 bits and multiplied again (decayed entries, states,
+    the products of q and k within a chunk of rows) in 16 bits for bfloat16, which has 8, 19 for float16, which has 11, and 22 for float32 and the state that is
+    answered, each with an exponent of its own: fast decays and rows or columns of very different size take no digits from one another.  A NaN or an infinite entry reaches its own
     row, all later ones and those before it of its chunk.  Results are the same from run to run; last bits depend on how a
-    sequence is cut, so on B, H and L, and on whether there are tangents.
+    sequence is cut, so on B, H and L, on whether there are tangents, and in the 16-bit types on whether the last state is answered, which
+    is then carried in more bits.
 
     The gradient goes to q, k, v and state, through values and tangents.  That of the values can be differentiated once more; that through the
     tangents cannot.  Gradients that are taken inside a forward-AD level carry their tangents, but for those through the tangent, which are
