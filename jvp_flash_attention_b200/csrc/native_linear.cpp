@@ -144,7 +144,7 @@ struct LinearOp : ModuleOp {
 
 bool decays_acceptable(const Tensor& w, const Tensor& like, int64_t heads) {
   return !w.defined() || (w.dim() == 1 && w.size(0) == heads && w.scalar_type() == at::kFloat && w.is_contiguous() && w.device() == like.device() &&
-                          !w.requires_grad() && !w._fw_grad(0).defined() && !is_wrapped(w));
+                          !(w.requires_grad() && at::GradMode::is_enabled()) && !w._fw_grad(0).defined() && !is_wrapped(w));
 }
 
 bool linear_acceptable(const Tensors& x, const Tensors& extras) {

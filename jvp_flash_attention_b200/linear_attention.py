@@ -30,7 +30,7 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor | None =
 
     q, k: (B, H, L, D), v: (B, H, L, E), bfloat16, float16 or float32, of any strides with contiguous entries, plain or dual; D and E from 1 to 128,
     fastest at 32, 64 and 128.  o has v's layout.  ``log_decay``: (H) float32, the logarithm of each head's decay, at most 0 (None: no decay; -inf:
-    a row sees itself alone); no gradient.  ``sm_scale``: 1 / sqrt(D) by default.  ``state``: (B, H, D, E) float32, S before the first row, plain or
+    a row sees itself alone); no gradient, so one that requires it is taken under ``torch.no_grad()`` alone.  ``sm_scale``: 1 / sqrt(D) by default.  ``state``: (B, H, D, E) float32, S before the first row, plain or
     dual.  ``lengths``: (B) int32, rows of each sequence; those behind are not read and their results are zero, and S is that behind the last one.
 
     Sums and states are in 32 bits.  Entries are multiplied as they are; what is formed of them in 32 bits and multiplied again (decayed entries, states,
@@ -100,7 +100,7 @@ def _check_operands(q, k, v, state, log_decay, B, H, D, E) -> None:
             raise TypeError(f"log_decay must be a float32 vector of {H} values, got {log_decay.dtype} {tuple(log_decay.shape)}")
         if not log_decay.is_contiguous():
             raise ValueError("log_decay must be contiguous")
-        if log_decay.requires_grad or fwAD.unpack_dual(log_decay).tangent is not None:
+        if (log_decay.requires_grad and torch.is_grad_enabled()) or fwAD.unpack_dual(log_decay).tangent is not None:
             raise NotImplementedError("linear attention has no derivative with respect to log_decay; pass log_decay.detach()")
     for name, x in (("k", k), ("v", v), ("state", state), ("log_decay", log_decay)):
         if x is not None and x.device != q.device:

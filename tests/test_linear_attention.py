@@ -151,6 +151,22 @@ def test_bad_arguments(cpu):
             call()
 
 
+def test_a_decay_that_is_a_parameter(cpu):
+    """Refused where a gradient would be lost, and only there."""
+    q, k, v, s = _operands(13)
+    w = DECAY.clone().requires_grad_()
+    want = la.linear_attention(q, k, v, DECAY, state=s, return_state=True)
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            _close(la.linear_attention(q, k, v, w, state=s, return_state=True), want)
+            la._check_step(q[:, :, 0], k[:, :, 0], v[:, :, 0], w, 1.0, s)
+    for call in (lambda: la.linear_attention(q, k, v, w), lambda: la.linear_attention_step(q[:, :, 0], k[:, :, 0], v[:, :, 0], w, s)):
+        with pytest.raises(NotImplementedError, match="log_decay"):
+            call()
+    with torch.no_grad(), fwAD.dual_level(), pytest.raises(NotImplementedError, match="log_decay"):
+        la.linear_attention(q, k, v, fwAD.make_dual(DECAY, DECAY))
+
+
 def test_rows_are_counted_in_32_bits():
     x = torch.ones(1, 1, 1, 1).expand(1, 1, 2**30 + 1, 1)
     with pytest.raises(ValueError, match="at most 2\\*\\*30 rows"):
