@@ -65,10 +65,11 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Scan 
 // Rows of a segment and segments (1: no workspace).
 void cut(Scan& s) {
   // Rounds of as many CTAs as SMs hold at once, each of a segment's rows, and the states that a segment costs, about 3/1000 of a sequence; no
-  // segment below 128 rows.  (us by segments: bf16 B4 H16 L2048 D64 with tangents and gradients, 296 CTAs at once, 4 / 6 / 8 / 11: 426 / 592 / 459 / 506;
-  // L8192 D128 forward and backward 4 / 8 / 9 / 16: 1584 / 1620 / 1552 / 1549; fp32 B2 H8 L1023 D128 with tangents, 148 at once, 4 / 6 / 8: 377 / 294 / 223.)
+  // segment below 128 rows.  (us by segments, those of the rule marked: bf16 B4 H16 L2048 D64 with tangents and gradients 4* / 6 / 8 / 11: 407 / 550 / 431 /
+  // 467; L8192 D128 forward and backward 4 / 6 / 8 / 9* / 16: 1587 / 1714 / 1615 / 1533 / 1510; fp32 B2 H8 L1023 D128 with tangents 4 / 6 / 8*: 363 / 281 / 218;
+  // B4 H16 L2048 D64 with tangents and gradients 4 / 6 / 11 / 16*: 2202 / 2461 / 2110 / 2041, without tangents 4 / 6* / 8 / 11: 715 / 687 / 698 / 670.)
   const int heads = s.B * s.H, width = s.D > s.E ? s.D : s.E, chunk = s.dtype == JVPFA_FP32 && width > 64 ? 32 : 64;
-  const int room = kSMs * (width <= 64 ? (s.dual ? 2 : width <= 32 || s.dtype == JVPFA_FP32 ? 4 : 3) : s.dual || s.dtype == JVPFA_FP32 ? 1 : 2);
+  const int room = kSMs * (s.dtype == JVPFA_FP32 ? scan_ctas(s) : s.dtype == JVPFA_BF16 ? chunk_ctas<__nv_bfloat16>(s) : chunk_ctas<__half>(s));
   s.segments = 1, s.segment = s.L;
   double least = 1e30;
   for (int n = 1; n <= kMostSegments; ++n) {

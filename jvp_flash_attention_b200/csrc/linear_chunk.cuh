@@ -634,7 +634,18 @@ int launch(const Scan& s, cudaStream_t stream) {
   return width <= 32 ? launch<T, 32, OUT>(s, stream) : width <= 64 ? launch<T, 64, OUT>(s, stream) : launch<T, 128, OUT>(s, stream);
 }
 
+template <typename T, int DT>
+int ctas_of(const Scan& s) {
+  return s.dual ? ChunkShape<T, DT, true, true>::CTAS : ChunkShape<T, DT, false, true>::CTAS;
+}
+
 }  // namespace
+
+template <typename T>
+int chunk_ctas(const Scan& s) {
+  const int width = s.D > s.E ? s.D : s.E;
+  return width <= 32 ? ctas_of<T, 32>(s) : width <= 64 ? ctas_of<T, 64>(s) : ctas_of<T, 128>(s);
+}
 
 template <typename T>
 int launch_chunks(const Scan& s, bool outputs, cudaStream_t stream) {

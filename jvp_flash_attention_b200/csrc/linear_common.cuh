@@ -41,6 +41,10 @@ struct Scan {
 template <typename T>
 int launch_chunks(const Scan& s, bool outputs, cudaStream_t stream);  // 16-bit types (linear_chunk.cuh)
 int launch_scan(const Scan& s, bool outputs, cudaStream_t stream);    // float32 (linear_scan.cu)
+// CTAs that an SM holds at once of those that form the outputs.
+template <typename T>
+int chunk_ctas(const Scan& s);
+int scan_ctas(const Scan& s);
 
 // Whether a tensor's rows are whole 16-byte pieces.
 template <typename T>

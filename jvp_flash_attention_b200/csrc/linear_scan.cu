@@ -67,11 +67,13 @@ struct ScanShape {
   static constexpr size_t bytes(bool dual, bool outs) {
     return (dual ? 2 : 1) * (sizeof(float) * (size_t)CH * LD * (outs ? 3 : 2) + (outs ? sizeof(float) * (size_t)CH * LP : 0));
   }
+  // CTAs of an SM: as its shared memory has room for (2 KB of each are the system's and the powers), one with D = 128, which takes all registers.
+  static constexpr int ctas(bool dual) { return DT == 128 ? 1 : (int)(227 * 1024 / (bytes(dual, true) + 2048)); }
 };
 
 // OUT: the outputs, from the states that the segments begin with; else the states that their rows leave, from nothing.
 template <int DT, bool DUAL, bool OUT>
-__global__ void __launch_bounds__(2 * DT) scan_kernel(const __grid_constant__ Scan p, const uint32_t wide) {
+__global__ void __launch_bounds__(2 * DT, ScanShape<DT>::ctas(DUAL)) scan_kernel(const __grid_constant__ Scan p, const uint32_t wide) {
   using S = ScanShape<DT>;
   constexpr int CH = S::CH, NT = S::NT, LD = S::LD, LP = S::LP, ND = DT / 8;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -334,6 +336,11 @@ int launch(const Scan& s, cudaStream_t stream) {
 }
 
 }  // namespace
+
+int scan_ctas(const Scan& s) {
+  const int width = s.D > s.E ? s.D : s.E;
+  return width <= 32 ? ScanShape<32>::ctas(s.dual) : width <= 64 ? ScanShape<64>::ctas(s.dual) : ScanShape<128>::ctas(s.dual);
+}
 
 int launch_scan(const Scan& s, bool outputs, cudaStream_t stream) { return outputs ? launch<true>(s, stream) : launch<false>(s, stream); }
 

@@ -222,3 +222,12 @@ def test_the_c_entries_refuse():
     for want, kw in [(-7, dict(struct_size=8)), (-3, dict(dtype=9)), (-2, dict(D=0)), (-2, dict(E=129)), (-1, dict(o=None)), (-8, dict(q=65)), (-8, dict(state=66)),
                      (-2, dict(state_stride=(0, 16))), (-2, dict(state_stride=(16, 16))), (-2, dict(state_stride=(24, 16))), (-2, dict(state_stride=(16, 8)))]:
         assert step(**kw) == want, kw
+
+
+def test_sequences_are_cut_into_rounds_that_fit():
+    """float32 of 64 columns with tangents: shared memory has room for one CTA of an SM, so 148 at once (the cut shows in what a forward keeps)."""
+    a = _lib.LinearArgs()
+    a.struct_size = ctypes.sizeof(a)
+    a.dtype, a.B, a.H, a.L, a.D, a.E, a.dual = 2, 3, 8, 1023, 64, 64, 1
+    segments = _lib.load().jvpfa_linear_kept_bytes(ctypes.byref(a)) / (2 * 4 * a.B * a.H * a.D * a.E)
+    assert segments > 1 and a.B * a.H * segments <= 148
