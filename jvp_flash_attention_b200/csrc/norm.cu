@@ -1,15 +1,18 @@
 // Entries of the norms and residual sums: argument checks, how a backward is cut, and the launch that adds up the parts of the vectors'
-// gradients.  With the parts P of a group (norm_bwd.cuh), sums over all groups for a vector that is not grouped:
+// gradients.  With the parts P of a group (norm_common.cuh), sums over all groups for a vector that is not grouped:
 //   dweight = (1 + scale) PG + tscale PtG     dscale = weight PG + tweight PtG + bias PO + tbias PtO    dshift = PO
 //   dbias = (1 + scale) PO + tscale PtO       dgate = alpha (post PE + tpost PtE)                       dpost = alpha (gate PE + tgate PtE)
 // and the tangents' the same with (PtG, PtO, PtE) for (PG, PO, PE) and nothing for their second terms.
-#include "norm_bwd.cuh"
+#include "norm_common.cuh"
 
 namespace jvpfa {
 namespace norms {
 
+// Instances in norm_fwd_*.cu and norm_bwd_*.cu.
 template <typename T>
 int launch_fwd(const jvpfa_norm_args& a, cudaStream_t s);
+template <typename T>
+int launch_bwd(const jvpfa_norm_args& a, const Cut& c, cudaStream_t s);
 
 namespace {
 

@@ -12,17 +12,9 @@
 namespace jvpfa {
 namespace norms {
 
-// The sums over a group's rows that the vectors' gradients are made of, by their place in the workspace.
-enum Part { PG, PO, PE, PtG, PtO, PtE, kParts };  // of gn n + gtn tn, gn, dr N + dtr tN, gtn n, gtn, dtr N
-
-struct Cut {
-  int groups, slices;  // of each group's rows
-  uint32_t parts;      // which sums are wanted, a bit for each
-  int n_parts;
-};
-
+// (One CTA, said so: else the compiler leaves 32 or 64 registers to the instances that hold least of a row in them.)
 template <typename T, int NC, Way WAY, bool TAN, bool HASY, bool HASN, int BOUND>
-__global__ void __launch_bounds__(BOUND) norm_bwd_kernel(const __grid_constant__ jvpfa_norm_args a, const Wide wide, const Layout lay, const bool aligned, const Cut cut) {
+__global__ void __launch_bounds__(BOUND, 1) norm_bwd_kernel(const __grid_constant__ jvpfa_norm_args a, const Wide wide, const Layout lay, const bool aligned, const Cut cut) {
   constexpr int V = 16 / (int)sizeof(T), E = V * NC, ET = TAN ? E : 1, SIDES = TAN ? 2 : 1;
   constexpr int TENSORS = SIDES * ((HASY ? 3 : 1) + (HASN ? 1 : 0));
   extern __shared__ __align__(16) unsigned char smem[];
@@ -321,14 +313,18 @@ int launch_bwd(const jvpfa_norm_args& a, const Cut& cut, bool aligned, cudaStrea
 // Entries of a thread: 8 with tangents or with the sum and its norm, else 16 of rows that give them to a whole warp; threads have 170 registers
 // with 16 entries or tangents, where a row takes at most 384 of them, else 128.  (us at 8 / 16 entries, 512 threads / 16 and 384: the norm of
 // fp16 3990 x 2731 rows 58 / 46 / 43, bf16 8192 x 4096 with sum and both norms 121 / 165 / 149, where 16 entries and their sums leave the
-// registers or, with 384 threads, one row in work on an SM.)
+// registers or, with 384 threads, one row in work on an SM.)  With tangents 16 from 4097 columns on, and 32 of any row from 8193 on, which
+// registers hold in part alone: 0.3 to 3.5 KB of a thread are in local memory with 16, 0.5 to 7.5 with 32 (bf16 2048 rows with tangents, the norm / sum and
+// both norms: 4096 columns 34 / 121 us; 4104 77 / 303, with 32 entries in 64 registers 336 / 1065; 8192 110 / 527, so 495 / 1499; 8200 287 / 1343).
 template <typename T, Way WAY, bool TAN, bool HASY, bool HASN>
 int launch_bwd(const jvpfa_norm_args& a, const Cut& c, bool al, cudaStream_t s) {
   if constexpr (WAY == DIRECT) {
+    if (a.C <= 8192) return launch_bwd<T, 16, WAY, TAN, HASY, HASN, 512>(a, c, al, s);
     return launch_bwd<T, 32, WAY, TAN, HASY, HASN, 512>(a, c, al, s);
   } else if constexpr (TAN) {
     if (a.C <= 8 * 384) return launch_bwd<T, 8, WAY, TAN, HASY, HASN, 384>(a, c, al, s);
-    return a.C <= 4096 ? launch_bwd<T, 8, WAY, TAN, HASY, HASN, 512>(a, c, al, s) : kDoesNotFit;
+    if (a.C <= 4096) return launch_bwd<T, 8, WAY, TAN, HASY, HASN, 512>(a, c, al, s);
+    return a.C <= 8192 ? launch_bwd<T, 16, WAY, TAN, HASY, HASN, 512>(a, c, al, s) : kDoesNotFit;
   } else {
     if (a.C <= 256 || (HASY && HASN && a.C <= 4096)) return launch_bwd<T, 8, WAY, TAN, HASY, HASN, 512>(a, c, al, s);
     if (a.C <= 16 * 384) return launch_bwd<T, 16, WAY, TAN, HASY, HASN, 384>(a, c, al, s);

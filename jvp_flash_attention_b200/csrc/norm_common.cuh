@@ -13,7 +13,6 @@ namespace norms {
 
 constexpr int kSMs = 148;
 
-
 // V entries in 16 bytes.
 template <typename T, int V>
 struct alignas(16) Pack {
@@ -201,8 +200,8 @@ constexpr int kSumFloats = 256;  // of a row's RowSum
 
 // Rows of several tensors on their way into shared memory, `depth` rows ahead, 16 bytes at a time.  Thread t's entries are pieces t, t + threads,
 // ... of each row.  ALIGNED: rows begin on 16 bytes, a thread fetches what it reads itself, and nobody waits for anybody.  RAGGED: rows begin
-// anywhere; the aligned pieces that a row touches are fetched, and a thread takes its entries out of two neighbours.  DIRECT: rows too wide for
-// shared memory, read and written as they are.
+// anywhere; the aligned pieces that a row touches are fetched, and a thread takes its entries out of two neighbours.  DIRECT: rows that shared
+// memory has no room for, or of more columns than a thread's 16 entries (with no tangents 32 in the forward) reach; read and written as they are.
 enum Way { ALIGNED, RAGGED, DIRECT };
 constexpr int kMostDepth = 4;
 struct Source {
@@ -470,6 +469,14 @@ inline Wide wide_vectors(const jvpfa_norm_args& a) {
   return w;
 }
 
+// The sums over a group's rows that the vectors' gradients are made of, by their place in the workspace.
+enum Part { PG, PO, PE, PtG, PtO, PtE, kParts };  // of gn n + gtn tn, gn, dr N + dtr tN, gtn n, gtn, dtr N
+
+struct Cut {
+  int groups, slices;  // of each group's rows
+  uint32_t parts;      // which sums are wanted, a bit for each
+  int n_parts;
+};
 
 }  // namespace norms
 }  // namespace jvpfa

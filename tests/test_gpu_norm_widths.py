@@ -1,0 +1,43 @@
+"""GPU tests of the norms' gradients at widths where another kernel takes over, several rows of each of a launch's CTAs.
+
+Bounds as in test_gpu_norms.py: half a step of the type and 2^-16 of the magnitudes that an entry is made of; of a vector's gradient 2^-15, here a
+sum of at most 400 / 148 rows of a CTA, 148 / 32 slices and 32 lanes, with tangents twice as many terms."""
+import pytest
+import torch
+
+from tests import _norm_formulas as formulas
+from tests.test_gpu_norms import ALL, DEV, DT, NAMES, _call, _near, _operands, _options
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("dual", [False, True])
+@pytest.mark.parametrize("present", [{"x", "weight", "bias"}, {"x", "y", "gate"}, ALL])
+@pytest.mark.parametrize("C", [4097, 4104, 6144, 8191, 8192, 8193, 8200])
+def test_gradients(C, present, dual, dt):
+    kind, post = (None, "rms") if present == {"x", "y", "gate"} else ("layer", "rms" if "y" in present else None)
+    shape, group = (2, 200, C), (2, 1)
+    x = _operands(present, shape, group, DT[dt], DT[dt], C, grad=True)
+    tx = _operands(present, shape, group, DT[dt], DT[dt], C + 1, mean=0.0, grad=True) if dual else [None] * 8
+    at = [i for i in range(8) if x[i] is not None]
+    options = _options(kind, post, x[1] is not None)
+
+    def f(*xs):
+        full = [None] * 8
+        for i, t in zip(at, xs):
+            full[i] = t
+        return _call(full, kind, post)
+
+    ys, tys = torch.func.jvp(f, tuple(x[i] for i in at), tuple(tx[i] for i in at)) if dual else (f(*(x[i] for i in at)), ())
+    g = torch.Generator(device=DEV).manual_seed(7)
+    gs, gts = ([torch.randn(shape, generator=g, device=DEV).to(DT[dt]) for _ in ts] for ts in (ys, tys))
+    leaves = [x[i] for i in at] + ([tx[i] for i in at] if dual else [])
+    grads = torch.autograd.grad((*ys, *tys), leaves, (*gs, *gts), materialize_grads=True)
+    where = lambda ts: ([ts[0], ts[1]] if len(ts) == 2 else [None, ts[0]] if x[1] is None else [ts[0], None]) if ts else [None, None]  # noqa: E731
+    _, dsize, dtsize = formulas.sizes(x, tx, where(gs), where(gts), options)
+    wanted = formulas.launch_bwd(x, tx, (), None, where(gs), where(gts), options, [True] * 16)
+    for k, d in enumerate(grads):
+        i = at[k % len(at)]
+        s = (dsize if k < len(at) else dtsize)[i]
+        _near(d, wanted[i if k < len(at) else 8 + i], s.expand(d.shape), 16 if i < 2 else 15, ("d" if k < len(at) else "dt") + NAMES[i])
