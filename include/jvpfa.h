@@ -516,7 +516,8 @@ int64_t jvpfa_norm_bwd_workspace(const jvpfa_norm_args* args);
  * q, k (and their tangents and gradients): (B, H, L, D); v, o: (B, H, L, E); any positive strides, entries contiguous; 1 <= D, E <= 128.
  * Rows from lengths[b] on are not read, and their results are zero; state_out is the state behind row lengths[b] - 1.  States are
  * (B, H, D, E) row-major, in 32 bits whatever the type, and so are all sums.  log_decay: H values, at most 0 in use (NULL: 0 for all;
- * below -1e4 it counts as -1e4, which leaves a row its own key alone).
+ * below -1e4 it counts as -1e4, which leaves a row its own key alone).  scale: at most 2^64 in size, and at least 2^-64 where the backward has gstate
+ * or gtstate, which it divides by it (else JVPFA_ERR_UNSUPPORTED).
  */
 typedef struct {
   const void* p; /* NULL: absent (a tangent: zero) */

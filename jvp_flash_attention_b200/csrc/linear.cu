@@ -191,7 +191,8 @@ int check(const jvpfa_linear_args* a, bool backward) {
   if (!a) return JVPFA_ERR_NULL;
   if (a->struct_size != (int32_t)sizeof(jvpfa_linear_args)) return JVPFA_ERR_STRUCT;
   if (const int rc = bad_sizes(*a)) return rc;
-  if (!(a->scale == a->scale) || (backward && a->scale == 0.f && (a->gstate || a->gtstate))) return JVPFA_ERR_UNSUPPORTED;
+  // (backwards, the cotangents of the last state are divided by the scale)
+  if (!(fabsf(a->scale) <= 0x1p64f) || (backward && fabsf(a->scale) < 0x1p-64f && (a->gstate || a->gtstate))) return JVPFA_ERR_UNSUPPORTED;
   if (!a->q.p || !a->k.p || !a->v.p) return JVPFA_ERR_NULL;
   if (!a->dual && (a->tq.p || a->tk.p || a->tv.p || a->tstate || a->to.p || a->tstate_out || a->gto.p || a->gtstate || a->dtq.p || a->dtk.p || a->dtv.p || a->dtstate))
     return JVPFA_ERR_NULL;

@@ -21,6 +21,7 @@ from . import _dual, _lib
 from .jvp_attention import _JVP, _is_tracing, _peek_functorch, _require_cuda
 
 MAX_WIDTH = 128
+_MIN_SCALE, _MAX_SCALE = 2.0**-64, 2.0**64  # (a last state's cotangent is divided by it, in 32 bits)
 
 
 def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor | None = None, *, sm_scale: float | None = None, state: Tensor | None = None,
@@ -30,7 +31,7 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor | None =
 
     q, k: (B, H, L, D), v: (B, H, L, E), bfloat16, float16 or float32, of any strides with contiguous entries, plain or dual; D and E from 1 to 128,
     fastest at 32, 64 and 128.  o has v's layout.  ``log_decay``: (H) float32, the logarithm of each head's decay, at most 0 (None: no decay; -inf:
-    a row sees itself alone); no gradient, so one that requires it is taken under ``torch.no_grad()`` alone.  ``sm_scale``: 1 / sqrt(D) by default.  ``state``: (B, H, D, E) float32, S before the first row, plain or
+    a row sees itself alone); no gradient, so one that requires it is taken under ``torch.no_grad()`` alone.  ``sm_scale``: 1 / sqrt(D) by default, 2**-64 to 2**64 in size.  ``state``: (B, H, D, E) float32, S before the first row, plain or
     dual.  ``lengths``: (B) int32, rows of each sequence; those behind are not read and their results are zero, and S is that behind the last one.
 
     Sums and states are in 32 bits.  Entries are multiplied as they are; what is formed of them in 32 bits and multiplied again (decayed entries, states,
@@ -45,12 +46,12 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor | None =
     third derivatives and NaN.  Under ``torch.func`` ``jvp``, ``vjp`` and ``grad`` nest as far as that goes; ``jvp`` of ``jvp`` and ``vmap`` are refused,
     and batched cotangents of ``torch.autograd.grad``.
     """
-    scale = 1.0 / math.sqrt(max(q.shape[-1], 1)) if sm_scale is None and q.dim() else sm_scale
+    scale = 1.0 / math.sqrt(max((1, *q.shape[-1:]))) if sm_scale is None else sm_scale
     options = (scale, return_state, "linear_attention")
     interp = _peek_functorch()
     out = None
     if (interp is None or (interp.level() == 1 and interp.key() == _JVP)) and not _is_tracing():
-        if not q.is_cuda or not (scale and math.isfinite(scale)):  # (the native layer checks CUDA tensors itself)
+        if not q.is_cuda or not _MIN_SCALE <= abs(scale) <= _MAX_SCALE:  # (the native layer checks CUDA tensors itself)
             _check(q, k, v, log_decay, scale, state, lengths)
         out = _lib.native().linear((q, k, v, state), log_decay, lengths, options)
     if out is None:
@@ -65,9 +66,9 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor | N
     q, k: (B, H, D), v: (B, H, E), of any strides; ``state``: (B, H, D, E) float32, as ``linear_attention`` answers it, or any (B, H) view of such
     matrices that has none twice (a slice of a larger store).  Else as ``linear_attention``.  No gradient and no tangents.
     """
-    scale = 1.0 / math.sqrt(max(q.shape[-1], 1)) if sm_scale is None and q.dim() else sm_scale
+    scale = 1.0 / math.sqrt(max((1, *q.shape[-1:]))) if sm_scale is None else sm_scale
     out = None
-    if q.is_cuda and scale and math.isfinite(scale):
+    if q.is_cuda and _MIN_SCALE <= abs(scale) <= _MAX_SCALE:
         out = _lib.native().linear_step(q, k, v, log_decay, state, scale)
     if out is None:
         _check_step(q, k, v, log_decay, scale, state)
@@ -76,8 +77,8 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor | N
 
 
 def _check_scale(scale) -> None:
-    if not scale or not math.isfinite(scale):
-        raise ValueError(f"sm_scale must be finite and not zero, got {scale}")
+    if not _MIN_SCALE <= abs(scale) <= _MAX_SCALE:
+        raise ValueError(f"sm_scale must be from 2**-64 to 2**64 in size, got {scale}")
 
 
 def _check_operands(q, k, v, state, log_decay, B, H, D, E) -> None:

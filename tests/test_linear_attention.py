@@ -231,3 +231,24 @@ def test_sequences_are_cut_into_rounds_that_fit():
     a.dtype, a.B, a.H, a.L, a.D, a.E, a.dual = 2, 3, 8, 1023, 64, 64, 1
     segments = _lib.load().jvpfa_linear_kept_bytes(ctypes.byref(a)) / (2 * 4 * a.B * a.H * a.D * a.E)
     assert segments > 1 and a.B * a.H * segments <= 148
+
+
+def test_scales_beyond_32_bits_are_refused(cpu):
+    """Backwards a last state's cotangent is divided by the scale, in 32 bits."""
+    q, k, v, s = _operands(14)
+    for scale in (1e-50, 1e-40, 1e-30, -1e-30, 1e30, 1e50):
+        for call in (lambda: la.linear_attention(q, k, v, sm_scale=scale), lambda: la.linear_attention_step(q[:, :, 0], k[:, :, 0], v[:, :, 0], None, s, sm_scale=scale)):  # noqa: B023
+            with pytest.raises(ValueError, match="sm_scale"):
+                call()
+    o, last = la.linear_attention(q, k, v, sm_scale=2.0**-64, return_state=True)
+    torch.testing.assert_close(o, ((q @ k.transpose(-1, -2)).tril() @ v) * 2.0**-64, rtol=1e-6, atol=0)
+    lib = _lib.load()
+    for scale, gstate, want in ((2.0**-65, 64, -9), (2.0**65, None, -9), (float("inf"), None, -9), (2.0**-65, None, 0)):
+        a = _lib.LinearArgs()
+        a.struct_size = ctypes.sizeof(a)
+        a.B = a.H = 1
+        a.L, a.D, a.E, a.scale = 4, 8, 8, scale
+        a.q.p = a.k.p = a.v.p = 64
+        a.gstate = gstate
+        got = lib.jvpfa_linear_bwd(ctypes.byref(a), None)
+        assert got == want if want else got != -9
