@@ -4,7 +4,7 @@ import torch
 
 import jvp_flash_attention_b200.linear_attention as la
 from tests import _linear_formulas as formulas
-from tests.test_gpu_linear_attention import DEV, _bits, _near
+from tests.test_gpu_linear_attention import DEV, DT, _bits, _near
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +49,30 @@ def test_scales_at_the_ends_of_their_range(scale):
     _near(o.detach(), want[0], size[0], _bits(150, 32), "o")
     for d, e, f in zip(grads, dwant, dsize):
         _near(d, e, f, _bits(150, 32))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("L,lengths", [(40, None), (1400, (1400, 515))])
+def test_tangents_without_their_gradient(L, lengths, dt):
+    """A call with tangents whose gradient is taken through the values alone, or through the tangents alone: the states that the forward kept are those
+    of a call with tangents."""
+    B, H, D, E = 2, 2, 64, 32
+    g = torch.Generator(device=DEV).manual_seed(L)
+    make = lambda std: [(torch.randn(*s, generator=g, device=DEV) * std).to(DT[dt] if i < 3 else torch.float32).requires_grad_()  # noqa: E731
+                        for i, s in enumerate([(B, H, L, D), (B, H, L, D), (B, H, L, E), (B, H, D, E)])]
+    x, tx = make(1.0), make(0.3)
+    w = torch.tensor([-0.001, -0.1], device=DEV)
+    n = None if lengths is None else torch.tensor(lengths, device=DEV, dtype=torch.int32)
+    cots = [torch.randn(B, H, L, E, generator=g, device=DEV).to(DT[dt]), torch.randn(B, H, D, E, generator=g, device=DEV)]
+    mag = lambda ts: [None if t is None else t.detach().abs() for t in ts]  # noqa: E731
+    bits = _bits(L, D)
+    outs = bits if dt == "fp32" else bits + 2.0**-11
+    for through in (0, 1):
+        y, ty = torch.func.jvp(lambda *a: la.linear_attention(*a[:3], w, sm_scale=0.3, state=a[3], lengths=n, return_state=True), tuple(x), tuple(tx))
+        grads = torch.autograd.grad(ty if through else y, (*x, *tx), cots, materialize_grads=True)
+        pair = ([None, None], cots) if through else (cots, [None, None])
+        args = ((w, n), None, *pair, (0.3, True, ""), [True] * 8)
+        want = formulas.launch_bwd(x, tx, *args)
+        size = formulas.launch_bwd(mag(x), mag(tx), (w, n), None, *map(mag, pair), (0.3, True, ""), [True] * 8)
+        for i, (d, e, f) in enumerate(zip(grads, want, size)):
+            _near(d, e, f, bits if i % 4 == 3 else outs, (through, i))
