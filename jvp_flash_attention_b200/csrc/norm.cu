@@ -41,34 +41,43 @@ __device__ __forceinline__ void write_vec(const jvpfa_norm_args& a, void* p, lon
     static_cast<__half*>(p)[at] = __float2half_rn(x);
 }
 
-// Column blockIdx.x * kCols + x of the groups of chunk blockIdx.y.  `totals`: 12 rows of C values for each chunk, where there are several.
-__global__ void __launch_bounds__(kCols * kLanes) norm_parts_kernel(const __grid_constant__ jvpfa_norm_args a, const Cut cut, float* totals) {
+// Column blockIdx.x * kCols + x of the groups of chunk blockIdx.y, `per` lanes for the slices of one group, so kLanes / per groups at once.  `totals`: 12 rows of
+// C values for each chunk, where there are several.  ALL: a group takes all lanes.  (8192 groups of one row of 1024, scale and shift of each: 180 us; with all
+// lanes for a group's one slice 4.2 ms.)
+template <bool ALL>
+__global__ void __launch_bounds__(kCols * kLanes) norm_parts_kernel(const __grid_constant__ jvpfa_norm_args a, const Cut cut, float* totals, const int lanes) {
   __shared__ float part[kParts][kLanes][kCols + 1];
   const int x = threadIdx.x % kCols, lane = threadIdx.x / kCols, col = blockIdx.x * kCols + x;
-  const bool live = col < a.C;
+  const int per = ALL ? kLanes : lanes, sub = lane % per, at = lane / per, at_once = kLanes / per;
   Totals t;
 #pragma unroll
   for (int i = 0; i < 6; ++i) t.d[i] = t.dt[i] = 0.f;
   const long long g0 = (long long)cut.groups * blockIdx.y / gridDim.y, g1 = (long long)cut.groups * (blockIdx.y + 1) / gridDim.y;
-  for (long long group = g0; group < g1; ++group) {
+  for (long long first = g0; first < g1; first += at_once) {
+    const long long group = first + at;
+    const bool live = col < a.C && group < g1;
     float p[kParts] = {};
     if (live)
 #pragma unroll 4
-      for (int slice = lane; slice < cut.slices; slice += kLanes) {
+      for (int slice = sub; slice < cut.slices; slice += per) {
         const float* from = static_cast<const float*>(a.workspace) + (group * cut.slices + slice) * cut.n_parts * (long long)a.C + col;
 #pragma unroll
         for (int k = 0; k < kParts; ++k)
           if (cut.parts >> k & 1) p[k] += *from, from += a.C;
       }
-    __syncthreads();
+    if (per > 1) {
+      __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kParts; ++k) part[k][lane][x] = p[k];
-    __syncthreads();
-    if (lane != 0 || !live) continue;
+      for (int k = 0; k < kParts; ++k) part[k][lane][x] = p[k];
+      __syncthreads();
+    }
+    if (sub != 0 || !live) continue;
+    if (per > 1) {
 #pragma unroll
-    for (int k = 0; k < kParts; ++k) {
-      p[k] = 0.f;
-      for (int l = 0; l < kLanes; ++l) p[k] += part[k][l][x];
+      for (int k = 0; k < kParts; ++k) {
+        p[k] = 0.f;
+        for (int l = 0; l < per; ++l) p[k] += part[k][lane + l][x];
+      }
     }
     auto v = [&](int which, bool tangent, float otherwise) { return vec_scalar(a, which, tangent, group, col, otherwise); };
     const float w = v(JVPFA_VEC_WEIGHT, false, 1.f), tw = v(JVPFA_VEC_WEIGHT, true, 0.f), b = v(JVPFA_VEC_BIAS, false, 0.f), tb = v(JVPFA_VEC_BIAS, true, 0.f);
@@ -88,7 +97,24 @@ __global__ void __launch_bounds__(kCols * kLanes) norm_parts_kernel(const __grid
       }
     }
   }
-  if (lane != 0 || !live) return;
+  static_assert(kParts >= 6, "a vector's sums go where the parts were");
+  if (at_once > 1) {  // what each of them has added up
+    auto over_groups = [&](float(&mine)[6]) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 6; ++i)
+        if (sub == 0) part[i][at][x] = mine[i];
+      __syncthreads();
+      if (lane != 0) return;
+#pragma unroll
+      for (int i = 0; i < 6; ++i) {
+        mine[i] = 0.f;
+        for (int l = 0; l < at_once; ++l) mine[i] += part[i][l][x];
+      }
+    };
+    over_groups(t.d), over_groups(t.dt);
+  }
+  if (lane != 0 || col >= a.C) return;
 #pragma unroll
   for (int i = 0; i < 6; ++i) {
     if (a.vec[i].grouped) continue;
@@ -153,7 +179,7 @@ int check(const jvpfa_norm_args* a, bool backward) {
 
 struct Plan {
   Cut cut;
-  int chunks;
+  int per, chunks;  // lanes for a group where parts are added up; CTAs that share the groups of a column
   int64_t parts_bytes, bytes;
 };
 
@@ -170,7 +196,9 @@ Plan plan_bwd(const jvpfa_norm_args& a) {
   if (wants(JVPFA_VEC_GATE) || wants(JVPFA_VEC_POST_WEIGHT)) p.cut.parts |= 1u << PE;
   if (a.dual) p.cut.parts |= p.cut.parts << PtG;
   for (int k = 0; k < kParts; ++k) p.cut.n_parts += p.cut.parts >> k & 1;
-  p.chunks = p.cut.groups < kMostChunks ? p.cut.groups : kMostChunks;
+  for (p.per = 1; p.per < p.cut.slices && p.per < kLanes;) p.per *= 2;
+  p.chunks = (p.cut.groups + kLanes / p.per - 1) / (kLanes / p.per);
+  if (p.chunks > kMostChunks) p.chunks = kMostChunks;
   p.parts_bytes = (int64_t)p.cut.groups * p.cut.slices * p.cut.n_parts * a.C * 4;
   p.bytes = p.cut.parts ? p.parts_bytes + (p.chunks > 1 ? (int64_t)p.chunks * 12 * a.C * 4 : 0) : 0;
   return p;
@@ -210,7 +238,8 @@ int jvpfa_norm_bwd(const jvpfa_norm_args* a, void* stream) {
     rc = a->dtype == JVPFA_BF16 ? norms::launch_bwd<__nv_bfloat16>(*a, p.cut, s) : norms::launch_bwd<__half>(*a, p.cut, s);
   if (rc || !p.cut.parts) return rc;
   float* totals = p.chunks > 1 ? reinterpret_cast<float*>(static_cast<char*>(a->workspace) + p.parts_bytes) : nullptr;
-  norms::norm_parts_kernel<<<dim3((a->C + norms::kCols - 1) / norms::kCols, p.chunks), norms::kCols * norms::kLanes, 0, s>>>(*a, p.cut, totals);
+  const auto parts = p.per == norms::kLanes ? norms::norm_parts_kernel<true> : norms::norm_parts_kernel<false>;
+  parts<<<dim3((a->C + norms::kCols - 1) / norms::kCols, p.chunks), norms::kCols * norms::kLanes, 0, s>>>(*a, p.cut, totals, p.per);
   bool ungrouped = false;
   for (int i = 0; i < 6; ++i) ungrouped = ungrouped || (!a->vec[i].grouped && (a->d[i] || a->dt[i]));
   if (totals && ungrouped) norms::norm_totals_kernel<<<dim3((a->C + 127) / 128, 12), 128, 0, s>>>(*a, totals, p.chunks);

@@ -45,8 +45,9 @@ def test_gradients(C, present, dual, dt):
 
 @pytest.mark.parametrize("dual", [False, True])
 def test_many_groups(dual):
-    """Several thousand groups with vectors of their own, and others of all rows.  The sum over rows goes by 3 rows, 4000 / 64 groups one after the other
-    and 64 parts of these: with the magnitudes of a row (2^-16) and 130 roundings of 2^-24, 2^-15."""
+    """Several thousand groups with vectors of their own, and others of all rows.  The sum over rows goes by 3 rows, the groups of one of
+    64 parts (at most 4000 / 64 one after the other, by the lanes that take turns with them fewer), and these: with the magnitudes of a row (2^-16) and at
+    most 130 roundings of 2^-24, 2^-15."""
     present, shape, group = {"x", "y", "weight", "bias", "scale", "gate", "post_weight"}, (4000, 3, 72), (4000, 1)
     x = _operands(present, shape, group, torch.float32, torch.float32, 1, grad=True)
     tx = _operands(present, shape, group, torch.float32, torch.float32, 2, mean=0.0, grad=True) if dual else [None] * 8
@@ -66,6 +67,35 @@ def test_many_groups(dual):
     options, gts = _options("layer", "rms", True), list(gts) or [None, None]
     _, dsize, dtsize = formulas.sizes(x, tx, list(gs), gts, options)
     wanted = formulas.launch_bwd(x, tx, (), None, list(gs), gts, options, [True] * 16)
+    for k, d in enumerate(grads):
+        i = at[k % len(at)]
+        s = (dsize if k < len(at) else dtsize)[i]
+        _near(d, wanted[i if k < len(at) else 8 + i], s.expand(d.shape), 16 if i < 2 else 15, ("d" if k < len(at) else "dt") + NAMES[i])
+
+
+@pytest.mark.parametrize("dual", [False, True])
+@pytest.mark.parametrize("groups,rows,C", [(3, 1, 40), (33, 2, 72), (65, 9, 33), (148, 1, 520), (149, 4, 40), (2049, 1, 72)])
+def test_groups_beside_vectors_of_all_rows(groups, rows, C, dual):
+    """As many slices of a group and groups at once as there are.  At most 148 rows and slices of a group, and 2049 / 64 groups and 64 parts of them: 2^-15."""
+    present, shape, group = {"x", "weight", "scale", "shift"}, (groups, rows, C), (groups, 1)
+    x = _operands(present, shape, group, torch.float32, torch.float32, 1, grad=True)
+    tx = _operands(present, shape, group, torch.float32, torch.float32, 2, mean=0.0, grad=True) if dual else [None] * 8
+    at = [i for i in range(8) if x[i] is not None]
+
+    def f(*xs):
+        full = [None] * 8
+        for i, t in zip(at, xs):
+            full[i] = t
+        return _call(full, "layer", None)
+
+    ys, tys = torch.func.jvp(f, tuple(x[i] for i in at), tuple(tx[i] for i in at)) if dual else (f(*(x[i] for i in at)), ())
+    g = torch.Generator(device=DEV).manual_seed(3)
+    gs, gts = ([torch.randn(shape, generator=g, device=DEV) for _ in ts] for ts in (ys, tys))
+    leaves = [x[i] for i in at] + ([tx[i] for i in at] if dual else [])
+    grads = torch.autograd.grad((*ys, *tys), leaves, (*gs, *gts), materialize_grads=True)
+    options, pair = _options("layer", None, False), ([None, *gs], [None, *gts] if dual else [None, None])
+    _, dsize, dtsize = formulas.sizes(x, tx, *pair, options)
+    wanted = formulas.launch_bwd(x, tx, (), None, *pair, options, [True] * 16)
     for k, d in enumerate(grads):
         i = at[k % len(at)]
         s = (dsize if k < len(at) else dtsize)[i]
