@@ -31,15 +31,16 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor | None =
 
     q, k: (B, H, L, D), v: (B, H, L, E), bfloat16, float16 or float32, of any strides with contiguous entries, plain or dual; D and E from 1 to 128,
     fastest at 32, 64 and 128.  o has v's layout.  ``log_decay``: (H) float32, the logarithm of each head's decay, at most 0 (None: no decay; -inf:
-    a row sees itself alone); no gradient, so one that requires it is taken under ``torch.no_grad()`` alone.  ``sm_scale``: 1 / sqrt(D) by default, 2**-64 to 2**64 in size.  ``state``: (B, H, D, E) float32, S before the first row, plain or
-    dual.  ``lengths``: (B) int32, rows of each sequence; those behind are not read and their results are zero, and S is that behind the last one.
+    a row sees itself alone); no gradient, so one that requires it is taken under ``torch.no_grad()`` alone.  ``sm_scale``: 1 / sqrt(D) by default,
+    2**-64 to 2**64 in size.  ``state``: (B, H, D, E) float32, S before the first row, plain or dual.  ``lengths``: (B) int32, rows of each
+    sequence; those behind are not read and their results are zero, and S is that behind the last one.
 
-    Sums and states are in 32 bits.  Entries are multiplied as they are; what is formed of them in 32 bits and multiplied again (decayed entries, states,
-    the products of q and k within a chunk of rows) in 16 bits for bfloat16, which has 8, 19 for float16, which has 11, and 22 for float32 and the state that is
-    answered, each with an exponent of its own: fast decays and rows or columns of very different size take no digits from one another.  A NaN or an infinite entry reaches its own
-    row, all later ones and those before it of its chunk.  Results are the same from run to run; last bits depend on how a
-    sequence is cut, so on B, H and L, on whether there are tangents, and in the 16-bit types on whether the last state is answered, which
-    is then carried in more bits.
+    Sums and states are in 32 bits.  Entries are multiplied as they are; what is formed of them in 32 bits and multiplied again (decayed entries,
+    states, the products of q and k within a chunk of rows) in 16 bits for bfloat16, which has 8, 19 for float16, which has 11, and 22 for float32 and
+    the state that is answered, each with an exponent of its own: fast decays and rows or columns of very different size take no digits from one
+    another.  A NaN or an infinite entry reaches its own row, all later ones and those before it of its chunk.  Results are the same from run to run;
+    last bits depend on how a sequence is cut, so on B, H and L, on whether there are tangents, and in the 16-bit types on whether the last
+    state is answered, which is then carried in more bits.
 
     The gradient goes to q, k, v and state, through values and tangents.  That of the values can be differentiated once more; that through the
     tangents cannot.  Gradients that are taken inside a forward-AD level carry their tangents, but for those through the tangent, which are
